@@ -14,7 +14,7 @@ import threading
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libb200gdn.so')
 
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 FWD_INTRA, FWD_SCAN, FWD_OUT = 1, 2, 4
 BWD_DVLOCAL, BWD_SCAN, BWD_DQKWG, BWD_WY = 1, 2, 4, 8
@@ -94,12 +94,47 @@ class FoldArgs(C.Structure):
     ]
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = [
+        ('struct_bytes', C.c_int32), ('D', C.c_int32), ('rows', C.c_int64), ('dtype', C.c_int32), ('param_dtype', C.c_int32),
+        ('eps', C.c_float),
+        ('x', _p), ('residual', _p), ('weight', _p), ('bias', _p), ('z', _p), ('y', _p), ('mean', _p), ('rstd', _p),
+        ('dy', _p), ('dz', _p), ('dx', _p), ('dweight', _p), ('dbias', _p), ('partials', _p),
+    ]
+
+
+_ROWS_OF_LOGITS = [('struct_bytes', C.c_int32), ('V', C.c_int32), ('rows', C.c_int64), ('inner', C.c_int64),
+                   ('stride_inner', C.c_int64), ('stride_outer', C.c_int64), ('dtype', C.c_int32)]
+MAX_TOP, MAX_LIST = 128, 256
+
+
+class LogprobArgs(C.Structure):
+    _fields_ = _ROWS_OF_LOGITS + [
+        ('top_k', C.c_int32), ('scale', C.c_float), ('token_bytes', C.c_int32),
+        ('logits', _p), ('tokens', _p), ('logprobs', _p), ('entropy', _p), ('top_logprobs', _p), ('top_ids', _p), ('stats', _p),
+        ('dlogprobs', _p), ('dentropy', _p), ('dtop_logprobs', _p), ('dlogits', _p),
+    ]
+
+
+DISTILL_BUCKET, DISTILL_MEAN, DISTILL_SCALAR, DISTILL_SKIP_ONE = 1, 2, 4, 8
+
+
+class DistillArgs(C.Structure):
+    _fields_ = _ROWS_OF_LOGITS + [
+        ('K', C.c_int32), ('scale', C.c_float), ('flags', C.c_uint32), ('id_bytes', C.c_int32), ('teacher_dtype', C.c_int32),
+        ('logits', _p), ('teacher', _p), ('ids', _p), ('row_loss', _p), ('loss', _p), ('stats', _p), ('counters', _p),
+        ('dloss', _p), ('dlogits', _p),
+    ]
+
+
 EXPORTS = (
     'b200gdn_chunk_fwd', 'b200gdn_chunk_bwd', 'b200gdn_recurrent_fwd', 'b200gdn_affine_apply',
     'b200gdn_saved_bytes', 'b200gdn_bwd_workspace_bytes', 'b200gdn_last_launch_count',
     'b200gdn_abi_version', 'b200gdn_last_error', 'b200gdn_device_status', 'b200gdn_prep_fwd', 'b200gdn_prep_bwd',
     'b200gdn_selftest_wait_expiry', 'b200gdn_chunk_fwd_static', 'b200gdn_cp_fold', 'b200gdn_cp_prefix',
     'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd', 'b200gdn_norm_gate_ctas',
+    'b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd', 'b200gdn_layer_norm_ctas', 'b200gdn_logprob_fwd', 'b200gdn_logprob_bwd',
+    'b200gdn_distill_fwd', 'b200gdn_distill_bwd',
 )
 
 _lib = None
@@ -125,7 +160,9 @@ def load():
         lib = C.CDLL(LIB_PATH)
         for name in ('b200gdn_chunk_fwd', 'b200gdn_chunk_bwd', 'b200gdn_recurrent_fwd', 'b200gdn_affine_apply',
                      'b200gdn_prep_fwd', 'b200gdn_prep_bwd', 'b200gdn_chunk_fwd_static', 'b200gdn_cp_fold', 'b200gdn_cp_prefix',
-                     'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd'):
+                     'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd',
+                     'b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd', 'b200gdn_logprob_fwd', 'b200gdn_logprob_bwd',
+                     'b200gdn_distill_fwd', 'b200gdn_distill_bwd'):
             fn = getattr(lib, name)
             fn.restype = C.c_int
             fn.argtypes = [C.c_void_p, C.c_void_p]
@@ -135,6 +172,8 @@ def load():
             fn.argtypes = [C.c_int32] * 6
         lib.b200gdn_norm_gate_ctas.restype = C.c_int
         lib.b200gdn_norm_gate_ctas.argtypes = [C.c_int64]
+        lib.b200gdn_layer_norm_ctas.restype = C.c_int
+        lib.b200gdn_layer_norm_ctas.argtypes = [C.c_int64, C.c_int32, C.c_int32]
         lib.b200gdn_last_launch_count.restype = C.c_int
         lib.b200gdn_device_status.restype = C.c_int
         lib.b200gdn_device_status.argtypes = []

@@ -1,14 +1,18 @@
-"""The two steps either side of the mixer in fla.layers.GatedDeltaNet, with the reference's interfaces:
+"""The steps either side of the mixer, with the reference's interfaces: in fla.layers.GatedDeltaNet
 
 * ``causal_conv1d`` / ``ShortConvolution`` — the short causal depthwise convolution (+ SiLU) applied to the q, k, v
   projections (fla/modules/conv/causal_conv1d.py:17-160, fla/modules/conv/short_conv.py:24-260), including the
   decode step on a cache and the context-parallel form whose first local sequence starts from the previous rank's
   last W-1 tokens (fla/modules/conv/cp/ops.py:15-260);
 * ``rms_norm_gated`` / ``FusedRMSNormGated`` — the gated RMS norm on the mixer's output
-  (fla/modules/fused_norm_gate.py:861-884, 1007-1068).
+  (fla/modules/fused_norm_gate.py:861-884, 1007-1068);
 
-Both run as HBM-streaming kernels of libb200gdn.so (b200gdn_conv_fwd/bwd, b200gdn_norm_gate_fwd/bwd); there is no
-fallback path.
+and ahead of it, in the block around the layer,
+
+* ``layer_norm`` / ``LayerNorm`` — layer norm with the residual sum (fla/modules/layernorm.py).
+
+All run as HBM-streaming kernels of libb200gdn.so (b200gdn_conv_fwd/bwd, b200gdn_norm_gate_fwd/bwd,
+b200gdn_layer_norm_fwd/bwd); there is no fallback path.
 """
 from __future__ import annotations
 
@@ -212,3 +216,30 @@ class FusedRMSNormGated(nn.Module):
                 return y
         return rms_norm_gated(x, g, weight, bias, self.activation, residual=residual, eps=self.eps,
                               prenorm=prenorm, residual_in_fp32=residual_in_fp32)
+
+
+def layer_norm(x, weight=None, bias=None, residual=None, eps: float = 1e-5, prenorm: bool = False):
+    """``(z - mean) rstd weight + bias`` over the last dimension of any width, with ``z = x + residual`` (rounded to the type of
+    both, as the rest of the model sees it) or ``z = x``.  ``prenorm=True`` returns ``(y, z)``: z goes on as the residual stream.
+    x and residual in bf16, fp16 or fp32; weight and bias in any of these or absent.  The reference's ``layer_norm``
+    (fla/modules/layernorm.py) with a residual of the type of x."""
+    if not x.is_cuda:
+        raise _lib.B200GDNError('layer_norm runs on a CUDA device only (no CPU path)')
+    args = (x, weight, bias, residual, eps, prenorm)
+    out = _lib.host().layer_norm(*args)
+    if out is NotImplemented:
+        out = RecordedCall.apply(_lib.host().layer_norm, *args)
+    return (out, x) if prenorm and residual is None else out
+
+
+class LayerNorm(nn.Module):
+    """The layer ahead of a mixer: parameters and forward contract of the reference's ``LayerNorm`` (fla/modules/layernorm.py)."""
+
+    def __init__(self, hidden_size: int, elementwise_affine: bool = True, bias: bool = False, eps: float = 1e-5, device=None, dtype=None):
+        super().__init__()
+        self.hidden_size, self.elementwise_affine, self.eps = hidden_size, elementwise_affine, eps
+        self.register_parameter('weight', nn.Parameter(torch.ones(hidden_size, device=device, dtype=dtype)) if elementwise_affine else None)
+        self.register_parameter('bias', nn.Parameter(torch.zeros(hidden_size, device=device, dtype=dtype)) if elementwise_affine and bias else None)
+
+    def forward(self, x, residual=None, prenorm=False):
+        return layer_norm(x, self.weight, self.bias, residual=residual, eps=self.eps, prenorm=prenorm)

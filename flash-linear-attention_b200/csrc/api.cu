@@ -338,6 +338,119 @@ int b200gdn_norm_gate_bwd(const b200gdn_norm_gate_args* a, void* stream) {
 
 int b200gdn_norm_gate_ctas(int64_t rows) { return gdn::norm_gate_grid(rows); }
 
+static int check_layer_norm_args(const b200gdn_layer_norm_args* a, const char* who, bool bwd) {
+  using namespace gdn;
+  if (a == nullptr) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: args is NULL", who);
+  if (a->struct_bytes != (int32_t)sizeof(b200gdn_layer_norm_args))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: struct_bytes %d != %zu (ABI mismatch)", who, a->struct_bytes,
+                     sizeof(b200gdn_layer_norm_args));
+  if (a->rows <= 0 || a->D <= 0) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: empty problem (rows=%lld D=%d)", who, (long long)a->rows, a->D);
+  if (a->rows > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows", who);
+  if (a->dtype < 0 || a->dtype > 2 || a->param_dtype < 0 || a->param_dtype > 2)
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: dtype codes %d, %d", who, a->dtype, a->param_dtype);
+  if (!bwd) {
+    REQUIRE(a->x, who); REQUIRE(a->y, who);
+    if ((a->mean == nullptr) != (a->rstd == nullptr)) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: mean and rstd come together", who);
+  } else {
+    REQUIRE(a->z, who); REQUIRE(a->mean, who); REQUIRE(a->rstd, who); REQUIRE(a->dy, who); REQUIRE(a->dx, who);
+    if (a->dweight != nullptr || a->dbias != nullptr) REQUIRE(a->partials, who);
+  }
+  return 0;
+}
+
+int b200gdn_layer_norm_fwd(const b200gdn_layer_norm_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_layer_norm_args(a, "layer_norm_fwd", false)) return e;
+  return gdn::launch_layer_norm(*a, static_cast<cudaStream_t>(stream), false);
+}
+
+int b200gdn_layer_norm_bwd(const b200gdn_layer_norm_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_layer_norm_args(a, "layer_norm_bwd", true)) return e;
+  return gdn::launch_layer_norm(*a, static_cast<cudaStream_t>(stream), true);
+}
+
+int b200gdn_layer_norm_ctas(int64_t rows, int32_t D, int32_t dtype) { return gdn::layer_norm_grid(rows, D, dtype); }
+
+// what the two operators on rows of logits have in common
+static int check_rows_of_logits(const char* who, int64_t rows, int64_t inner, int32_t V, int32_t dtype, float scale, const void* logits,
+                                const void* dlogits) {
+  using namespace gdn;
+  if (rows <= 0 || V <= 0 || inner <= 0)
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: empty problem (rows=%lld V=%d inner=%lld)", who, (long long)rows, V, (long long)inner);
+  if (rows > (1 << 27)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^27 rows", who);
+  if (V > (1 << 30)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^30 entries a row", who);
+  if (dtype < 0 || dtype > 2) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: dtype code %d", who, dtype);
+  if (!(scale > 0.f) || !(scale <= 1e6f)) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: scale %g (above 0, at most 1e6)", who, scale);
+  REQUIRE(logits, who);
+  const uintptr_t off = (reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) % (dtype == 2 ? 4 : 2);
+  if (off != 0) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: logits or dlogits off their elements' boundary", who);
+  return 0;
+}
+
+static int check_logprob_args(const b200gdn_logprob_args* a, const char* who, bool bwd) {
+  using namespace gdn;
+  if (a == nullptr) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: args is NULL", who);
+  if (a->struct_bytes != (int32_t)sizeof(b200gdn_logprob_args))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: struct_bytes %d != %zu (ABI mismatch)", who, a->struct_bytes, sizeof(b200gdn_logprob_args));
+  if (int e = check_rows_of_logits(who, a->rows, a->inner, a->V, a->dtype, a->scale, a->logits, a->dlogits)) return e;
+  if (a->top_k < 0 || a->top_k > B200GDN_MAX_TOP || a->top_k > a->V)
+    return set_error(B200GDN_ERR_UNSUPPORTED, "%s: top_k=%d (0 to %d, at most V=%d)", who, a->top_k, B200GDN_MAX_TOP, a->V);
+  if (a->tokens != nullptr && a->token_bytes != 4 && a->token_bytes != 8)
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: token_bytes %d (4 or 8)", who, a->token_bytes);
+  if (!bwd) {
+    if (a->logprobs != nullptr) REQUIRE(a->tokens, who);
+    if (a->top_k > 0) { REQUIRE(a->top_ids, who); REQUIRE(a->top_logprobs, who); }
+  } else {
+    REQUIRE(a->stats, who); REQUIRE(a->dlogits, who);
+    if (a->dlogprobs != nullptr) REQUIRE(a->tokens, who);
+    if (a->dentropy != nullptr) REQUIRE(a->entropy, who);
+    if (a->dtop_logprobs != nullptr) REQUIRE(a->top_ids, who);
+  }
+  return 0;
+}
+
+int b200gdn_logprob_fwd(const b200gdn_logprob_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_logprob_args(a, "logprob_fwd", false)) return e;
+  return gdn::launch_logprob(*a, static_cast<cudaStream_t>(stream), false);
+}
+
+int b200gdn_logprob_bwd(const b200gdn_logprob_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_logprob_args(a, "logprob_bwd", true)) return e;
+  return gdn::launch_logprob(*a, static_cast<cudaStream_t>(stream), true);
+}
+
+static int check_distill_args(const b200gdn_distill_args* a, const char* who, bool bwd) {
+  using namespace gdn;
+  if (a == nullptr) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: args is NULL", who);
+  if (a->struct_bytes != (int32_t)sizeof(b200gdn_distill_args))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: struct_bytes %d != %zu (ABI mismatch)", who, a->struct_bytes, sizeof(b200gdn_distill_args));
+  if (int e = check_rows_of_logits(who, a->rows, a->inner, a->V, a->dtype, a->scale, a->logits, a->dlogits)) return e;
+  if (a->K < 1 || a->K > B200GDN_MAX_LIST)
+    return set_error(B200GDN_ERR_UNSUPPORTED, "%s: K=%d (1 to %d entries a row)", who, a->K, B200GDN_MAX_LIST);
+  if (a->id_bytes != 4 && a->id_bytes != 8) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: id_bytes %d (4 or 8)", who, a->id_bytes);
+  if (a->teacher_dtype < 0 || a->teacher_dtype > 2) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: teacher_dtype %d", who, a->teacher_dtype);
+  REQUIRE(a->teacher, who); REQUIRE(a->ids, who);
+  if (a->flags & B200GDN_DISTILL_MEAN) REQUIRE(a->counters, who);
+  if (!bwd) { REQUIRE(a->row_loss, who); }
+  else { REQUIRE(a->stats, who); REQUIRE(a->dloss, who); REQUIRE(a->dlogits, who); }
+  return 0;
+}
+
+int b200gdn_distill_fwd(const b200gdn_distill_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_distill_args(a, "distill_fwd", false)) return e;
+  return gdn::launch_distill(*a, static_cast<cudaStream_t>(stream), false);
+}
+
+int b200gdn_distill_bwd(const b200gdn_distill_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_distill_args(a, "distill_bwd", true)) return e;
+  return gdn::launch_distill(*a, static_cast<cudaStream_t>(stream), true);
+}
+
 int b200gdn_selftest_wait_expiry(void* stream) {
   gdn::g_launches = 0;
   gdn::selftest_wait_expiry_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(2000u);

@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/custom_class.h>
 
@@ -815,6 +816,346 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
   }
 };
 
+// ---- layer norm ------------------------------------------------------------------------------------------------
+// the gradients of these nodes have no derivative of their own: asking for one raises, and is not answered by zero
+variable_list once(const char* who, variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach();
+    torch::autograd::create_gradient_edge(g, std::make_shared<torch::autograd::Error>(std::string(who) + " has no second derivative"));
+  }
+  return grads;
+}
+
+struct LayerNormForward {
+  Tensor y, z, w, b, mean, rstd;   // z: what was normalised, x itself where no residual was added
+  int32_t param_dtype = 0;
+};
+
+LayerNormForward layer_norm_forward(const Tensor& x_in, const Tensor& weight, const Tensor& bias, const Tensor& residual, double eps,
+                                    bool keep_z, bool need_grad) {
+  LayerNormForward r;
+  const at::Device dev = x_in.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const at::ScalarType t = x_in.scalar_type();
+  const Tensor x = dense(x_in), res = dense(residual);
+  r.w = weight;
+  r.b = bias;
+  if (weight.defined() || bias.defined()) r.param_dtype = gate_types(r.w, r.b);
+  const int64_t D = x.size(-1), rows = x.numel() / D;
+  r.y = new_tensor(x.sizes(), t, dev);
+  if (!res.defined()) r.z = x;
+  else if (keep_z || need_grad) r.z = new_tensor(x.sizes(), t, dev);
+  if (need_grad) {
+    r.mean = new_tensor({rows}, at::kFloat, dev);
+    r.rstd = new_tensor({rows}, at::kFloat, dev);
+  }
+  if (rows == 0) return r;
+  b200gdn_layer_norm_args a{};
+  a.D = (int32_t)D;
+  a.rows = rows;
+  a.dtype = act_code(t);
+  a.param_dtype = r.param_dtype;
+  a.eps = (float)eps;
+  a.x = ptr(x);
+  a.residual = ptr(res);
+  a.weight = ptr(r.w);
+  a.bias = ptr(r.b);
+  a.z = res.defined() ? ptr(r.z) : nullptr;
+  a.y = ptr(r.y);
+  a.mean = fptr(r.mean);
+  a.rstd = fptr(r.rstd);
+  call("b200gdn_layer_norm_fwd", b200gdn_layer_norm_fwd, a);
+  return r;
+}
+
+class LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                               const std::optional<Tensor>& residual, double eps, bool prenorm) {
+    const Tensor w = val(weight), b = val(bias), res = val(residual);
+    LayerNormForward r = layer_norm_forward(x, w, b, res, eps, prenorm, true);
+    ctx->save_for_backward({r.z, r.w, r.mean, r.rstd});
+    auto ty = [](const Tensor& p) { return (int64_t)(p.defined() ? p.scalar_type() : at::kFloat); };
+    auto wanted = [](const Tensor& p) { return p.defined() && p.requires_grad(); };
+    ctx->saved_data["s"] = std::vector<int64_t>{r.param_dtype, wanted(w), wanted(b), ty(w), ty(b), res.defined()};
+    ctx->set_materialize_grads(false);
+    if (prenorm && res.defined()) return {r.y, r.z};
+    return {r.y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &z = saved[0], &w = saved[1], &mean = saved[2], &rstd = saved[3];
+    const auto s = ctx->saved_data["s"].toIntVector();
+    const at::Device dev = z.device();
+    c10::cuda::CUDAGuard guard(dev);
+    const at::ScalarType t = z.scalar_type(), pt = s[0] == B200GDN_F32 ? at::kFloat : s[0] == B200GDN_BF16 ? at::kBFloat16 : at::kHalf;
+    const int64_t D = z.size(-1), rows = z.numel() / D;
+    const Tensor dy = grads[0].defined() ? dense(grads[0], t) : new_tensor(z.sizes(), t, dev, true);
+    const Tensor dz = grads.size() > 1 && grads[1].defined() ? dense(grads[1], t) : Tensor();
+    Tensor dx = new_tensor(z.sizes(), t, dev), dw, db, partials;
+    if (s[1]) dw = new_tensor({D}, pt, dev, rows == 0);
+    if (s[2]) db = new_tensor({D}, pt, dev, rows == 0);
+    if (rows > 0) {
+      b200gdn_layer_norm_args a{};
+      a.D = (int32_t)D;
+      a.rows = rows;
+      a.dtype = act_code(t);
+      a.param_dtype = (int32_t)s[0];
+      if (s[1] || s[2]) partials = new_tensor({(int64_t)b200gdn_layer_norm_ctas(rows, a.D, a.dtype) * 2 * D}, at::kFloat, dev);
+      a.weight = ptr(w);
+      a.z = ptr(z);
+      a.mean = fptr(mean);
+      a.rstd = fptr(rstd);
+      a.dy = ptr(dy);
+      a.dz = ptr(dz);
+      a.dx = ptr(dx);
+      a.dweight = ptr(dw);
+      a.dbias = ptr(db);
+      a.partials = fptr(partials);
+      call("b200gdn_layer_norm_bwd", b200gdn_layer_norm_bwd, a);
+    }
+    return once("layer_norm", {dx, s[1] ? cast(dw, (at::ScalarType)s[3]) : Tensor(), s[2] ? cast(db, (at::ScalarType)s[4]) : Tensor(),
+                               s[5] ? dx : Tensor(), Tensor(), Tensor()});
+  }
+};
+
+// ---- rows of logits --------------------------------------------------------------------------------------------
+// The rows as the kernels address them: row r at (r / inner) outer + (r % inner) step.  Slices of a sequence or of a padded
+// vocabulary are read where they lie; what has more levels is copied.
+struct LogitRows {
+  Tensor x;
+  int64_t rows = 0, inner = 1, step = 0, outer = 0;
+};
+
+LogitRows logit_rows(const Tensor& x) {
+  LogitRows r;
+  r.x = x;
+  const int64_t V = x.size(-1), n = x.dim() - 1;
+  r.rows = x.numel() / V;
+  if (V > 1 && x.stride(-1) != 1) r.x = x.contiguous();
+  int levels = 0;
+  int64_t size[2] = {1, 1}, step[2] = {0, 0};
+  for (int64_t i = n - 1; i >= 0 && levels <= 2; --i) {
+    const int64_t len = r.x.size(i), st = r.x.stride(i);
+    if (len == 1) continue;
+    if (levels > 0 && st == size[levels - 1] * step[levels - 1]) {
+      size[levels - 1] *= len;
+    } else {
+      if (levels < 2) {
+        size[levels] = len;
+        step[levels] = st;
+      }
+      ++levels;
+    }
+  }
+  if (levels > 2) {
+    r.x = x.contiguous();
+    size[0] = r.rows;
+    step[0] = V;
+    size[1] = 1;
+  }
+  r.inner = size[0] > 0 ? size[0] : 1;
+  r.step = step[0];
+  r.outer = step[1];
+  return r;
+}
+
+template <typename Args>
+void set_rows(Args& a, const LogitRows& r, double scale) {
+  a.V = (int32_t)r.x.size(-1);
+  a.rows = r.rows;
+  a.inner = r.inner;
+  a.stride_inner = r.step;
+  a.stride_outer = r.outer;
+  a.dtype = act_code(r.x.scalar_type());
+  a.scale = (float)scale;
+  a.logits = ptr(r.x);
+}
+
+struct LogprobForward {
+  Tensor tokens, logprobs, entropy, top, ids, stats;
+};
+
+LogprobForward logprob_forward(const Tensor& logits, const Tensor& tokens, int64_t top_k, double scale, bool entropy, bool need_grad) {
+  LogprobForward r;
+  const at::Device dev = logits.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const LogitRows rows = logit_rows(logits);
+  const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
+  if (tokens.defined()) {
+    r.tokens = tokens.contiguous();
+    r.logprobs = new_tensor(lead, at::kFloat, dev);
+  }
+  if (entropy) r.entropy = new_tensor(lead, at::kFloat, dev);
+  if (top_k > 0) {
+    std::vector<int64_t> sizes = lead.vec();
+    sizes.push_back(top_k);
+    r.top = new_tensor(sizes, at::kFloat, dev);
+    r.ids = new_tensor(sizes, at::kLong, dev);
+  }
+  if (need_grad) r.stats = new_tensor({rows.rows, 2}, at::kFloat, dev);
+  if (rows.rows == 0) return r;
+  b200gdn_logprob_args a{};
+  set_rows(a, rows, scale);
+  a.top_k = (int32_t)top_k;
+  a.token_bytes = r.tokens.defined() ? (int32_t)r.tokens.element_size() : 0;
+  a.tokens = ptr(r.tokens);
+  a.logprobs = fptr(r.logprobs);
+  a.entropy = fptr(r.entropy);
+  a.top_logprobs = fptr(r.top);
+  a.top_ids = static_cast<int64_t*>(ptr(r.ids));
+  a.stats = fptr(r.stats);
+  call("b200gdn_logprob_fwd", b200gdn_logprob_fwd, a);
+  return r;
+}
+
+class LogprobFunction : public torch::autograd::Function<LogprobFunction> {
+ public:
+  // returns what there is of: logprobs, entropy, top_logprobs, top_ids
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const std::optional<Tensor>& tokens, int64_t top_k, double scale,
+                               bool entropy) {
+    LogprobForward r = logprob_forward(logits, val(tokens), top_k, scale, entropy, true);
+    ctx->save_for_backward({logits, r.tokens, r.stats, r.entropy, r.ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    variable_list out;
+    for (const Tensor& x : {r.logprobs, r.entropy, r.top, r.ids})
+      if (x.defined()) out.push_back(x);
+    if (r.ids.defined()) ctx->mark_non_differentiable({r.ids});
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2], &entropy = saved[3], &ids = saved[4];
+    const at::Device dev = logits.device();
+    c10::cuda::CUDAGuard guard(dev);
+    const LogitRows rows = logit_rows(logits);
+    Tensor dlogits = new_tensor(logits.sizes(), logits.scalar_type(), dev);
+    if (rows.rows > 0) {
+      size_t at = 0;
+      auto next = [&](const Tensor& there) {
+        Tensor g;
+        if (there.defined() && grads[at++].defined()) g = dense(grads[at - 1], at::kFloat);
+        return g;
+      };
+      const Tensor dlp = next(tokens), dh = next(entropy), dtop = next(ids);
+      b200gdn_logprob_args a{};
+      set_rows(a, rows, ctx->saved_data["scale"].toDouble());
+      a.top_k = ids.defined() ? (int32_t)ids.size(-1) : 0;
+      a.token_bytes = tokens.defined() ? (int32_t)tokens.element_size() : 0;
+      a.tokens = ptr(tokens);
+      a.entropy = fptr(entropy);
+      a.top_ids = static_cast<int64_t*>(ptr(ids));
+      a.stats = fptr(stats);
+      a.dlogprobs = fptr(dlp);
+      a.dentropy = fptr(dh);
+      a.dtop_logprobs = fptr(dtop);
+      a.dlogits = ptr(dlogits);
+      call("b200gdn_logprob_bwd", b200gdn_logprob_bwd, a);
+    }
+    return once("token_logprobs", {dlogits, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+enum Reduction { kNone = 0, kSum = 1, kMean = 2 };
+
+struct DistillForward {
+  Tensor teacher, ids, out, stats, counters, dlogits;
+};
+
+b200gdn_distill_args distill_args(const LogitRows& rows, const Tensor& teacher, const Tensor& ids, double scale, bool bucket, int64_t reduction,
+                                  const Tensor& stats, const Tensor& counters, const Tensor& dlogits) {
+  b200gdn_distill_args a{};
+  set_rows(a, rows, scale);
+  a.K = (int32_t)teacher.size(-1);
+  a.flags = (bucket ? B200GDN_DISTILL_BUCKET : 0) | (reduction == kMean ? B200GDN_DISTILL_MEAN : 0);
+  a.id_bytes = (int32_t)ids.element_size();
+  a.teacher_dtype = param_code(teacher.scalar_type());
+  a.teacher = ptr(teacher);
+  a.ids = ptr(ids);
+  a.stats = fptr(stats);
+  a.counters = static_cast<int32_t*>(ptr(counters));
+  a.dlogits = ptr(dlogits);
+  return a;
+}
+
+// `need_grad`: what the backward pass needs is kept; of a sum or mean the gradient is formed here, while the rows are on the chip
+DistillForward distill_forward(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double scale, bool bucket, int64_t reduction,
+                               bool need_grad) {
+  DistillForward r;
+  const at::Device dev = logits.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const LogitRows rows = logit_rows(logits);
+  const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
+  r.teacher = teacher.contiguous();
+  r.ids = ids.contiguous();
+  const Tensor row_loss = new_tensor(lead, at::kFloat, dev);
+  r.out = reduction == kNone ? row_loss : new_tensor({}, at::kFloat, dev, rows.rows == 0);
+  if (need_grad) {
+    r.stats = new_tensor({rows.rows, 4}, at::kFloat, dev);
+    if (reduction != kNone) r.dlogits = new_tensor(logits.sizes(), logits.scalar_type(), dev);
+  }
+  if (rows.rows == 0) return r;
+  if (reduction != kNone) r.counters = new_tensor({2}, at::kInt, dev);
+  b200gdn_distill_args a = distill_args(rows, r.teacher, r.ids, scale, bucket, reduction, r.stats, r.counters, r.dlogits);
+  a.row_loss = fptr(row_loss);
+  a.loss = reduction == kNone ? nullptr : fptr(r.out);
+  call("b200gdn_distill_fwd", b200gdn_distill_fwd, a);
+  return r;
+}
+
+// the gradient that the forward pass formed: handed out once
+struct DistillGradient : torch::CustomClassHolder {
+  std::mutex lock;
+  Tensor dlogits;
+  Tensor take() {
+    std::lock_guard<std::mutex> g(lock);
+    return std::exchange(dlogits, Tensor());
+  }
+};
+
+class DistillFunction : public torch::autograd::Function<DistillFunction> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& ids, double scale, bool bucket,
+                        int64_t reduction) {
+    DistillForward r = distill_forward(logits, teacher, ids, scale, bucket, reduction, true);
+    ctx->save_for_backward({logits, r.teacher, r.ids, r.stats, r.counters});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["bucket"] = bucket;
+    ctx->saved_data["reduction"] = reduction;
+    auto g = c10::make_intrusive<DistillGradient>();
+    g->dlogits = r.dlogits;
+    ctx->saved_data["g"] = at::IValue::make_capsule(g);
+    return r.out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &teacher = saved[1], &ids = saved[2], &stats = saved[3], &counters = saved[4];
+    const at::Device dev = logits.device();
+    c10::cuda::CUDAGuard guard(dev);
+    const LogitRows rows = logit_rows(logits);
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
+    const auto capsule = ctx->saved_data["g"].toCapsule();
+    Tensor dlogits = static_cast<DistillGradient*>(capsule.get())->take();
+    const bool formed = dlogits.defined();
+    if (!formed) dlogits = new_tensor(logits.sizes(), logits.scalar_type(), dev);
+    if (rows.rows > 0) {
+      const Tensor dloss = dense(grads[0], at::kFloat);
+      b200gdn_distill_args a = distill_args(rows, teacher, ids, ctx->saved_data["scale"].toDouble(), ctx->saved_data["bucket"].toBool(),
+                                            reduction, stats, counters, dlogits);
+      if (reduction != kNone) a.flags |= B200GDN_DISTILL_SCALAR | (formed ? B200GDN_DISTILL_SKIP_ONE : 0);
+      a.dloss = fptr(dloss);
+      call("b200gdn_distill_bwd", b200gdn_distill_bwd, a);
+    }
+    return once("topk_distill_loss", {dlogits, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
 // ---- Python side -----------------------------------------------------------------------------------------------
 struct NoGil {
   PyThreadState* st = PyEval_SaveThread();
@@ -1003,6 +1344,142 @@ PyObject* py_norm_gate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// layer_norm(x, weight, bias, residual, eps, prenorm) -> y, or (y, z) with a residual and prenorm; NotImplemented while a trace is recorded
+PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(6);
+  if (tracing()) Py_RETURN_NOTIMPLEMENTED;
+  Tensor x, w, b, res;
+  if (!get(args[0], x) || !get(args[1], w) || !get(args[2], b) || !get(args[3], res) || !x.defined()) {
+    PyErr_SetString(PyExc_TypeError, "layer_norm: a tensor is expected");
+    return nullptr;
+  }
+  const double eps = PyFloat_AsDouble(args[4]);
+  const bool prenorm = truth(args[5]);
+  if (PyErr_Occurred()) return nullptr;
+  Tensor y, z;
+  {
+    NoGil nogil;
+    if (act_code(x.scalar_type()) < 0) raise(std::string("layer_norm: dtype ") + c10::toString(x.scalar_type()) + " is not supported");
+    if (x.dim() == 0 || x.size(-1) == 0) raise("layer_norm: rows without elements");
+    for (const Tensor* p : {&w, &b})
+      if (p->defined() && (p->dim() != 1 || p->size(0) != x.size(-1) || !p->is_floating_point()))
+        raise("layer_norm: weight and bias are vectors of the " + std::to_string(x.size(-1)) + " elements of a row");
+    check("weight", w, x.size(-1), x.device());
+    check("bias", b, x.size(-1), x.device());
+    check("residual", res, x.numel(), x.device());
+    if (res.defined() && (res.sizes() != x.sizes() || res.scalar_type() != x.scalar_type()))
+      raise("layer_norm: residual has the shape and the type of x");
+    if (wants_grad({&x, &w, &b, &res})) {
+      variable_list out = LayerNormFunction::apply(x, opt(w), opt(b), opt(res), eps, prenorm);
+      y = out[0];
+      if (out.size() > 1) z = out[1];
+    } else {
+      LayerNormForward r = layer_norm_forward(x, w, b, res, eps, prenorm, false);
+      y = r.y;
+      if (prenorm && res.defined()) z = r.z;
+    }
+  }
+  return z.defined() ? wrap_pair(y, z) : wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+void check_logits(const char* who, const Tensor& logits) {
+  if (act_code(logits.scalar_type()) < 0) raise(std::string(who) + ": dtype " + c10::toString(logits.scalar_type()) + " is not supported");
+  if (logits.dim() == 0 || logits.size(-1) == 0) raise(std::string(who) + ": a vocabulary without entries");
+}
+void check_indices(const char* who, const char* what, const Tensor& x, at::IntArrayRef sizes, const at::Device& dev) {
+  if (x.scalar_type() != at::kLong && x.scalar_type() != at::kInt) raise(std::string(who) + ": " + what + " are int32 or int64");
+  if (x.sizes() != sizes) raise(std::string(who) + ": " + what + " of another shape than the rows of logits");
+  check(what, x, 0, dev);
+}
+
+// logprob(logits, tokens, top_k, scale, entropy) -> (logprobs, entropy, top_logprobs, top_ids); NotImplemented while a trace is recorded
+PyObject* py_logprob(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(5);
+  if (tracing()) Py_RETURN_NOTIMPLEMENTED;
+  Tensor x, tokens;
+  if (!get(args[0], x) || !get(args[1], tokens) || !x.defined()) {
+    PyErr_SetString(PyExc_TypeError, "token_logprobs: a tensor is expected");
+    return nullptr;
+  }
+  const int64_t top_k = PyLong_AsLongLong(args[2]);
+  const double scale = PyFloat_AsDouble(args[3]);
+  const bool entropy = truth(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  Tensor out[4];
+  {
+    NoGil nogil;
+    check_logits("token_logprobs", x);
+    if (tokens.defined()) check_indices("token_logprobs", "tokens", tokens, x.sizes().slice(0, x.dim() - 1), x.device());
+    if (top_k < 0 || top_k > B200GDN_MAX_TOP || top_k > x.size(-1))
+      raise("token_logprobs: top_k=" + std::to_string(top_k) + " (0 to " + std::to_string(B200GDN_MAX_TOP) + ", at most the vocabulary)");
+    if (!tokens.defined() && top_k == 0 && !entropy) raise("token_logprobs: nothing is asked for");
+    if (wants_grad({&x})) {
+      variable_list got = LogprobFunction::apply(x, opt(tokens), top_k, scale, entropy);
+      size_t at = 0;
+      if (tokens.defined()) out[0] = got[at++];
+      if (entropy) out[1] = got[at++];
+      if (top_k > 0) {
+        out[2] = got[at++];
+        out[3] = got[at++];
+      }
+    } else {
+      LogprobForward r = logprob_forward(x, tokens, top_k, scale, entropy, false);
+      out[0] = r.logprobs;
+      out[1] = r.entropy;
+      out[2] = r.top;
+      out[3] = r.ids;
+    }
+  }
+  PyObject* r = PyTuple_New(4);
+  for (int i = 0; r != nullptr && i < 4; ++i) {
+    PyObject* o = wrap(out[i]);
+    if (o == nullptr) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i, o);
+  }
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// distill(logits, teacher, ids, scale, bucket, reduction) -> loss; NotImplemented while a trace is recorded
+PyObject* py_distill(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(6);
+  if (tracing()) Py_RETURN_NOTIMPLEMENTED;
+  Tensor x, teacher, ids;
+  if (!get(args[0], x) || !get(args[1], teacher) || !get(args[2], ids) || !x.defined() || !teacher.defined() || !ids.defined()) {
+    PyErr_SetString(PyExc_TypeError, "topk_distill_loss: a tensor is expected");
+    return nullptr;
+  }
+  const double scale = PyFloat_AsDouble(args[3]);
+  const bool bucket = truth(args[4]);
+  const int64_t reduction = PyLong_AsLongLong(args[5]);
+  if (PyErr_Occurred()) return nullptr;
+  Tensor loss;
+  {
+    NoGil nogil;
+    check_logits("topk_distill_loss", x);
+    std::vector<int64_t> sizes = x.sizes().vec();
+    if (teacher.dim() == x.dim()) sizes.back() = teacher.size(-1);
+    if (teacher.sizes() != at::IntArrayRef(sizes)) raise("topk_distill_loss: teacher_logprobs of another shape than the rows of logits");
+    if (sizes.back() < 1 || sizes.back() > B200GDN_MAX_LIST)
+      raise("topk_distill_loss: " + std::to_string(sizes.back()) + " entries a row (1 to " + std::to_string(B200GDN_MAX_LIST) + ")");
+    if (param_code(teacher.scalar_type()) < 0) raise(std::string("topk_distill_loss: teacher_logprobs of type ") + c10::toString(teacher.scalar_type()));
+    check("teacher_logprobs", teacher, 0, x.device());
+    check_indices("topk_distill_loss", "teacher_ids", ids, sizes, x.device());
+    if (wants_grad({&teacher})) raise("topk_distill_loss: teacher_logprobs have no gradient here: detach them");
+    if (wants_grad({&x})) loss = DistillFunction::apply(x, teacher, ids, scale, bucket, reduction);
+    else loss = distill_forward(x, teacher, ids, scale, bucket, reduction, false).out;
+  }
+  return wrap(loss);
+  END_HANDLE_TH_ERRORS
+}
+
 // plan(chunk_meta, seq_meta, n_chunks, n_seq, covered, empty_seqs, stream, seq_order or None
 //      [, chains, pre_fwd, pre_bwd, first_piece, last_piece, n_chains, n_pre])
 PyObject* py_plan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -1071,6 +1548,9 @@ PyMethodDef methods[] = {
     {"chunk", FAST(py_chunk), "chunked rule, differentiable"},
     {"conv", FAST(py_conv), "short causal convolution, differentiable"},
     {"norm_gate", FAST(py_norm_gate), "gated RMS norm, differentiable"},
+    {"layer_norm", FAST(py_layer_norm), "layer norm with the residual sum, differentiable"},
+    {"logprob", FAST(py_logprob), "log probabilities, entropy and top entries of rows of logits, differentiable"},
+    {"distill", FAST(py_distill), "divergence from a teacher's top entries, differentiable"},
     {"plan", FAST(py_plan), "chunk tables (and split plan) of a shape as one handle"},
     {"in_use", py_in_use, METH_O, "the tables of a plan are about to be read on the current stream"},
     {"plans_alive", py_plans_alive, METH_NOARGS, "plans that are cached, saved for a backward pass or held by a graph"},

@@ -37,7 +37,7 @@ extern "C" {
 
 /* 2: element types of gates, betas and of the convolution's and norm's parameters (gb_dtype, param_dtype); the L2 norm in the
  * forward chunk pass (qn, kn); the order of the sequences (seq_order).  Argument blocks changed size with it. */
-#define B200GDN_ABI_VERSION 2
+#define B200GDN_ABI_VERSION 3
 #define B200GDN_CHUNK 64
 
 /* element type of small per-head / per-channel tensors that are read (or written) in the caller's own precision:
@@ -384,6 +384,105 @@ typedef struct b200gdn_norm_gate_args {
 int b200gdn_norm_gate_fwd(const b200gdn_norm_gate_args* args, void* stream);
 int b200gdn_norm_gate_bwd(const b200gdn_norm_gate_args* args, void* stream);
 int b200gdn_norm_gate_ctas(int64_t rows);
+
+/* Layer norm over rows of D with the residual sum ahead of it (fla/modules/layernorm.py, layer_norm):
+ *   z = x + residual, rounded to the element type (z = x without a residual);  n = (z - mean) rstd;  y = n weight + bias
+ * with mean and 1/sqrt(variance + eps) of each row in fp32.  The backward pass reads z again with `mean` and `rstd`:
+ *   h = dy weight;  dx = rstd (h - mean(h) - n mean(h n)) + dz;  dweight = sum of dy n;  dbias = sum of dy
+ * and needs `partials` of b200gdn_layer_norm_ctas(rows, D, dtype) x 2 x D floats.  dx is the gradient of x and of residual. */
+typedef struct b200gdn_layer_norm_args {
+  int32_t struct_bytes;
+  int32_t D;
+  int64_t rows;
+  int32_t dtype;                 /* 0 = bf16, 1 = fp16, 2 = fp32: x, residual, z, y, dy, dz, dx */
+  int32_t param_dtype;           /* B200GDN_F32 / BF16 / F16: weight, bias, dweight, dbias */
+  float eps;
+  const void* x;                 /* [rows, D] (forward) */
+  const void* residual;          /* [rows, D] or NULL (forward) */
+  const void* weight;            /* [D] or NULL: ones */
+  const void* bias;              /* [D] or NULL: zeros */
+  void* z;                       /* [rows, D]: written by the forward pass (NULL: not wanted), read by the backward pass (x where there was no residual) */
+  void* y;                       /* [rows, D] (forward) */
+  float* mean;                   /* [rows]: written by the forward pass (NULL: not wanted), read by the backward pass */
+  float* rstd;                   /* [rows] */
+  const void* dy;                /* [rows, D] */
+  const void* dz;                /* [rows, D]: gradient of the z that was handed on, or NULL */
+  void* dx;                      /* [rows, D] */
+  void* dweight;                 /* [D] or NULL */
+  void* dbias;                   /* [D] or NULL */
+  float* partials;               /* with dweight or dbias */
+} b200gdn_layer_norm_args;
+int b200gdn_layer_norm_fwd(const b200gdn_layer_norm_args* args, void* stream);
+int b200gdn_layer_norm_bwd(const b200gdn_layer_norm_args* args, void* stream);
+int b200gdn_layer_norm_ctas(int64_t rows, int32_t D, int32_t dtype);
+
+/* Rows of logits over a vocabulary of V.  Row r starts at element (r / inner) stride_outer + (r % inner) stride_inner; the
+ * entries of a row lie side by side and need no alignment beyond their own.  scale = 1 / temperature; with m the largest entry:
+ *   lp_j = scale (x_j - m) - log(sum exp(scale (x - m)));  p = exp(lp)
+ * A row with nothing above minus infinity has lp = -infinity, entropy 0 and gradient 0. */
+typedef struct b200gdn_logprob_args {
+  int32_t struct_bytes;
+  int32_t V;
+  int64_t rows, inner, stride_inner, stride_outer;
+  int32_t dtype;                 /* 0 = bf16, 1 = fp16, 2 = fp32: logits, dlogits */
+  int32_t top_k;                 /* 0 .. min(V, B200GDN_MAX_TOP) */
+  float scale;
+  int32_t token_bytes;           /* 4 or 8: int32 or int64 tokens */
+  const void* logits;
+  const void* tokens;            /* [rows] or NULL; a token outside [0, V) asks for nothing: its log probability is 0, without gradient */
+  float* logprobs;               /* [rows] or NULL (without tokens) */
+  float* entropy;                /* [rows] or NULL: -sum p lp */
+  float* top_logprobs;           /* [rows, top_k], most probable first */
+  int64_t* top_ids;              /* [rows, top_k]: equal entries in the order of their indices */
+  float* stats;                  /* [rows, 2]: m and the logarithm of the sum; written by the forward pass (NULL: not wanted), read by the backward pass */
+  /* backward: entropy (with dentropy) and top_ids are read.  Upstream gradients, NULL: zero */
+  const float* dlogprobs;        /* [rows] */
+  const float* dentropy;         /* [rows] */
+  const float* dtop_logprobs;    /* [rows, top_k] */
+  void* dlogits;                 /* [rows, V], contiguous */
+} b200gdn_logprob_args;
+#define B200GDN_MAX_TOP 128
+int b200gdn_logprob_fwd(const b200gdn_logprob_args* args, void* stream);
+int b200gdn_logprob_bwd(const b200gdn_logprob_args* args, void* stream);
+
+/* Cross-entropy difference (Kullback-Leibler divergence) of a student's rows of logits, laid out as above, from a teacher's K
+ * entries a row: log probabilities l and their places id.
+ *   q = softmax(l)                  loss = sum q_i (log q_i - lp_id_i)
+ *   with B200GDN_DISTILL_BUCKET: q = exp(l), q_t = 1 - sum q (0 below 1e-6: rounding of the sum), p_t = sum of p off the list,
+ *                                   loss = sum q_i (log q_i - lp_id_i) + q_t (log q_t - log p_t)
+ * An entry with an id outside [0, V) or l = -infinity is absent; a row without entries is left out: loss 0, gradient 0, not counted.
+ * A row with a teacher whose logits are all minus infinity has an infinite loss and gradient 0.
+ * The forward pass writes row_loss; `loss` (NULL: not wanted) is their sum, with B200GDN_DISTILL_MEAN over the number of rows
+ * counted (at least 1).  With dlogits it writes the gradient of `loss` in the same pass.  The backward pass forms
+ * dlogits for an upstream gradient: dloss [rows] of row_loss, or with B200GDN_DISTILL_SCALAR dloss [1] of `loss`; with
+ * B200GDN_DISTILL_SKIP_ONE as well it returns at once where dloss is one (dlogits holds that gradient already). */
+#define B200GDN_DISTILL_BUCKET 1u
+#define B200GDN_DISTILL_MEAN 2u
+#define B200GDN_DISTILL_SCALAR 4u
+#define B200GDN_DISTILL_SKIP_ONE 8u
+typedef struct b200gdn_distill_args {
+  int32_t struct_bytes;
+  int32_t V;
+  int64_t rows, inner, stride_inner, stride_outer;
+  int32_t dtype;                 /* 0 = bf16, 1 = fp16, 2 = fp32: logits, dlogits */
+  int32_t K;                     /* 1 .. B200GDN_MAX_LIST */
+  float scale;
+  uint32_t flags;
+  int32_t id_bytes;              /* 4 or 8 */
+  int32_t teacher_dtype;         /* B200GDN_F32 / BF16 / F16 */
+  const void* logits;
+  const void* teacher;           /* [rows, K] */
+  const void* ids;               /* [rows, K] */
+  float* row_loss;               /* [rows] */
+  float* loss;                   /* [1] or NULL */
+  float* stats;                  /* [rows, 4]: what the backward pass needs of each row (NULL: not wanted) */
+  int32_t* counters;             /* [2]: workspace, kept for the backward pass with B200GDN_DISTILL_MEAN */
+  const float* dloss;
+  void* dlogits;                 /* [rows, V], contiguous */
+} b200gdn_distill_args;
+#define B200GDN_MAX_LIST 256
+int b200gdn_distill_fwd(const b200gdn_distill_args* args, void* stream);
+int b200gdn_distill_bwd(const b200gdn_distill_args* args, void* stream);
 
 /* Bytes of forward-saved tensors and of backward workspace for a problem (what the caller allocates; the latter with what
  * single stages of the backward pass need). */

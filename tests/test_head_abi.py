@@ -1,0 +1,100 @@
+"""The C ABI of layer norm and of the operators on logits: struct layouts, and arguments that are refused before any CUDA call."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), '..'))
+
+
+def test_struct_layouts_match_header(tmp_path):
+    from b200gdn import _lib
+    structs = {'b200gdn_layer_norm_args': _lib.LayerNormArgs, 'b200gdn_logprob_args': _lib.LogprobArgs, 'b200gdn_distill_args': _lib.DistillArgs}
+    lines, want = [], []
+    for name, cls in structs.items():
+        lines.append(f'printf("%zu\\n", sizeof({name}));')
+        want.append(C.sizeof(cls))
+        for field, _ in cls._fields_:
+            lines.append(f'printf("%zu\\n", offsetof({name}, {field}));')
+            want.append(getattr(cls, field).offset)
+    lines += ['printf("%d\\n", B200GDN_MAX_TOP);', 'printf("%d\\n", B200GDN_MAX_LIST);']
+    want += [_lib.MAX_TOP, _lib.MAX_LIST]
+    prog = tmp_path / 'sz.c'
+    prog.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "b200gdn.h"\nint main(void){' + '\n'.join(lines) + 'return 0;}\n')
+    exe = tmp_path / 'sz'
+    subprocess.check_call(['gcc', '-I', os.path.join(ROOT, 'include'), str(prog), '-o', str(exe)])
+    assert [int(x) for x in subprocess.check_output([str(exe)]).split()] == want
+
+
+def refused(fn, args, code, text):
+    from b200gdn import _lib
+    lib = _lib.load()
+    args.struct_bytes = C.sizeof(args)
+    assert getattr(lib, fn)(C.byref(args), None) == code
+    assert text in lib.b200gdn_last_error().decode(), lib.b200gdn_last_error()
+
+
+def test_bad_arguments_of_layer_norm():
+    from b200gdn import _lib
+    for fn in ('b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd'):
+        assert getattr(_lib.load(), fn)(None, None) == -1
+        refused(fn, _lib.LayerNormArgs(), -1, 'empty problem')
+        refused(fn, _lib.LayerNormArgs(rows=1 << 31, D=8), -2, 'rows')
+        refused(fn, _lib.LayerNormArgs(rows=4, D=8, dtype=3), -1, 'dtype')
+    refused('b200gdn_layer_norm_fwd', _lib.LayerNormArgs(rows=4, D=8), -1, 'a->x is NULL')
+    refused('b200gdn_layer_norm_fwd', _lib.LayerNormArgs(rows=4, D=8, x=256, y=256, mean=256), -1, 'come together')
+    refused('b200gdn_layer_norm_bwd', _lib.LayerNormArgs(rows=4, D=8, z=256, mean=256, rstd=256, dy=256, dx=256, dweight=256), -1, 'partials is NULL')
+    a = _lib.LayerNormArgs(rows=4, D=8)
+    a.struct_bytes = 8
+    assert _lib.load().b200gdn_layer_norm_fwd(C.byref(a), None) == -1 and b'ABI mismatch' in _lib.load().b200gdn_last_error()
+    assert _lib.load().b200gdn_layer_norm_ctas(1, 64, 0) >= 1
+
+
+@pytest.mark.parametrize('name', ['logprob', 'distill'])
+def test_bad_rows_of_logits(name):
+    from b200gdn import _lib
+    cls = {'logprob': _lib.LogprobArgs, 'distill': _lib.DistillArgs}[name]
+    for way in ('fwd', 'bwd'):
+        fn = f'b200gdn_{name}_{way}'
+        assert getattr(_lib.load(), fn)(None, None) == -1
+        refused(fn, cls(), -1, 'empty problem')
+        refused(fn, cls(rows=2, V=5, inner=0), -1, 'empty problem')
+        refused(fn, cls(rows=(1 << 27) + 1, V=5, inner=1), -2, 'rows')
+        refused(fn, cls(rows=2, V=(1 << 30) + 1, inner=1), -2, 'entries')
+        refused(fn, cls(rows=2, V=5, inner=1, dtype=4), -1, 'dtype')
+        for scale in (0.0, -1.0, float('nan'), float('inf')):
+            refused(fn, cls(rows=2, V=5, inner=1, scale=scale), -1, 'scale')
+        refused(fn, cls(rows=2, V=5, inner=1, scale=1), -1, 'logits is NULL')
+        refused(fn, cls(rows=2, V=5, inner=1, scale=1, logits=257), -1, 'boundary')
+        refused(fn, cls(rows=2, V=5, inner=1, scale=1, dtype=2, logits=256, dlogits=258), -1, 'boundary')
+
+
+def test_bad_arguments_of_logprob_and_distill():
+    from b200gdn import _lib
+    rows = dict(rows=2, V=50, inner=1, scale=1.0, logits=256)
+    for k in (-1, 51, 129):
+        refused('b200gdn_logprob_fwd', _lib.LogprobArgs(top_k=k, **rows), -2, 'top_k')
+    refused('b200gdn_logprob_fwd', _lib.LogprobArgs(tokens=256, token_bytes=2, **rows), -1, 'token_bytes')
+    refused('b200gdn_logprob_fwd', _lib.LogprobArgs(logprobs=256, **rows), -1, 'tokens is NULL')
+    refused('b200gdn_logprob_fwd', _lib.LogprobArgs(top_k=3, **rows), -1, 'top_ids is NULL')
+    refused('b200gdn_logprob_bwd', _lib.LogprobArgs(**rows), -1, 'stats is NULL')
+    refused('b200gdn_logprob_bwd', _lib.LogprobArgs(stats=256, dlogits=256, dentropy=256, **rows), -1, 'entropy is NULL')
+    for k in (0, 257):
+        refused('b200gdn_distill_fwd', _lib.DistillArgs(K=k, **rows), -2, 'entries a row')
+    refused('b200gdn_distill_fwd', _lib.DistillArgs(K=3, id_bytes=1, **rows), -1, 'id_bytes')
+    refused('b200gdn_distill_fwd', _lib.DistillArgs(K=3, id_bytes=8, teacher_dtype=7, **rows), -1, 'teacher_dtype')
+    lists = dict(K=3, id_bytes=8, teacher=256, ids=256, **rows)
+    refused('b200gdn_distill_fwd', _lib.DistillArgs(**lists), -1, 'row_loss is NULL')
+    refused('b200gdn_distill_fwd', _lib.DistillArgs(flags=_lib.DISTILL_MEAN, row_loss=256, **lists), -1, 'counters is NULL')
+    refused('b200gdn_distill_bwd', _lib.DistillArgs(row_loss=256, **lists), -1, 'stats is NULL')
+
+
+def test_cpu_tensors_are_refused():
+    import torch
+    from b200gdn import B200GDNError, LayerNorm, layer_norm, token_logprobs, topk_distill_loss
+    x = torch.zeros(2, 8)
+    for call in (lambda: layer_norm(x), lambda: LayerNorm(8)(x), lambda: token_logprobs(x, torch.zeros(2, dtype=torch.long)),
+                 lambda: topk_distill_loss(x, x, x.long())):
+        with pytest.raises(B200GDNError, match='CUDA device only'):
+            call()
