@@ -112,7 +112,7 @@ class LogprobArgs(C.Structure):
     _fields_ = _ROWS_OF_LOGITS + [
         ('top_k', C.c_int32), ('scale', C.c_float), ('token_bytes', C.c_int32),
         ('logits', _p), ('tokens', _p), ('logprobs', _p), ('entropy', _p), ('top_logprobs', _p), ('top_ids', _p), ('stats', _p),
-        ('dlogprobs', _p), ('dentropy', _p), ('dtop_logprobs', _p), ('dlogits', _p),
+        ('dlogprobs', _p), ('dentropy', _p), ('dtop_logprobs', _p), ('dlogits', _p), ('workspace', _p),
     ]
 
 
@@ -134,7 +134,7 @@ EXPORTS = (
     'b200gdn_selftest_wait_expiry', 'b200gdn_chunk_fwd_static', 'b200gdn_cp_fold', 'b200gdn_cp_prefix',
     'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd', 'b200gdn_norm_gate_ctas',
     'b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd', 'b200gdn_layer_norm_ctas', 'b200gdn_logprob_fwd', 'b200gdn_logprob_bwd',
-    'b200gdn_distill_fwd', 'b200gdn_distill_bwd',
+    'b200gdn_logprob_workspace_bytes', 'b200gdn_distill_fwd', 'b200gdn_distill_bwd',
 )
 
 _lib = None
@@ -172,6 +172,8 @@ def load():
             fn.argtypes = [C.c_int32] * 6
         lib.b200gdn_norm_gate_ctas.restype = C.c_int
         lib.b200gdn_norm_gate_ctas.argtypes = [C.c_int64]
+        lib.b200gdn_logprob_workspace_bytes.restype = C.c_int64
+        lib.b200gdn_logprob_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
         lib.b200gdn_layer_norm_ctas.restype = C.c_int
         lib.b200gdn_layer_norm_ctas.argtypes = [C.c_int64, C.c_int32, C.c_int32]
         lib.b200gdn_last_launch_count.restype = C.c_int

@@ -401,6 +401,7 @@ static int check_logprob_args(const b200gdn_logprob_args* a, const char* who, bo
   if (!bwd) {
     if (a->logprobs != nullptr) REQUIRE(a->tokens, who);
     if (a->top_k > 0) { REQUIRE(a->top_ids, who); REQUIRE(a->top_logprobs, who); }
+    REQUIRE(a->workspace, who);
   } else {
     REQUIRE(a->stats, who); REQUIRE(a->dlogits, who);
     if (a->dlogprobs != nullptr) REQUIRE(a->tokens, who);
@@ -421,6 +422,8 @@ int b200gdn_logprob_bwd(const b200gdn_logprob_args* a, void* stream) {
   if (int e = check_logprob_args(a, "logprob_bwd", true)) return e;
   return gdn::launch_logprob(*a, static_cast<cudaStream_t>(stream), true);
 }
+
+int64_t b200gdn_logprob_workspace_bytes(int64_t rows, int32_t V, int32_t dtype, int32_t top_k) { return gdn::logprob_workspace(rows, V, dtype, top_k); }
 
 static int check_distill_args(const b200gdn_distill_args* a, const char* who, bool bwd) {
   using namespace gdn;

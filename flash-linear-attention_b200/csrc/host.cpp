@@ -1008,6 +1008,8 @@ LogprobForward logprob_forward(const Tensor& logits, const Tensor& tokens, int64
   a.top_logprobs = fptr(r.top);
   a.top_ids = static_cast<int64_t*>(ptr(r.ids));
   a.stats = fptr(r.stats);
+  const Tensor workspace = new_tensor({b200gdn_logprob_workspace_bytes(a.rows, a.V, a.dtype, a.top_k)}, at::kByte, dev);
+  a.workspace = ptr(workspace);
   call("b200gdn_logprob_fwd", b200gdn_logprob_fwd, a);
   return r;
 }

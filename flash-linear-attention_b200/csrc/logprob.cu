@@ -1,78 +1,415 @@
 // Log probabilities of given tokens, entropy and the most probable entries of rows of logits, and their gradient.
-// The simplest form: one CTA per row, three passes over it (largest entry, sums, and one search for each of the top entries).
+//
+// Forward: one look at each logit, by warps that know nothing of one another.  (A row in one cluster, its pieces joined through shared
+// memory, came to 4.0 TB/s at best and less with top entries: what has to be said about a row is a chain of a few thousand clocks.)
+// A warp takes a span of 32 W words of 16 bytes of a row into registers, and leaves the span's largest entry m and the sums
+// s = sum 2^u, t = sum u 2^u; with top entries also the largest entry of each lane's words (a group).  A second kernel joins a row's
+// spans: lp_j = (u_j - log2 s) ln 2, entropy = (log2 s - t / s) ln 2.
+//
+// Top entries: the k-th largest of the groups' largest entries, tau, is a bound that at least k entries reach and few more than k exceed; only
+// the groups that reach it are read again (k of 2048 in a row of 131072 16-bit logits), and each of the entries found counts how many
+// of them are larger, which is its place.
 #include "vocab.cuh"
 
 namespace gdn {
 namespace {
 
-constexpr int NT = 256;
+// log probability of an entry x; log_s: the base-2 logarithm of the sum, -infinity where nothing is above -infinity
+__device__ __forceinline__ float lp_of(float x, float m, float log_s, float scale) {
+  return log_s == -INFINITY ? -INFINITY : exponent(x, m, scale) - log_s * kLn2;
+}
 
+// ---- spans -------------------------------------------------------------------------------------------------------------
+constexpr int kSpanWarps = 4;
+
+// How rows are cut: `w` words a lane, for as many words of 16 bytes as a row has at most (off a word's boundary it has one more).  By the
+// width alone: a row's results are the same bits whatever rows it comes with.
+struct Spans {
+  int w, per_row;
+  __host__ __device__ int groups() const { return 32 * per_row; }
+};
+Spans spans_of(int V, int size) {
+  const int64_t words = ((int64_t)V * size + 15) / 16 + 1;
+  int w = 8;
+  while (w > 1 && words <= 16 * w) w >>= 1;   // short rows: no more lanes without words than have to be
+  return Spans{w, (int)((words + 32 * w - 1) / (32 * w))};
+}
+
+// values in order as unsigned integers of 16 or 32 bits; 0 for no value at all.  The zeros are one value.
 template <typename T>
-__global__ void __launch_bounds__(NT) logprob_fwd_kernel(const b200gdn_logprob_args a) {
-  __shared__ float fs[NT / 32];
-  __shared__ uint64_t ks[NT / 32];
-  const int64_t r = blockIdx.x;
-  const T* x = static_cast<const T*>(a.logits) + row_offset(a, r);
-  float m = -INFINITY;
-  for (int j = threadIdx.x; j < a.V; j += NT) m = fmaxf(m, Io<T>::ld(x, j));
-  m = cta_reduce<NT>(m, fs, MaxOf());
-  const float base = m == -INFINITY ? 0.f : m;
-  float ss[8] = {}, ts[8] = {};   // eight chains of additions: an eighth of the rounding
-  for (int j0 = threadIdx.x; j0 < a.V; j0 += 8 * NT) {
+__device__ __forceinline__ uint32_t ordered(float x) {
+  uint32_t b = __float_as_uint(x + 0.f);
+  if constexpr (std::is_same<T, __half>::value) b = (uint32_t)__half_as_ushort(__float2half_rn(x + 0.f));
+  else if constexpr (sizeof(T) == 2) b >>= 16;
+  constexpr uint32_t sign = sizeof(T) == 2 ? 0x8000u : 0x80000000u, all = sizeof(T) == 2 ? 0xffffu : 0xffffffffu;
+  return b & sign ? ~b & all : b | sign;
+}
+template <typename T> using Order = typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type;
+template <typename T>
+__device__ __forceinline__ float from_ordered(uint32_t o) {
+  constexpr uint32_t sign = sizeof(T) == 2 ? 0x8000u : 0x80000000u, all = sizeof(T) == 2 ? 0xffffu : 0xffffffffu;
+  const uint32_t b = o & sign ? o & ~sign : ~o & all;
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)b));
+  else return __uint_as_float(sizeof(T) == 2 ? b << 16 : b);
+}
+
+// A row by words: word j holds the entries from first + j EPW on; the first and the last may hold something else beside (every word that is
+// read holds an entry of the row, so no read leaves the 16 bytes that hold one).
+template <typename T>
+struct Words {
+  static constexpr int EPW = 16 / sizeof(T);
+  const uint4* at;
+  int first, n;
+  __device__ __forceinline__ Words(const T* row, int V) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(row);
+    const int shift = (int)(b & 15) / (int)sizeof(T);
+    at = reinterpret_cast<const uint4*>(b & ~(uintptr_t)15);
+    first = -shift;
+    n = (shift + V + EPW - 1) / EPW;
+  }
+  // word j with minus infinity for what is not of the row
+  __device__ __forceinline__ uint4 edge(int j, int V) const {
+    uint4 q = at[j];
+    T* x = reinterpret_cast<T*>(&q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int j = j0 + i * NT;
-      if (j >= a.V) break;
-      const float u = (Io<T>::ld(x, j) - base) * a.scale, e = exp2_approx(u * kLog2e);
-      ss[i] += e;
-      if (!(e <= 0.f)) ts[i] += e * u;
+    for (int e = 0; e < EPW; ++e) {
+      const int i = first + j * EPW + e;
+      if (i < 0 || i >= V) x[e] = static_cast<T>(-INFINITY);
     }
+    return q;
   }
-  float s = 0.f, t = 0.f;
+};
+
+template <typename T, int W, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(32 * kSpanWarps) logprob_spans_kernel(const b200gdn_logprob_args a, const Spans spans, float4* part, void* largest) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task = (int64_t)blockIdx.x * kSpanWarps + (threadIdx.x >> 5), r = task / spans.per_row;
+  const int span = (int)(task - r * spans.per_row);
+  if (r >= a.rows) return;
+  const Words<T> x(static_cast<const T*>(a.logits) + row_offset(a, r), a.V);
+  const float c = a.scale * kLog2e;
+  const int j0 = span * 32 * W + lane;
+  uint4 q[W];
+  // nothing but entries
+  const bool inner = (span > 0 || x.first == 0) && ((span + 1) * 32 * W < x.n || ((span + 1) * 32 * W == x.n && x.first + x.n * Words<T>::EPW == a.V));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    s += ss[i];
-    t += ts[i];
+  for (int i = 0; i < W; ++i) {
+    const int j = j0 + 32 * i;
+    if (inner) q[i] = x.at[j];
+    else if (j < x.n) q[i] = x.edge(j, a.V);
+    else q[i] = make_uint4(kMinusInfWord<T>, kMinusInfWord<T>, kMinusInfWord<T>, kMinusInfWord<T>);
   }
-  s = cta_reduce<NT>(s, fs, SumOf());
-  t = cta_reduce<NT>(t, fs, SumOf());
-  const bool empty = s == 0.f;
-  const float logs = logf(s);
-  auto lp = [&](float v) { return empty ? -INFINITY : (v - base) * a.scale - logs; };
-  if (threadIdx.x == 0) {
-    if (a.logprobs) {
-      const int token = load_index(a.tokens, r, a.token_bytes, a.V);
-      a.logprobs[r] = token < 0 ? 0.f : lp(Io<T>::ld(x, token));
+  PieceSums<T, ENTROPY> p;
+  constexpr int G = W < 4 ? W : 4;
+  bool bounded = !inner;
+  if (inner) {
+#pragma unroll
+    for (int i = 0; i < W; i += G) {
+      uint4 w[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) w[g] = q[i + g];
+      p.template add<false>(w, c);
     }
-    if (a.entropy) a.entropy[r] = empty ? 0.f : logs - t / s;
-    if (a.stats) {
-      a.stats[2 * r] = base;
-      a.stats[2 * r + 1] = logs;
-    }
+    p.flush();
+    // entries of minus infinity: once more, with bounded exponents
+    bounded = ENTROPY && p.a.t != p.a.t && p.a.s == p.a.s;
   }
-  uint64_t below = ~0ull;
-  for (int i = 0; i < a.top_k; ++i) {
-    uint64_t best = 0;
-    for (int j = threadIdx.x; j < a.V; j += NT) {
-      const uint64_t k = entry_key(Io<T>::ld(x, j), j);
-      if (k < below && k > best) best = k;
+  if (bounded) {
+    p = PieceSums<T, ENTROPY>();
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const uint4 w[1] = {q[i]};
+      p.template add<true>(w, c);
     }
-    below = cta_reduce<NT>(best, ks, MaxOf());
-    if (threadIdx.x == 0) {
-      a.top_ids[r * a.top_k + i] = key_index(below);
-      a.top_logprobs[r * a.top_k + i] = lp(key_value(below));
-    }
+    p.flush();
+  }
+  const Sums v = warp_sums<ENTROPY>(p.a, c);
+  if (lane == 0) part[r * spans.per_row + span] = make_float4(v.m, v.s, v.t, 0.f);
+  if constexpr (TOP) {
+    // (a lane without words leaves 0)
+    static_cast<Order<T>*>(largest)[r * spans.groups() + span * 32 + lane] = (Order<T>)(j0 < x.n ? ordered<T>(p.a.m) : 0u);
   }
 }
 
+// ---- joining a row's spans ---------------------------------------------------------------------------------------------
+constexpr int NT = 128, kRoom = 1024;   // threads of a row with top entries; keys of entries that may be among them
+static_assert(kRoom >= 2 * B200GDN_MAX_TOP, "entries above tau and as many equal to it as are wanted");
+
+// a whole warp
+__device__ __forceinline__ Sums joined_spans(const float4* part, int n, float c, int lane) {
+  Sums v{-INFINITY, 0.f, 0.f};
+  for (int i = lane; i < n; i += 32) {
+    const float4 f = part[i];
+    const Sums o{f.x, f.y, f.z};
+    const float m = fmaxf(v.m, o.m);
+    const Sums p = moved(o, m, c);
+    v = moved(v, m, c);
+    v.s += p.s;
+    v.t += p.t;
+  }
+  return warp_sums<true>(v, c);
+}
+
+// one thread
+template <typename T>
+__device__ __forceinline__ void row_results(const b200gdn_logprob_args& a, int64_t r, const Sums& v, float log_s) {
+  if (a.logprobs) {
+    const int token = load_index(a.tokens, r, a.token_bytes, a.V);
+    a.logprobs[r] = token < 0 ? 0.f : lp_of(Io<T>::ld(static_cast<const T*>(a.logits) + row_offset(a, r), token), v.m, log_s, a.scale);
+  }
+  if (a.entropy) a.entropy[r] = v.s == 0.f ? 0.f : (log_s - v.t / v.s) * kLn2;
+  if (a.stats) {
+    a.stats[2 * r] = v.m;
+    a.stats[2 * r + 1] = log_s;
+  }
+}
+
+// without top entries: a warp a row
+template <typename T>
+__global__ void __launch_bounds__(NT) logprob_join_kernel(const b200gdn_logprob_args a, const Spans spans, const float4* part) {
+  wait_for_predecessor();
+  const int64_t r = (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
+  if (r >= a.rows) return;
+  const int lane = threadIdx.x & 31;
+  const Sums v = joined_spans(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
+  if (lane == 0) row_results<T>(a, r, v, log2f(v.s));
+}
+
+// The k-th largest of n <= 2 NT values (0 where fewer than k are there), two bits at a time from the highest down; of 32 bits the upper 22,
+// which bounds it from below as well as tau needs.  One warp.
+template <typename T>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t* values, int n, int k, int lane) {
+  uint32_t v[2 * NT / 32];
+#pragma unroll
+  for (int i = 0; i < 2 * NT / 32; ++i) v[i] = i * 32 + lane < n ? values[i * 32 + lane] : 0u;
+  uint32_t t = 0;
+#pragma unroll 1
+  for (int bit = sizeof(T) == 2 ? 14 : 30; bit >= (sizeof(T) == 2 ? 0 : 10); bit -= 2) {
+    const uint32_t n1 = t | 1u << bit, n2 = t | 2u << bit, n3 = t | 3u << bit;
+    uint32_t c = 0;   // three counts of up to 2 NT in one sum
+#pragma unroll
+    for (int i = 0; i < 2 * NT / 32; ++i)
+      if (i * 32 < n) c += (v[i] >= n1 ? 1u : 0u) + (v[i] >= n2 ? 1u << 10 : 0u) + (v[i] >= n3 ? 1u << 20 : 0u);
+    c = __reduce_add_sync(0xffffffffu, c);
+    t = (c >> 20) >= (uint32_t)k ? n3 : (c >> 10 & 0x3ffu) >= (uint32_t)k ? n2 : (c & 0x3ffu) >= (uint32_t)k ? n1 : t;
+  }
+  return t == 0 ? 0 : max(t, ordered<T>(-INFINITY));   // (the lower bits left out: below minus infinity there are only NaNs)
+}
+
+// The keys of a row's entries above tau (with `everything`: of all) and of the first k equal to it, in the order of their indices: for rows with
+// NaN (above everything) and with many entries equal to tau.  Returns how many there are (those beyond the room are not kept).  One warp.
+template <typename T>
+__device__ __noinline__ int keys_in_order(const Words<T>& x, int V, uint32_t tau_bits, int k, uint64_t* keys, int lane) {
+  const bool everything = tau_bits == 0;
+  const float tau = from_ordered<T>(tau_bits);
+  int found = 0, equal = 0;   // keys, and of entries that are equal to tau the number met
+  for (int j0 = 0; j0 < x.n; j0 += 32) {
+    const int j = j0 + lane, at = x.first + j * Words<T>::EPW;
+    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+    if (j < x.n) q = x.at[j];
+    const T* w = reinterpret_cast<const T*>(&q);
+    uint32_t n = 0;   // above tau, and in the upper half equal to it
+#pragma unroll
+    for (int e = 0; e < Words<T>::EPW; ++e) {
+      const float v = Io<T>::ld(w, e);
+      if (j < x.n && at + e >= 0 && at + e < V) n += everything || !(v <= tau) ? 1u : v == tau ? 0x10000u : 0u;
+    }
+    if (!__any_sync(0xffffffffu, n != 0)) continue;
+    uint32_t before = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
+    }
+    const uint32_t total = __shfl_sync(0xffffffffu, before, 31);
+    before -= n;
+    int eq = equal + (int)(before >> 16), to = found + (int)(before & 0xffffu) + min(eq, k) - min(equal, k);
+    if (n != 0)
+#pragma unroll
+      for (int e = 0; e < Words<T>::EPW; ++e) {
+        const float v = Io<T>::ld(w, e);
+        if (at + e < 0 || at + e >= V) continue;
+        const bool above = everything || !(v <= tau);
+        if (!above && (v != tau || eq++ >= k)) continue;
+        if (to < kRoom) keys[to] = entry_key(v, at + e);
+        ++to;
+      }
+    found += (int)(total & 0xffffu) + min(equal + (int)(total >> 16), k) - min(equal, k);
+    equal += (int)(total >> 16);
+  }
+  return found;
+}
+
+// with top entries: a CTA a row
+template <typename T>
+__global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logprob_args a, const Spans spans, const float4* part, const void* largest) {
+  __shared__ uint64_t keys[kRoom], ks[NT / 32];
+  __shared__ uint32_t own[2 * NT], bound;
+  __shared__ uint16_t list[kRoom];
+  __shared__ float stats[4];
+  __shared__ int n_list, found;
+  wait_for_predecessor();
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.top_k, groups = spans.groups();
+  const Words<T> x(static_cast<const T*>(a.logits) + row_offset(a, r), a.V);
+  const Order<T>* of_groups = static_cast<const Order<T>*>(largest) + r * groups;
+  // tau from as many values as threads, or twice that: the largest of the groups i NT + tid.  With few groups tau would be low, and the
+  // row is gone through again: the largest entry of each thread's words.
+  const bool by_groups = 2 * groups >= 3 * k && groups <= 65536, twice = by_groups && 2 * k > NT;
+  uint32_t most = 0, odd = 0;
+  if (by_groups) {
+#pragma unroll 4
+    for (int i = tid; i < groups; i += 2 * NT) {
+      most = max(most, (uint32_t)of_groups[i]);
+      if (i + NT < groups) odd = max(odd, (uint32_t)of_groups[i + NT]);
+    }
+    if (!twice) most = max(most, odd);
+  } else {
+    float m = -INFINITY;
+    for (int j = tid; j < x.n; j += NT) m = fmaxf(m, max_of_word<T>(largest_of<T>(x.edge(j, a.V))));
+    most = tid < x.n ? ordered<T>(m) : 0u;
+  }
+  own[tid] = most;
+  own[NT + tid] = odd;
+  __syncthreads();
+  if (warp == 0) {
+    const uint32_t t = kth_largest<T>(own, twice ? 2 * NT : NT, k, lane);
+    if (lane == 0) bound = t;
+  } else if (warp == 1) {
+    const Sums v = joined_spans(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
+    if (lane == 0) {
+      stats[0] = v.m;
+      stats[1] = log2f(v.s);
+      stats[2] = v.s;
+      stats[3] = v.t;
+      n_list = found = 0;
+    }
+  }
+  __syncthreads();
+  const uint32_t tau = bound;
+  const float m = stats[0], log_s = stats[1], least = from_ordered<T>(tau);
+  if (tid == NT - 1) row_results<T>(a, r, Sums{m, stats[2], stats[3]}, log_s);
+  const bool usable = tau != 0 && stats[2] == stats[2];   // entries that reach tau may be looked for (no NaN among them)
+  auto look = [&](const uint4& q, int j) {
+    if (!(max_of_word<T>(largest_of<T>(q)) >= least)) return;
+#pragma unroll
+    for (int e = 0; e < Words<T>::EPW; ++e) {
+      const float2 p = unpack2(pair_of<T>(q, e / 2));
+      const float v = e & 1 ? p.y : p.x;
+      const int at = x.first + j * Words<T>::EPW + e;
+      if (v >= least && at >= 0 && at < a.V) {
+        const int to = atomicAdd(&found, 1);
+        if (to < kRoom) keys[to] = entry_key(v, at);
+      }
+    }
+  };
+  if (usable && by_groups) {
+    if (max(most, odd) >= tau)
+      for (int g = tid; g < groups; g += NT)
+        if (of_groups[g] >= tau) {
+          const int to = atomicAdd(&n_list, 1);
+          if (to < kRoom) list[to] = (uint16_t)g;
+        }
+    __syncthreads();
+    const int n = n_list;
+    if (n > kRoom) {
+      if (tid == 0) found = kRoom + 1;   // as many groups equal to tau: in order
+    } else {
+      constexpr int U = 4;   // words of a thread on their way at once
+      for (int i = tid; i < n * spans.w; i += U * NT) {
+        uint4 q[U];
+        int j[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int at = i + u * NT, g = at < n * spans.w ? list[at / spans.w] : 0;
+          j[u] = at < n * spans.w ? g / 32 * 32 * spans.w + at % spans.w * 32 + g % 32 : x.n;
+          q[u] = j[u] < x.n ? x.at[j[u]] : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (j[u] < x.n) look(q[u], j[u]);
+      }
+    }
+  } else if (usable) {
+    if (most >= tau)
+      for (int j = tid; j < x.n; j += NT) look(x.at[j], j);
+  } else if (tid == 0) {
+    found = kRoom + 1;
+  }
+  __syncthreads();
+  int n = found;
+  __syncthreads();
+  if (n > kRoom) {
+    if (warp == 0) {
+      n = keys_in_order<T>(x, a.V, tau, k, keys, lane);
+      if (lane == 0) found = n;
+    }
+    __syncthreads();
+    n = found;
+  }
+  auto result = [&](int place, uint64_t key) {
+    a.top_ids[r * k + place] = key_index(key);
+    a.top_logprobs[r * k + place] = lp_of(key_value(key), m, log_s, a.scale);
+  };
+  if (n > kRoom) {   // some thousand entries above tau, all in fewer than k groups: one search through the row for each top entry
+    uint64_t below = ~0ull;
+    for (int i = 0; i < k; ++i) {
+      uint64_t best = 0;
+      for (int j = tid; j < a.V; j += NT) {
+        const uint64_t key = entry_key(Io<T>::ld(x.at, j - x.first), j);
+        if (key < below && key > best) best = key;
+      }
+      below = cta_reduce<NT>(best, ks, MaxOf());
+      if (tid == 0) result(i, below);
+    }
+    return;
+  }
+  for (int i = tid; i < n; i += NT) {
+    const uint64_t key = keys[i];
+    int larger = 0;
+#pragma unroll 4
+    for (int o = 0; o < n; ++o) larger += keys[o] > key;
+    if (larger < k) result(larger, key);
+  }
+}
+
+template <typename T, int W>
+int launch_spans(const b200gdn_logprob_args& a, const Spans& spans, float4* part, void* largest, cudaStream_t st) {
+  const unsigned grid = (unsigned)((a.rows * spans.per_row + kSpanWarps - 1) / kSpanWarps);
+  auto go = [&](auto kern) { kern<<<grid, 32 * kSpanWarps, 0, st>>>(a, spans, part, largest); };
+  if (a.top_k > 0) {
+    if (a.entropy) go(logprob_spans_kernel<T, W, true, true>);
+    else go(logprob_spans_kernel<T, W, false, true>);
+  } else {
+    if (a.entropy) go(logprob_spans_kernel<T, W, true, false>);
+    else go(logprob_spans_kernel<T, W, false, false>);
+  }
+  return check_launch("logprob_spans");
+}
+
+template <typename T>
+int launch_fwd(const b200gdn_logprob_args& a, cudaStream_t st) {
+  const Spans spans = spans_of(a.V, sizeof(T));
+  if (a.rows * spans.per_row > (int64_t)INT32_MAX * kSpanWarps) return set_error(B200GDN_ERR_UNSUPPORTED, "logprob_fwd: more than 2^34 spans");
+  float4* part = static_cast<float4*>(a.workspace);
+  void* largest = part + a.rows * spans.per_row;
+  int e = spans.w == 8 ? launch_spans<T, 8>(a, spans, part, largest, st) : spans.w == 4 ? launch_spans<T, 4>(a, spans, part, largest, st)
+          : spans.w == 2 ? launch_spans<T, 2>(a, spans, part, largest, st) : launch_spans<T, 1>(a, spans, part, largest, st);
+  if (e) return e;
+  if (a.top_k > 0) launch_overlapped(true, logprob_top_kernel<T>, dim3((unsigned)a.rows), NT, 0, st, a, spans, part, largest);
+  else launch_overlapped(true, logprob_join_kernel<T>, dim3((unsigned)((a.rows + NT / 32 - 1) / (NT / 32))), NT, 0, st, a, spans, part);
+  return check_launch(a.top_k > 0 ? "logprob_top" : "logprob_join");
+}
+
+// ---- gradient ----------------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(NT) logprob_bwd_kernel(const b200gdn_logprob_args a) {
   __shared__ float fs[NT / 32];
   const int64_t r = blockIdx.x;
   const T* x = static_cast<const T*>(a.logits) + row_offset(a, r);
   const int64_t out = r * a.V;
-  const float base = a.stats[2 * r], logs = a.stats[2 * r + 1];
-  if (logs == -INFINITY) {   // nothing in this row
+  const float m = a.stats[2 * r], log_s = a.stats[2 * r + 1], c = a.scale * kLog2e;
+  if (log_s == -INFINITY) {   // nothing in this row
     for (int j = threadIdx.x; j < a.V; j += NT) Io<T>::st(a.dlogits, out + j, 0.f);
     return;
   }
@@ -83,8 +420,8 @@ __global__ void __launch_bounds__(NT) logprob_bwd_kernel(const b200gdn_logprob_a
   for (int i = threadIdx.x; i < k; i += NT) all += a.dtop_logprobs[r * k + i];
   all = cta_reduce<NT>(all, fs, SumOf()) + dlp;
   auto grad = [&](int j) {
-    const float lp = (Io<T>::ld(x, j) - base) * a.scale - logs, p = exp2_approx(lp * kLog2e);
-    return p == 0.f ? 0.f : -p * (all + dh * (lp + h));
+    const float l2 = exponent(Io<T>::ld(x, j), m, c) - log_s, p = exp2_approx(l2);
+    return p == 0.f ? 0.f : -p * (all + dh * (l2 * kLn2 + h));
   };
   for (int j = threadIdx.x; j < a.V; j += NT) Io<T>::st(a.dlogits, out + j, grad(j) * a.scale);
   __syncthreads();
@@ -99,12 +436,17 @@ __global__ void __launch_bounds__(NT) logprob_bwd_kernel(const b200gdn_logprob_a
 
 template <typename T>
 int launch_t(const b200gdn_logprob_args& a, cudaStream_t st, bool bwd) {
-  if (bwd) logprob_bwd_kernel<T><<<(unsigned)a.rows, NT, 0, st>>>(a);
-  else logprob_fwd_kernel<T><<<(unsigned)a.rows, NT, 0, st>>>(a);
-  return check_launch(bwd ? "logprob_bwd" : "logprob_fwd");
+  if (!bwd) return launch_fwd<T>(a, st);
+  logprob_bwd_kernel<T><<<(unsigned)a.rows, NT, 0, st>>>(a);
+  return check_launch("logprob_bwd");
 }
 
 }  // namespace
+
+int64_t logprob_workspace(int64_t rows, int V, int dtype, int top_k) {
+  const Spans spans = spans_of(V, dtype == 2 ? 4 : 2);
+  return rows * spans.per_row * (16 + (top_k > 0 ? 32 * (dtype == 2 ? 4 : 2) : 0));
+}
 
 int launch_logprob(const b200gdn_logprob_args& a, cudaStream_t st, bool bwd) {
   return a.dtype == 0 ? launch_t<__nv_bfloat16>(a, st, bwd) : a.dtype == 1 ? launch_t<__half>(a, st, bwd) : launch_t<float>(a, st, bwd);

@@ -9,6 +9,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <typename Args>
 __device__ __forceinline__ int64_t row_offset(const Args& a, int64_t r) {
+  if (r < a.inner) return r * a.stride_inner;   // the usual case, without a division
   return (r / a.inner) * a.stride_outer + (r % a.inner) * a.stride_inner;
 }
 
@@ -18,9 +19,17 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Exponents of two: 2^u is an entry's weight beside m, the largest entry of some part of its row, c = scale log2(e).  The difference
+// first: it is exact for what counts, is 0 at m, and leaves fp32's range only where the weight is zero.  m = -infinity (nothing above
+// it yet) counts as 0.
+__device__ __forceinline__ float exponent(float x, float m, float c) { return (x - (m == -INFINITY ? 0.f : m)) * c; }
+
 // an index as int32 or int64; whatever lies outside [0, V) is -1
+__device__ __forceinline__ int64_t raw_index(const void* p, int64_t i, int bytes) {
+  return bytes == 8 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
+}
 __device__ __forceinline__ int load_index(const void* p, int64_t i, int bytes, int V) {
-  const int64_t v = bytes == 8 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
+  const int64_t v = raw_index(p, i, bytes);
   return v >= 0 && v < V ? (int)v : -1;
 }
 
@@ -60,5 +69,139 @@ __device__ __forceinline__ T cta_reduce(T v, T* scratch, Op op) {
   __syncthreads();
   return v;
 }
+
+// ---- running maximum and sums ----------------------------------------------------------------------------------------
+// m: the largest entry (-infinity: none yet);  s = sum 2^u, t = sum u 2^u with the exponents u beside m
+struct Sums {
+  float m, s, t;
+};
+__device__ __forceinline__ Sums moved(Sums a, float m, float c) {   // the same sums beside another, larger m
+  if (a.m == -INFINITY) return {m, a.s, a.t};   // of no entries above -infinity: zeros, or NaN with NaN among them
+  const float d = (a.m - m) * c, f = exp2_approx(d);
+  return {m, a.s * f, f == 0.f ? 0.f : f * (a.t + d * a.s)};
+}
+__device__ __forceinline__ float warp_max(float x) {   // (NaN is left out)
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool WITH_T>
+__device__ __forceinline__ Sums warp_sums(Sums a, float c) {
+  a = moved(a, warp_max(a.m), c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    if constexpr (WITH_T) a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+  }
+  return a;
+}
+
+// the larger of two words' elements, pair by pair (what is NaN is left out), and the largest of a word of pairs
+template <typename T>
+__device__ __forceinline__ uint32_t max_words(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float max_of_word(uint32_t a) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(a);
+  else {
+    const float2 f = unpack2(widen2<T>(a));
+    return fmaxf(f.x, f.y);
+  }
+}
+template <typename T>
+constexpr uint32_t kMinusInfWord = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+
+// elements 2 i, 2 i + 1 of a 16-byte word as an fp32 pair
+template <typename T>
+__device__ __forceinline__ uint64_t pair_of(const uint4& w, int i) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  if constexpr (sizeof(T) == 2) return widen2<T>(u[i]);
+  else return pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t largest_of(const uint4& w) {
+  if constexpr (sizeof(T) == 4) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(m) : "f"(__uint_as_float(w.x)), "f"(__uint_as_float(w.y)), "f"(__uint_as_float(w.z)));
+    return __float_as_uint(fmaxf(m, __uint_as_float(w.w)));
+  } else {
+    return max_words<T>(max_words<T>(w.x, w.y), max_words<T>(w.z, w.w));
+  }
+}
+
+// One thread's running sums.  A group of words at a time: their largest entry first, so that the sums are moved seldom.  Per pair of
+// 16-bit entries: one operation for the largest, two to widen, two for the exponents, two exponentials, one to add and one more for the
+// entropy: 4.5 instructions an entry.  (At the memory's rate an SM gets 11.7 entries of 16 bits a clock, for which it can issue 128 instructions;
+// the exponentials' unit takes 16.)
+// BOUNDED: u is at least -2^10, of entries whose 2^u is zero long before: 0 x -infinity is no number.
+template <typename T, bool WITH_T>
+struct PieceSums {
+  static constexpr int PAIRS = sizeof(T) == 2 ? 4 : 2;
+  Sums a{-INFINITY, 0.f, 0.f};
+  uint64_t s2 = 0ull, t2 = 0ull, s3 = 0ull, t3 = 0ull, m2 = 0ull;   // two running sums each, of pairs; minus the largest
+
+  __device__ __forceinline__ void flush() {
+    const float2 s = unpack2(add2(s2, s3)), t = unpack2(add2(t2, t3));
+    a.s = s.x + s.y;
+    a.t = t.x + t.y;
+  }
+  template <bool BOUNDED, int N>
+  __device__ __forceinline__ void add(const uint4 (&w)[N], float c) {
+    uint32_t top = largest_of<T>(w[0]);
+#pragma unroll
+    for (int g = 1; g < N; ++g) top = max_words<T>(top, largest_of<T>(w[g]));
+    const float m = max_of_word<T>(top);
+    if (m > a.m) {
+      flush();
+      a = moved(a, m, c);
+      s2 = pack2(a.s, 0.f);
+      t2 = pack2(a.t, 0.f);
+      s3 = t3 = 0ull;
+      m2 = pack2(-m, -m);
+    }
+    if (!(BOUNDED && WITH_T)) {
+      const uint64_t c2 = pack2(c, c);
+#pragma unroll
+      for (int g = 0; g < N; ++g)
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          const uint64_t u2 = mul2(add2(pair_of<T>(w[g], i), m2), c2);
+          const float2 u = unpack2(u2);
+          const uint64_t e2 = pack2(exp2_approx(u.x), exp2_approx(u.y));
+          if (i & 1) s3 = add2(s3, e2);
+          else s2 = add2(s2, e2);
+          if constexpr (WITH_T) {
+            if (i & 1) t3 = fma2(e2, u2, t3);
+            else t2 = fma2(e2, u2, t2);
+          }
+        }
+    } else {
+#pragma unroll 1
+      for (int g = 0; g < N; ++g) {
+        uint4 q = w[0];
+#pragma unroll
+        for (int o = 1; o < N; ++o)
+          if (g == o) q = w[o];
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          const float2 x = unpack2(pair_of<T>(q, i));
+          const float u0 = exponent(x.x, a.m, c), u1 = exponent(x.y, a.m, c), e0 = exp2_approx(u0), e1 = exp2_approx(u1);
+          s2 = add2(s2, pack2(e0, e1));
+          if constexpr (WITH_T) t2 = fma2(pack2(e0, e1), pack2(fmaxf(u0, -1024.f), fmaxf(u1, -1024.f)), t2);
+        }
+      }
+    }
+  }
+};
 
 }  // namespace gdn

@@ -434,16 +434,18 @@ typedef struct b200gdn_logprob_args {
   float* entropy;                /* [rows] or NULL: -sum p lp */
   float* top_logprobs;           /* [rows, top_k], most probable first */
   int64_t* top_ids;              /* [rows, top_k]: equal entries in the order of their indices */
-  float* stats;                  /* [rows, 2]: m and the logarithm of the sum; written by the forward pass (NULL: not wanted), read by the backward pass */
+  float* stats;                  /* [rows, 2]: m and the base-2 logarithm of the sum; written by the forward pass (NULL: not wanted), read by the backward pass */
   /* backward: entropy (with dentropy) and top_ids are read.  Upstream gradients, NULL: zero */
   const float* dlogprobs;        /* [rows] */
   const float* dentropy;         /* [rows] */
   const float* dtop_logprobs;    /* [rows, top_k] */
   void* dlogits;                 /* [rows, V], contiguous */
+  void* workspace;               /* forward: b200gdn_logprob_workspace_bytes(rows, V, dtype, top_k), 16-byte aligned */
 } b200gdn_logprob_args;
 #define B200GDN_MAX_TOP 128
 int b200gdn_logprob_fwd(const b200gdn_logprob_args* args, void* stream);
 int b200gdn_logprob_bwd(const b200gdn_logprob_args* args, void* stream);
+int64_t b200gdn_logprob_workspace_bytes(int64_t rows, int32_t V, int32_t dtype, int32_t top_k);
 
 /* Cross-entropy difference (Kullback-Leibler divergence) of a student's rows of logits, laid out as above, from a teacher's K
  * entries a row: log probabilities l and their places id.
