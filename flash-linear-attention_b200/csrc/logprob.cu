@@ -19,22 +19,6 @@ __device__ __forceinline__ float lp_of(float x, float m, float log_s, float scal
   return log_s == -INFINITY ? -INFINITY : exponent(x, m, scale) - log_s * kLn2;
 }
 
-// ---- spans -------------------------------------------------------------------------------------------------------------
-constexpr int kSpanWarps = 4;
-
-// How rows are cut: `w` words a lane, for as many words of 16 bytes as a row has at most (off a word's boundary it has one more).  By the
-// width alone: a row's results are the same bits whatever rows it comes with.
-struct Spans {
-  int w, per_row;
-  __host__ __device__ int groups() const { return 32 * per_row; }
-};
-Spans spans_of(int V, int size) {
-  const int64_t words = ((int64_t)V * size + 15) / 16 + 1;
-  int w = 8;
-  while (w > 1 && words <= 16 * w) w >>= 1;   // short rows: no more lanes without words than have to be
-  return Spans{w, (int)((words + 32 * w - 1) / (32 * w))};
-}
-
 // values in order as unsigned integers of 16 or 32 bits; 0 for no value at all.  The zeros are one value.
 template <typename T>
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -53,33 +37,6 @@ __device__ __forceinline__ float from_ordered(uint32_t o) {
   else return __uint_as_float(sizeof(T) == 2 ? b << 16 : b);
 }
 
-// A row by words: word j holds the entries from first + j EPW on; the first and the last may hold something else beside (every word that is
-// read holds an entry of the row, so no read leaves the 16 bytes that hold one).
-template <typename T>
-struct Words {
-  static constexpr int EPW = 16 / sizeof(T);
-  const uint4* at;
-  int first, n;
-  __device__ __forceinline__ Words(const T* row, int V) {
-    const uintptr_t b = reinterpret_cast<uintptr_t>(row);
-    const int shift = (int)(b & 15) / (int)sizeof(T);
-    at = reinterpret_cast<const uint4*>(b & ~(uintptr_t)15);
-    first = -shift;
-    n = (shift + V + EPW - 1) / EPW;
-  }
-  // word j with minus infinity for what is not of the row
-  __device__ __forceinline__ uint4 edge(int j, int V) const {
-    uint4 q = at[j];
-    T* x = reinterpret_cast<T*>(&q);
-#pragma unroll
-    for (int e = 0; e < EPW; ++e) {
-      const int i = first + j * EPW + e;
-      if (i < 0 || i >= V) x[e] = static_cast<T>(-INFINITY);
-    }
-    return q;
-  }
-};
-
 template <typename T, int W, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(32 * kSpanWarps) logprob_spans_kernel(const b200gdn_logprob_args a, const Spans spans, float4* part, void* largest) {
   const int lane = threadIdx.x & 31;
@@ -88,67 +45,16 @@ __global__ void __launch_bounds__(32 * kSpanWarps) logprob_spans_kernel(const b2
   if (r >= a.rows) return;
   const Words<T> x(static_cast<const T*>(a.logits) + row_offset(a, r), a.V);
   const float c = a.scale * kLog2e;
-  const int j0 = span * 32 * W + lane;
-  uint4 q[W];
-  // nothing but entries
-  const bool inner = (span > 0 || x.first == 0) && ((span + 1) * 32 * W < x.n || ((span + 1) * 32 * W == x.n && x.first + x.n * Words<T>::EPW == a.V));
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const int j = j0 + 32 * i;
-    if (inner) q[i] = x.at[j];
-    else if (j < x.n) q[i] = x.edge(j, a.V);
-    else q[i] = make_uint4(kMinusInfWord<T>, kMinusInfWord<T>, kMinusInfWord<T>, kMinusInfWord<T>);
-  }
-  PieceSums<T, ENTROPY> p;
-  constexpr int G = W < 4 ? W : 4;
-  bool bounded = !inner;
-  if (inner) {
-#pragma unroll
-    for (int i = 0; i < W; i += G) {
-      uint4 w[G];
-#pragma unroll
-      for (int g = 0; g < G; ++g) w[g] = q[i + g];
-      p.template add<false>(w, c);
-    }
-    p.flush();
-    // entries of minus infinity: once more, with bounded exponents
-    bounded = ENTROPY && p.a.t != p.a.t && p.a.s == p.a.s;
-  }
-  if (bounded) {
-    p = PieceSums<T, ENTROPY>();
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const uint4 w[1] = {q[i]};
-      p.template add<true>(w, c);
-    }
-    p.flush();
-  }
-  const Sums v = warp_sums<ENTROPY>(p.a, c);
-  if (lane == 0) part[r * spans.per_row + span] = make_float4(v.m, v.s, v.t, 0.f);
-  if constexpr (TOP) {
-    // (a lane without words leaves 0)
-    static_cast<Order<T>*>(largest)[r * spans.groups() + span * 32 + lane] = (Order<T>)(j0 < x.n ? ordered<T>(p.a.m) : 0u);
-  }
+  const SpanWords<T, W> words(x, a.V, span, lane);
+  const Sums mine = words.template sums<ENTROPY>(c), v = warp_sums<ENTROPY>(mine, c);
+  if (lane == 0) part[task] = make_float4(v.m, v.s, v.t, 0.f);
+  // (a lane without words leaves 0)
+  if constexpr (TOP) static_cast<Order<T>*>(largest)[task * 32 + lane] = (Order<T>)(words.j0 < x.n ? ordered<T>(mine.m) : 0u);
 }
 
 // ---- joining a row's spans ---------------------------------------------------------------------------------------------
 constexpr int NT = 128, kRoom = 1024;   // threads of a row with top entries; keys of entries that may be among them
 static_assert(kRoom >= 2 * B200GDN_MAX_TOP, "entries above tau and as many equal to it as are wanted");
-
-// a whole warp
-__device__ __forceinline__ Sums joined_spans(const float4* part, int n, float c, int lane) {
-  Sums v{-INFINITY, 0.f, 0.f};
-  for (int i = lane; i < n; i += 32) {
-    const float4 f = part[i];
-    const Sums o{f.x, f.y, f.z};
-    const float m = fmaxf(v.m, o.m);
-    const Sums p = moved(o, m, c);
-    v = moved(v, m, c);
-    v.s += p.s;
-    v.t += p.t;
-  }
-  return warp_sums<true>(v, c);
-}
 
 // one thread
 template <typename T>
@@ -171,7 +77,7 @@ __global__ void __launch_bounds__(NT) logprob_join_kernel(const b200gdn_logprob_
   const int64_t r = (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
   if (r >= a.rows) return;
   const int lane = threadIdx.x & 31;
-  const Sums v = joined_spans(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
+  const Sums v = joined_spans<false>(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
   if (lane == 0) row_results<T>(a, r, v, log2f(v.s));
 }
 
@@ -276,7 +182,7 @@ __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logpr
     const uint32_t t = kth_largest<T>(own, twice ? 2 * NT : NT, k, lane);
     if (lane == 0) bound = t;
   } else if (warp == 1) {
-    const Sums v = joined_spans(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
+    const Sums v = joined_spans<false>(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
     if (lane == 0) {
       stats[0] = v.m;
       stats[1] = log2f(v.s);
@@ -390,7 +296,7 @@ int launch_spans(const b200gdn_logprob_args& a, const Spans& spans, float4* part
 template <typename T>
 int launch_fwd(const b200gdn_logprob_args& a, cudaStream_t st) {
   const Spans spans = spans_of(a.V, sizeof(T));
-  if (a.rows * spans.per_row > (int64_t)INT32_MAX * kSpanWarps) return set_error(B200GDN_ERR_UNSUPPORTED, "logprob_fwd: more than 2^34 spans");
+  if (a.rows * spans.per_row > (int64_t)INT32_MAX * kSpanWarps) return set_error(B200GDN_ERR_UNSUPPORTED, "logprob_fwd: more than 2^33 spans");
   float4* part = static_cast<float4*>(a.workspace);
   void* largest = part + a.rows * spans.per_row;
   int e = spans.w == 8 ? launch_spans<T, 8>(a, spans, part, largest, st) : spans.w == 4 ? launch_spans<T, 4>(a, spans, part, largest, st)
@@ -402,44 +308,77 @@ int launch_fwd(const b200gdn_logprob_args& a, cudaStream_t st) {
 }
 
 // ---- gradient ----------------------------------------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(NT) logprob_bwd_kernel(const b200gdn_logprob_args a) {
-  __shared__ float fs[NT / 32];
-  const int64_t r = blockIdx.x;
-  const T* x = static_cast<const T*>(a.logits) + row_offset(a, r);
-  const int64_t out = r * a.V;
+// dx = scale p (-(A + dH (lp + H))) plus what the given entries get: with l = log2 p,  p (a0 + a1 l).  Two exponent instructions for
+// every four bytes moved: HBM's.
+template <typename T, int W>
+__global__ void __launch_bounds__(32 * kSpanWarps) logprob_bwd_kernel(const b200gdn_logprob_args a, const Spans spans) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task = (int64_t)blockIdx.x * kSpanWarps + (threadIdx.x >> 5), r = task / spans.per_row;
+  const int span = (int)(task - r * spans.per_row);
+  if (r >= a.rows) return;
+  const T* row = static_cast<const T*>(a.logits) + row_offset(a, r);
+  T* out = static_cast<T*>(a.dlogits) + r * a.V;
   const float m = a.stats[2 * r], log_s = a.stats[2 * r + 1], c = a.scale * kLog2e;
   if (log_s == -INFINITY) {   // nothing in this row
-    for (int j = threadIdx.x; j < a.V; j += NT) Io<T>::st(a.dlogits, out + j, 0.f);
+    write_span<T, W>(out, out, a.V, span, lane, [](uint64_t) { return 0ull; });
     return;
   }
   const int token = a.dlogprobs ? load_index(a.tokens, r, a.token_bytes, a.V) : -1;
   const float dlp = token < 0 ? 0.f : a.dlogprobs[r], dh = a.dentropy ? a.dentropy[r] : 0.f, h = a.dentropy ? a.entropy[r] : 0.f;
   const int k = a.dtop_logprobs ? a.top_k : 0;
-  float all = 0.f;
-  for (int i = threadIdx.x; i < k; i += NT) all += a.dtop_logprobs[r * k + i];
-  all = cta_reduce<NT>(all, fs, SumOf()) + dlp;
-  auto grad = [&](int j) {
-    const float l2 = exponent(Io<T>::ld(x, j), m, c) - log_s, p = exp2_approx(l2);
-    return p == 0.f ? 0.f : -p * (all + dh * (l2 * kLn2 + h));
-  };
-  for (int j = threadIdx.x; j < a.V; j += NT) Io<T>::st(a.dlogits, out + j, grad(j) * a.scale);
-  __syncthreads();
-  bool listed = false;
-  for (int i = 0; i < k; ++i) listed |= (int)a.top_ids[r * k + i] == token;
-  for (int i = threadIdx.x; i < k; i += NT) {
-    const int j = (int)a.top_ids[r * k + i];
-    Io<T>::st(a.dlogits, out + j, (grad(j) + a.dtop_logprobs[r * k + i] + (j == token ? dlp : 0.f)) * a.scale);
+  constexpr int L = B200GDN_MAX_TOP / 32;
+  int id[L];
+  float d[L], all = 0.f;
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    const bool there = i * 32 + lane < k;
+    id[i] = there ? (int)a.top_ids[r * k + i * 32 + lane] : -1;
+    d[i] = there ? a.dtop_logprobs[r * k + i * 32 + lane] : 0.f;
+    all += d[i];
   }
-  if (threadIdx.x == 0 && token >= 0 && !listed) Io<T>::st(a.dlogits, out + token, (grad(token) + dlp) * a.scale);
+  if (k > 0)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  all += dlp;
+  const float a0 = -(all + dh * h) * a.scale, a1 = -dh * kLn2 * a.scale, base = m == -INFINITY ? 0.f : m;
+  const uint64_t m2 = pack2(-base, -base), c2 = pack2(c, c), s2 = pack2(-log_s, -log_s), a02 = pack2(a0, a0), a12 = pack2(a1, a1);
+  auto grad = [&](uint64_t x) {   // (of masked entries p is zero, and l bounded)
+    const float2 l = unpack2(add2(mul2(add2(x, m2), c2), s2));
+    return mul2(pack2(exp2_approx(l.x), exp2_approx(l.y)), fma2(a12, pack2(fmaxf(l.x, -1024.f), fmaxf(l.y, -1024.f)), a02));
+  };
+  write_span<T, W>(row, out, a.V, span, lane, grad);
+  // the given entries again, from the lanes that hold them
+  __syncwarp();
+  auto again = [&](int j, float more) {
+    const float x = Io<T>::ld(row, j);
+    Io<T>::st(out, j, unpack2(grad(pack2(x, x))).x + more * a.scale);
+  };
+  bool listed = false;
+#pragma unroll
+  for (int i = 0; i < L; ++i) {
+    if (id[i] < 0) continue;
+    listed |= id[i] == token;
+    if (in_span<T, W>(out, span, id[i])) again(id[i], d[i] + (id[i] == token ? dlp : 0.f));
+  }
+  listed = __any_sync(0xffffffffu, listed);
+  if (lane == 0 && token >= 0 && !listed && in_span<T, W>(out, span, token)) again(token, dlp);
 }
 
 template <typename T>
-int launch_t(const b200gdn_logprob_args& a, cudaStream_t st, bool bwd) {
-  if (!bwd) return launch_fwd<T>(a, st);
-  logprob_bwd_kernel<T><<<(unsigned)a.rows, NT, 0, st>>>(a);
+int launch_bwd(const b200gdn_logprob_args& a, cudaStream_t st) {
+  const Spans spans = spans_of(a.V, sizeof(T));
+  if (a.rows * spans.per_row > (int64_t)INT32_MAX * kSpanWarps) return set_error(B200GDN_ERR_UNSUPPORTED, "logprob_bwd: more than 2^33 spans");
+  const unsigned grid = (unsigned)((a.rows * spans.per_row + kSpanWarps - 1) / kSpanWarps);
+  auto go = [&](auto kern) { kern<<<grid, 32 * kSpanWarps, 0, st>>>(a, spans); };
+  if (spans.w == 8) go(logprob_bwd_kernel<T, 8>);
+  else if (spans.w == 4) go(logprob_bwd_kernel<T, 4>);
+  else if (spans.w == 2) go(logprob_bwd_kernel<T, 2>);
+  else go(logprob_bwd_kernel<T, 1>);
   return check_launch("logprob_bwd");
 }
+
+template <typename T>
+int launch_t(const b200gdn_logprob_args& a, cudaStream_t st, bool bwd) { return bwd ? launch_bwd<T>(a, st) : launch_fwd<T>(a, st); }
 
 }  // namespace
 

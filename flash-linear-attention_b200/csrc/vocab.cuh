@@ -204,4 +204,173 @@ struct PieceSums {
   }
 };
 
+
+// ---- spans -------------------------------------------------------------------------------------------------------------
+constexpr int kSpanWarps = 4;
+
+// How rows are cut: `w` words a lane, for as many words of 16 bytes as a row has at most (off a word's boundary it has one more).  By the
+// width alone: a row's results are the same bits whatever rows it comes with.
+struct Spans {
+  int w, per_row;
+  __host__ __device__ int groups() const { return 32 * per_row; }
+};
+inline Spans spans_of(int V, int size) {
+  const int64_t words = ((int64_t)V * size + 15) / 16 + 1;
+  int w = 8;
+  while (w > 1 && words <= 16 * w) w >>= 1;   // short rows: no more lanes without words than have to be
+  return Spans{w, (int)((words + 32 * w - 1) / (32 * w))};
+}
+
+// A row by words: word j holds the entries from first + j EPW on; the first and the last may hold something else beside (every word that is
+// read holds an entry of the row, so no read leaves the 16 bytes that hold one).
+template <typename T>
+struct Words {
+  static constexpr int EPW = 16 / sizeof(T);
+  const uint4* at;
+  int first, n;
+  __device__ __forceinline__ Words(const T* row, int V) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(row);
+    const int shift = (int)(b & 15) / (int)sizeof(T);
+    at = reinterpret_cast<const uint4*>(b & ~(uintptr_t)15);
+    first = -shift;
+    n = (shift + V + EPW - 1) / EPW;
+  }
+  // word j with minus infinity for what is not of the row
+  __device__ __forceinline__ uint4 edge(int j, int V) const {
+    uint4 q = at[j];
+    T* x = reinterpret_cast<T*>(&q);
+#pragma unroll
+    for (int e = 0; e < EPW; ++e) {
+      const int i = first + j * EPW + e;
+      if (i < 0 || i >= V) x[e] = static_cast<T>(-INFINITY);
+    }
+    return q;
+  }
+};
+
+// A span's words in a warp's registers: word i of lane l is word (32 W span) + 32 i + l of the row; minus infinity for what is not of it.
+template <typename T, int W>
+struct SpanWords {
+  uint4 q[W];
+  int j0;       // of this lane
+  bool inner;   // nothing but entries
+  __device__ __forceinline__ SpanWords(const Words<T>& x, int V, int span, int lane) {
+    j0 = span * 32 * W + lane;
+    inner = (span > 0 || x.first == 0) && ((span + 1) * 32 * W < x.n || ((span + 1) * 32 * W == x.n && x.first + x.n * Words<T>::EPW == V));
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int j = j0 + 32 * i;
+      if (inner) q[i] = x.at[j];
+      else if (j < x.n) q[i] = x.edge(j, V);
+      else q[i] = make_uint4(kMinusInfWord<T>, kMinusInfWord<T>, kMinusInfWord<T>, kMinusInfWord<T>);
+    }
+  }
+  // this lane's sums
+  template <bool WITH_T>
+  __device__ __forceinline__ Sums sums(float c) const {
+    PieceSums<T, WITH_T> p;
+    constexpr int G = W < 4 ? W : 4;
+    bool bounded = !inner;
+    if (inner) {
+#pragma unroll
+      for (int i = 0; i < W; i += G) {
+        uint4 w[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) w[g] = q[i + g];
+        p.template add<false>(w, c);
+      }
+      p.flush();
+      // entries of minus infinity: once more, with bounded exponents
+      bounded = WITH_T && p.a.t != p.a.t && p.a.s == p.a.s;
+    }
+    if (bounded) {
+      p = PieceSums<T, WITH_T>();
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const uint4 w[1] = {q[i]};
+        p.template add<true>(w, c);
+      }
+      p.flush();
+    }
+    return p.a;
+  }
+};
+
+// A row's spans joined; a whole warp.  L2: the parts may be of other CTAs of the same kernel.
+template <bool L2>
+__device__ __forceinline__ Sums joined_spans(const float4* part, int n, float c, int lane) {
+  Sums v{-INFINITY, 0.f, 0.f};
+  for (int i = lane; i < n; i += 32) {
+    const float4 f = L2 ? __ldcg(part + i) : part[i];
+    const Sums o{f.x, f.y, f.z};
+    const float m = fmaxf(v.m, o.m);
+    const Sums p = moved(o, m, c);
+    v = moved(v, m, c);
+    v.s += p.s;
+    v.t += p.t;
+  }
+  return warp_sums<true>(v, c);
+}
+
+// ---- gradients: a span of dlogits ----------------------------------------------------------------------------------------
+// Words of dlogits, each written by one lane: f(x) of the entry's logit.  Where a row of dlogits lies in its words as the row of logits does,
+// logits are read by words as well, else entry by entry.
+template <typename T, int W, typename F>
+__device__ __forceinline__ void write_span(const T* row, T* out, int V, int span, int lane, F f) {
+  constexpr int EPW = Words<T>::EPW;
+  const Words<T> y(out, V);
+  const bool alike = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
+  uint4 q[W];
+  const int j0 = span * 32 * W + lane;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const int j = j0 + 32 * i;
+    if (j >= y.n) continue;
+    if (alike) {
+      q[i] = src[j];
+    } else {
+      T* x = reinterpret_cast<T*>(&q[i]);
+#pragma unroll
+      for (int e = 0; e < EPW; ++e) {
+        const int at = y.first + j * EPW + e;
+        x[e] = at >= 0 && at < V ? row[at] : static_cast<T>(0.f);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const int j = j0 + 32 * i, at = y.first + j * EPW;
+    if (j >= y.n) continue;
+    uint32_t g[4];
+#pragma unroll
+    for (int e = 0; e < EPW / 2; ++e) {
+      const uint64_t d = f(pair_of<T>(q[i], e));
+      if constexpr (sizeof(T) == 2) {
+        g[e] = narrow2<T>(d);
+      } else {
+        const float2 p = unpack2(d);
+        g[2 * e] = __float_as_uint(p.x);
+        g[2 * e + 1] = __float_as_uint(p.y);
+      }
+    }
+    const uint4 w = make_uint4(g[0], g[1], g[2], g[3]);
+    if (at >= 0 && at + EPW <= V) {
+      __stcs(const_cast<uint4*>(y.at) + j, w);
+    } else {
+      const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int e = 0; e < EPW; ++e)
+        if (at + e >= 0 && at + e < V) out[at + e] = x[e];
+    }
+  }
+}
+// the entries that the words of a span of dlogits hold
+template <typename T, int W>
+__device__ __forceinline__ bool in_span(const T* out, int span, int j) {
+  constexpr int EPW = Words<T>::EPW;
+  const int word = (j + (int)(reinterpret_cast<uintptr_t>(out) & 15) / (int)sizeof(T)) / EPW;
+  return j >= 0 && word / (32 * W) == span;
+}
+
 }  // namespace gdn
