@@ -122,7 +122,7 @@ DISTILL_BUCKET, DISTILL_MEAN, DISTILL_SCALAR, DISTILL_SKIP_ONE = 1, 2, 4, 8
 class DistillArgs(C.Structure):
     _fields_ = _ROWS_OF_LOGITS + [
         ('K', C.c_int32), ('scale', C.c_float), ('flags', C.c_uint32), ('id_bytes', C.c_int32), ('teacher_dtype', C.c_int32),
-        ('logits', _p), ('teacher', _p), ('ids', _p), ('row_loss', _p), ('loss', _p), ('stats', _p), ('counters', _p),
+        ('logits', _p), ('teacher', _p), ('ids', _p), ('row_loss', _p), ('loss', _p), ('workspace', _p),
         ('dloss', _p), ('dlogits', _p),
     ]
 
@@ -134,7 +134,7 @@ EXPORTS = (
     'b200gdn_selftest_wait_expiry', 'b200gdn_chunk_fwd_static', 'b200gdn_cp_fold', 'b200gdn_cp_prefix',
     'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd', 'b200gdn_norm_gate_ctas',
     'b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd', 'b200gdn_layer_norm_ctas', 'b200gdn_logprob_fwd', 'b200gdn_logprob_bwd',
-    'b200gdn_logprob_workspace_bytes', 'b200gdn_distill_fwd', 'b200gdn_distill_bwd',
+    'b200gdn_logprob_workspace_bytes', 'b200gdn_distill_fwd', 'b200gdn_distill_bwd', 'b200gdn_distill_workspace_bytes',
 )
 
 _lib = None
@@ -172,8 +172,10 @@ def load():
             fn.argtypes = [C.c_int32] * 6
         lib.b200gdn_norm_gate_ctas.restype = C.c_int
         lib.b200gdn_norm_gate_ctas.argtypes = [C.c_int64]
-        lib.b200gdn_logprob_workspace_bytes.restype = C.c_int64
-        lib.b200gdn_logprob_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
+        for name in ('b200gdn_logprob_workspace_bytes', 'b200gdn_distill_workspace_bytes'):
+            fn = getattr(lib, name)
+            fn.restype = C.c_int64
+            fn.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
         lib.b200gdn_layer_norm_ctas.restype = C.c_int
         lib.b200gdn_layer_norm_ctas.argtypes = [C.c_int64, C.c_int32, C.c_int32]
         lib.b200gdn_last_launch_count.restype = C.c_int

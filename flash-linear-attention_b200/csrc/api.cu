@@ -436,11 +436,15 @@ static int check_distill_args(const b200gdn_distill_args* a, const char* who, bo
   if (a->id_bytes != 4 && a->id_bytes != 8) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: id_bytes %d (4 or 8)", who, a->id_bytes);
   if (a->teacher_dtype < 0 || a->teacher_dtype > 2) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: teacher_dtype %d", who, a->teacher_dtype);
   REQUIRE(a->teacher, who); REQUIRE(a->ids, who);
-  if (a->flags & B200GDN_DISTILL_MEAN) REQUIRE(a->counters, who);
   if (!bwd) { REQUIRE(a->row_loss, who); }
-  else { REQUIRE(a->stats, who); REQUIRE(a->dloss, who); REQUIRE(a->dlogits, who); }
+  else { REQUIRE(a->dloss, who); REQUIRE(a->dlogits, who); }
+  if ((a->flags & B200GDN_DISTILL_SKIP_ONE) && !(bwd && (a->flags & B200GDN_DISTILL_SCALAR)))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: SKIP_ONE goes with a scalar upstream gradient", who);
+  REQUIRE(a->workspace, who);
   return 0;
 }
+
+int64_t b200gdn_distill_workspace_bytes(int64_t rows, int32_t V, int32_t dtype, int32_t K) { return gdn::distill_workspace(rows, V, dtype, K); }
 
 int b200gdn_distill_fwd(const b200gdn_distill_args* a, void* stream) {
   gdn::g_launches = 0;

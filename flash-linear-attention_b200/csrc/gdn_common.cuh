@@ -155,6 +155,7 @@ int launch_layer_norm(const b200gdn_layer_norm_args& a, cudaStream_t st, bool bw
 int layer_norm_grid(int64_t rows, int D, int dtype);
 int64_t logprob_workspace(int64_t rows, int V, int dtype, int top_k);
 int launch_logprob(const b200gdn_logprob_args& a, cudaStream_t st, bool bwd);
+int64_t distill_workspace(int64_t rows, int V, int dtype, int K);
 int launch_distill(const b200gdn_distill_args& a, cudaStream_t st, bool bwd);
 int decode_timeout_flag();
 int intra_fwd_timeout_flag();

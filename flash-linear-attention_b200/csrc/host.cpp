@@ -1066,11 +1066,11 @@ class LogprobFunction : public torch::autograd::Function<LogprobFunction> {
 enum Reduction { kNone = 0, kSum = 1, kMean = 2 };
 
 struct DistillForward {
-  Tensor teacher, ids, out, stats, counters, dlogits;
+  Tensor teacher, ids, out, workspace, dlogits;
 };
 
 b200gdn_distill_args distill_args(const LogitRows& rows, const Tensor& teacher, const Tensor& ids, double scale, bool bucket, int64_t reduction,
-                                  const Tensor& stats, const Tensor& counters, const Tensor& dlogits) {
+                                  const Tensor& workspace, const Tensor& dlogits) {
   b200gdn_distill_args a{};
   set_rows(a, rows, scale);
   a.K = (int32_t)teacher.size(-1);
@@ -1079,8 +1079,7 @@ b200gdn_distill_args distill_args(const LogitRows& rows, const Tensor& teacher, 
   a.teacher_dtype = param_code(teacher.scalar_type());
   a.teacher = ptr(teacher);
   a.ids = ptr(ids);
-  a.stats = fptr(stats);
-  a.counters = static_cast<int32_t*>(ptr(counters));
+  a.workspace = ptr(workspace);
   a.dlogits = ptr(dlogits);
   return a;
 }
@@ -1097,13 +1096,11 @@ DistillForward distill_forward(const Tensor& logits, const Tensor& teacher, cons
   r.ids = ids.contiguous();
   const Tensor row_loss = new_tensor(lead, at::kFloat, dev);
   r.out = reduction == kNone ? row_loss : new_tensor({}, at::kFloat, dev, rows.rows == 0);
-  if (need_grad) {
-    r.stats = new_tensor({rows.rows, 4}, at::kFloat, dev);
-    if (reduction != kNone) r.dlogits = new_tensor(logits.sizes(), logits.scalar_type(), dev);
-  }
+  if (need_grad && reduction != kNone) r.dlogits = new_tensor(logits.sizes(), logits.scalar_type(), dev);
   if (rows.rows == 0) return r;
-  if (reduction != kNone) r.counters = new_tensor({2}, at::kInt, dev);
-  b200gdn_distill_args a = distill_args(rows, r.teacher, r.ids, scale, bucket, reduction, r.stats, r.counters, r.dlogits);
+  r.workspace = new_tensor({b200gdn_distill_workspace_bytes(rows.rows, (int32_t)logits.size(-1), act_code(logits.scalar_type()), (int32_t)teacher.size(-1))},
+                           at::kByte, dev);
+  b200gdn_distill_args a = distill_args(rows, r.teacher, r.ids, scale, bucket, reduction, r.workspace, r.dlogits);
   a.row_loss = fptr(row_loss);
   a.loss = reduction == kNone ? nullptr : fptr(r.out);
   call("b200gdn_distill_fwd", b200gdn_distill_fwd, a);
@@ -1125,7 +1122,7 @@ class DistillFunction : public torch::autograd::Function<DistillFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& teacher, const Tensor& ids, double scale, bool bucket,
                         int64_t reduction) {
     DistillForward r = distill_forward(logits, teacher, ids, scale, bucket, reduction, true);
-    ctx->save_for_backward({logits, r.teacher, r.ids, r.stats, r.counters});
+    ctx->save_for_backward({logits, r.teacher, r.ids, r.workspace});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["bucket"] = bucket;
     ctx->saved_data["reduction"] = reduction;
@@ -1137,7 +1134,7 @@ class DistillFunction : public torch::autograd::Function<DistillFunction> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &teacher = saved[1], &ids = saved[2], &stats = saved[3], &counters = saved[4];
+    const Tensor &logits = saved[0], &teacher = saved[1], &ids = saved[2], &workspace = saved[3];
     const at::Device dev = logits.device();
     c10::cuda::CUDAGuard guard(dev);
     const LogitRows rows = logit_rows(logits);
@@ -1149,7 +1146,7 @@ class DistillFunction : public torch::autograd::Function<DistillFunction> {
     if (rows.rows > 0) {
       const Tensor dloss = dense(grads[0], at::kFloat);
       b200gdn_distill_args a = distill_args(rows, teacher, ids, ctx->saved_data["scale"].toDouble(), ctx->saved_data["bucket"].toBool(),
-                                            reduction, stats, counters, dlogits);
+                                            reduction, workspace, dlogits);
       if (reduction != kNone) a.flags |= B200GDN_DISTILL_SCALAR | (formed ? B200GDN_DISTILL_SKIP_ONE : 0);
       a.dloss = fptr(dloss);
       call("b200gdn_distill_bwd", b200gdn_distill_bwd, a);

@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(NT) logprob_join_kernel(const b200gdn_logprob_
   const int64_t r = (int64_t)blockIdx.x * (NT / 32) + (threadIdx.x >> 5);
   if (r >= a.rows) return;
   const int lane = threadIdx.x & 31;
-  const Sums v = joined_spans<false>(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
+  const Sums v = joined_spans(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
   if (lane == 0) row_results<T>(a, r, v, log2f(v.s));
 }
 
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logpr
     const uint32_t t = kth_largest<T>(own, twice ? 2 * NT : NT, k, lane);
     if (lane == 0) bound = t;
   } else if (warp == 1) {
-    const Sums v = joined_spans<false>(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
+    const Sums v = joined_spans(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
     if (lane == 0) {
       stats[0] = v.m;
       stats[1] = log2f(v.s);
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(32 * kSpanWarps) logprob_bwd_kernel(const b200
   T* out = static_cast<T*>(a.dlogits) + r * a.V;
   const float m = a.stats[2 * r], log_s = a.stats[2 * r + 1], c = a.scale * kLog2e;
   if (log_s == -INFINITY) {   // nothing in this row
-    write_span<T, W>(out, out, a.V, span, lane, [](uint64_t) { return 0ull; });
+    zero_span<T, W>(out, a.V, span, lane);
     return;
   }
   const int token = a.dlogprobs ? load_index(a.tokens, r, a.token_bytes, a.V) : -1;
@@ -346,7 +346,9 @@ __global__ void __launch_bounds__(32 * kSpanWarps) logprob_bwd_kernel(const b200
     const float2 l = unpack2(add2(mul2(add2(x, m2), c2), s2));
     return mul2(pack2(exp2_approx(l.x), exp2_approx(l.y)), fma2(a12, pack2(fmaxf(l.x, -1024.f), fmaxf(l.y, -1024.f)), a02));
   };
-  write_span<T, W>(row, out, a.V, span, lane, grad);
+  GradientSpan<T, W> g;
+  g.load(row, out, a.V, span, lane);
+  g.store(out, a.V, span, lane, grad);
   // the given entries again, from the lanes that hold them
   __syncwarp();
   auto again = [&](int j, float more) {

@@ -296,12 +296,11 @@ struct SpanWords {
   }
 };
 
-// A row's spans joined; a whole warp.  L2: the parts may be of other CTAs of the same kernel.
-template <bool L2>
+// A row's spans joined; a whole warp.
 __device__ __forceinline__ Sums joined_spans(const float4* part, int n, float c, int lane) {
   Sums v{-INFINITY, 0.f, 0.f};
   for (int i = lane; i < n; i += 32) {
-    const float4 f = L2 ? __ldcg(part + i) : part[i];
+    const float4 f = part[i];
     const Sums o{f.x, f.y, f.z};
     const float m = fmaxf(v.m, o.m);
     const Sums p = moved(o, m, c);
@@ -315,55 +314,68 @@ __device__ __forceinline__ Sums joined_spans(const float4* part, int n, float c,
 // ---- gradients: a span of dlogits ----------------------------------------------------------------------------------------
 // Words of dlogits, each written by one lane: f(x) of the entry's logit.  Where a row of dlogits lies in its words as the row of logits does,
 // logits are read by words as well, else entry by entry.
-template <typename T, int W, typename F>
-__device__ __forceinline__ void write_span(const T* row, T* out, int V, int span, int lane, F f) {
-  constexpr int EPW = Words<T>::EPW;
-  const Words<T> y(out, V);
-  const bool alike = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
+template <typename T, int W>
+struct GradientSpan {
+  static constexpr int EPW = Words<T>::EPW;
   uint4 q[W];
-  const int j0 = span * 32 * W + lane;
+  // (as SpanWords: word i of lane l is word (32 W span) + 32 i + l)
+  __device__ __forceinline__ void load(const T* row, const T* out, int V, int span, int lane) {
+    const Words<T> y(out, V);
+    const bool alike = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const int j = j0 + 32 * i;
-    if (j >= y.n) continue;
-    if (alike) {
-      q[i] = src[j];
-    } else {
-      T* x = reinterpret_cast<T*>(&q[i]);
-#pragma unroll
-      for (int e = 0; e < EPW; ++e) {
-        const int at = y.first + j * EPW + e;
-        x[e] = at >= 0 && at < V ? row[at] : static_cast<T>(0.f);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const int j = j0 + 32 * i, at = y.first + j * EPW;
-    if (j >= y.n) continue;
-    uint32_t g[4];
-#pragma unroll
-    for (int e = 0; e < EPW / 2; ++e) {
-      const uint64_t d = f(pair_of<T>(q[i], e));
-      if constexpr (sizeof(T) == 2) {
-        g[e] = narrow2<T>(d);
+    for (int i = 0; i < W; ++i) {
+      const int j = span * 32 * W + lane + 32 * i;
+      if (j >= y.n) continue;
+      if (alike) {
+        q[i] = src[j];
       } else {
-        const float2 p = unpack2(d);
-        g[2 * e] = __float_as_uint(p.x);
-        g[2 * e + 1] = __float_as_uint(p.y);
+        T* x = reinterpret_cast<T*>(&q[i]);
+#pragma unroll
+        for (int e = 0; e < EPW; ++e) {
+          const int at = y.first + j * EPW + e;
+          x[e] = at >= 0 && at < V ? row[at] : static_cast<T>(0.f);
+        }
       }
     }
-    const uint4 w = make_uint4(g[0], g[1], g[2], g[3]);
-    if (at >= 0 && at + EPW <= V) {
-      __stcs(const_cast<uint4*>(y.at) + j, w);
-    } else {
-      const T* x = reinterpret_cast<const T*>(&w);
+  }
+  template <typename F>
+  __device__ __forceinline__ void store(T* out, int V, int span, int lane, F f) const {
+    const Words<T> y(out, V);
 #pragma unroll
-      for (int e = 0; e < EPW; ++e)
-        if (at + e >= 0 && at + e < V) out[at + e] = x[e];
+    for (int i = 0; i < W; ++i) {
+      const int j = span * 32 * W + lane + 32 * i, at = y.first + j * EPW;
+      if (j >= y.n) continue;
+      uint32_t g[4];
+#pragma unroll
+      for (int e = 0; e < EPW / 2; ++e) {
+        const uint64_t d = f(pair_of<T>(q[i], e));
+        if constexpr (sizeof(T) == 2) {
+          g[e] = narrow2<T>(d);
+        } else {
+          const float2 p = unpack2(d);
+          g[2 * e] = __float_as_uint(p.x);
+          g[2 * e + 1] = __float_as_uint(p.y);
+        }
+      }
+      const uint4 w = make_uint4(g[0], g[1], g[2], g[3]);
+      if (at >= 0 && at + EPW <= V) {
+        __stcs(const_cast<uint4*>(y.at) + j, w);
+      } else {
+        const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int e = 0; e < EPW; ++e)
+          if (at + e >= 0 && at + e < V) out[at + e] = x[e];
+      }
     }
   }
+};
+template <typename T, int W>
+__device__ __forceinline__ void zero_span(T* out, int V, int span, int lane) {
+  GradientSpan<T, W> z;
+#pragma unroll
+  for (int i = 0; i < W; ++i) z.q[i] = make_uint4(0u, 0u, 0u, 0u);
+  z.store(out, V, span, lane, [](uint64_t x) { return x; });
 }
 // the entries that the words of a span of dlogits hold
 template <typename T, int W>

@@ -477,14 +477,14 @@ typedef struct b200gdn_distill_args {
   const void* ids;               /* [rows, K] */
   float* row_loss;               /* [rows] */
   float* loss;                   /* [1] or NULL */
-  float* stats;                  /* [rows, 4]: what the backward pass needs of each row (NULL: not wanted) */
-  int32_t* counters;             /* [2]: workspace, kept for the backward pass with B200GDN_DISTILL_MEAN */
+  void* workspace;               /* b200gdn_distill_workspace_bytes(rows, V, dtype, K), 16-byte aligned; the backward pass reads the forward pass's */
   const float* dloss;
   void* dlogits;                 /* [rows, V], contiguous */
 } b200gdn_distill_args;
 #define B200GDN_MAX_LIST 256
 int b200gdn_distill_fwd(const b200gdn_distill_args* args, void* stream);
 int b200gdn_distill_bwd(const b200gdn_distill_args* args, void* stream);
+int64_t b200gdn_distill_workspace_bytes(int64_t rows, int32_t V, int32_t dtype, int32_t K);
 
 /* Bytes of forward-saved tensors and of backward workspace for a problem (what the caller allocates; the latter with what
  * single stages of the backward pass need). */

@@ -86,8 +86,11 @@ def test_bad_arguments_of_logprob_and_distill():
     refused('b200gdn_distill_fwd', _lib.DistillArgs(K=3, id_bytes=8, teacher_dtype=7, **rows), -1, 'teacher_dtype')
     lists = dict(K=3, id_bytes=8, teacher=256, ids=256, **rows)
     refused('b200gdn_distill_fwd', _lib.DistillArgs(**lists), -1, 'row_loss is NULL')
-    refused('b200gdn_distill_fwd', _lib.DistillArgs(flags=_lib.DISTILL_MEAN, row_loss=256, **lists), -1, 'counters is NULL')
-    refused('b200gdn_distill_bwd', _lib.DistillArgs(row_loss=256, **lists), -1, 'stats is NULL')
+    refused('b200gdn_distill_fwd', _lib.DistillArgs(row_loss=256, **lists), -1, 'workspace is NULL')
+    refused('b200gdn_distill_bwd', _lib.DistillArgs(row_loss=256, workspace=256, **lists), -1, 'dloss is NULL')
+    lib = _lib.load()
+    assert lib.b200gdn_distill_workspace_bytes(4, 1000, 0, 8) > lib.b200gdn_distill_workspace_bytes(2, 1000, 0, 8) > 0
+    assert lib.b200gdn_logprob_workspace_bytes(4, 1000, 0, 8) > lib.b200gdn_logprob_workspace_bytes(4, 1000, 0, 0) > 0
 
 
 def test_cpu_tensors_are_refused():
