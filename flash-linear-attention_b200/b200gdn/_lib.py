@@ -177,7 +177,7 @@ def load():
             fn.restype = C.c_int64
             fn.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
         lib.b200gdn_layer_norm_ctas.restype = C.c_int
-        lib.b200gdn_layer_norm_ctas.argtypes = [C.c_int64, C.c_int32, C.c_int32]
+        lib.b200gdn_layer_norm_ctas.argtypes = [C.c_int64]
         lib.b200gdn_last_launch_count.restype = C.c_int
         lib.b200gdn_device_status.restype = C.c_int
         lib.b200gdn_device_status.argtypes = []

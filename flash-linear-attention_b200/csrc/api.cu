@@ -370,7 +370,7 @@ int b200gdn_layer_norm_bwd(const b200gdn_layer_norm_args* a, void* stream) {
   return gdn::launch_layer_norm(*a, static_cast<cudaStream_t>(stream), true);
 }
 
-int b200gdn_layer_norm_ctas(int64_t rows, int32_t D, int32_t dtype) { return gdn::layer_norm_grid(rows, D, dtype); }
+int b200gdn_layer_norm_ctas(int64_t rows) { return gdn::layer_norm_grid(rows); }
 
 // what the two operators on rows of logits have in common
 static int check_rows_of_logits(const char* who, int64_t rows, int64_t inner, int32_t V, int32_t dtype, float scale, const void* logits,

@@ -904,7 +904,7 @@ class LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
       a.rows = rows;
       a.dtype = act_code(t);
       a.param_dtype = (int32_t)s[0];
-      if (s[1] || s[2]) partials = new_tensor({(int64_t)b200gdn_layer_norm_ctas(rows, a.D, a.dtype) * 2 * D}, at::kFloat, dev);
+      if (s[1] || s[2]) partials = new_tensor({(int64_t)b200gdn_layer_norm_ctas(rows) * 2 * D}, at::kFloat, dev);
       a.weight = ptr(w);
       a.z = ptr(z);
       a.mean = fptr(mean);

@@ -389,7 +389,7 @@ int b200gdn_norm_gate_ctas(int64_t rows);
  *   z = x + residual, rounded to the element type (z = x without a residual);  n = (z - mean) rstd;  y = n weight + bias
  * with mean and 1/sqrt(variance + eps) of each row in fp32.  The backward pass reads z again with `mean` and `rstd`:
  *   h = dy weight;  dx = rstd (h - mean(h) - n mean(h n)) + dz;  dweight = sum of dy n;  dbias = sum of dy
- * and needs `partials` of b200gdn_layer_norm_ctas(rows, D, dtype) x 2 x D floats.  dx is the gradient of x and of residual. */
+ * and needs `partials` of b200gdn_layer_norm_ctas(rows) x 2 x D floats.  dx is the gradient of x and of residual. */
 typedef struct b200gdn_layer_norm_args {
   int32_t struct_bytes;
   int32_t D;
@@ -414,7 +414,7 @@ typedef struct b200gdn_layer_norm_args {
 } b200gdn_layer_norm_args;
 int b200gdn_layer_norm_fwd(const b200gdn_layer_norm_args* args, void* stream);
 int b200gdn_layer_norm_bwd(const b200gdn_layer_norm_args* args, void* stream);
-int b200gdn_layer_norm_ctas(int64_t rows, int32_t D, int32_t dtype);
+int b200gdn_layer_norm_ctas(int64_t rows);
 
 /* Rows of logits over a vocabulary of V.  Row r starts at element (r / inner) stride_outer + (r % inner) stride_inner; the
  * entries of a row lie side by side and need no alignment beyond their own.  scale = 1 / temperature; with m the largest entry:

@@ -48,7 +48,7 @@ def test_bad_arguments_of_layer_norm():
     a = _lib.LayerNormArgs(rows=4, D=8)
     a.struct_bytes = 8
     assert _lib.load().b200gdn_layer_norm_fwd(C.byref(a), None) == -1 and b'ABI mismatch' in _lib.load().b200gdn_last_error()
-    assert _lib.load().b200gdn_layer_norm_ctas(1, 64, 0) >= 1
+    assert _lib.load().b200gdn_layer_norm_ctas(1) >= 1
 
 
 @pytest.mark.parametrize('name', ['logprob', 'distill'])
