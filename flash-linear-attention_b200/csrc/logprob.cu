@@ -102,23 +102,25 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t* values, int n, i
   return t == 0 ? 0 : max(t, ordered<T>(-INFINITY));   // (the lower bits left out: below minus infinity there are only NaNs)
 }
 
-// The keys of a row's entries above tau (with `everything`: of all) and of the first k equal to it, in the order of their indices: for rows with
-// NaN (above everything) and with many entries equal to tau.  Returns how many there are (those beyond the room are not kept).  One warp.
+// Keys of a row's entries in the order of their indices, from `found` on; returns how many there are then (those beyond the room are
+// not kept).  Of rows with NaN (above everything): those above tau (with tau 0: all) and the first k equal to it.  Of others
+// (`ties`) the first k equal to tau alone, and no further than that.  One warp.
 template <typename T>
-__device__ __noinline__ int keys_in_order(const Words<T>& x, int V, uint32_t tau_bits, int k, uint64_t* keys, int lane) {
+__device__ __noinline__ int keys_in_order(const Words<T>& x, int V, uint32_t tau_bits, int k, bool ties, uint64_t* keys, int found, int lane) {
   const bool everything = tau_bits == 0;
   const float tau = from_ordered<T>(tau_bits);
-  int found = 0, equal = 0;   // keys, and of entries that are equal to tau the number met
-  for (int j0 = 0; j0 < x.n; j0 += 32) {
+  int equal = 0;   // entries equal to tau that were met
+  for (int j0 = 0; j0 < x.n && !(ties && equal >= k); j0 += 32) {
     const int j = j0 + lane, at = x.first + j * Words<T>::EPW;
     uint4 q = make_uint4(0u, 0u, 0u, 0u);
     if (j < x.n) q = x.at[j];
     const T* w = reinterpret_cast<const T*>(&q);
+    auto above = [&](float v) { return !ties && (everything || !(v <= tau)); };
     uint32_t n = 0;   // above tau, and in the upper half equal to it
 #pragma unroll
     for (int e = 0; e < Words<T>::EPW; ++e) {
       const float v = Io<T>::ld(w, e);
-      if (j < x.n && at + e >= 0 && at + e < V) n += everything || !(v <= tau) ? 1u : v == tau ? 0x10000u : 0u;
+      if (j < x.n && at + e >= 0 && at + e < V) n += above(v) ? 1u : v == tau ? 0x10000u : 0u;
     }
     if (!__any_sync(0xffffffffu, n != 0)) continue;
     uint32_t before = n;
@@ -135,8 +137,7 @@ __device__ __noinline__ int keys_in_order(const Words<T>& x, int V, uint32_t tau
       for (int e = 0; e < Words<T>::EPW; ++e) {
         const float v = Io<T>::ld(w, e);
         if (at + e < 0 || at + e >= V) continue;
-        const bool above = everything || !(v <= tau);
-        if (!above && (v != tau || eq++ >= k)) continue;
+        if (!above(v) && (v != tau || eq++ >= k)) continue;
         if (to < kRoom) keys[to] = entry_key(v, at + e);
         ++to;
       }
@@ -195,32 +196,33 @@ __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logpr
   const uint32_t tau = bound;
   const float m = stats[0], log_s = stats[1], least = from_ordered<T>(tau);
   if (tid == NT - 1) row_results<T>(a, r, Sums{m, stats[2], stats[3]}, log_s);
-  const bool usable = tau != 0 && stats[2] == stats[2];   // entries that reach tau may be looked for (no NaN among them)
-  auto look = [&](const uint4& q, int j) {
+  // The entries that reach tau, of the groups (or threads) whose largest does; `strictly`: that are above it.
+  auto look = [&](const uint4& q, int j, bool strictly) {
     if (!(max_of_word<T>(largest_of<T>(q)) >= least)) return;
 #pragma unroll
     for (int e = 0; e < Words<T>::EPW; ++e) {
       const float2 p = unpack2(pair_of<T>(q, e / 2));
       const float v = e & 1 ? p.y : p.x;
       const int at = x.first + j * Words<T>::EPW + e;
-      if (v >= least && at >= 0 && at < a.V) {
+      if ((strictly ? v > least : v >= least) && at >= 0 && at < a.V) {
         const int to = atomicAdd(&found, 1);
         if (to < kRoom) keys[to] = entry_key(v, at);
       }
     }
   };
-  if (usable && by_groups) {
-    if (max(most, odd) >= tau)
-      for (int g = tid; g < groups; g += NT)
-        if (of_groups[g] >= tau) {
-          const int to = atomicAdd(&n_list, 1);
-          if (to < kRoom) list[to] = (uint16_t)g;
-        }
-    __syncthreads();
-    const int n = n_list;
-    if (n > kRoom) {
-      if (tid == 0) found = kRoom + 1;   // as many groups equal to tau: in order
-    } else {
+  auto collect = [&](bool strictly) {   // returns how many there are, more than the room where they are not all kept
+    if (by_groups) {
+      auto reaches = [&](uint32_t most) { return strictly ? most > tau : most >= tau; };
+      if (reaches(max(most, odd)))
+        for (int g = tid; g < groups; g += NT)
+          if (reaches(of_groups[g])) {
+            const int to = atomicAdd(&n_list, 1);
+            if (to < kRoom) list[to] = (uint16_t)g;
+          }
+      __syncthreads();
+      const int n = n_list;
+      // (many more groups than entries are wanted: most of them no more than equal to tau)
+      if (n > (strictly ? kRoom : 128 + 4 * k)) return kRoom + 1;
       constexpr int U = 4;   // words of a thread on their way at once
       for (int i = tid; i < n * spans.w; i += U * NT) {
         uint4 q[U];
@@ -233,22 +235,37 @@ __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logpr
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (j[u] < x.n) look(q[u], j[u]);
+          if (j[u] < x.n) look(q[u], j[u], strictly);
       }
+    } else if (most >= tau) {
+      for (int j = tid; j < x.n; j += NT) look(x.at[j], j, strictly);
     }
-  } else if (usable) {
-    if (most >= tau)
-      for (int j = tid; j < x.n; j += NT) look(x.at[j], j);
-  } else if (tid == 0) {
-    found = kRoom + 1;
-  }
-  __syncthreads();
-  int n = found;
-  __syncthreads();
-  if (n > kRoom) {
+    __syncthreads();
+    return found;
+  };
+  const bool numbers = stats[2] == stats[2];   // no NaN (nor infinity) in the row
+  int n = kRoom + 1;
+  if (tau != 0 && numbers) {
+    n = collect(false);
+    if (n > kRoom) {   // masked rows and the like: those above tau, then of those equal to it the first
+      __syncthreads();
+      if (tid == 0) n_list = found = 0;
+      __syncthreads();
+      n = collect(true);
+    }
+    __syncthreads();
+    if (n < k) {
+      if (warp == 0) {
+        const int more = keys_in_order<T>(x, a.V, tau, k - n, true, keys, n, lane);
+        if (lane == 0) found = more;
+      }
+      __syncthreads();
+      n = found;
+    }
+  } else {
     if (warp == 0) {
-      n = keys_in_order<T>(x, a.V, tau, k, keys, lane);
-      if (lane == 0) found = n;
+      const int more = keys_in_order<T>(x, a.V, tau, k, false, keys, 0, lane);
+      if (lane == 0) found = more;
     }
     __syncthreads();
     n = found;
