@@ -6,8 +6,10 @@
 // registers.  The next rows are on their way while the present ones are worked on.  What a row's threads have to agree on takes one
 // barrier, forward as well: a warp's mean and the squares about it are joined to the row's, which loses nothing.  Each CTA of the
 // backward pass leaves one partial row of dw and db, which a second kernel adds in a fixed order.
-// What held the first forms back was instructions, not bytes: conversions one by one and scalar arithmetic came to 24 instructions an
-// element; by pairs it is about 8.
+// What held the first forms back was instructions, not bytes: 24 an element with conversions one by one, scalar arithmetic, divisions
+// and parameters converted row after row.
+// Measured: 65536 x 4096 bf16 forward 180 us (164 at copy rate), backward 295 (246); 16384 x 2048 with a residual 50 (41) forward;
+// 65536 x 1024 fp32 with a residual backward 170 (164); 32768 x 1001 bf16, two bytes at a time, 56 and 76 (20 and 30).
 #include "gdn_common.cuh"
 #include "rowio.cuh"
 
@@ -92,6 +94,8 @@ __device__ __forceinline__ void load_params(const void* p, int dtype, int d, flo
 
 constexpr int threads_of(int tpr) { return tpr > 32 ? tpr : 128; }   // rows of several warps have a CTA to themselves
 // forward, an SM's: by the registers of the rows on their way (NV pieces, with a residual twice that) and at work
+// (with a residual there is more to move for the same arithmetic: the cache does: 16384 rows of 8192, 169 us, 192 with shared memory)
+constexpr bool shares_params(int nv, int n, bool res) { return !res && n >= 4 && nv * n > 8 && nv <= 4; }
 constexpr int fwd_ctas(int tpr, int nv, bool res) {
   return tpr > 32 ? 512 / threads_of(tpr) : nv >= 16 ? (res ? 2 : 3) : nv == 8 ? (res ? 3 : 4) : nv == 4 ? (res ? 5 : 6) : 8;
 }
@@ -130,11 +134,14 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
   __shared__ float scratch[2][2 * R * NW];
   const int sub = threadIdx.x % TPR, group = threadIdx.x / TPR, lane = threadIdx.x & 31;
   const float inv = 1.f / a.D, root = sqrtf(inv);
-  // weight and bias stay in registers where a thread has few columns, else they come from the first-level cache row by row
-  constexpr bool HELD = NV * N <= (N <= 2 ? 16 : 8), LARGE = R * NV * N > 16;   // large: widened anew at each step; kept wide the rows would not fit the registers
+  // Weight and bias as fp32 pairs: in registers where a thread has few columns, else in shared memory, where row after row finds them
+  // without conversions (and without a bank conflict: 16 bytes a thread side by side); of very wide rows from the first-level cache.
   constexpr int P = pairs(N);
+  constexpr bool HELD = NV * N <= (N <= 2 ? 16 : 8), SHARED = shares_params(NV, N, RES);
+  constexpr bool LARGE = R * NV * N > 16;   // widened anew at each step; kept wide the rows would not fit the registers
+  extern __shared__ __align__(16) ulonglong2 shared_params[];   // [2][P / 2][TPR NV]
   uint64_t w[HELD ? NV : 1][P], b[HELD ? NV : 1][P];
-  if constexpr (HELD)
+  if constexpr (HELD) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int d = (v * TPR + sub) * N;
@@ -145,6 +152,18 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
         load_params<N>(a.bias, a.param_dtype, d, 0.f, b[v]);
       }
     }
+  } else if constexpr (SHARED) {
+    for (int q = threadIdx.x; q * N < a.D; q += threads_of(TPR)) {
+      load_params<N>(a.weight, a.param_dtype, q * N, 1.f, w[0]);
+      load_params<N>(a.bias, a.param_dtype, q * N, 0.f, b[0]);
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        shared_params[i * TPR * NV + q] = make_ulonglong2(w[0][2 * i], w[0][2 * i + 1]);
+        shared_params[(P / 2 + i) * TPR * NV + q] = make_ulonglong2(b[0][2 * i], b[0][2 * i + 1]);
+      }
+    }
+    __syncthreads();
+  }
   // elements that a warp holds of a row (for lane l: of warp l modulo NW)
   float held = a.D;
   if constexpr (TPR > 32) {
@@ -153,7 +172,7 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
     for (int v = 0; v < NV; ++v) n += min(max(a.D - (v * TPR + (lane & (NW - 1)) * 32) * N, 0), 32 * N);
     held = n;
   }
-  const float held_here = TPR > 32 ? __shfl_sync(0xffffffffu, held, threadIdx.x >> 5) : held;
+  const float per_held = held > 0.f ? 1.f / held : 0.f, per_held_here = TPR > 32 ? __shfl_sync(0xffffffffu, per_held, threadIdx.x >> 5) : per_held;
   Vec<T, N> x[R][NV], res[RES ? R : 1][NV];
   auto fetch = [&](int64_t r0) {
 #pragma unroll
@@ -201,7 +220,7 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
     shuffle_sums<(TPR < 32 ? TPR : 32)>(s);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float mean = held_here > 0.f ? s[r] / held_here : 0.f;
+      const float mean = s[r] * per_held_here;
       const uint64_t by = spread<N>(root), off = spread<N>(-mean * root);
       uint64_t sum = 0ull;
 #pragma unroll
@@ -230,7 +249,7 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
       for (int r = 0; r < R; ++r) {
         s[r] = scratch[turn][2 * r * NW + (lane & (NW - 1))];
         q[r] = scratch[turn][(2 * r + 1) * NW + (lane & (NW - 1))];
-        of[r] = held > 0.f ? s[r] / held : 0.f;
+        of[r] = s[r] * per_held;
       }
       shuffle_sums<NW>(s);
 #pragma unroll
@@ -244,7 +263,7 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
     for (int r = 0; r < R; ++r) {
       const int64_t row = now + r * RPC + group;
       if (row >= a.rows) continue;
-      const float mean = s[r] * inv, rstd = 1.f / sqrtf(q[r] + a.eps);
+      const float mean = s[r] * inv, rstd = __frsqrt_rn(q[r] + a.eps);
       const uint64_t by = spread<N>(rstd), off = spread<N>(-mean * rstd);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
@@ -252,7 +271,14 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
         if (d >= a.D) continue;
         if (RES && a.z) z[r][v].store(a.z, row * a.D + d);
         if (LARGE) z[r][v].again();
-        if constexpr (!HELD) {
+        if constexpr (SHARED) {
+#pragma unroll
+          for (int i = 0; i < P / 2; ++i) {
+            const ulonglong2 p = shared_params[i * TPR * NV + v * TPR + sub], q = shared_params[(P / 2 + i) * TPR * NV + v * TPR + sub];
+            w[0][2 * i] = p.x, w[0][2 * i + 1] = p.y;
+            b[0][2 * i] = q.x, b[0][2 * i + 1] = q.y;
+          }
+        } else if constexpr (!HELD) {
           load_params<N>(a.weight, a.param_dtype, d, 1.f, w[0]);
           load_params<N>(a.bias, a.param_dtype, d, 0.f, b[0]);
         }
@@ -501,9 +527,15 @@ int grid_of(int64_t rows, int each, int per_sm) {   // CTAs that take `each` row
 template <typename T, int N, int TPR, int NV>
 int launch_fwd(const b200gdn_layer_norm_args& a, cudaStream_t st) {
   const int n = grid_of(a.rows, threads_of(TPR) / TPR * rows_at_once(NV, N), fwd_ctas(TPR, NV, a.residual != nullptr));
-  if (a.residual) layer_norm_fwd_kernel<T, N, TPR, NV, true><<<n, threads_of(TPR), 0, st>>>(a);
-  else layer_norm_fwd_kernel<T, N, TPR, NV, false><<<n, threads_of(TPR), 0, st>>>(a);
-  return check_launch("layer_norm_fwd");
+  auto go = [&](auto kern, bool shared) {
+    const size_t smem = shared ? 2 * sizeof(float) * TPR * NV * N : 0;
+    if (smem > 48 * 1024)
+      if (int e = ensure_smem(kern, smem)) return e;
+    kern<<<n, threads_of(TPR), smem, st>>>(a);
+    return check_launch("layer_norm_fwd");
+  };
+  return a.residual ? go(layer_norm_fwd_kernel<T, N, TPR, NV, true>, shares_params(NV, N, true))
+                    : go(layer_norm_fwd_kernel<T, N, TPR, NV, false>, shares_params(NV, N, false));
 }
 template <typename T, int N, int TPR, int NV>
 int launch_bwd(const b200gdn_layer_norm_args& a, cudaStream_t st) {
@@ -529,8 +561,8 @@ int launch_wide(const b200gdn_layer_norm_args& a, cudaStream_t st, bool bwd) {
   return reduce_partials(a, n, st);
 }
 
-// Pieces of a row, of 16 bytes.  Forward four a thread, from 2048 16-bit elements on by several warps (65536 rows of 4096: 217 us with four
-// pieces a thread, 232 with two, 226 with one, 318 with sixteen, a warp a row).  Backward, beside the sums: one a thread as far
+// Pieces of a row, of 16 bytes.  Forward four a thread, from 2048 16-bit elements on by several warps (65536 rows of 4096, with parameters from
+// the cache: 217 us with four pieces a thread, 232 with two, 226 with one, 318 with sixteen, a warp a row; from shared memory 180).  Backward, beside the sums: one a thread as far
 // as 512 go.  Smaller pieces (odd widths): up to eight a thread first (8191 rows of 1003 fp32, forward: 17 us with eight, 29 with four).
 template <typename T, int N>
 int launch_n(const b200gdn_layer_norm_args& a, cudaStream_t st, bool bwd) {
