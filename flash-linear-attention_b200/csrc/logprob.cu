@@ -150,7 +150,8 @@ __device__ __noinline__ int keys_in_order(const Words<T>& x, int V, uint32_t tau
 // with top entries: a CTA a row
 template <typename T>
 __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logprob_args a, const Spans spans, const float4* part, const void* largest) {
-  __shared__ uint64_t keys[kRoom], ks[NT / 32];
+  __shared__ __align__(16) uint64_t keys[kRoom];
+  __shared__ uint64_t ks[NT / 32];
   __shared__ uint32_t own[2 * NT], bound;
   __shared__ uint16_t list[kRoom];
   __shared__ float stats[4];
@@ -224,13 +225,14 @@ __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logpr
       // (many more groups than entries are wanted: most of them no more than equal to tau)
       if (n > (strictly ? kRoom : 128 + 4 * k)) return kRoom + 1;
       constexpr int U = 4;   // words of a thread on their way at once
-      for (int i = tid; i < n * spans.w; i += U * NT) {
+      const int shift = spans.shift();
+      for (int i = tid; i < n << shift; i += U * NT) {
         uint4 q[U];
         int j[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int at = i + u * NT, g = at < n * spans.w ? list[at / spans.w] : 0;
-          j[u] = at < n * spans.w ? g / 32 * 32 * spans.w + at % spans.w * 32 + g % 32 : x.n;
+          const int at = i + u * NT, g = at < n << shift ? list[at >> shift] : 0;
+          j[u] = at < n << shift ? (((g >> 5) << shift) + (at & ((1 << shift) - 1))) * 32 + (g & 31) : x.n;
           q[u] = j[u] < x.n ? x.at[j[u]] : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
@@ -287,11 +289,17 @@ __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logpr
     }
     return;
   }
+  if (tid == 0 && n % 2 != 0 && n < kRoom) keys[n] = 0;   // (below every entry's)
+  __syncthreads();
+  const ulonglong2* two = reinterpret_cast<const ulonglong2*>(keys);
   for (int i = tid; i < n; i += NT) {
     const uint64_t key = keys[i];
     int larger = 0;
 #pragma unroll 4
-    for (int o = 0; o < n; ++o) larger += keys[o] > key;
+    for (int o = 0; o < (n + 1) / 2; ++o) {
+      const ulonglong2 p = two[o];
+      larger += (p.x > key) + (p.y > key);
+    }
     if (larger < k) result(larger, key);
   }
 }

@@ -211,7 +211,8 @@ constexpr int kSpanWarps = 4;
 // How rows are cut: `w` words a lane, for as many words of 16 bytes as a row has at most (off a word's boundary it has one more).  By the
 // width alone: a row's results are the same bits whatever rows it comes with.
 struct Spans {
-  int w, per_row;
+  int w, per_row;   // w: a power of two
+  __device__ __forceinline__ int shift() const { return 31 - __clz(w); }
   __host__ __device__ int groups() const { return 32 * per_row; }
 };
 inline Spans spans_of(int V, int size) {

@@ -107,6 +107,25 @@ def test_top_entries_in_any_order(kind, V, dtype):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('k', [1, 20, 128])
+def test_top_entries_that_lie_together(k, dtype):
+    """Thousands of entries above all others, at the places that few lanes of the kernels hold; few entries that are not masked."""
+    from b200gdn import token_logprobs
+    V = 131072
+    at = torch.arange(V, device='cuda')
+    x = torch.randn(4, V, device='cuda', generator=gen())
+    x[:, at // (4 if dtype == torch.float32 else 8) % 32 < 2] += 20
+    x[1] = torch.where(torch.rand(V, device='cuda', generator=gen(1)) < 1e-4, x[1], -math.inf)
+    x[2] = torch.where(at < 3, x[2], torch.finfo(dtype).min)
+    x[3] = torch.where(at >= V - 300, 2.0, -math.inf)
+    check_logprobs(x.to(dtype), tokens_of(4, V), k, upstream=False)
+    for temperature in (1e-4, 3e4):
+        r, want = token_logprobs(x.to(dtype), top_k=k, temperature=temperature), H.logprobs(x.to(dtype), tokens_of(4, V), k, temperature)
+        assert torch.equal(r.top_ids, want['top_ids'])
+        close_lp('entropy', r.entropy, want['entropy'])
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('V', [40, 1003, 33000])
 def test_masked_entries(V, dtype):
     """Minus infinity and the type's lowest value in masked places, rows with little or nothing left, a token that is masked."""
