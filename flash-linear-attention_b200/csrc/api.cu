@@ -346,6 +346,7 @@ static int check_layer_norm_args(const b200gdn_layer_norm_args* a, const char* w
                      sizeof(b200gdn_layer_norm_args));
   if (a->rows <= 0 || a->D <= 0) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: empty problem (rows=%lld D=%d)", who, (long long)a->rows, a->D);
   if (a->rows > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows", who);
+  if (a->D > (1 << 23)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: D=%d (at most 2^23)", who, a->D);
   if (a->dtype < 0 || a->dtype > 2 || a->param_dtype < 0 || a->param_dtype > 2)
     return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: dtype codes %d, %d", who, a->dtype, a->param_dtype);
   if (!bwd) {

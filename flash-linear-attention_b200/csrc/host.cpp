@@ -1361,6 +1361,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     NoGil nogil;
     if (act_code(x.scalar_type()) < 0) raise(std::string("layer_norm: dtype ") + c10::toString(x.scalar_type()) + " is not supported");
     if (x.dim() == 0 || x.size(-1) == 0) raise("layer_norm: rows without elements");
+    if (x.size(-1) > (1 << 23)) raise("layer_norm: rows of more than 2^23 elements");
     for (const Tensor* p : {&w, &b})
       if (p->defined() && (p->dim() != 1 || p->size(0) != x.size(-1) || !p->is_floating_point()))
         raise("layer_norm: weight and bias are vectors of the " + std::to_string(x.size(-1)) + " elements of a row");
@@ -1386,6 +1387,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 void check_logits(const char* who, const Tensor& logits) {
   if (act_code(logits.scalar_type()) < 0) raise(std::string(who) + ": dtype " + c10::toString(logits.scalar_type()) + " is not supported");
   if (logits.dim() == 0 || logits.size(-1) == 0) raise(std::string(who) + ": a vocabulary without entries");
+  if (logits.size(-1) > (1 << 30)) raise(std::string(who) + ": more than 2^30 entries a row");
 }
 void check_indices(const char* who, const char* what, const Tensor& x, at::IntArrayRef sizes, const at::Device& dev) {
   if (x.scalar_type() != at::kLong && x.scalar_type() != at::kInt) raise(std::string(who) + ": " + what + " are int32 or int64");

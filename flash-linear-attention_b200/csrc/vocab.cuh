@@ -25,11 +25,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ float exponent(float x, float m, float c) { return (x - (m == -INFINITY ? 0.f : m)) * c; }
 
 // an index as int32 or int64; whatever lies outside [0, V) is -1
-__device__ __forceinline__ int64_t raw_index(const void* p, int64_t i, int bytes) {
-  return bytes == 8 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
-}
 __device__ __forceinline__ int load_index(const void* p, int64_t i, int bytes, int V) {
-  const int64_t v = raw_index(p, i, bytes);
+  const int64_t v = bytes == 8 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
   return v >= 0 && v < V ? (int)v : -1;
 }
 
@@ -52,7 +49,6 @@ struct SumOf {
   template <typename T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
 };
 struct MaxOf {
-  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
   __device__ __forceinline__ uint64_t operator()(uint64_t a, uint64_t b) const { return a > b ? a : b; }
 };
 // the whole CTA's value, to every thread; `scratch` has a place for each warp and is free again on return
@@ -128,6 +124,7 @@ __device__ __forceinline__ uint64_t pair_of(const uint4& w, int i) {
   else return pack2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
 }
 
+// the largest entries of a 16-byte word, as max_words leaves them
 template <typename T>
 __device__ __forceinline__ uint32_t largest_of(const uint4& w) {
   if constexpr (sizeof(T) == 4) {
@@ -203,7 +200,6 @@ struct PieceSums {
     }
   }
 };
-
 
 // ---- spans -------------------------------------------------------------------------------------------------------------
 constexpr int kSpanWarps = 4;

@@ -64,6 +64,12 @@ def test_forward_and_backward(D, dtype):
                 assert torch.equal(layer_norm(x, w, b, residual=res), out[0])
 
 
+@pytest.mark.parametrize('dtype,D', [(torch.bfloat16, 40000), (torch.bfloat16, 10002), (torch.float32, 20000), (torch.float32, 9001)])
+def test_wide_rows(D, dtype):
+    """Wider than the registers of a CTA, forward or backward."""
+    test_forward_and_backward(D, dtype)
+
+
 def test_gradient_of_differences():
     """In fp32, along a direction: (f(x + h d) - f(x - h d)) / 2h.  With h = 2^-6 the third derivative leaves about h^2 / 6 of the
     value's own size (4e-5 of it; y is smooth on the scale of a row's spread), rounding 2^-24 / h x sqrt(terms): 1e-3 in all."""

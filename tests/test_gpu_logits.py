@@ -205,6 +205,16 @@ def test_logprobs_options():
         assert empty.logprobs.shape == (0,) and empty.top_ids.shape == (0, 2)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_long_rows(dtype):
+    """Rows of millions of entries: more spans than a warp joins in one go, more groups than the top entries are sought by."""
+    V = 4_500_001
+    x = logits_of(2, V, dtype)
+    check_logprobs(x, torch.tensor([V - 1, 7], device='cuda'), 20)
+    t, ids = lists_of(2, V, 16, absent=False)
+    check_distill(x, t, ids, 1.0, True, ('sum',))
+
+
 def test_logprobs_past_32_bits():
     """Offsets of more than 2^31 elements; the rows at the end are the same as alone."""
     from b200gdn import token_logprobs

@@ -42,6 +42,7 @@ def test_bad_arguments_of_layer_norm():
         refused(fn, _lib.LayerNormArgs(), -1, 'empty problem')
         refused(fn, _lib.LayerNormArgs(rows=1 << 31, D=8), -2, 'rows')
         refused(fn, _lib.LayerNormArgs(rows=4, D=8, dtype=3), -1, 'dtype')
+        refused(fn, _lib.LayerNormArgs(rows=4, D=(1 << 23) + 1), -2, 'D=')
     refused('b200gdn_layer_norm_fwd', _lib.LayerNormArgs(rows=4, D=8), -1, 'a->x is NULL')
     refused('b200gdn_layer_norm_fwd', _lib.LayerNormArgs(rows=4, D=8, x=256, y=256, mean=256), -1, 'come together')
     refused('b200gdn_layer_norm_bwd', _lib.LayerNormArgs(rows=4, D=8, z=256, mean=256, rstd=256, dy=256, dx=256, dweight=256), -1, 'partials is NULL')
@@ -84,9 +85,12 @@ def test_bad_arguments_of_logprob_and_distill():
         refused('b200gdn_distill_fwd', _lib.DistillArgs(K=k, **rows), -2, 'entries a row')
     refused('b200gdn_distill_fwd', _lib.DistillArgs(K=3, id_bytes=1, **rows), -1, 'id_bytes')
     refused('b200gdn_distill_fwd', _lib.DistillArgs(K=3, id_bytes=8, teacher_dtype=7, **rows), -1, 'teacher_dtype')
+    refused('b200gdn_logprob_fwd', _lib.LogprobArgs(**rows), -1, 'workspace is NULL')
     lists = dict(K=3, id_bytes=8, teacher=256, ids=256, **rows)
     refused('b200gdn_distill_fwd', _lib.DistillArgs(**lists), -1, 'row_loss is NULL')
     refused('b200gdn_distill_fwd', _lib.DistillArgs(row_loss=256, **lists), -1, 'workspace is NULL')
+    for fn, flags in (('b200gdn_distill_fwd', _lib.DISTILL_SKIP_ONE | _lib.DISTILL_SCALAR), ('b200gdn_distill_bwd', _lib.DISTILL_SKIP_ONE)):
+        refused(fn, _lib.DistillArgs(row_loss=256, workspace=256, dloss=256, dlogits=256, flags=flags, **lists), -1, 'SKIP_ONE')
     refused('b200gdn_distill_bwd', _lib.DistillArgs(row_loss=256, workspace=256, **lists), -1, 'dloss is NULL')
     lib = _lib.load()
     assert lib.b200gdn_distill_workspace_bytes(4, 1000, 0, 8) > lib.b200gdn_distill_workspace_bytes(2, 1000, 0, 8) > 0
