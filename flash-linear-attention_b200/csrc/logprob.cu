@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(32 * kSpanWarps) logprob_spans_kernel(const b2
 
 // ---- joining a row's spans ---------------------------------------------------------------------------------------------
 constexpr int NT = 128, kRoom = 1024;   // threads of a row with top entries; keys of entries that may be among them
-static_assert(kRoom >= 2 * B200GDN_MAX_TOP, "entries above tau and as many equal to it as are wanted");
+constexpr int kBounds = 4 * NT;         // values that tau is the k-th largest of, at most
+static_assert(kBounds >= 4 * B200GDN_MAX_TOP && kBounds < 1 << 10 && kRoom >= 2 * B200GDN_MAX_TOP, "entries above tau and as many equal to it as are wanted");
 
 // one thread
 template <typename T>
@@ -81,20 +82,20 @@ __global__ void __launch_bounds__(NT) logprob_join_kernel(const b200gdn_logprob_
   if (lane == 0) row_results<T>(a, r, v, log2f(v.s));
 }
 
-// The k-th largest of n <= 2 NT values (0 where fewer than k are there), two bits at a time from the highest down; of 32 bits the upper 22,
+// The k-th largest of n <= kBounds values (0 where fewer than k are there), two bits at a time from the highest down; of 32 bits the upper 22,
 // which bounds it from below as well as tau needs.  One warp.
 template <typename T>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t* values, int n, int k, int lane) {
-  uint32_t v[2 * NT / 32];
+  uint32_t v[kBounds / 32];
 #pragma unroll
-  for (int i = 0; i < 2 * NT / 32; ++i) v[i] = i * 32 + lane < n ? values[i * 32 + lane] : 0u;
+  for (int i = 0; i < kBounds / 32; ++i) v[i] = i * 32 + lane < n ? values[i * 32 + lane] : 0u;
   uint32_t t = 0;
 #pragma unroll 1
   for (int bit = sizeof(T) == 2 ? 14 : 30; bit >= (sizeof(T) == 2 ? 0 : 10); bit -= 2) {
     const uint32_t n1 = t | 1u << bit, n2 = t | 2u << bit, n3 = t | 3u << bit;
-    uint32_t c = 0;   // three counts of up to 2 NT in one sum
+    uint32_t c = 0;   // three counts in one sum
 #pragma unroll
-    for (int i = 0; i < 2 * NT / 32; ++i)
+    for (int i = 0; i < kBounds / 32; ++i)
       if (i * 32 < n) c += (v[i] >= n1 ? 1u : 0u) + (v[i] >= n2 ? 1u << 10 : 0u) + (v[i] >= n3 ? 1u << 20 : 0u);
     c = __reduce_add_sync(0xffffffffu, c);
     t = (c >> 20) >= (uint32_t)k ? n3 : (c >> 10 & 0x3ffu) >= (uint32_t)k ? n2 : (c & 0x3ffu) >= (uint32_t)k ? n1 : t;
@@ -152,36 +153,39 @@ template <typename T>
 __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logprob_args a, const Spans spans, const float4* part, const void* largest) {
   __shared__ __align__(16) uint64_t keys[kRoom];
   __shared__ uint64_t ks[NT / 32];
-  __shared__ uint32_t own[2 * NT], bound;
+  __shared__ uint32_t own[kBounds], bound;
   __shared__ uint16_t list[kRoom];
   __shared__ float stats[4];
   __shared__ int n_list, found;
   wait_for_predecessor();
-  const int64_t r = blockIdx.x;
+  const int64_t r = a.rows - 1 - blockIdx.x;   // the last rows are still in the second-level cache
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.top_k, groups = spans.groups();
   const Words<T> x(static_cast<const T*>(a.logits) + row_offset(a, r), a.V);
   const Order<T>* of_groups = static_cast<const Order<T>*>(largest) + r * groups;
-  // tau from as many values as threads, or twice that: the largest of the groups i NT + tid.  With few groups tau would be low, and the
-  // row is gone through again: the largest entry of each thread's words.
-  const bool by_groups = 2 * groups >= 3 * k && groups <= 65536, twice = by_groups && 2 * k > NT;
-  uint32_t most = 0, odd = 0;
+  // tau from at least four values for each entry that is wanted (of 2 k it would be exceeded by 1.4 k entries, of 4 k by 1.15 k): the
+  // largest of the groups i NT + tid, in one, two or four parts.  With few groups tau would be low, and the row is gone through again:
+  // the largest entry of each thread's words.
+  const bool by_groups = 2 * groups >= 3 * k && groups <= 65536;
+  const int parts = !by_groups || k <= NT / 4 ? 1 : k <= NT / 2 ? 2 : 4;
+  uint32_t most[4] = {0, 0, 0, 0};
   if (by_groups) {
-#pragma unroll 4
-    for (int i = tid; i < groups; i += 2 * NT) {
-      most = max(most, (uint32_t)of_groups[i]);
-      if (i + NT < groups) odd = max(odd, (uint32_t)of_groups[i + NT]);
-    }
-    if (!twice) most = max(most, odd);
+#pragma unroll 2
+    for (int i = tid; i < groups; i += 4 * NT)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e * NT < groups) most[e] = max(most[e], (uint32_t)of_groups[i + e * NT]);
   } else {
     float m = -INFINITY;
     for (int j = tid; j < x.n; j += NT) m = fmaxf(m, max_of_word<T>(largest_of<T>(x.edge(j, a.V))));
-    most = tid < x.n ? ordered<T>(m) : 0u;
+    most[0] = tid < x.n ? ordered<T>(m) : 0u;
   }
-  own[tid] = most;
-  own[NT + tid] = odd;
+  const uint32_t even = max(most[0], most[2]), odd = max(most[1], most[3]), mine = max(even, odd);
+  own[tid] = parts == 1 ? mine : parts == 2 ? even : most[0];
+  if (parts > 1) own[NT + tid] = parts == 2 ? odd : most[1];
+  if (parts > 2) own[2 * NT + tid] = most[2], own[3 * NT + tid] = most[3];
   __syncthreads();
   if (warp == 0) {
-    const uint32_t t = kth_largest<T>(own, twice ? 2 * NT : NT, k, lane);
+    const uint32_t t = kth_largest<T>(own, parts * NT, k, lane);
     if (lane == 0) bound = t;
   } else if (warp == 1) {
     const Sums v = joined_spans(part + r * spans.per_row, spans.per_row, a.scale * kLog2e, lane);
@@ -200,21 +204,24 @@ __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logpr
   // The entries that reach tau, of the groups (or threads) whose largest does; `strictly`: that are above it.
   auto look = [&](const uint4& q, int j, bool strictly) {
     if (!(max_of_word<T>(largest_of<T>(q)) >= least)) return;
+    unsigned hits = 0;   // seldom more than one
 #pragma unroll
-    for (int e = 0; e < Words<T>::EPW; ++e) {
-      const float2 p = unpack2(pair_of<T>(q, e / 2));
-      const float v = e & 1 ? p.y : p.x;
-      const int at = x.first + j * Words<T>::EPW + e;
-      if ((strictly ? v > least : v >= least) && at >= 0 && at < a.V) {
-        const int to = atomicAdd(&found, 1);
-        if (to < kRoom) keys[to] = entry_key(v, at);
-      }
+    for (int e = 0; e < Words<T>::EPW / 2; ++e) {
+      const float2 p = unpack2(pair_of<T>(q, e));
+      hits |= ((strictly ? p.x > least : p.x >= least) ? 1u << (2 * e) : 0u) | ((strictly ? p.y > least : p.y >= least) ? 2u << (2 * e) : 0u);
+    }
+    while (hits != 0) {
+      const int e = __ffs(hits) - 1, at = x.first + j * Words<T>::EPW + e;
+      hits &= hits - 1;
+      if (at < 0 || at >= a.V) continue;
+      const int to = atomicAdd(&found, 1);
+      if (to < kRoom) keys[to] = entry_key(Io<T>::ld(x.at, (int64_t)j * Words<T>::EPW + e), at);
     }
   };
   auto collect = [&](bool strictly) {   // returns how many there are, more than the room where they are not all kept
     if (by_groups) {
-      auto reaches = [&](uint32_t most) { return strictly ? most > tau : most >= tau; };
-      if (reaches(max(most, odd)))
+      auto reaches = [&](uint32_t largest) { return strictly ? largest > tau : largest >= tau; };
+      if (reaches(mine))
         for (int g = tid; g < groups; g += NT)
           if (reaches(of_groups[g])) {
             const int to = atomicAdd(&n_list, 1);
@@ -239,7 +246,7 @@ __global__ void __launch_bounds__(NT, 12) logprob_top_kernel(const b200gdn_logpr
         for (int u = 0; u < U; ++u)
           if (j[u] < x.n) look(q[u], j[u], strictly);
       }
-    } else if (most >= tau) {
+    } else if (mine >= tau) {
       for (int j = tid; j < x.n; j += NT) look(x.at[j], j, strictly);
     }
     __syncthreads();
@@ -338,9 +345,10 @@ int launch_fwd(const b200gdn_logprob_args& a, cudaStream_t st) {
 template <typename T, int W>
 __global__ void __launch_bounds__(32 * kSpanWarps) logprob_bwd_kernel(const b200gdn_logprob_args a, const Spans spans) {
   const int lane = threadIdx.x & 31;
-  const int64_t task = (int64_t)blockIdx.x * kSpanWarps + (threadIdx.x >> 5), r = task / spans.per_row;
+  // from the last row to the first: behind the forward pass the last rows are still in the second-level cache
+  const int64_t task = a.rows * spans.per_row - 1 - ((int64_t)blockIdx.x * kSpanWarps + (threadIdx.x >> 5)), r = task / spans.per_row;
+  if (task < 0) return;
   const int span = (int)(task - r * spans.per_row);
-  if (r >= a.rows) return;
   const T* row = static_cast<const T*>(a.logits) + row_offset(a, r);
   T* out = static_cast<T*>(a.dlogits) + r * a.V;
   const float m = a.stats[2 * r], log_s = a.stats[2 * r + 1], c = a.scale * kLog2e;
