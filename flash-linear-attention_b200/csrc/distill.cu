@@ -25,8 +25,12 @@ struct RowList {
   float total, rest;   // sum q; what is left of one
   int counted;
 };
-struct RowSums {   // m, log2 of the sum; the factor of p in the gradient off the list and on it
-  float m, log_s, off, on;
+// Largest entry and log2 of the sum, of what the list leaves (renormalised: of the row; log_s -infinity: the gradient is zero) and of the
+// whole row.  The gradient is the softmax of what is off the list times `by` there, the softmax of the row times `by`, minus q, on it.
+struct __align__(16) RowSums {
+  struct __align__(16) Part {
+    float m, log_s, by, unused;
+  } off, row;
 };
 
 // The workspace of a call: kept from the forward pass for the backward pass.
@@ -36,7 +40,7 @@ struct Work {
   RowSums* sums;     // [rows]
   Entry* entries;    // [rows, K]
   float4* part;      // [rows, spans]
-  static int64_t bytes(int64_t rows, int K, int per_row) { return rows * (16 + 16 + 8 * (int64_t)K + 16 * (int64_t)per_row) + 16; }
+  static int64_t bytes(int64_t rows, int K, int per_row) { return rows * (16 + 32 + 8 * (int64_t)K + 16 * (int64_t)per_row) + 16; }
   Work(void* p, int64_t rows, int K, int per_row) {
     part = static_cast<float4*>(p);
     lists = reinterpret_cast<RowList*>(part + rows * per_row);
@@ -208,14 +212,19 @@ __device__ __forceinline__ void join_row(const b200gdn_distill_args& a, const Wo
     if (e.id >= 0 && e.q != 0.f) loss -= e.q * (exponent(Io<T>::ld(row, e.id), v.m, a.scale) - ln_s);
   }
   loss = warp_sum(loss) + list.constant;
-  RowSums s{v.m, log_s, list.total + list.rest, list.total + list.rest};
-  if (list.rest != 0.f) {
-    const float p_rest = moved(off, v.m, c).s;   // beside the row's largest entry
-    loss -= list.rest * (logf(p_rest) - ln_s);
-    s.off = p_rest == 0.f ? 0.f : s.off - list.rest * (v.s / p_rest);
+  // What is off the list keeps its own largest entry: its mass P = sum 2^((x - m) c) / s is zero in 32 bits from 87 / scale below the
+  // list on, its logarithm and its softmax w are not.  p_j Q - rest p_j / P = w_j (P Q - rest): nothing in it leaves fp32's range.
+  const float all = list.total + list.rest;
+  RowSums s{{off.m, 0.f, 0.f, 0.f}, {v.m, log_s, all, 0.f}};
+  if (off.s != 0.f) {   // something is
+    s.off.log_s = log2f(off.s);
+    s.off.by = moved(off, v.m, c).s / v.s * all - list.rest;
   }
-  if (!list.counted) loss = s.off = s.on = 0.f;
-  else if (v.s == 0.f) loss = INFINITY;
+  if (list.rest != 0.f) loss -= list.rest * (exponent(off.m, v.m, a.scale) + logf(off.s) - ln_s);
+  if (!list.counted || v.s == 0.f) {   // none of a teacher's, or no row
+    loss = list.counted ? INFINITY : 0.f;
+    s.off.log_s = -INFINITY;
+  }
   if (lane == 0) {
     a.row_loss[r] = loss;
     w.sums[r] = s;
@@ -228,23 +237,25 @@ __device__ __forceinline__ void gradient_span(const b200gdn_distill_args& a, con
                                               int lane) {
   const T* row = static_cast<const T*>(a.logits) + row_offset(a, r);
   T* out = static_cast<T*>(a.dlogits) + r * a.V;
-  const RowSums s = w.sums[r];
-  if (s.log_s == -INFINITY || (s.off == 0.f && s.on == 0.f)) {   // no row, or none of a teacher's
+  const RowSums::Part off = w.sums[r].off;
+  if (off.log_s == -INFINITY) {
     zero_span<T, W>(out, a.V, span, lane);
     return;
   }
-  const float c = a.scale * kLog2e, base = s.m == -INFINITY ? 0.f : s.m, by = s.off * weight;
-  const uint64_t m2 = pack2(-base, -base), c2 = pack2(c, c), s2 = pack2(-s.log_s, -s.log_s), by2 = pack2(by, by);
+  const float c = a.scale * kLog2e, off_base = off.m == -INFINITY ? 0.f : off.m, by = off.by * weight;
+  const uint64_t m2 = pack2(-off_base, -off_base), c2 = pack2(c, c), s2 = pack2(-off.log_s, -off.log_s), by2 = pack2(by, by);
   g.store(out, a.V, span, lane, [&](uint64_t x) {
     const float2 l = unpack2(add2(mul2(add2(x, m2), c2), s2));
     return mul2(pack2(exp2_approx(l.x), exp2_approx(l.y)), by2);
   });
   __syncwarp();
+  const RowSums::Part all = w.sums[r].row;
+  const float base = all.m == -INFINITY ? 0.f : all.m;
   for (int i = lane; i < a.K; i += 32) {
     const Entry e = w.entries[r * a.K + i];
     if (!in_span<T, W>(out, span, e.id)) continue;
-    const float p = exp2_approx((Io<T>::ld(row, e.id) - base) * c - s.log_s);
-    Io<T>::st(out, e.id, (p * s.on - e.q) * weight);
+    const float p = exp2_approx((Io<T>::ld(row, e.id) - base) * c - all.log_s);
+    Io<T>::st(out, e.id, (p * all.by - e.q) * weight);
   }
 }
 

@@ -454,6 +454,8 @@ int64_t b200gdn_logprob_workspace_bytes(int64_t rows, int32_t V, int32_t dtype, 
  *                                   loss = sum q_i (log q_i - lp_id_i) + q_t (log q_t - log p_t)
  * An entry with an id outside [0, V) or l = -infinity is absent; a row without entries is left out: loss 0, gradient 0, not counted.
  * A row with a teacher whose logits are all minus infinity has an infinite loss and gradient 0.
+ * With B200GDN_DISTILL_BUCKET a row with q_t > 0 and nothing above minus infinity off its list has an infinite loss too.  However far
+ * the list is above the rest, or below it, loss and gradient are finite otherwise.
  * The forward pass writes row_loss; `loss` (NULL: not wanted) is their sum, with B200GDN_DISTILL_MEAN over the number of rows
  * counted (at least 1).  With dlogits it writes the gradient of `loss` in the same pass.  The backward pass forms
  * dlogits for an upstream gradient: dloss [rows] of row_loss, or with B200GDN_DISTILL_SCALAR dloss [1] of `loss`; with

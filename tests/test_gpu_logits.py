@@ -479,3 +479,80 @@ def test_forward_mode_tangents_are_refused():
         for call in (lambda: token_logprobs(dual, tok), lambda: topk_distill_loss(dual, t, ids), lambda: layer_norm(dual)):
             with pytest.raises((NotImplementedError, RuntimeError), match='jvp'):
                 call()
+
+
+# ---- a list far above or below the rest of the vocabulary -----------------------------------------------------------
+def lists_with_a_rest(n, v, k):
+    """Lists that leave 1 to 50 per cent to the rest of the vocabulary."""
+    _, ids = lists_of(n, v, k, absent=False)
+    left = torch.linspace(0.01, 0.5, n, device='cuda')[:, None]
+    return torch.log_softmax(torch.randn(n, k, device='cuda', generator=gen(1)) * 2, -1) + torch.log1p(-left), ids
+
+
+def check_far(x, t, ids, temperature):
+    """The rest as an entry, in 64 bits and in logarithms, so that no distance between the list and the rest is too large:
+    with w the softmax of what is off the list and P its mass, the gradient there is w (P (total + rest) - rest).
+
+    Tolerances: the file's, and what the rest being one minus a sum in 32 bits adds: the sum is off by 2^-22 (its exponentials)
+    and a few 2^-24 (its additions), 2^-21 in all, times the derivative of the loss by it."""
+    from b200gdn import topk_distill_loss
+    lp = torch.log_softmax(x.double() / temperature, -1)
+    q = t.double().exp()
+    total, given = q.sum(-1, keepdim=True), lp.gather(1, ids)
+    rest = 1.0 - total
+    off = lp.scatter(1, ids, -math.inf)
+    log_rest, w = torch.logsumexp(off, -1, keepdim=True), torch.softmax(off, -1)
+    rows = (q * (t.double() - given)).sum(-1) + (rest * (rest.log() - log_rest))[:, 0]
+    size = (q * (t.double().abs() + given.abs())).sum(-1) + (rest * (rest.log().abs() + log_rest.abs() + 2.0))[:, 0]
+    limit = 2.0 ** -20 + 2.0 ** -22 * size + 2.0 ** -21 * (rest.log().abs() + log_rest.abs() + 1.0)[:, 0]
+    dx = (w * (log_rest.exp() * (total + rest) - rest)).scatter(1, ids, given.exp() * (total + rest) - q) / temperature
+    reach = (w * (log_rest.exp() * (total + rest) + rest + 1.0)).scatter(1, ids, given.exp() * (total + rest) + q) / temperature
+    options = dict(temperature=temperature, remainder='bucket')
+    leaf = x.detach().requires_grad_(True)
+    got = topk_distill_loss(leaf, t, ids, reduction='none', **options)
+    off_by = (got.detach().double() - rows).abs()
+    assert (off_by <= limit).all(), f'loss off by {off_by.tolist()}, allowed {limit.tolist()}'
+    up = torch.randn(got.shape, device='cuda', generator=gen(9))
+    close_grad('dlogits', torch.autograd.grad(got, leaf, up)[0], dx * up[:, None], reach * up[:, None].abs())
+    total_loss = topk_distill_loss(leaf, t, ids, reduction='mean', **options)
+    assert (total_loss.detach().double() - rows.mean()).abs() <= limit.mean() + 2.0 ** -22 * rows.abs().mean()
+    close_grad('dlogits', torch.autograd.grad(total_loss, leaf, retain_graph=True)[0], dx / len(rows), reach / len(rows))
+    close_grad('dlogits', torch.autograd.grad(0.5 * total_loss, leaf)[0], dx / (2 * len(rows)), reach / (2 * len(rows)))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('V,k', [(70, 16), (5003, 64), (33001, 256)])
+@pytest.mark.parametrize('temperature', [1.0, 0.1])
+def test_distill_bucket_with_the_rest_far_away(temperature, V, k, dtype):
+    """A student that puts next to nothing off the list, or on it: distances at which a mass beside the row's largest entry leaves
+    what fp32 holds, as they count after the temperature; some of the rest masked."""
+    gaps = [60.0, 75.0, 82.0, 84.0, 85.5, 86.0, 87.0, 88.0, 95.0, 103.0, 200.0, 700.0, 5000.0, -50.0, -86.0, -88.0, -104.0, -200.0, -5000.0]
+    n = len(gaps)
+    t, ids = lists_with_a_rest(n, V, k)
+    x = torch.randn(n, V, device='cuda', generator=gen(2))
+    x[torch.rand(n, V, device='cuda', generator=gen(3)) < 0.3] = -math.inf
+    x.scatter_(1, ids, torch.randn(n, k, device='cuda', generator=gen(4)) + torch.tensor(gaps, device='cuda')[:, None])
+    free = torch.ones(n, V, device='cuda').scatter_(1, ids, 0.0).argmax(-1, keepdim=True)
+    x.scatter_(1, free, 0.5)     # something is left off the list
+    check_far((x * temperature).to(dtype), t, ids, temperature)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_distill_bucket_with_one_entry_far_above_the_others(dtype):
+    """Off the list one entry, and the others so far below it that they are nothing beside it, not beside the list alone."""
+    n, V, k = 9, 3001, 64
+    t, ids = lists_with_a_rest(n, V, k)
+    x = torch.full((n, V), -200.0, device='cuda')
+    free = torch.ones(n, V, device='cuda').scatter_(1, ids, 0.0).argmax(-1, keepdim=True)
+    x.scatter_(1, free, -torch.tensor([80.0, 83.0, 84.0, 85.0, 86.0, 87.0, 88.0, 90.0, 120.0], device='cuda')[:, None])
+    x.scatter_(1, ids, 0.0)
+    check_far(x.to(dtype), t, ids, 1.0)
+
+
+def test_distill_bucket_with_the_rest_at_the_lowest_values():
+    """Masked with large finite numbers: a large loss, and the gradient of a uniform rest."""
+    n, V, k = 4, 2000, 32
+    t, ids = lists_with_a_rest(n, V, k)
+    x = torch.tensor([-1e4, -1e9, -1e20, -1e30], device='cuda')[:, None].expand(n, V).contiguous()
+    x.scatter_(1, ids, torch.randn(n, k, device='cuda', generator=gen(4)))
+    check_far(x, t, ids, 1.0)
