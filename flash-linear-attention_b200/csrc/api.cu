@@ -356,6 +356,15 @@ static int check_layer_norm_args(const b200gdn_layer_norm_args* a, const char* w
     REQUIRE(a->z, who); REQUIRE(a->mean, who); REQUIRE(a->rstd, who); REQUIRE(a->dy, who); REQUIRE(a->dx, who);
     if (a->dweight != nullptr || a->dbias != nullptr) REQUIRE(a->partials, who);
   }
+  const uintptr_t size = a->dtype == 2 ? 4 : 2, param_size = a->param_dtype == B200GDN_F32 ? 4 : 2;
+  auto off = [](uintptr_t boundary, std::initializer_list<const void*> all) {
+    for (const void* p : all)
+      if (reinterpret_cast<uintptr_t>(p) % boundary != 0) return true;
+    return false;
+  };
+  if (off(size, {a->x, a->residual, a->z, a->y, a->dy, a->dz, a->dx}) || off(param_size, {a->weight, a->bias, a->dweight, a->dbias}) ||
+      off(4, {a->mean, a->rstd, a->partials}))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: a tensor off its elements' boundary", who);
   return 0;
 }
 

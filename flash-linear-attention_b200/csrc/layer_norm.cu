@@ -11,6 +11,7 @@
 // Measured: 65536 x 4096 bf16 forward 180 us (164 at copy rate), backward 295 (246); 16384 x 2048 with a residual 50 (41) forward;
 // 65536 x 1024 fp32 with a residual backward 170 (164); 32768 x 1001 bf16, two bytes at a time, 56 and 76 (20 and 30).
 #include "gdn_common.cuh"
+#include "layer_norm_pieces.h"
 #include "rowio.cuh"
 
 namespace gdn {
@@ -611,13 +612,10 @@ int launch_n(const b200gdn_layer_norm_args& a, cudaStream_t st, bool bwd) {
 
 template <typename T>
 int launch_t(const b200gdn_layer_norm_args& a, cudaStream_t st, bool bwd) {
-  // the boundary that every tensor the kernels read or write by pieces starts on
-  uintptr_t off = 0;
-  for (const void* p : {a.x, a.residual, a.weight, a.bias, (const void*)a.z, (const void*)a.y, a.dy, a.dz, (const void*)a.dx}) off |= reinterpret_cast<uintptr_t>(p);
-  constexpr int N = 16 / sizeof(T);
-  if (a.D % N == 0 && off % 16 == 0) return launch_n<T, N>(a, st, bwd);
+  const int n = layer_norm_piece(a);
+  if (n == 16 / sizeof(T)) return launch_n<T, 16 / sizeof(T)>(a, st, bwd);
   if constexpr (sizeof(T) == 2)
-    if (a.D % 2 == 0 && off % 4 == 0) return launch_n<T, 2>(a, st, bwd);
+    if (n == 2) return launch_n<T, 2>(a, st, bwd);
   return launch_n<T, 1>(a, st, bwd);
 }
 

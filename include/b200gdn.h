@@ -389,7 +389,8 @@ int b200gdn_norm_gate_ctas(int64_t rows);
  *   z = x + residual, rounded to the element type (z = x without a residual);  n = (z - mean) rstd;  y = n weight + bias
  * with mean and 1/sqrt(variance + eps) of each row in fp32.  The backward pass reads z again with `mean` and `rstd`:
  *   h = dy weight;  dx = rstd (h - mean(h) - n mean(h n)) + dz;  dweight = sum of dy n;  dbias = sum of dy
- * and needs `partials` of b200gdn_layer_norm_ctas(rows) x 2 x D floats.  dx is the gradient of x and of residual. */
+ * and needs `partials` of b200gdn_layer_norm_ctas(rows) x 2 x D floats.  dx is the gradient of x and of residual.
+ * Tensors need no alignment beyond their elements' own; on 16-byte boundaries (fp32 parameters included) they are read fastest. */
 typedef struct b200gdn_layer_norm_args {
   int32_t struct_bytes;
   int32_t D;

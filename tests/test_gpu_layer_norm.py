@@ -209,3 +209,35 @@ def test_refusals():
     dx, = torch.autograd.grad(layer_norm(leaf).square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match='no second derivative'):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('D', [10, 1002, 2048])
+def test_tensors_at_any_element_of_a_buffer(D, dtype):
+    """By the C ABI, which copies nothing: rows and fp32 or 16-bit parameters that begin one, two or four elements into their buffers."""
+    import ctypes as C
+    from b200gdn import _lib
+    lib, rows = _lib.load(), 19
+    code = {torch.float32: 0, torch.bfloat16: 1}
+    for ptype in (torch.float32, torch.bfloat16):
+        for i, (xo, wo, bo) in enumerate([(0, 1, 0), (0, 0, 1), (0, 2, 2), (2, 1, 3), (1, 0, 0), (4, 4, 4), (0, 3, 5), (0, 0, 0)]):
+            x, w, b, _, dy, _ = make(rows, D, dtype, ptype, False, True, seed=i)
+
+            def at(t, off):
+                buf = torch.zeros(t.numel() + off + 8, dtype=t.dtype, device='cuda')
+                buf[off:off + t.numel()] = t.flatten()
+                return buf[off:off + t.numel()].view(t.shape)
+            x, w, b, dy = at(x, xo), at(w, wo), at(b, bo), at(dy, xo)
+            y, dx = at(torch.zeros_like(x), xo), at(torch.zeros_like(x), xo)
+            mean, rstd = torch.zeros(rows, device='cuda'), torch.zeros(rows, device='cuda')
+            dw, db = at(torch.zeros_like(w), wo), at(torch.zeros_like(b), bo)
+            partials = torch.zeros(lib.b200gdn_layer_norm_ctas(rows) * 2 * D, device='cuda')
+            shape = dict(struct_bytes=C.sizeof(_lib.LayerNormArgs), D=D, rows=rows, dtype=2 if dtype == torch.float32 else 0, param_dtype=code[ptype], eps=1e-5)
+            p = {k: v.data_ptr() for k, v in dict(x=x, w=w, b=b, y=y, mean=mean, rstd=rstd, dy=dy, dx=dx, dw=dw, db=db, partials=partials).items()}
+            stream = torch.cuda.current_stream().cuda_stream
+            assert lib.b200gdn_layer_norm_fwd(C.byref(_lib.LayerNormArgs(x=p['x'], weight=p['w'], bias=p['b'], y=p['y'], mean=p['mean'], rstd=p['rstd'], **shape)), stream) == 0
+            assert lib.b200gdn_layer_norm_bwd(C.byref(_lib.LayerNormArgs(z=p['x'], weight=p['w'], mean=p['mean'], rstd=p['rstd'], dy=p['dy'], dx=p['dx'],
+                                                                         dweight=p['dw'], dbias=p['db'], partials=p['partials'], **shape)), stream) == 0
+            want = H.layer_norm(x, w, b, None, 1e-5, dy)
+            for name, got in (('y', y), ('dx', dx), ('dweight', dw), ('dbias', db)):
+                close(name, got, want[name], want[name + '_size'])

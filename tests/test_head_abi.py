@@ -105,3 +105,61 @@ def test_cpu_tensors_are_refused():
                  lambda: topk_distill_loss(x, x, x.long())):
         with pytest.raises(B200GDNError, match='CUDA device only'):
             call()
+
+
+PIECES = r'''
+#include <stdio.h>
+#include "layer_norm_pieces.h"
+int main() {   // dtype, param_dtype, D, addresses of rows, weight and bias; prints the elements that are moved at a time
+  b200gdn_layer_norm_args a{};
+  long x, w, b;
+  while (scanf("%d %d %d %ld %ld %ld", &a.dtype, &a.param_dtype, &a.D, &x, &w, &b) == 6) {
+    a.x = a.y = (void*)x;
+    a.weight = (void*)w;
+    a.bias = (void*)b;
+    printf("%d\n", gdn::layer_norm_piece(a));
+  }
+}
+'''
+
+
+def test_layer_norm_moves_no_more_than_every_tensor_is_aligned_for(tmp_path):
+    """The rule that chooses the kernels, by arithmetic: N elements of a row are one access, N parameters accesses of N times their
+    own size, 16 bytes at most.  A slice of a flat buffer of fp32 parameters begins on any boundary of 4."""
+    src, exe = tmp_path / 'pieces.cpp', tmp_path / 'pieces'
+    src.write_text(PIECES)
+    csrc = os.path.join(ROOT, 'flash-linear-attention_b200', 'csrc')
+    subprocess.check_call(['g++', '-std=c++17', '-I', csrc, '-I', os.path.join(ROOT, 'include'), str(src), '-o', str(exe)])
+    base, cases = 1 << 12, []
+    for dtype in (0, 1, 2):
+        size = 4 if dtype == 2 else 2
+        for ptype in (0, 1, 2):
+            psize = 4 if ptype == 0 else 2
+            for D in (1, 2, 7, 10, 1000, 1002, 2048, 2052):
+                for x in (0, 1, 2, 4, 8):
+                    for w, b in ((0, 0), (1, 0), (0, 1), (2, 2), (4, 0), (3, None), (None, 5), (None, None), (8, 8)):
+                        cases.append((dtype, ptype, D, base + x * size, *(0 if o is None else base + o * psize for o in (w, b))))
+    out = subprocess.run([str(exe)], input='\n'.join(' '.join(map(str, c)) for c in cases), capture_output=True, text=True, check=True).stdout.split()
+    assert len(out) == len(cases)
+
+    def fits(n, dtype, ptype, D, x, w, b):
+        size, psize = 4 if dtype == 2 else 2, 4 if ptype == 0 else 2
+        return D % n == 0 and x % (n * size) == 0 and all(p % min(16, n * psize) == 0 for p in (w, b))
+    for got, c in zip(map(int, out), cases):
+        assert fits(got, *c), (got, c)
+        assert got == max(n for n in ((4, 1) if c[0] == 2 else (8, 2, 1)) if fits(n, *c)), (got, c)
+
+
+def test_layer_norm_refuses_tensors_off_their_elements_boundary():
+    from b200gdn import _lib
+    fwd = dict(rows=4, D=8, x=256, y=256, residual=256, z=256, weight=256, bias=256, mean=256, rstd=256)
+    bwd = dict(rows=4, D=8, z=256, mean=256, rstd=256, dy=256, dz=256, dx=256, weight=256, dweight=256, dbias=256, partials=256)
+    for fn, good in (('b200gdn_layer_norm_fwd', fwd), ('b200gdn_layer_norm_bwd', bwd)):
+        for name in good:
+            if name in ('rows', 'D'):
+                continue
+            rows, params = name in ('x', 'y', 'residual', 'z', 'dy', 'dz', 'dx'), name in ('weight', 'bias', 'dweight', 'dbias')
+            for dtype, ptype, at in ((0, 1, 257), (2, 1, 258), (1, 0, 258)):
+                size = {'rows': 4 if dtype == 2 else 2, 'params': 4 if ptype == 0 else 2, 'sums': 4}['rows' if rows else 'params' if params else 'sums']
+                if at % size:
+                    refused(fn, _lib.LayerNormArgs(dtype=dtype, param_dtype=ptype, **{**good, name: at}), -1, 'boundary')
