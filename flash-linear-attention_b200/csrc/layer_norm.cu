@@ -94,11 +94,12 @@ __device__ __forceinline__ void load_params(const void* p, int dtype, int d, flo
 }
 
 constexpr int threads_of(int tpr) { return tpr > 32 ? tpr : 128; }   // rows of several warps have a CTA to themselves
-// forward, an SM's: by the registers of the rows on their way (NV pieces, with a residual twice that) and at work
+// forward, an SM's: by the registers of the rows on their way (NV pieces, with a residual twice that) and at work.  One or two pieces a thread:
+// 7, with a residual 5, since at 8 rows spill (65536 x 256 bf16 with a residual 25 us at 5, 28 at 6, 36 at 8; 131072 x 100 fp32 without 25 at 7, 28 at 8)
 // (with a residual there is more to move for the same arithmetic: the cache does: 16384 rows of 8192, 169 us, 192 with shared memory)
 constexpr bool shares_params(int nv, int n, bool res) { return !res && n >= 4 && nv * n > 8 && nv <= 4; }
 constexpr int fwd_ctas(int tpr, int nv, bool res) {
-  return tpr > 32 ? 512 / threads_of(tpr) : nv >= 16 ? (res ? 2 : 3) : nv == 8 ? (res ? 3 : 4) : nv == 4 ? (res ? 5 : 6) : 8;
+  return tpr > 32 ? 512 / threads_of(tpr) : nv >= 16 ? (res ? 2 : 3) : nv == 8 ? (res ? 3 : 4) : nv == 4 ? (res ? 5 : 6) : res ? 5 : 7;
 }
 constexpr int bwd_ctas(int tpr) { return tpr <= 32 ? 4 : tpr == 64 ? 8 : tpr == 128 ? 4 : tpr == 256 ? 2 : 1; }
 constexpr int rows_at_once(int nv, int n) { return nv * n <= 4 ? 4 : nv == 1 ? 2 : 1; }   // of a group of TPR threads
@@ -134,7 +135,9 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
   constexpr int RPC = threads_of(TPR) / TPR, R = rows_at_once(NV, N), NW = TPR > 32 ? TPR / 32 : 1;
   __shared__ float scratch[2][2 * R * NW];
   const int sub = threadIdx.x % TPR, group = threadIdx.x / TPR, lane = threadIdx.x & 31;
-  const float inv = 1.f / a.D, root = sqrtf(inv);
+  // down: a power of two, down^2 in [1 / 4 D, 1 / D].  Products with it are exact, so one fused operation is (z - mean) down with one
+  // rounding, and the sum of its squares is within range wherever the variance is; times `up` it is the variance.
+  const float inv = 1.f / a.D, down = __int_as_float((127 - (33 - __clz(a.D - 1)) / 2) << 23), up = inv / (down * down);
   // Weight and bias as fp32 pairs: in registers where a thread has few columns, else in shared memory, where row after row finds them
   // without conversions (and without a bank conflict: 16 bytes a thread side by side); of very wide rows from the first-level cache.
   constexpr int P = pairs(N);
@@ -216,13 +219,12 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
     }
     r0 += step;
     fetch(r0);
-    // the mean of what a warp (a row's lanes) holds, the squares about it (divided by D each: the sum is within range wherever the
-    // variance is), then the row's
+    // the mean of what a warp (a row's lanes) holds, the squares about it, then the row's
     shuffle_sums<(TPR < 32 ? TPR : 32)>(s);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float mean = s[r] * per_held_here;
-      const uint64_t by = spread<N>(root), off = spread<N>(-mean * root);
+      const uint64_t by = spread<N>(down), off = spread<N>(-mean * down);
       uint64_t sum = 0ull;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
           sum = fma2(c, c, sum);
         }
       }
-      q[r] = both(sum);
+      q[r] = both(sum) * up;
     }
     shuffle_sums<(TPR < 32 ? TPR : 32)>(q);
     if constexpr (TPR > 32) {
@@ -265,7 +267,8 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
       const int64_t row = now + r * RPC + group;
       if (row >= a.rows) continue;
       const float mean = s[r] * inv, rstd = __frsqrt_rn(q[r] + a.eps);
-      const uint64_t by = spread<N>(rstd), off = spread<N>(-mean * rstd);
+      // (the difference first: z rstd - mean rstd in one operation would leave the rounding of mean rstd where z is the mean)
+      const uint64_t by = spread<N>(rstd), off = spread<N>(-mean);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int d = (v * TPR + sub) * N;
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__(threads_of(TPR), fwd_ctas(TPR, NV, RES)) layer
           load_params<N>(a.bias, a.param_dtype, d, 0.f, b[0]);
         }
 #pragma unroll
-        for (int i = 0; i < P; ++i) z[r][v].set(i, fma2(fma2(z[r][v].pair(i), by, off), w[HELD ? v : 0][i], b[HELD ? v : 0][i]));
+        for (int i = 0; i < P; ++i) z[r][v].set(i, fma2(mul2(add2(z[r][v].pair(i), off), by), w[HELD ? v : 0][i], b[HELD ? v : 0][i]));
         z[r][v].store(a.y, row * a.D + d);
       }
       if (sub == 0 && a.mean) {
@@ -348,28 +351,28 @@ __global__ void __launch_bounds__(threads_of(TPR), bwd_ctas(TPR)) layer_norm_bwd
     float s[2 * R];   // of h and of h n
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint64_t by = spread<N>(cur.rstd[r]), off = spread<N>(-cur.mean[r] * cur.rstd[r]);
+      const uint64_t by = spread<N>(cur.rstd[r]), off = spread<N>(-cur.mean[r]);
       uint64_t s1 = 0ull, s2 = 0ull;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const uint64_t n = fma2(cur.z[r][v].pair(i), by, off), g = cur.dy[r][v].pair(i), h = mul2(g, w[v][i]);
+          const uint64_t c = add2(cur.z[r][v].pair(i), off), g = cur.dy[r][v].pair(i), h = mul2(g, w[v][i]);   // c = n / rstd
           s1 = add2(s1, h);
-          s2 = fma2(h, n, s2);
-          dw[v][i] = fma2(g, n, dw[v][i]);
+          s2 = fma2(h, c, s2);
+          dw[v][i] = fma2(mul2(g, by), c, dw[v][i]);
           db[v][i] = add2(db[v][i], g);
         }
       s[2 * r] = both(s1);
-      s[2 * r + 1] = both(s2);
+      s[2 * r + 1] = both(s2) * cur.rstd[r];
     }
     row_sums<TPR>(s, scratch[turn]);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int64_t row = now + r * RPC + group;
       if (row >= a.rows) continue;
-      const uint64_t by = spread<N>(cur.rstd[r]), off = spread<N>(-cur.mean[r] * cur.rstd[r]);
-      const uint64_t h_mean = spread<N>(-s[2 * r] * inv), hn_mean = spread<N>(-s[2 * r + 1] * inv);
+      const uint64_t by = spread<N>(cur.rstd[r]), off = spread<N>(-cur.mean[r]);
+      const uint64_t h_mean = spread<N>(-s[2 * r] * inv), hn_mean = spread<N>(-s[2 * r + 1] * inv * cur.rstd[r]);   // (of z - mean)
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int d = (v * TPR + sub) * N;
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(threads_of(TPR), bwd_ctas(TPR)) layer_norm_bwd
         cur.dy[r][v].again();
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const uint64_t n = fma2(cur.z[r][v].pair(i), by, off), e = fma2(n, hn_mean, fma2(cur.dy[r][v].pair(i), w[v][i], h_mean));
+          const uint64_t e = fma2(add2(cur.z[r][v].pair(i), off), hn_mean, fma2(cur.dy[r][v].pair(i), w[v][i], h_mean));
           if constexpr (DZ) cur.z[r][v].set(i, fma2(e, by, cur.dz[r][v].pair(i)));
           else cur.z[r][v].set(i, mul2(e, by));
         }

@@ -241,3 +241,26 @@ def test_tensors_at_any_element_of_a_buffer(D, dtype):
             want = H.layer_norm(x, w, b, None, 1e-5, dy)
             for name, got in (('y', y), ('dx', dx), ('dweight', dw), ('dbias', db)):
                 close(name, got, want[name], want[name + '_size'])
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize('D', [1, 2, 8, 64, 256, 512, 1024, 2048, 4096, 8192, 16384, 32768, 65536])
+def test_constant_rows(D, dtype):
+    """Rows of one value v of at most 8 bits: sums of a power of two of them and their mean are exact, and z - mean is zero.  So y is
+    the bias, the weight's gradient zero and dx = rstd (h - mean(h)), whatever eps makes of rstd."""
+    from b200gdn import layer_norm
+    v = torch.tensor([0.1, 100.0, 1000.0, -7.3, 0.0, 3.0, 1e-3]).bfloat16().float().cuda()
+    x = v[:, None].expand(len(v), D).to(dtype).contiguous().requires_grad_(True)
+    x_half = (x.detach().float() / 2).to(dtype)   # (exact) twice that, as a residual sum
+    w = (1 + 0.3 * torch.randn(D, device='cuda', generator=torch.Generator('cuda').manual_seed(0))).requires_grad_(True)
+    b = torch.randn(D, device='cuda', generator=torch.Generator('cuda').manual_seed(1)).requires_grad_(True)
+    dy = torch.randn(len(v), D, device='cuda', generator=torch.Generator('cuda').manual_seed(2)).to(dtype)
+    h = dy.double() * w.detach().double()
+    for eps in (1e-5, 1e-12):
+        r = eps ** -0.5
+        for y in (layer_norm(x, w, b, eps=eps), layer_norm(x_half.requires_grad_(True), w, b, residual=x_half, eps=eps)):
+            assert torch.equal(y.detach(), b.detach().to(dtype).expand_as(y))
+        dx, dw = torch.autograd.grad(layer_norm(x, w, b, eps=eps), [x, w], dy)
+        assert (dw == 0).all()
+        if dtype is not torch.float16 or eps == 1e-5:   # (1e6 leaves what fp16 holds)
+            close('dx', dx, r * (h - h.mean(-1, keepdim=True)), r * (h.abs() + h.abs().mean(-1, keepdim=True)))
