@@ -338,6 +338,13 @@ int b200gdn_norm_gate_bwd(const b200gdn_norm_gate_args* a, void* stream) {
 
 int b200gdn_norm_gate_ctas(int64_t rows) { return gdn::norm_gate_grid(rows); }
 
+// any of the addresses off a boundary (NULL is on every one)
+static bool off_boundary(uintptr_t boundary, std::initializer_list<const void*> all) {
+  for (const void* p : all)
+    if (reinterpret_cast<uintptr_t>(p) % boundary != 0) return true;
+  return false;
+}
+
 static int check_layer_norm_args(const b200gdn_layer_norm_args* a, const char* who, bool bwd) {
   using namespace gdn;
   if (a == nullptr) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: args is NULL", who);
@@ -357,13 +364,8 @@ static int check_layer_norm_args(const b200gdn_layer_norm_args* a, const char* w
     if (a->dweight != nullptr || a->dbias != nullptr) REQUIRE(a->partials, who);
   }
   const uintptr_t size = a->dtype == 2 ? 4 : 2, param_size = a->param_dtype == B200GDN_F32 ? 4 : 2;
-  auto off = [](uintptr_t boundary, std::initializer_list<const void*> all) {
-    for (const void* p : all)
-      if (reinterpret_cast<uintptr_t>(p) % boundary != 0) return true;
-    return false;
-  };
-  if (off(size, {a->x, a->residual, a->z, a->y, a->dy, a->dz, a->dx}) || off(param_size, {a->weight, a->bias, a->dweight, a->dbias}) ||
-      off(4, {a->mean, a->rstd, a->partials}))
+  if (off_boundary(size, {a->x, a->residual, a->z, a->y, a->dy, a->dz, a->dx}) || off_boundary(param_size, {a->weight, a->bias, a->dweight, a->dbias}) ||
+      off_boundary(4, {a->mean, a->rstd, a->partials}))
     return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: a tensor off its elements' boundary", who);
   return 0;
 }
@@ -418,6 +420,10 @@ static int check_logprob_args(const b200gdn_logprob_args* a, const char* who, bo
     if (a->dentropy != nullptr) REQUIRE(a->entropy, who);
     if (a->dtop_logprobs != nullptr) REQUIRE(a->top_ids, who);
   }
+  if (off_boundary(4, {a->logprobs, a->entropy, a->top_logprobs, a->stats, a->dlogprobs, a->dentropy, a->dtop_logprobs}) || off_boundary(8, {a->top_ids}) ||
+      (a->tokens != nullptr && off_boundary(a->token_bytes, {a->tokens})))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: a tensor off its elements' boundary", who);
+  if (!bwd && off_boundary(16, {a->workspace})) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: workspace off a 16-byte boundary", who);
   return 0;
 }
 
@@ -451,6 +457,10 @@ static int check_distill_args(const b200gdn_distill_args* a, const char* who, bo
   if ((a->flags & B200GDN_DISTILL_SKIP_ONE) && !(bwd && (a->flags & B200GDN_DISTILL_SCALAR)))
     return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: SKIP_ONE goes with a scalar upstream gradient", who);
   REQUIRE(a->workspace, who);
+  if (off_boundary(4, {a->row_loss, a->loss, a->dloss}) || off_boundary(a->id_bytes, {a->ids}) ||
+      off_boundary(a->teacher_dtype == B200GDN_F32 ? 4 : 2, {a->teacher}))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: a tensor off its elements' boundary", who);
+  if (off_boundary(16, {a->workspace})) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: workspace off a 16-byte boundary", who);
   return 0;
 }
 

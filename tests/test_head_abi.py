@@ -163,3 +163,25 @@ def test_layer_norm_refuses_tensors_off_their_elements_boundary():
                 size = {'rows': 4 if dtype == 2 else 2, 'params': 4 if ptype == 0 else 2, 'sums': 4}['rows' if rows else 'params' if params else 'sums']
                 if at % size:
                     refused(fn, _lib.LayerNormArgs(dtype=dtype, param_dtype=ptype, **{**good, name: at}), -1, 'boundary')
+
+
+def test_logprob_and_distill_refuse_tensors_off_their_boundary():
+    from b200gdn import _lib
+    rows = dict(rows=2, V=50, inner=1, scale=1.0, logits=256, workspace=256)
+    both = dict(tokens=256, token_bytes=8, entropy=256, top_k=3, top_ids=256, stats=256, **rows)
+    fwd = dict(logprobs=256, top_logprobs=256, **both)
+    bwd = dict(dlogprobs=256, dentropy=256, dtop_logprobs=256, dlogits=256, **both)
+    for fn, good in (('b200gdn_logprob_fwd', fwd), ('b200gdn_logprob_bwd', bwd)):
+        for name in ('logprobs', 'entropy', 'top_logprobs', 'stats', 'dlogprobs', 'dentropy', 'dtop_logprobs'):
+            if name in good:
+                refused(fn, _lib.LogprobArgs(**{**good, name: 258}), -1, 'boundary')
+        for name in ('tokens', 'top_ids'):
+            refused(fn, _lib.LogprobArgs(**{**good, name: 260}), -1, 'boundary')
+        refused(fn, _lib.LogprobArgs(**{**good, 'token_bytes': 4, 'tokens': 258}), -1, 'boundary')
+    refused('b200gdn_logprob_fwd', _lib.LogprobArgs(**{**fwd, 'workspace': 264}), -1, 'workspace')
+    good = dict(K=3, id_bytes=8, teacher=256, ids=256, row_loss=256, loss=256, dloss=256, dlogits=256, **rows)
+    for fn in ('b200gdn_distill_fwd', 'b200gdn_distill_bwd'):
+        for name, at in (('teacher', 258), ('ids', 260), ('row_loss', 258), ('loss', 257), ('dloss', 258), ('workspace', 264)):
+            refused(fn, _lib.DistillArgs(**{**good, name: at}), -1, 'boundary')
+        refused(fn, _lib.DistillArgs(**{**good, 'teacher_dtype': 1, 'teacher': 257}), -1, 'boundary')
+        refused(fn, _lib.DistillArgs(**{**good, 'id_bytes': 4, 'ids': 258}), -1, 'boundary')
