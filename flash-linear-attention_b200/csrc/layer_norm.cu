@@ -589,7 +589,8 @@ int launch_n(const b200gdn_layer_norm_args& a, cudaStream_t st, bool bwd) {
     }
     if (pieces <= 2048) return launch_fwd<T, N, 256, 8>(a, st);
     if (pieces <= 4096) return launch_fwd<T, N, 512, 8>(a, st);
-    if (N == 1 && pieces <= 8192) return launch_fwd<T, N, 512, 16>(a, st);
+    if constexpr (N == 1)
+      if (pieces <= 8192) return launch_fwd<T, N, 512, 16>(a, st);
   } else if constexpr (full) {
     if (pieces <= 8) return launch_bwd<T, N, 8, 1>(a, st);
     if (pieces <= 16) return launch_bwd<T, N, 16, 1>(a, st);
@@ -608,7 +609,8 @@ int launch_n(const b200gdn_layer_norm_args& a, cudaStream_t st, bool bwd) {
     if (pieces <= 1024) return launch_bwd<T, N, 128, 8>(a, st);
     if (pieces <= 2048) return launch_bwd<T, N, 256, 8>(a, st);
     if (pieces <= 4096) return launch_bwd<T, N, 512, 8>(a, st);
-    if (N == 1 && pieces <= 8192) return launch_bwd<T, N, 512, 16>(a, st);
+    if constexpr (N == 1)
+      if (pieces <= 8192) return launch_bwd<T, N, 512, 16>(a, st);
   }
   return launch_wide<T>(a, st, bwd);
 }
