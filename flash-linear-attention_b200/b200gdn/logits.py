@@ -3,7 +3,7 @@ against a teacher's top alternatives.
 
 * ``token_logprobs`` — scoring and sampling interfaces, a teacher's pass, policy losses; differentiable.
 * ``topk_distill_loss`` — a student's divergence from the entries that ``token_logprobs(..., top_k=...)`` gave of a teacher;
-  the gradient of a sum or mean is formed in the same pass over the logits.
+  the gradient of a sum or mean is formed in the same call, by a second look at the logits.
 
 Both read logits ``[..., V]`` in bf16, fp16 or fp32 where they lie (a slice of a sequence, a padded vocabulary), hold every
 sum in fp32 and run as kernels of libb200gdn.so (b200gdn_logprob_fwd/bwd, b200gdn_distill_fwd/bwd); there is no fallback path.
@@ -67,7 +67,9 @@ def topk_distill_loss(logits: torch.Tensor, teacher_logprobs: torch.Tensor, teac
     An entry with an id outside ``[0, V)`` or a log probability of minus infinity is absent.  A row without entries (a prompt) is
     left out: its loss is 0, it has no gradient and the mean does not count it.  ``reduction``: ``'mean'`` over the rows that
     count, ``'sum'`` or ``'none'`` (``[...]``).  With sum or mean and logits that require a gradient, the gradient is formed in the
-    forward pass; the backward pass only hands it on where the upstream gradient is one, else it forms it anew with that factor.
+    forward pass (and held until the backward pass); the backward pass only hands it on where the upstream gradient is one, else it
+    forms it anew with that factor, which costs as much again: a weight or an accumulation divisor is cheaper in ``reduction='none'``,
+    whose gradient is formed in the backward pass alone.
     """
     if not logits.is_cuda:
         raise _lib.B200GDNError('topk_distill_loss runs on a CUDA device only (no CPU path)')

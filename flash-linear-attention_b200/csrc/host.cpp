@@ -1084,7 +1084,8 @@ b200gdn_distill_args distill_args(const LogitRows& rows, const Tensor& teacher, 
   return a;
 }
 
-// `need_grad`: what the backward pass needs is kept; of a sum or mean the gradient is formed here, while the rows are on the chip
+// `need_grad`: what the backward pass needs is kept; of a sum or mean the gradient is formed here, by a second look at the
+// rows: the backward call has nothing left to do where the upstream gradient is one
 DistillForward distill_forward(const Tensor& logits, const Tensor& teacher, const Tensor& ids, double scale, bool bucket, int64_t reduction,
                                bool need_grad) {
   DistillForward r;

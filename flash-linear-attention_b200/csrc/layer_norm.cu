@@ -8,8 +8,10 @@
 // backward pass leaves one partial row of dw and db, which a second kernel adds in a fixed order.
 // What held the first forms back was instructions, not bytes: 24 an element with conversions one by one, scalar arithmetic, divisions
 // and parameters converted row after row.
-// Measured: 65536 x 4096 bf16 forward 180 us (164 at copy rate), backward 295 (246); 16384 x 2048 with a residual 50 (41) forward;
-// 65536 x 1024 fp32 with a residual backward 170 (164); 32768 x 1001 bf16, two bytes at a time, 56 and 76 (20 and 30).
+// Measured: 65536 x 4096 bf16 forward 180 us (164 at copy rate), backward 292 (246); 16384 x 2048 with a residual 50 (41) forward;
+// 65536 x 1024 fp32 with a residual backward 173 (164); 32768 x 1001 bf16, two bytes at a time, 51 to 56 and 75 (20 and 30).  Beyond the
+// registers, in several looks: 16384 x 8192 fp32 backward 880 (246), 8192 x 16384 bf16 954 (123).  Forward rows of 16-bit elements from
+// 8193 on are held at the cost of spills: 8192 x 16384 155 (82), with a residual 346 (164).
 #include "gdn_common.cuh"
 #include "layer_norm_pieces.h"
 #include "rowio.cuh"

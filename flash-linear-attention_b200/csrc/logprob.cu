@@ -11,8 +11,8 @@
 // of them are larger, which is its place.  (Groups of a lane's words, 512 bytes from one another, cost no exchange but ten times
 // the bytes when they are read again: 2048 rows of 131072, k = 64, 130 us for 122.)
 //
-// Measured, 131072 16-bit logits a row: 4096 rows with token and entropy 169 us, 6.4 TB/s (the copy rate is 6.56); 2048 rows 90, with 20 top
-// entries 113, with 128 138; backward 4096 rows 373 us, 5.8 TB/s.
+// Measured, 131072 16-bit logits a row: 4096 rows with token and entropy 169 us, 6.4 TB/s (the copy rate is 6.56); 2048 rows 89, with 20 top
+// entries 113, with 128 138; backward 4096 rows 376 us, 5.7 TB/s.
 #include "vocab.cuh"
 
 namespace gdn {

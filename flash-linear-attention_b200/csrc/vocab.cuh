@@ -137,9 +137,9 @@ __device__ __forceinline__ uint32_t largest_of(const uint4& w) {
 }
 
 // One thread's running sums.  A group of words at a time: their largest entry first, so that the sums are moved seldom.  Per pair of
-// 16-bit entries: one operation for the largest, two to widen, two for the exponents, two exponentials, one to add and one more for the
-// entropy: 4.5 instructions an entry.  (At the memory's rate an SM gets 11.7 entries of 16 bits a clock, for which it can issue 128 instructions;
-// the exponentials' unit takes 16.)
+// 16-bit entries the arithmetic is one operation for the largest, two to widen, two for the exponents, two exponentials, one to add and one
+// more for the entropy; with moves, loads and the joining of lanes the kernel was counted at 8.0 instructions an entry.  (At the memory's
+// rate an SM gets 11.7 entries of 16 bits a clock, for which it can issue 128 instructions; the exponentials' unit takes 16.)
 // BOUNDED: u is at least -2^10, of entries whose 2^u is zero long before: 0 x -infinity is no number.
 template <typename T, bool WITH_T>
 struct PieceSums {

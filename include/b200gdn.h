@@ -458,7 +458,7 @@ int64_t b200gdn_logprob_workspace_bytes(int64_t rows, int32_t V, int32_t dtype, 
  * With B200GDN_DISTILL_BUCKET a row with q_t > 0 and nothing above minus infinity off its list has an infinite loss too.  However far
  * the list is above the rest, or below it, loss and gradient are finite otherwise.
  * The forward pass writes row_loss; `loss` (NULL: not wanted) is their sum, with B200GDN_DISTILL_MEAN over the number of rows
- * counted (at least 1).  With dlogits it writes the gradient of `loss` in the same pass.  The backward pass forms
+ * counted (at least 1).  With dlogits it writes the gradient of `loss` in the same call, by a second look at the logits.  The backward pass forms
  * dlogits for an upstream gradient: dloss [rows] of row_loss, or with B200GDN_DISTILL_SCALAR dloss [1] of `loss`; with
  * B200GDN_DISTILL_SKIP_ONE as well it returns at once where dloss is one (dlogits holds that gradient already). */
 #define B200GDN_DISTILL_BUCKET 1u
