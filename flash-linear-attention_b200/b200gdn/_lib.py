@@ -103,6 +103,28 @@ class LayerNormArgs(C.Structure):
     ]
 
 
+NORMS_POST, NORMS_SIGMOID, NORMS_SILU = 1, 2, 4
+
+
+class RmsNormsArgs(C.Structure):
+    _fields_ = [
+        ('struct_bytes', C.c_int32), ('D', C.c_int32), ('rows', C.c_int64), ('dtype', C.c_int32), ('param_dtype', C.c_int32),
+        ('flags', C.c_uint32), ('eps', C.c_float), ('alpha', C.c_float),
+        ('y', _p), ('residual', _p), ('gate', _p), ('weight', _p), ('post_weight', _p), ('scale', _p), ('z', _p), ('out', _p),
+        ('rstd_y', _p), ('rstd_z', _p), ('dout', _p), ('dz', _p), ('dy', _p), ('dresidual', _p), ('dgate', _p),
+        ('dweight', _p), ('dpost_weight', _p), ('dscale', _p), ('partials', _p),
+    ]
+
+
+class GatedRecurrenceArgs(C.Structure):
+    _fields_ = [
+        ('struct_bytes', C.c_int32), ('D', C.c_int32), ('rows', C.c_int64), ('n_seq', C.c_int32), ('seq_len', C.c_int32), ('n_chunks', C.c_int32),
+        ('dtype', C.c_int32), ('gate_dtype', C.c_int32), ('reserved', C.c_int32), ('stride_x', C.c_int64), ('stride_g', C.c_int64),
+        ('chunk_meta', _p), ('seq_meta', _p), ('seq_order', _p), ('x', _p), ('g', _p), ('h0', _p), ('h', _p), ('ht', _p), ('states', _p),
+        ('dh', _p), ('dht', _p), ('dx', _p), ('dg', _p), ('dh0', _p),
+    ]
+
+
 _ROWS_OF_LOGITS = [('struct_bytes', C.c_int32), ('V', C.c_int32), ('rows', C.c_int64), ('inner', C.c_int64),
                    ('stride_inner', C.c_int64), ('stride_outer', C.c_int64), ('dtype', C.c_int32)]
 MAX_TOP, MAX_LIST = 128, 256
@@ -134,6 +156,7 @@ EXPORTS = (
     'b200gdn_selftest_wait_expiry', 'b200gdn_chunk_fwd_static', 'b200gdn_cp_fold', 'b200gdn_cp_prefix',
     'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd', 'b200gdn_norm_gate_ctas',
     'b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd', 'b200gdn_layer_norm_ctas', 'b200gdn_logprob_fwd', 'b200gdn_logprob_bwd',
+    'b200gdn_gated_recurrence_fwd', 'b200gdn_gated_recurrence_bwd', 'b200gdn_rms_norms_fwd', 'b200gdn_rms_norms_bwd', 'b200gdn_rms_norms_partials',
     'b200gdn_logprob_workspace_bytes', 'b200gdn_distill_fwd', 'b200gdn_distill_bwd', 'b200gdn_distill_workspace_bytes',
 )
 
@@ -162,7 +185,8 @@ def load():
                      'b200gdn_prep_fwd', 'b200gdn_prep_bwd', 'b200gdn_chunk_fwd_static', 'b200gdn_cp_fold', 'b200gdn_cp_prefix',
                      'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd',
                      'b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd', 'b200gdn_logprob_fwd', 'b200gdn_logprob_bwd',
-                     'b200gdn_distill_fwd', 'b200gdn_distill_bwd'):
+                     'b200gdn_distill_fwd', 'b200gdn_distill_bwd', 'b200gdn_gated_recurrence_fwd', 'b200gdn_gated_recurrence_bwd',
+                     'b200gdn_rms_norms_fwd', 'b200gdn_rms_norms_bwd'):
             fn = getattr(lib, name)
             fn.restype = C.c_int
             fn.argtypes = [C.c_void_p, C.c_void_p]
@@ -178,6 +202,8 @@ def load():
             fn.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
         lib.b200gdn_layer_norm_ctas.restype = C.c_int
         lib.b200gdn_layer_norm_ctas.argtypes = [C.c_int64]
+        lib.b200gdn_rms_norms_partials.restype = C.c_int64
+        lib.b200gdn_rms_norms_partials.argtypes = [C.c_int64, C.c_int32]
         lib.b200gdn_last_launch_count.restype = C.c_int
         lib.b200gdn_device_status.restype = C.c_int
         lib.b200gdn_device_status.argtypes = []

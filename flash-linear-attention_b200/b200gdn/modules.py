@@ -9,10 +9,11 @@
 
 and ahead of it, in the block around the layer,
 
-* ``layer_norm`` / ``LayerNorm`` — layer norm with the residual sum (fla/modules/layernorm.py).
+* ``layer_norm`` / ``LayerNorm`` — layer norm with the residual sum (fla/modules/layernorm.py);
+* ``residual_rms_norm`` / ``ResidualRMSNorm`` — the RMS norms either side of a block with its gate, residual scale and residual sum.
 
 All run as HBM-streaming kernels of libb200gdn.so (b200gdn_conv_fwd/bwd, b200gdn_norm_gate_fwd/bwd,
-b200gdn_layer_norm_fwd/bwd); there is no fallback path.
+b200gdn_layer_norm_fwd/bwd, b200gdn_rms_norms_fwd/bwd); there is no fallback path.
 """
 from __future__ import annotations
 
@@ -243,3 +244,52 @@ class LayerNorm(nn.Module):
 
     def forward(self, x, residual=None, prenorm=False):
         return layer_norm(x, self.weight, self.bias, residual=residual, eps=self.eps, prenorm=prenorm)
+
+
+_GATES = {None: 0, 'sigmoid': _lib.NORMS_SIGMOID, 'silu': _lib.NORMS_SILU, 'swish': _lib.NORMS_SILU}
+
+
+def residual_rms_norm(y, weight=None, residual=None, post_norm: bool = False, post_weight=None, gate=None, gate_activation: Optional[str] = None,
+                      scale=None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What lies between two blocks in one pass over the rows: ``p = y / rms(y) post_weight`` (with ``post_norm``; else y),
+    ``z = residual + scale act(gate) p`` and ``out = z / rms(z) weight``, with ``rms(v) = sqrt(mean(v^2) + eps)``; returns ``(out, z)``,
+    out for the next block and z as the residual stream.  With nothing but ``y`` and ``weight`` it is the plain RMS norm.
+
+    y is a block's output ``[..., D]`` in bf16, fp16 or fp32; residual and gate are of its shape and type.  ``gate_activation``: None (the
+    gate as it is), ``'sigmoid'`` or ``'silu'`` / ``'swish'``.  weight, post_weight ``[D]`` in any of the three types, ones where absent;
+    scale is such a vector too, or a number.  z is normalised as it is summed, in fp32; only what is handed on is rounded.  Gradients of
+    both results reach all tensors.
+    """
+    if not y.is_cuda:
+        raise _lib.B200GDNError('residual_rms_norm runs on a CUDA device only (no CPU path)')
+    if gate_activation not in _GATES:
+        raise ValueError(f'Unsupported activation: {gate_activation}')
+    if post_weight is not None and not post_norm:
+        raise ValueError('`post_weight` belongs to the norm of the block\'s output: it needs `post_norm`')
+    if gate_activation is not None and gate is None:
+        raise ValueError('`gate_activation` without a `gate`')
+    vector = isinstance(scale, torch.Tensor)
+    args = (y, weight, residual, post_weight, gate, scale if vector else None, _GATES[gate_activation] | (_lib.NORMS_POST if post_norm else 0),
+            1.0 if vector or scale is None else float(scale), eps)
+    out = _lib.host().residual_rms_norm(*args)
+    return RecordedCall.apply(_lib.host().residual_rms_norm, *args) if out is NotImplemented else out
+
+
+class ResidualRMSNorm(nn.Module):
+    """The step between two blocks with its parameters: ``forward(y, residual, gate)`` returns ``(out, z)`` of ``residual_rms_norm``.
+    ``post_norm``: the block's output has a norm of its own; ``scale``: the start value of the residual scale, None for none."""
+
+    def __init__(self, hidden_size: int, post_norm: bool = False, scale: Optional[float] = None, gate_activation: Optional[str] = None,
+                 elementwise_affine: bool = True, eps: float = 1e-6, device=None, dtype=None):
+        super().__init__()
+        if gate_activation not in _GATES:
+            raise ValueError(f'Unsupported activation: {gate_activation}')
+        self.hidden_size, self.post_norm, self.gate_activation, self.eps = hidden_size, post_norm, gate_activation, eps
+        kw = dict(device=device, dtype=dtype)
+        self.register_parameter('weight', nn.Parameter(torch.ones(hidden_size, **kw)) if elementwise_affine else None)
+        self.register_parameter('post_weight', nn.Parameter(torch.ones(hidden_size, **kw)) if elementwise_affine and post_norm else None)
+        self.register_parameter('scale', nn.Parameter(torch.full((hidden_size,), float(scale), **kw)) if scale is not None else None)
+
+    def forward(self, y, residual=None, gate=None):
+        return residual_rms_norm(y, self.weight, residual, self.post_norm, self.post_weight, gate, self.gate_activation if gate is not None else None,
+                                 self.scale, self.eps)

@@ -384,6 +384,91 @@ int b200gdn_layer_norm_bwd(const b200gdn_layer_norm_args* a, void* stream) {
 
 int b200gdn_layer_norm_ctas(int64_t rows) { return gdn::layer_norm_grid(rows); }
 
+static int check_gated_recurrence_args(const b200gdn_gated_recurrence_args* a, const char* who, bool bwd) {
+  using namespace gdn;
+  if (a == nullptr) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: args is NULL", who);
+  if (a->struct_bytes != (int32_t)sizeof(b200gdn_gated_recurrence_args))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: struct_bytes %d != %zu (ABI mismatch)", who, a->struct_bytes,
+                     sizeof(b200gdn_gated_recurrence_args));
+  if (a->rows <= 0 || a->D <= 0 || a->n_seq <= 0 || a->seq_len < 0 || (a->seq_len == 0 && a->n_chunks < 0))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: empty problem (rows=%lld D=%d n_seq=%d seq_len=%d n_chunks=%d)", who, (long long)a->rows, a->D,
+                     a->n_seq, a->seq_len, a->n_chunks);
+  if (a->rows > (1 << 30)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^30 rows", who);
+  if (a->D > (1 << 23)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: D=%d (at most 2^23)", who, a->D);
+  if (a->seq_len > 0 && (int64_t)a->n_seq * a->seq_len > a->rows)
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: %d sequences of %d tokens in %lld rows", who, a->n_seq, a->seq_len, (long long)a->rows);
+  if (a->seq_len == 0) { REQUIRE(a->chunk_meta, who); REQUIRE(a->seq_meta, who); }
+  if (a->dtype < 0 || a->dtype > 2 || (a->gate_dtype != a->dtype && a->gate_dtype != 2))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: dtype codes %d, %d (the gate's is 2 or that of x)", who, a->dtype, a->gate_dtype);
+  if (a->stride_x < a->D || a->stride_g < a->D)
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: strides %lld, %lld of rows of %d", who, (long long)a->stride_x, (long long)a->stride_g, a->D);
+  REQUIRE(a->x, who); REQUIRE(a->g, who);
+  if (!bwd) { REQUIRE(a->h, who); }
+  else { REQUIRE(a->states, who); REQUIRE(a->dx, who); }
+  const uintptr_t size = a->dtype == 2 ? 4 : 2, gate = a->gate_dtype == 2 ? 4 : 2;
+  if (off_boundary(size, {a->x, a->h, a->dh, a->dx}) || off_boundary(gate, {a->g, a->dg}) ||
+      off_boundary(4, {a->h0, a->ht, a->states, a->dht, a->dh0, a->seq_meta, a->seq_order}) || off_boundary(16, {a->chunk_meta}))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: a tensor off its elements' boundary", who);
+  return 0;
+}
+
+int b200gdn_gated_recurrence_fwd(const b200gdn_gated_recurrence_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_gated_recurrence_args(a, "gated_recurrence_fwd", false)) return e;
+  return gdn::launch_gated_recurrence(*a, static_cast<cudaStream_t>(stream), false);
+}
+
+int b200gdn_gated_recurrence_bwd(const b200gdn_gated_recurrence_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_gated_recurrence_args(a, "gated_recurrence_bwd", true)) return e;
+  return gdn::launch_gated_recurrence(*a, static_cast<cudaStream_t>(stream), true);
+}
+
+static int check_rms_norms_args(const b200gdn_rms_norms_args* a, const char* who, bool bwd) {
+  using namespace gdn;
+  if (a == nullptr) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: args is NULL", who);
+  if (a->struct_bytes != (int32_t)sizeof(b200gdn_rms_norms_args))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: struct_bytes %d != %zu (ABI mismatch)", who, a->struct_bytes, sizeof(b200gdn_rms_norms_args));
+  if (a->rows <= 0 || a->D <= 0) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: empty problem (rows=%lld D=%d)", who, (long long)a->rows, a->D);
+  if (a->rows > (1 << 30)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^30 rows", who);
+  if (a->D > (1 << 23)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: D=%d (at most 2^23)", who, a->D);
+  if (a->dtype < 0 || a->dtype > 2 || a->param_dtype < 0 || a->param_dtype > 2)
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: dtype codes %d, %d", who, a->dtype, a->param_dtype);
+  const uint32_t both = B200GDN_NORMS_SIGMOID | B200GDN_NORMS_SILU;
+  if ((a->flags & both) == both || (a->flags & ~(both | B200GDN_NORMS_POST)) != 0)
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: flags %u", who, a->flags);
+  if (a->post_weight != nullptr && !(a->flags & B200GDN_NORMS_POST))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: post_weight without B200GDN_NORMS_POST", who);
+  REQUIRE(a->y, who);
+  if ((a->rstd_y == nullptr) != (a->rstd_z == nullptr)) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: rstd_y and rstd_z come together", who);
+  if (!bwd) { REQUIRE(a->out, who); }
+  else {
+    REQUIRE(a->rstd_z, who);
+    if (a->dweight != nullptr || a->dpost_weight != nullptr || a->dscale != nullptr) REQUIRE(a->partials, who);
+    if (a->dgate != nullptr && a->gate == nullptr) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: dgate without a gate", who);
+  }
+  const uintptr_t size = a->dtype == 2 ? 4 : 2, param_size = a->param_dtype == B200GDN_F32 ? 4 : 2;
+  if (off_boundary(size, {a->y, a->residual, a->gate, a->z, a->out, a->dout, a->dz, a->dy, a->dresidual, a->dgate}) ||
+      off_boundary(param_size, {a->weight, a->post_weight, a->scale, a->dweight, a->dpost_weight, a->dscale}) ||
+      off_boundary(4, {a->rstd_y, a->rstd_z, a->partials}))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: a tensor off its elements' boundary", who);
+  return 0;
+}
+
+int b200gdn_rms_norms_fwd(const b200gdn_rms_norms_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_rms_norms_args(a, "rms_norms_fwd", false)) return e;
+  return gdn::launch_rms_norms(*a, static_cast<cudaStream_t>(stream), false);
+}
+
+int b200gdn_rms_norms_bwd(const b200gdn_rms_norms_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_rms_norms_args(a, "rms_norms_bwd", true)) return e;
+  return gdn::launch_rms_norms(*a, static_cast<cudaStream_t>(stream), true);
+}
+
+int64_t b200gdn_rms_norms_partials(int64_t rows, int32_t D) { return gdn::rms_norms_partials(rows, D); }
+
 // what the two operators on rows of logits have in common
 static int check_rows_of_logits(const char* who, int64_t rows, int64_t inner, int32_t V, int32_t dtype, float scale, const void* logits,
                                 const void* dlogits) {

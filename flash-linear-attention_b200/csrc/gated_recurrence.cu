@@ -1,0 +1,377 @@
+// Gated recurrence, elementwise: h_t = exp(g_t) h_{t-1} + x_t along each sequence, forward and backward.
+//     forward   over R tokens of a warp with a = exp(g): h' = their recurrence from 0 and A = their product of a; entered with s they leave
+//               A s + h'
+//     backward  u_t = a_t (dh_t + u_{t+1}) from the right in the same way; dx_t = dh_t + u_{t+1}, dg_t = dx_t a_t h_{t-1}
+// HBM streaming: what counts is that every tensor is read once.  A CTA owns 32 C neighbouring channels of a sequence and walks it in steps
+// of W R tokens, R for each of its W warps, which hold them in registers (the next step's are on their way meanwhile): each warp joins its
+// own tokens, leaves (A, h') in shared memory, and after one barrier a step goes through the warps ahead of it for the state its first
+// token sees, then through its tokens again.  Where sequences x channels give fewer CTAs than there are SMs, CTAs of a cluster share a
+// sequence: step by step each takes its turn of W R tokens, and their joined pairs go to one another's shared memory.
+// The backward pass does not read h, which is rounded to its type, but forms it again from x in fp32; the forward pass leaves the state
+// ahead of every 64 tokens (a 32nd of x's bytes in bf16) so that this needs no pass of its own from the left.
+#include <cooperative_groups.h>
+
+#include "gdn_common.cuh"
+#include "rowio.cuh"
+
+namespace gdn {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int MOST_WARPS = 16, MOST_RANKS = 8;
+
+// C neighbouring channels of a token, as loaded
+template <typename T, int C>
+struct Piece {
+  using Raw = std::conditional_t<sizeof(T) * C == 8, uint2, std::conditional_t<sizeof(T) * C == 4, uint32_t, uint16_t>>;
+  Raw u;
+  __device__ __forceinline__ void zero() { u = Raw{}; }
+  __device__ __forceinline__ void load(const T* p) { u = __ldcs(reinterpret_cast<const Raw*>(p)); }
+  __device__ __forceinline__ uint64_t pair() const {   // of one channel: the second half is zero
+    if constexpr (C == 1) return pack2((float)*reinterpret_cast<const T*>(&u), 0.f);
+    else if constexpr (sizeof(T) == 2) return widen2<T>(u);
+    else return pack2(__uint_as_float(u.x), __uint_as_float(u.y));
+  }
+  static __device__ __forceinline__ void store(T* p, uint64_t x) {
+    const float2 f = unpack2(x);
+    if constexpr (C == 1) *p = static_cast<T>(f.x);
+    else if constexpr (sizeof(T) == 2) __stcs(reinterpret_cast<uint32_t*>(p), narrow2<T>(x));
+    else __stcs(reinterpret_cast<float2*>(p), f);
+  }
+};
+
+// exp of a pair: 2^n 2^f with n the nearest integer to g log2 e and a polynomial of degree six for 2^f on [-1/2, 1/2] (least squares of the
+// relative error, 2e-9), in pairs of operations.  Off by 1.5 units of 2^-24 at most and 0.1
+// on average where |g| < 1 (beyond, log2 e as a float adds |g| / 4).  The average is what counts here: a
+// channel that remembers a thousand tokens multiplies as many decays, and ex2.approx, which is 0.4 units too small on average (measured),
+// would leave its state off by 2.4e-5.  Below 2^-126.5 the result is zero.
+__device__ __forceinline__ uint64_t decay(uint64_t g) {
+  float2 x = unpack2(g);
+  asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(x.x));   // [-88, 89]: there 2^n is zero, infinity
+  asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(x.y));
+  g = pack2(x.x, x.y);
+  const uint64_t log2e = pack2(1.4426950408889634f, 1.4426950408889634f), bias = pack2(12582912.f, 12582912.f);
+  const uint64_t t = fma2(g, log2e, bias);   // 1.5 2^23 + n: n in the lowest bits
+  const uint64_t f = fma2(g, log2e, fma2(t, pack2(-1.f, -1.f), bias));
+  auto k = [](float c) { return pack2(c, c); };
+  uint64_t p = fma2(k(1.5353350318036973e-4f), f, k(1.3398875016719103e-3f));
+  p = fma2(p, f, k(9.618437848985195e-3f));
+  p = fma2(p, f, k(5.5503323674201965e-2f));
+  p = fma2(p, f, k(0.24022647738456726f));
+  p = fma2(p, f, k(0.6931471824645996f));
+  p = fma2(p, f, k(1.f));
+  const float2 n = unpack2(t);
+  const float lo = __uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u), hi = __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u);
+  return mul2(p, pack2(lo, hi));
+}
+
+struct Span {   // the tokens of a sequence, and the index of its first chunk
+  int64_t first;
+  int len, chunk;
+};
+__device__ __forceinline__ Span span_of(const b200gdn_gated_recurrence_args& a, int seq) {
+  if (a.seq_len > 0) return Span{(int64_t)seq * a.seq_len, a.seq_len, (int)(seq * (int64_t)((a.seq_len + BT - 1) / BT))};
+  const int c = a.seq_meta[2 * seq], n = a.seq_meta[2 * seq + 1];
+  if (n == 0) return Span{0, 0, 0};
+  const ChunkMeta head = load_chunk_meta(a.chunk_meta, c), tail = load_chunk_meta(a.chunk_meta, c + n - 1);
+  return Span{head.row, tail.row + tail.len - head.row, c};
+}
+
+__device__ __forceinline__ uint64_t load_state(const float* p, int64_t at, bool there, bool two) {
+  if (p == nullptr || !there) return 0ull;
+  return pack2(p[at], two ? p[at + 1] : 0.f);
+}
+__device__ __forceinline__ void store_state(float* p, int64_t at, uint64_t x, bool two) {
+  const float2 f = unpack2(x);
+  p[at] = f.x;
+  if (two) p[at + 1] = f.y;
+}
+
+// [0]: the product of the decays, [1]: what the tokens leave of themselves
+struct Joined {
+  uint64_t a, h;
+};
+
+// The two buffers of what the warps, and the CTAs of a cluster, leave for one another.  A buffer is written again two steps later, with
+// another barrier in between that everyone passes after reading it.
+template <bool CLUSTER>
+struct Exchange {
+  ulonglong2 warps[2][MOST_WARPS][32];
+  ulonglong2 ranks[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][32];
+};
+
+// What enters warp `warp` of this CTA, and (in `s`) what leaves the whole step: W warps of each of the cluster's CTAs, from the first
+// one to the last (REVERSE: from the last to the first).
+template <bool CLUSTER, bool REVERSE>
+__device__ __forceinline__ uint64_t join(Exchange<CLUSTER>& x, int turn, int rank, int n_ranks, Joined own, uint64_t& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
+  x.warps[turn][warp][lane] = make_ulonglong2(own.a, own.h);
+  __syncthreads();
+  auto warp_at = [&](int i) { return REVERSE ? W - 1 - i : i; };
+  if constexpr (!CLUSTER) {
+    uint64_t mine = 0ull;
+    for (int i = 0; i < W; ++i) {
+      const int w = warp_at(i);
+      const ulonglong2 p = x.warps[turn][w][lane];
+      if (w == warp) mine = s;
+      s = fma2(p.x, s, p.y);
+    }
+    return mine;
+  } else {
+    Joined ahead = {0, 0}, all = {pack2(1.f, 1.f), 0ull};
+    for (int i = 0; i < W; ++i) {
+      const int w = warp_at(i);
+      const ulonglong2 p = x.warps[turn][w][lane];
+      if (w == warp) ahead = all;
+      all.h = fma2(p.x, all.h, p.y);
+      all.a = mul2(p.x, all.a);
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    if (warp < n_ranks)   // warp i tells CTA i
+      *cluster.map_shared_rank(&x.ranks[turn][rank][lane], warp) = make_ulonglong2(all.a, all.h);
+    for (int i = warp + W; i < n_ranks; i += W) *cluster.map_shared_rank(&x.ranks[turn][rank][lane], i) = make_ulonglong2(all.a, all.h);
+    cluster.sync();
+    uint64_t entering = 0ull;
+    for (int i = 0; i < n_ranks; ++i) {
+      const int r = REVERSE ? n_ranks - 1 - i : i;
+      const ulonglong2 p = x.ranks[turn][r][lane];
+      if (r == rank) entering = s;
+      s = fma2(p.x, s, p.y);
+    }
+    return fma2(ahead.a, entering, ahead.h);
+  }
+}
+
+struct Place {   // of a CTA
+  int seq, channel, rank, n_ranks;
+};
+template <int C, bool CLUSTER>
+__device__ __forceinline__ Place place_of(const b200gdn_gated_recurrence_args& a) {
+  const int tiles = (a.D + 32 * C - 1) / (32 * C);
+  const int n = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
+  const int i = blockIdx.x / n, seq = i / tiles;
+  return Place{a.seq_order ? a.seq_order[seq] : seq, (i % tiles) * 32 * C + (int)(threadIdx.x & 31) * C, CLUSTER ? (int)(blockIdx.x % n) : 0, n};
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------
+template <typename T, typename G, int C, int R, bool CLUSTER>
+__global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_fwd_kernel(const b200gdn_gated_recurrence_args a) {
+  __shared__ Exchange<CLUSTER> exchange;
+  const Place at = place_of<C, CLUSTER>(a);
+  const Span seq = span_of(a, at.seq);
+  const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, step = at.n_ranks * W * R;
+  const bool live = at.channel < a.D, two = C == 2;
+  Piece<T, C> x[R];
+  Piece<G, C> g[R];
+  int t0 = (at.rank * W + warp) * R;
+  auto fetch = [&](int t) {
+    const T* px = static_cast<const T*>(a.x) + (seq.first + t) * a.stride_x + at.channel;
+    const G* pg = static_cast<const G*>(a.g) + (seq.first + t) * a.stride_g + at.channel;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      x[r].zero();   // past the end: a decay of one, and nothing added
+      g[r].zero();
+      if (live && t + r < seq.len) {
+        x[r].load(px + r * a.stride_x);
+        g[r].load(pg + r * a.stride_g);
+      }
+    }
+  };
+  uint64_t s = load_state(a.h0, (int64_t)at.seq * a.D + at.channel, live, two);
+  fetch(t0);
+  const int n = (seq.len + step - 1) / step;
+  for (int i = 0; i < n; ++i, t0 += step) {
+    uint64_t decays[R];
+    Piece<T, C> now[R];
+    Joined own = {pack2(1.f, 1.f), 0ull};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      now[r] = x[r];
+      decays[r] = decay(g[r].pair());
+    }
+    if (i + 1 < n) fetch(t0 + step);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      own.h = fma2(decays[r], own.h, now[r].pair());
+      own.a = mul2(decays[r], own.a);
+    }
+    uint64_t h = join<CLUSTER, false>(exchange, i & 1, at.rank, at.n_ranks, own, s);
+    if (!live) continue;
+    if (a.states && (t0 & (BT - 1)) == 0 && t0 < seq.len) store_state(a.states, (int64_t)(seq.chunk + t0 / BT) * a.D + at.channel, h, two);
+    T* ph = static_cast<T*>(a.h) + (seq.first + t0) * a.D + at.channel;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      h = fma2(decays[r], h, now[r].pair());
+      if (t0 + r < seq.len) Piece<T, C>::store(ph + (int64_t)r * a.D, h);
+    }
+  }
+  if (a.ht && live && at.rank == 0 && warp == 0) store_state(a.ht, (int64_t)at.seq * a.D + at.channel, s, two);
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------
+template <typename T, typename G, int C, int R, bool CLUSTER>
+__global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_bwd_kernel(const b200gdn_gated_recurrence_args a) {
+  __shared__ Exchange<CLUSTER> exchange;
+  __shared__ ulonglong2 left[2][MOST_WARPS][32];   // (product of decays, tokens' own state) of the warps, from the left
+  const Place at = place_of<C, CLUSTER>(a);
+  const Span seq = span_of(a, at.seq);
+  const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = at.n_ranks * W * R;
+  const bool live = at.channel < a.D, two = C == 2;
+  Piece<T, C> x[R], dh[R];
+  Piece<G, C> g[R];
+  uint64_t start;   // the state ahead of the 64 tokens that this warp's belong to (of one token's warps: ahead of its step)
+  const int n = (seq.len + step - 1) / step;
+  int t0 = ((n - 1) * at.n_ranks + at.rank) * W * R + warp * R;
+  // a step's 64-token blocks begin with it: W R is a multiple of 64, or a CTA's only step begins at the sequence's first token
+  const int in_block = min(W, BT / R), first_warp = warp / in_block * in_block;
+  auto fetch = [&](int t) {
+    const T* px = static_cast<const T*>(a.x) + (seq.first + t) * a.stride_x + at.channel;
+    const G* pg = static_cast<const G*>(a.g) + (seq.first + t) * a.stride_g + at.channel;
+    const T* pd = static_cast<const T*>(a.dh) + (seq.first + t) * a.D + at.channel;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      x[r].zero();
+      g[r].zero();
+      dh[r].zero();
+      if (live && t + r < seq.len) {
+        x[r].load(px + r * a.stride_x);
+        g[r].load(pg + r * a.stride_g);
+        if (a.dh) dh[r].load(pd + (int64_t)r * a.D);
+      }
+    }
+    start = load_state(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, live && t < seq.len, two);
+  };
+  uint64_t s = load_state(a.dht, (int64_t)at.seq * a.D + at.channel, live, two);
+  if (n > 0) fetch(t0);
+  for (int i = 0; i < n; ++i, t0 -= step) {
+    uint64_t decays[R], kept[R];
+    Piece<T, C> up[R];
+    uint64_t h = start;
+    Joined own = {pack2(1.f, 1.f), 0ull};
+    uint64_t own_left = 0ull;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      decays[r] = decay(g[r].pair());
+      up[r] = dh[r];
+      kept[r] = x[r].pair();
+    }
+    if (i + 1 < n) fetch(t0 - step);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      own_left = fma2(decays[r], own_left, kept[r]);
+      own.a = mul2(decays[r], own.a);
+      const int q = R - 1 - r;
+      own.h = mul2(decays[q], add2(up[q].pair(), own.h));
+    }
+    left[i & 1][warp][lane] = make_ulonglong2(own.a, own_left);
+    uint64_t u = join<CLUSTER, true>(exchange, i & 1, at.rank, at.n_ranks, own, s);
+    for (int w = first_warp; w < warp; ++w) {
+      const ulonglong2 p = left[i & 1][w][lane];
+      h = fma2(p.x, h, p.y);
+    }
+    if (!live) continue;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint64_t from_before = mul2(decays[r], h);
+      h = fma2(decays[r], h, kept[r]);
+      kept[r] = from_before;
+    }
+    T* px = static_cast<T*>(a.dx) + (seq.first + t0) * a.D + at.channel;
+    G* pg = static_cast<G*>(a.dg) + (seq.first + t0) * a.D + at.channel;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const int r = R - 1 - q;
+      const uint64_t d = add2(up[r].pair(), u);
+      u = mul2(decays[r], d);
+      if (t0 + r < seq.len) {
+        Piece<T, C>::store(px + (int64_t)r * a.D, d);
+        if (a.dg) Piece<G, C>::store(pg + (int64_t)r * a.D, mul2(d, kept[r]));
+      }
+    }
+  }
+  if (a.dh0 && live && at.rank == 0 && warp == 0) store_state(a.dh0, (int64_t)at.seq * a.D + at.channel, s, two);
+}
+
+// ---- one token a sequence ------------------------------------------------------------------------------------------------
+template <typename T, typename G, int C>
+__global__ void __launch_bounds__(128) recurrence_step_kernel(const b200gdn_gated_recurrence_args a) {
+  const int d = (blockIdx.x * 128 + threadIdx.x) * C;
+  if (d >= a.D) return;
+  for (int seq = blockIdx.y; seq < a.n_seq; seq += gridDim.y) {
+    Piece<T, C> x;
+    Piece<G, C> g;
+    x.load(static_cast<const T*>(a.x) + (int64_t)seq * a.stride_x + d);
+    g.load(static_cast<const G*>(a.g) + (int64_t)seq * a.stride_g + d);
+    const int64_t at = (int64_t)seq * a.D + d;
+    const uint64_t before = load_state(a.h0, at, true, C == 2), h = fma2(decay(g.pair()), before, x.pair());
+    if (a.states) store_state(a.states, at, before, C == 2);
+    Piece<T, C>::store(static_cast<T*>(a.h) + at, h);
+    if (a.ht) store_state(a.ht, at, h, C == 2);
+  }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------------
+template <typename Kern>
+int launch_walk(Kern kern, const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, int C) {
+  const int64_t ctas = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)) * ranks;
+  if (ctas > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 pieces of work", what);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(W * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  (void)cudaLaunchKernelEx(&cfg, kern, a);   // (an error is check_launch's to name)
+  return check_launch(what);
+}
+
+template <typename T, typename G, int C>
+int launch_c(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd) {
+  if (!bwd && a.seq_len == 1) {
+    const int n = a.n_seq < 65535 ? a.n_seq : 65535;
+    recurrence_step_kernel<T, G, C><<<dim3((a.D + 128 * C - 1) / (128 * C), n), 128, 0, st>>>(a);
+    return check_launch("recurrence_step");
+  }
+  constexpr int R = 8;
+  const int64_t tokens = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT / a.n_seq + 1;   // of a sequence, on average
+  int W = 1;
+  while (W < MOST_WARPS && W * R < tokens) W *= 2;
+  if (bwd && a.seq_len == 0 && W * R < BT) W = BT / R;   // a sequence may be longer than the others: its steps begin where chunks do
+  const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)), most = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT;
+  int ranks = 1;
+  while (ranks < MOST_RANKS && work * ranks * 2 <= sm_count() && (int64_t)ranks * 2 * W * R <= most) ranks *= 2;
+  if (ranks > 1)
+    return bwd ? launch_walk(recurrence_bwd_kernel<T, G, C, R, true>, "recurrence_bwd", a, st, W, ranks, C)
+               : launch_walk(recurrence_fwd_kernel<T, G, C, R, true>, "recurrence_fwd", a, st, W, ranks, C);
+  return bwd ? launch_walk(recurrence_bwd_kernel<T, G, C, R, false>, "recurrence_bwd", a, st, W, 1, C)
+             : launch_walk(recurrence_fwd_kernel<T, G, C, R, false>, "recurrence_fwd", a, st, W, 1, C);
+}
+
+// two channels a thread where every row of every tensor allows it
+template <typename T, typename G>
+int launch_tg(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd) {
+  auto bits = [](std::initializer_list<const void*> all) {
+    uintptr_t b = 0;
+    for (const void* p : all) b |= reinterpret_cast<uintptr_t>(p);
+    return b;
+  };
+  const bool pairs = ((a.D | a.stride_x | a.stride_g) & 1) == 0 && bits({a.x, a.h, a.dh, a.dx}) % (2 * sizeof(T)) == 0 &&
+                     bits({a.g, a.dg}) % (2 * sizeof(G)) == 0;
+  return pairs ? launch_c<T, G, 2>(a, st, bwd) : launch_c<T, G, 1>(a, st, bwd);
+}
+
+}  // namespace
+
+int launch_gated_recurrence(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd) {
+  const bool wide = a.gate_dtype == 2;
+  if (a.dtype == 2) return launch_tg<float, float>(a, st, bwd);
+  if (a.dtype == 0) return wide ? launch_tg<__nv_bfloat16, float>(a, st, bwd) : launch_tg<__nv_bfloat16, __nv_bfloat16>(a, st, bwd);
+  return wide ? launch_tg<__half, float>(a, st, bwd) : launch_tg<__half, __half>(a, st, bwd);
+}
+
+}  // namespace gdn

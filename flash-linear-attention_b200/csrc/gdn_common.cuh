@@ -153,6 +153,10 @@ int launch_norm_gate(const b200gdn_norm_gate_args& a, cudaStream_t st, bool bwd)
 int norm_gate_grid(int64_t rows);
 int launch_layer_norm(const b200gdn_layer_norm_args& a, cudaStream_t st, bool bwd);
 int layer_norm_grid(int64_t rows);
+int launch_gated_recurrence(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd);
+int launch_rms_norms(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd);
+int rms_norms_grid(int64_t rows);
+int64_t rms_norms_partials(int64_t rows, int D);
 int64_t logprob_workspace(int64_t rows, int V, int dtype, int top_k);
 int launch_logprob(const b200gdn_logprob_args& a, cudaStream_t st, bool bwd);
 int64_t distill_workspace(int64_t rows, int V, int dtype, int K);

@@ -922,6 +922,281 @@ class LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
   }
 };
 
+// ---- gated recurrence ------------------------------------------------------------------------------------------
+struct RecurrenceSaved : torch::CustomClassHolder {
+  PlanPtr plan;   // null: sequences of one length
+  bool has_h0 = false, want_x = false, want_g = false, want_h0 = false;
+  at::ScalarType gt = at::kFloat, ht = at::kFloat;
+};
+
+struct RecurrenceForward {
+  Tensor h, final_state, x, g, states;
+};
+
+// [B, T, D] as rows of one distance, which is returned: x itself where it lies so, else a copy
+Tensor token_rows(const Tensor& x, int64_t& stride) {
+  const int64_t B = x.size(0), T = x.size(1), D = x.size(2);
+  stride = T > 1 ? x.stride(1) : B > 1 ? x.stride(0) : D;
+  const bool as_it_is = (D == 1 || x.stride(2) == 1) && stride >= D && (B == 1 || T == 1 || x.stride(0) == T * stride);
+  if (as_it_is) return x;
+  stride = D;
+  return x.contiguous();
+}
+
+b200gdn_gated_recurrence_args recurrence_args(const Tensor& x, const Tensor& g, int64_t n_seq, const Plan* plan) {
+  b200gdn_gated_recurrence_args a{};
+  a.D = (int32_t)x.size(2);
+  a.rows = x.size(0) * x.size(1);
+  a.n_seq = (int32_t)n_seq;
+  if (plan) {
+    a.n_chunks = plan->n_chunks;
+    a.chunk_meta = iptr(plan->chunk_meta);
+    a.seq_meta = iptr(plan->seq_meta);
+    a.seq_order = iptr(plan->seq_order);
+  } else {
+    a.seq_len = (int32_t)x.size(1);
+    a.n_chunks = (int32_t)(n_seq * ((x.size(1) + B200GDN_CHUNK - 1) / B200GDN_CHUNK));
+  }
+  a.dtype = act_code(x.scalar_type());
+  a.gate_dtype = act_code(g.scalar_type());
+  token_rows(x, a.stride_x);
+  token_rows(g, a.stride_g);
+  a.x = ptr(x);
+  a.g = ptr(g);
+  return a;
+}
+
+RecurrenceForward recurrence_forward(const Tensor& x_in, const Tensor& g_in, const Tensor& initial_state, bool output_final_state, bool inplace_state,
+                                     const PlanPtr& plan, bool need_grad) {
+  RecurrenceForward r;
+  const at::Device dev = x_in.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const at::ScalarType t = x_in.scalar_type();
+  const int64_t D = x_in.size(2), n_seq = plan ? plan->n_seq : x_in.size(0), tokens = x_in.size(1);
+  int64_t stride;
+  r.x = token_rows(x_in, stride);
+  r.g = token_rows(g_in.scalar_type() == t ? g_in : cast(g_in, at::kFloat), stride);
+  const Tensor h0 = dense_state(initial_state, at::kFloat);
+  r.h = new_tensor(x_in.sizes(), t, dev, plan && !plan->covered);
+  if (output_final_state) {
+    if (inplace_state) {
+      if (!h0.defined() || h0.data_ptr() != initial_state.data_ptr())
+        raise("gated_recurrence: inplace_state needs a contiguous initial_state in fp32");
+      r.final_state = initial_state;
+    } else {
+      r.final_state = new_tensor({n_seq, D}, at::kFloat, dev);
+    }
+  }
+  const int64_t n_chunks = plan ? plan->n_chunks : n_seq * ((tokens + B200GDN_CHUNK - 1) / B200GDN_CHUNK);
+  if (need_grad) r.states = new_tensor({n_chunks, D}, at::kFloat, dev);
+  if (n_chunks == 0) {   // no token: the states stay as they are
+    if (r.final_state.defined() && !inplace_state) {
+      if (h0.defined()) r.final_state.copy_(h0);
+      else r.final_state.zero_();
+    }
+    return r;
+  }
+  b200gdn_gated_recurrence_args a = recurrence_args(r.x, r.g, n_seq, plan.get());
+  a.h0 = fptr(h0);
+  a.h = ptr(r.h);
+  a.ht = fptr(r.final_state);
+  a.states = fptr(r.states);
+  if (plan) in_use(plan);
+  call("b200gdn_gated_recurrence_fwd", b200gdn_gated_recurrence_fwd, a);
+  return r;
+}
+
+class RecurrenceFunction : public torch::autograd::Function<RecurrenceFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const std::optional<Tensor>& initial_state,
+                               bool output_final_state, const PlanPtr& plan) {
+    const Tensor h0 = val(initial_state);
+    RecurrenceForward r = recurrence_forward(x, g, h0, output_final_state, false, plan, true);
+    auto s = c10::make_intrusive<RecurrenceSaved>();
+    s->plan = plan;
+    s->has_h0 = h0.defined();
+    s->want_x = x.requires_grad();
+    s->want_g = g.requires_grad();
+    s->want_h0 = h0.defined() && h0.requires_grad();
+    s->gt = g.scalar_type();
+    if (h0.defined()) s->ht = h0.scalar_type();
+    ctx->save_for_backward({r.x, r.g, r.states});
+    ctx->saved_data["s"] = at::IValue::make_capsule(s);
+    ctx->set_materialize_grads(false);
+    if (r.final_state.defined()) return {r.h, r.final_state};
+    return {r.h};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &g = saved[1], &states = saved[2];
+    const auto capsule = ctx->saved_data["s"].toCapsule();
+    const RecurrenceSaved& s = *static_cast<const RecurrenceSaved*>(capsule.get());
+    const at::Device dev = x.device();
+    c10::cuda::CUDAGuard guard(dev);
+    const at::ScalarType t = x.scalar_type();
+    const int64_t D = x.size(2), n_seq = s.plan ? s.plan->n_seq : x.size(0);
+    const bool uncovered = s.plan && !s.plan->covered;
+    const Tensor dh = grads[0].defined() ? dense(grads[0], t) : Tensor();
+    const Tensor dht = grads.size() > 1 && grads[1].defined() ? dense(grads[1], at::kFloat) : Tensor();
+    Tensor dx = new_tensor(x.sizes(), t, dev, uncovered), dg, dh0;
+    if (s.want_g) dg = new_tensor(g.sizes(), g.scalar_type(), dev, uncovered);
+    if (s.want_h0) dh0 = new_tensor({n_seq, D}, at::kFloat, dev);
+    if (states.numel() == 0) {   // no token
+      if (dh0.defined()) {
+        if (dht.defined()) dh0.copy_(dht);
+        else dh0.zero_();
+      }
+    } else {
+      b200gdn_gated_recurrence_args a = recurrence_args(x, g, n_seq, s.plan.get());
+      a.states = fptr(states);
+      a.dh = ptr(dh);
+      a.dht = fptr(dht);
+      a.dx = ptr(dx);
+      a.dg = ptr(dg);
+      a.dh0 = fptr(dh0);
+      if (s.plan) in_use(s.plan);
+      call("b200gdn_gated_recurrence_bwd", b200gdn_gated_recurrence_bwd, a);
+    }
+    return once("gated_recurrence", {s.want_x ? dx : Tensor(), cast(dg, s.gt), dh0.defined() ? cast(dh0, s.ht) : Tensor(), Tensor(), Tensor()});
+  }
+};
+
+// ---- the RMS norms either side of a block ------------------------------------------------------------------------
+struct NormsCall {   // what the forward and the backward pass are given alike
+  Tensor y, residual, gate, w, post, scale;
+  int32_t param_dtype = 0;
+  uint32_t flags = 0;
+  double alpha = 1, eps = 0;
+
+  b200gdn_rms_norms_args args() const {
+    b200gdn_rms_norms_args a{};
+    a.D = (int32_t)y.size(-1);
+    a.rows = y.numel() / y.size(-1);
+    a.dtype = act_code(y.scalar_type());
+    a.param_dtype = param_dtype;
+    a.flags = flags;
+    a.eps = (float)eps;
+    a.alpha = (float)alpha;
+    a.y = ptr(y);
+    a.residual = ptr(residual);
+    a.gate = ptr(gate);
+    a.weight = ptr(w);
+    a.post_weight = ptr(post);
+    a.scale = ptr(scale);
+    return a;
+  }
+};
+
+// weight, post_weight and scale in one element type the kernels read: their own where it is common, else fp32
+int norms_param_types(Tensor& w, Tensor& post, Tensor& scale) {
+  int code = -2;
+  for (const Tensor* p : {&w, &post, &scale}) {
+    if (!p->defined()) continue;
+    const int c = param_code(p->scalar_type());
+    code = code == -2 || code == c ? c : -1;
+  }
+  if (code == -2) return B200GDN_F32;
+  for (Tensor* p : {&w, &post, &scale}) *p = code < 0 ? dense(*p, at::kFloat) : dense(*p);
+  return code < 0 ? B200GDN_F32 : code;
+}
+at::ScalarType norms_param_type(int32_t code) { return code == B200GDN_F32 ? at::kFloat : code == B200GDN_BF16 ? at::kBFloat16 : at::kHalf; }
+
+struct NormsForward {
+  NormsCall call;
+  Tensor out, z, rstd;   // rstd [2, rows]
+};
+
+NormsForward norms_forward(const Tensor& y, const Tensor& weight, const Tensor& residual, const Tensor& post, const Tensor& gate, const Tensor& scale,
+                           uint32_t flags, double alpha, double eps, bool need_grad) {
+  NormsForward r;
+  const at::Device dev = y.device();
+  c10::cuda::CUDAGuard guard(dev);
+  NormsCall& c = r.call;
+  c.y = dense(y);
+  c.residual = dense(residual);
+  c.gate = dense(gate);
+  c.w = weight;
+  c.post = post;
+  c.scale = scale;
+  c.param_dtype = norms_param_types(c.w, c.post, c.scale);
+  c.flags = flags;
+  c.alpha = alpha;
+  c.eps = eps;
+  const int64_t rows = y.numel() / y.size(-1);
+  r.out = new_tensor(y.sizes(), y.scalar_type(), dev);
+  r.z = new_tensor(y.sizes(), y.scalar_type(), dev);
+  if (need_grad) r.rstd = new_tensor({2, rows}, at::kFloat, dev);
+  if (rows == 0) return r;
+  b200gdn_rms_norms_args a = c.args();
+  a.z = ptr(r.z);
+  a.out = ptr(r.out);
+  a.rstd_y = fptr(r.rstd);
+  a.rstd_z = need_grad ? fptr(r.rstd) + rows : nullptr;
+  call("b200gdn_rms_norms_fwd", b200gdn_rms_norms_fwd, a);
+  return r;
+}
+
+class NormsFunction : public torch::autograd::Function<NormsFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& y, const std::optional<Tensor>& weight, const std::optional<Tensor>& residual,
+                               const std::optional<Tensor>& post, const std::optional<Tensor>& gate, const std::optional<Tensor>& scale, int64_t flags,
+                               double alpha, double eps) {
+    const Tensor w = val(weight), res = val(residual), p = val(post), g = val(gate), sc = val(scale);
+    NormsForward r = norms_forward(y, w, res, p, g, sc, (uint32_t)flags, alpha, eps, true);
+    const NormsCall& c = r.call;
+    ctx->save_for_backward({c.y, c.residual, c.gate, c.w, c.post, c.scale, r.rstd});
+    auto ty = [](const Tensor& t) { return (int64_t)(t.defined() ? t.scalar_type() : at::kFloat); };
+    auto wanted = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    ctx->saved_data["s"] = std::vector<int64_t>{c.param_dtype, flags, wanted(y), wanted(w), wanted(res), wanted(p), wanted(g), wanted(sc), ty(w), ty(p), ty(sc)};
+    ctx->saved_data["alpha"] = alpha;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    return {r.out, r.z};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto s = ctx->saved_data["s"].toIntVector();
+    NormsCall c;
+    c.y = saved[0], c.residual = saved[1], c.gate = saved[2], c.w = saved[3], c.post = saved[4], c.scale = saved[5];
+    const Tensor& rstd = saved[6];
+    c.param_dtype = (int32_t)s[0];
+    c.flags = (uint32_t)s[1];
+    c.alpha = ctx->saved_data["alpha"].toDouble();
+    c.eps = ctx->saved_data["eps"].toDouble();
+    const at::Device dev = c.y.device();
+    c10::cuda::CUDAGuard guard(dev);
+    const at::ScalarType t = c.y.scalar_type(), pt = norms_param_type(c.param_dtype);
+    const int64_t D = c.y.size(-1), rows = c.y.numel() / D;
+    const Tensor dout = grads[0].defined() ? dense(grads[0], t) : Tensor(), dz = grads[1].defined() ? dense(grads[1], t) : Tensor();
+    auto rows_of = [&](bool wanted) { return wanted ? new_tensor(c.y.sizes(), t, dev) : Tensor(); };
+    auto vector = [&](bool wanted) { return wanted ? new_tensor({D}, pt, dev, rows == 0) : Tensor(); };
+    // where the block's output goes into the sum as it is, its gradient is the residual's
+    const bool same = !(c.flags & B200GDN_NORMS_POST) && !c.gate.defined() && !c.scale.defined() && c.alpha == 1.0;
+    Tensor dy = rows_of(s[2] || (same && s[4])), dres = rows_of(s[4] && !same), dgate = rows_of(s[6]);
+    Tensor dw = vector(s[3]), dpost = vector(s[5]), dscale = vector(s[7]), partials;
+    if (rows > 0) {
+      b200gdn_rms_norms_args a = c.args();
+      if (s[3] || s[5] || s[7]) partials = new_tensor({b200gdn_rms_norms_partials(rows, (int32_t)D)}, at::kFloat, dev);
+      a.rstd_y = fptr(rstd);
+      a.rstd_z = fptr(rstd) + rows;
+      a.dout = ptr(dout);
+      a.dz = ptr(dz);
+      a.dy = ptr(dy);
+      a.dresidual = ptr(dres);
+      a.dgate = ptr(dgate);
+      a.dweight = ptr(dw);
+      a.dpost_weight = ptr(dpost);
+      a.dscale = ptr(dscale);
+      a.partials = fptr(partials);
+      call("b200gdn_rms_norms_bwd", b200gdn_rms_norms_bwd, a);
+    }
+    return once("residual_rms_norm", {s[2] ? dy : Tensor(), cast(dw, (at::ScalarType)s[8]), s[4] ? (same ? dy : dres) : Tensor(), cast(dpost, (at::ScalarType)s[9]),
+                                      dgate, cast(dscale, (at::ScalarType)s[10]), Tensor(), Tensor(), Tensor()});
+  }
+};
+
 // ---- rows of logits --------------------------------------------------------------------------------------------
 // The rows as the kernels address them: row r at (r / inner) outer + (r % inner) step.  Slices of a sequence or of a padded
 // vocabulary are read where they lie; what has more levels is copied.
@@ -1385,6 +1660,93 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// residual_rms_norm(y, weight, residual, post_weight, gate, scale, flags, alpha, eps) -> (out, z); NotImplemented while a trace is recorded
+PyObject* py_residual_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(9);
+  if (tracing()) Py_RETURN_NOTIMPLEMENTED;
+  Tensor y, w, res, post, gate, scale;
+  if (!get(args[0], y) || !get(args[1], w) || !get(args[2], res) || !get(args[3], post) || !get(args[4], gate) || !get(args[5], scale) || !y.defined()) {
+    PyErr_SetString(PyExc_TypeError, "residual_rms_norm: a tensor is expected");
+    return nullptr;
+  }
+  const int64_t flags = PyLong_AsLongLong(args[6]);
+  const double alpha = PyFloat_AsDouble(args[7]), eps = PyFloat_AsDouble(args[8]);
+  if (PyErr_Occurred()) return nullptr;
+  Tensor out, z;
+  {
+    NoGil nogil;
+    const std::string who = "residual_rms_norm: ";
+    if (act_code(y.scalar_type()) < 0) raise(who + "dtype " + c10::toString(y.scalar_type()) + " is not supported");
+    if (y.dim() == 0 || y.size(-1) == 0) raise(who + "rows without elements");
+    if (y.size(-1) > (1 << 23)) raise(who + "rows of more than 2^23 elements");
+    for (const Tensor* p : {&w, &post, &scale}) {
+      if (p->defined() && (p->dim() != 1 || p->size(0) != y.size(-1) || !p->is_floating_point()))
+        raise(who + "weight, post_weight and scale are vectors of the " + std::to_string(y.size(-1)) + " elements of a row");
+      check("a parameter", *p, 0, y.device());
+    }
+    for (const Tensor* p : {&res, &gate}) {
+      if (p->defined() && (p->sizes() != y.sizes() || p->scalar_type() != y.scalar_type())) raise(who + "residual and gate have the shape and the type of the block's output");
+      check("residual or gate", *p, 0, y.device());
+    }
+    if (wants_grad({&y, &w, &res, &post, &gate, &scale})) {
+      variable_list r = NormsFunction::apply(y, opt(w), opt(res), opt(post), opt(gate), opt(scale), flags, alpha, eps);
+      out = r[0];
+      z = r[1];
+    } else {
+      NormsForward r = norms_forward(y, w, res, post, gate, scale, (uint32_t)flags, alpha, eps, false);
+      out = r.out;
+      z = r.z;
+    }
+  }
+  return wrap_pair(out, z);
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_recurrence(x, g, initial_state, output_final_state, inplace_state, plan or None) -> (h, final_state); NotImplemented while a
+// trace is recorded
+PyObject* py_gated_recurrence(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(6);
+  if (tracing()) Py_RETURN_NOTIMPLEMENTED;
+  Tensor x, g, h0;
+  if (!get(args[0], x) || !get(args[1], g) || !get(args[2], h0) || !x.defined() || !g.defined()) {
+    PyErr_SetString(PyExc_TypeError, "gated_recurrence: a tensor is expected");
+    return nullptr;
+  }
+  const bool out_state = truth(args[3]), inplace = truth(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  PlanPtr plan;
+  if (args[5] != Py_None) plan = plan_of(args[5]);
+  Tensor h, fin;
+  {
+    NoGil nogil;
+    if (act_code(x.scalar_type()) < 0) raise(std::string("gated_recurrence: dtype ") + c10::toString(x.scalar_type()) + " is not supported");
+    if (x.dim() != 3 || x.size(2) == 0) raise("gated_recurrence: x is [batch, tokens, channels]");
+    if (g.sizes() != x.sizes() || !g.is_floating_point()) raise("gated_recurrence: g has the shape of x");
+    if (x.size(2) > (1 << 23)) raise("gated_recurrence: more than 2^23 channels");
+    if (x.size(0) > (1 << 30) || x.size(1) > (1 << 30) || x.size(0) * x.size(1) > (1 << 30)) raise("gated_recurrence: more than 2^30 tokens");
+    const int64_t n_seq = plan ? plan->n_seq : x.size(0);
+    if (h0.defined() && (h0.dim() != 2 || h0.size(0) != n_seq || h0.size(1) != x.size(2) || !h0.is_floating_point()))
+      raise("gated_recurrence: initial_state is [" + std::to_string(n_seq) + ", " + std::to_string(x.size(2)) + "], a state a sequence");
+    check("g", g, x.numel(), x.device());
+    check("initial_state", h0, 0, x.device());
+    if (wants_grad({&x, &g, &h0})) {
+      if (inplace && out_state) raise("gated_recurrence: inplace_state where gradients are asked for");
+      variable_list out = RecurrenceFunction::apply(x, g, opt(h0), out_state, plan);
+      h = out[0];
+      if (out.size() > 1) fin = out[1];
+    } else {
+      RecurrenceForward r = recurrence_forward(x, g, h0, out_state, inplace, plan, false);
+      if (inplace && out_state && !r.final_state.is_inference()) torch::autograd::impl::bump_version(r.final_state);
+      h = r.h;
+      fin = r.final_state;
+    }
+  }
+  return wrap_pair(h, fin);
+  END_HANDLE_TH_ERRORS
+}
+
 void check_logits(const char* who, const Tensor& logits) {
   if (act_code(logits.scalar_type()) < 0) raise(std::string(who) + ": dtype " + c10::toString(logits.scalar_type()) + " is not supported");
   if (logits.dim() == 0 || logits.size(-1) == 0) raise(std::string(who) + ": a vocabulary without entries");
@@ -1551,6 +1913,8 @@ PyMethodDef methods[] = {
     {"conv", FAST(py_conv), "short causal convolution, differentiable"},
     {"norm_gate", FAST(py_norm_gate), "gated RMS norm, differentiable"},
     {"layer_norm", FAST(py_layer_norm), "layer norm with the residual sum, differentiable"},
+    {"residual_rms_norm", FAST(py_residual_rms_norm), "RMS norms either side of a block with gate, scale and residual sum, differentiable"},
+    {"gated_recurrence", FAST(py_gated_recurrence), "elementwise gated recurrence, differentiable"},
     {"logprob", FAST(py_logprob), "log probabilities, entropy and top entries of rows of logits, differentiable"},
     {"distill", FAST(py_distill), "divergence from a teacher's top entries, differentiable"},
     {"plan", FAST(py_plan), "chunk tables (and split plan) of a shape as one handle"},

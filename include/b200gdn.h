@@ -417,6 +417,84 @@ int b200gdn_layer_norm_fwd(const b200gdn_layer_norm_args* args, void* stream);
 int b200gdn_layer_norm_bwd(const b200gdn_layer_norm_args* args, void* stream);
 int b200gdn_layer_norm_ctas(int64_t rows);
 
+/* Gated recurrence, elementwise over D channels and token by token along each sequence:
+ *   h_t = exp(g_t) h_{t-1} + x_t,   h_{-1} = h0 (or 0)
+ * and, with dh the upstream gradient of h and dht that of the last state of each sequence,
+ *   dx_t = dh_t + exp(g_{t+1}) dx_{t+1} (+ dht at the last token),   dg_t = dx_t exp(g_t) h_{t-1},   dh0 = exp(g_0) dx_0
+ * g is a logarithm of a decay; above 0 the products of exp(g) over neighbouring tokens have to stay within fp32's range.  States are fp32.
+ * Sequences: seq_len > 0: n_seq of that many tokens, one behind the other, without tables; else the tables of the chunk passes, whose
+ * 64-token chunks n_chunks counts.  Rows that no sequence covers are neither read nor written.  ht may be h0 itself. */
+typedef struct b200gdn_gated_recurrence_args {
+  int32_t struct_bytes;
+  int32_t D;
+  int64_t rows;                  /* token rows of the tensors */
+  int32_t n_seq, seq_len, n_chunks;
+  int32_t dtype;                 /* 0 = bf16, 1 = fp16, 2 = fp32: x, h, dh, dx */
+  int32_t gate_dtype;            /* the same codes: g, dg; that of x, or 2 */
+  int32_t reserved;
+  int64_t stride_x, stride_g;    /* elements from one row of x (of g) to the next; all else is contiguous */
+  const int32_t* chunk_meta;     /* with seq_len = 0 */
+  const int32_t* seq_meta;
+  const int32_t* seq_order;      /* [n_seq] or NULL: the order in which the sequences are taken */
+  const void* x;                 /* [rows, D] */
+  const void* g;                 /* [rows, D] */
+  const float* h0;               /* [n_seq, D] or NULL: zeros */
+  void* h;                       /* [rows, D] (forward) */
+  float* ht;                     /* [n_seq, D] or NULL (forward) */
+  float* states;                 /* [n_chunks, D]: the state ahead of each chunk; written by the forward pass (NULL: not wanted), read by the backward pass */
+  const void* dh;                /* [rows, D] or NULL: zeros */
+  const float* dht;              /* [n_seq, D] or NULL: zeros */
+  void* dx;                      /* [rows, D] */
+  void* dg;                      /* [rows, D] or NULL */
+  float* dh0;                    /* [n_seq, D] or NULL */
+} b200gdn_gated_recurrence_args;
+int b200gdn_gated_recurrence_fwd(const b200gdn_gated_recurrence_args* args, void* stream);
+int b200gdn_gated_recurrence_bwd(const b200gdn_gated_recurrence_args* args, void* stream);
+
+/* The RMS norms either side of a block over rows of D, with the block's gate, its residual scale and the residual sum.  y is the block's output:
+ *   p = y r1 post_weight, r1 = 1/sqrt(mean(y^2) + eps)   (B200GDN_NORMS_POST; else p = y)
+ *   z = residual + alpha scale act(gate) p;   r2 = 1/sqrt(mean(z^2) + eps);   out = z r2 weight
+ * act is the sigmoid, the SiLU or, without a flag, the gate as it is; no gate, scale, weight or residual: ones and zeros.  z is normalised
+ * in fp32, as it is summed; what is stored is rounded.  Gradients, of the out and the z that were handed on (either may be NULL: zeros):
+ *   h = dout weight;  e = dz + r2 (h - z r2 mean(h z r2)) = dresidual;  dgate = e alpha scale p act'(gate);
+ *   f = e alpha scale act(gate) post_weight;  dy = r1 (f - y r1 mean(f y r1))  (without the norm: f);
+ *   dweight = sum of dout z r2;  dpost_weight = sum of e alpha scale act(gate) y r1;  dscale = sum of e alpha act(gate) p
+ * Tensors need no alignment beyond their elements' own; on 16-byte boundaries (fp32 parameters included) they are read fastest. */
+#define B200GDN_NORMS_POST 1u
+#define B200GDN_NORMS_SIGMOID 2u
+#define B200GDN_NORMS_SILU 4u
+typedef struct b200gdn_rms_norms_args {
+  int32_t struct_bytes;
+  int32_t D;
+  int64_t rows;
+  int32_t dtype;                 /* 0 = bf16, 1 = fp16, 2 = fp32: the [rows, D] tensors, which are contiguous */
+  int32_t param_dtype;           /* B200GDN_F32 / BF16 / F16: weight, post_weight, scale and their gradients */
+  uint32_t flags;
+  float eps, alpha;
+  const void* y;                 /* [rows, D] */
+  const void* residual;          /* [rows, D] or NULL */
+  const void* gate;              /* [rows, D] or NULL */
+  const void* weight;            /* [D] or NULL */
+  const void* post_weight;       /* [D] or NULL (only with B200GDN_NORMS_POST) */
+  const void* scale;             /* [D] or NULL */
+  void* z;                       /* [rows, D] or NULL (forward) */
+  void* out;                     /* [rows, D] (forward) */
+  float* rstd_y;                 /* [rows]: r1 and r2, written by the forward pass (NULL: not wanted), read by the backward pass */
+  float* rstd_z;                 /* [rows] */
+  const void* dout;              /* [rows, D] or NULL */
+  const void* dz;                /* [rows, D] or NULL */
+  void* dy;                      /* [rows, D] or NULL, as all gradients */
+  void* dresidual;               /* [rows, D] */
+  void* dgate;                   /* [rows, D] */
+  void* dweight;                 /* [D] */
+  void* dpost_weight;            /* [D] */
+  void* dscale;                  /* [D] */
+  float* partials;               /* b200gdn_rms_norms_partials(rows, D) floats, with any of the last three */
+} b200gdn_rms_norms_args;
+int b200gdn_rms_norms_fwd(const b200gdn_rms_norms_args* args, void* stream);
+int b200gdn_rms_norms_bwd(const b200gdn_rms_norms_args* args, void* stream);
+int64_t b200gdn_rms_norms_partials(int64_t rows, int32_t D);
+
 /* Rows of logits over a vocabulary of V.  Row r starts at element (r / inner) stride_outer + (r % inner) stride_inner; the
  * entries of a row lie side by side and need no alignment beyond their own.  scale = 1 / temperature; with m the largest entry:
  *   lp_j = scale (x_j - m) - log(sum exp(scale (x - m)));  p = exp(lp)
