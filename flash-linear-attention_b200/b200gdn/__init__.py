@@ -9,8 +9,8 @@ from .chunk import chunk_gated_delta_rule, chunk_gdn
 from .fused_recurrent import fused_recurrent_gated_delta_rule, fused_recurrent_gdn
 from .cp import FLACPContext, build_cp_context, get_cp_cu_seqlens
 from .backend import B200GDNBackend, install, uninstall
-from .modules import (FusedRMSNormGated, LayerNorm, ResidualRMSNorm, ShortConvolution, causal_conv1d, layer_norm, residual_rms_norm,
-                      rms_norm_gated)
+from .modules import (FusedLinear, FusedRMSNormGated, LayerNorm, ResidualRMSNorm, ShortConvolution, causal_conv1d, fused_linear,
+                      layer_norm, residual_rms_norm, rms_norm_gated)
 from .recurrence import gated_recurrence
 from .logits import TokenLogprobs, token_logprobs, topk_distill_loss
 
@@ -20,6 +20,6 @@ __all__ = [
     'FLACPContext', 'build_cp_context', 'get_cp_cu_seqlens', 'B200GDNBackend', 'install', 'uninstall',
     'B200GDNError', 'load_library', 'launch_count', 'device_status',
     'causal_conv1d', 'ShortConvolution', 'rms_norm_gated', 'FusedRMSNormGated', 'layer_norm', 'LayerNorm',
-    'gated_recurrence', 'residual_rms_norm', 'ResidualRMSNorm',
+    'gated_recurrence', 'residual_rms_norm', 'ResidualRMSNorm', 'fused_linear', 'FusedLinear',
     'TokenLogprobs', 'token_logprobs', 'topk_distill_loss',
 ]

@@ -103,6 +103,18 @@ class LayerNormArgs(C.Structure):
     ]
 
 
+LINEAR_SILU, LINEAR_SIGMOID, LINEAR_GELU = 1, 2, 3
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [
+        ('struct_bytes', C.c_int32), ('dtype', C.c_int32), ('rows', C.c_int64), ('K', C.c_int32), ('N', C.c_int32), ('activation', C.c_int32),
+        ('reserved', C.c_int32),
+        ('x', _p), ('weight', _p), ('bias', _p), ('residual', _p), ('y', _p), ('z', _p), ('dy', _p), ('dx', _p), ('dweight', _p), ('dbias', _p),
+        ('workspace', _p), ('workspace_bytes', C.c_int64),
+    ]
+
+
 NORMS_POST, NORMS_SIGMOID, NORMS_SILU = 1, 2, 4
 
 
@@ -157,6 +169,7 @@ EXPORTS = (
     'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd', 'b200gdn_norm_gate_ctas',
     'b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd', 'b200gdn_layer_norm_ctas', 'b200gdn_logprob_fwd', 'b200gdn_logprob_bwd',
     'b200gdn_gated_recurrence_fwd', 'b200gdn_gated_recurrence_bwd', 'b200gdn_rms_norms_fwd', 'b200gdn_rms_norms_bwd', 'b200gdn_rms_norms_partials',
+    'b200gdn_linear_fwd', 'b200gdn_linear_bwd', 'b200gdn_linear_workspace_bytes',
     'b200gdn_logprob_workspace_bytes', 'b200gdn_distill_fwd', 'b200gdn_distill_bwd', 'b200gdn_distill_workspace_bytes',
 )
 
@@ -186,7 +199,7 @@ def load():
                      'b200gdn_conv_fwd', 'b200gdn_conv_bwd', 'b200gdn_norm_gate_fwd', 'b200gdn_norm_gate_bwd',
                      'b200gdn_layer_norm_fwd', 'b200gdn_layer_norm_bwd', 'b200gdn_logprob_fwd', 'b200gdn_logprob_bwd',
                      'b200gdn_distill_fwd', 'b200gdn_distill_bwd', 'b200gdn_gated_recurrence_fwd', 'b200gdn_gated_recurrence_bwd',
-                     'b200gdn_rms_norms_fwd', 'b200gdn_rms_norms_bwd'):
+                     'b200gdn_rms_norms_fwd', 'b200gdn_rms_norms_bwd', 'b200gdn_linear_fwd', 'b200gdn_linear_bwd'):
             fn = getattr(lib, name)
             fn.restype = C.c_int
             fn.argtypes = [C.c_void_p, C.c_void_p]
@@ -204,6 +217,8 @@ def load():
         lib.b200gdn_layer_norm_ctas.argtypes = [C.c_int64]
         lib.b200gdn_rms_norms_partials.restype = C.c_int64
         lib.b200gdn_rms_norms_partials.argtypes = [C.c_int64, C.c_int32]
+        lib.b200gdn_linear_workspace_bytes.restype = C.c_int64
+        lib.b200gdn_linear_workspace_bytes.argtypes = [C.c_void_p, C.c_int32]
         lib.b200gdn_last_launch_count.restype = C.c_int
         lib.b200gdn_device_status.restype = C.c_int
         lib.b200gdn_device_status.argtypes = []

@@ -10,9 +10,10 @@
 and ahead of it, in the block around the layer,
 
 * ``layer_norm`` / ``LayerNorm`` — layer norm with the residual sum (fla/modules/layernorm.py);
-* ``residual_rms_norm`` / ``ResidualRMSNorm`` — the RMS norms either side of a block with its gate, residual scale and residual sum.
+* ``residual_rms_norm`` / ``ResidualRMSNorm`` — the RMS norms either side of a block with its gate, residual scale and residual sum;
+* ``fused_linear`` / ``FusedLinear`` — the projections with bias, activation and residual (b200gdn_linear_fwd/bwd, tcgen05).
 
-All run as HBM-streaming kernels of libb200gdn.so (b200gdn_conv_fwd/bwd, b200gdn_norm_gate_fwd/bwd,
+All others run as HBM-streaming kernels of libb200gdn.so (b200gdn_conv_fwd/bwd, b200gdn_norm_gate_fwd/bwd,
 b200gdn_layer_norm_fwd/bwd, b200gdn_rms_norms_fwd/bwd); there is no fallback path.
 """
 from __future__ import annotations
@@ -293,3 +294,36 @@ class ResidualRMSNorm(nn.Module):
     def forward(self, y, residual=None, gate=None):
         return residual_rms_norm(y, self.weight, residual, self.post_norm, self.post_weight, gate, self.gate_activation if gate is not None else None,
                                  self.scale, self.eps)
+
+
+_ACTIVATIONS = {None: 0, 'silu': _lib.LINEAR_SILU, 'swish': _lib.LINEAR_SILU, 'sigmoid': _lib.LINEAR_SIGMOID, 'gelu': _lib.LINEAR_GELU}
+
+
+def fused_linear(x, weight, bias=None, residual=None, activation: Optional[str] = None) -> torch.Tensor:
+    """``act(x weight^T + bias) + residual``: the projection into or out of a block with what follows it.
+
+    x ``[..., K]``, weight ``[N, K]``, bias ``[N]``, residual ``[..., N]``, all in bf16 or all in fp16; ``activation``: None, ``'silu'`` /
+    ``'swish'``, ``'sigmoid'`` or ``'gelu'`` (by the error function).  Sums are held in fp32 and rounded once.  Gradients reach all tensors;
+    with an activation what it is applied to is kept for them in the type of x.  Any number of tokens from one on and any width are served;
+    widths that are a multiple of eight are read in place, others cost a copy of the operand a call.
+    """
+    if not x.is_cuda:
+        raise _lib.B200GDNError('fused_linear runs on a CUDA device only (no CPU path)')
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f'Unsupported activation: {activation}')
+    args = (x, weight, bias, residual, _ACTIVATIONS[activation])
+    y = _lib.host().fused_linear(*args)
+    return RecordedCall.apply(_lib.host().fused_linear, *args) if y is NotImplemented else y
+
+
+class FusedLinear(nn.Linear):
+    """``nn.Linear`` with an activation, and a residual in its call: ``forward(x, residual)``."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: Optional[str] = None, device=None, dtype=None):
+        super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f'Unsupported activation: {activation}')
+        self.activation = activation
+
+    def forward(self, x, residual=None):
+        return fused_linear(x, self.weight, self.bias, residual, self.activation)

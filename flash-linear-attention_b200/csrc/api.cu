@@ -469,6 +469,53 @@ int b200gdn_rms_norms_bwd(const b200gdn_rms_norms_args* a, void* stream) {
 
 int64_t b200gdn_rms_norms_partials(int64_t rows, int32_t D) { return gdn::rms_norms_partials(rows, D); }
 
+static int check_linear_args(const b200gdn_linear_args* a, const char* who, bool bwd) {
+  using namespace gdn;
+  if (a == nullptr) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: args is NULL", who);
+  if (a->struct_bytes != (int32_t)sizeof(b200gdn_linear_args))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: struct_bytes %d != %zu (ABI mismatch)", who, a->struct_bytes, sizeof(b200gdn_linear_args));
+  if (a->rows <= 0 || a->K <= 0 || a->N <= 0)
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: empty problem (rows=%lld K=%d N=%d)", who, (long long)a->rows, a->K, a->N);
+  if (a->rows > (1 << 30)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^30 rows", who);
+  if (a->K > (1 << 23) || a->N > (1 << 23)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: K=%d, N=%d (at most 2^23)", who, a->K, a->N);
+  if (a->dtype < 0 || a->dtype > 1) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: dtype code %d (0 or 1)", who, a->dtype);
+  if (a->activation < 0 || a->activation > B200GDN_LINEAR_GELU) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: activation %d", who, a->activation);
+  if (!bwd) { REQUIRE(a->x, who); REQUIRE(a->weight, who); REQUIRE(a->y, who); }
+  else {
+    REQUIRE(a->dy, who);
+    if (a->dx != nullptr) REQUIRE(a->weight, who);
+    if (a->dweight != nullptr) REQUIRE(a->x, who);
+    if (a->activation != 0) REQUIRE(a->z, who);
+  }
+  if (off_boundary(2, {a->x, a->weight, a->bias, a->residual, a->y, a->z, a->dy, a->dx, a->dweight, a->dbias}))
+    return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: a tensor off its elements' boundary", who);
+  const int64_t need = linear_workspace(*a, bwd);
+  if (need > 0) {
+    REQUIRE(a->workspace, who);
+    if (a->workspace_bytes < need)
+      return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: a workspace of %lld bytes where %lld are needed", who, (long long)a->workspace_bytes, (long long)need);
+    if (off_boundary(256, {a->workspace})) return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: workspace off its boundary of 256", who);
+  }
+  return 0;
+}
+
+int b200gdn_linear_fwd(const b200gdn_linear_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_linear_args(a, "linear_fwd", false)) return e;
+  return gdn::launch_linear(*a, static_cast<cudaStream_t>(stream), false);
+}
+
+int b200gdn_linear_bwd(const b200gdn_linear_args* a, void* stream) {
+  gdn::g_launches = 0;
+  if (int e = check_linear_args(a, "linear_bwd", true)) return e;
+  return gdn::launch_linear(*a, static_cast<cudaStream_t>(stream), true);
+}
+
+int64_t b200gdn_linear_workspace_bytes(const b200gdn_linear_args* a, int32_t backward) {
+  if (a == nullptr || a->rows <= 0 || a->K <= 0 || a->N <= 0) return 0;
+  return gdn::linear_workspace(*a, backward != 0);
+}
+
 // what the two operators on rows of logits have in common
 static int check_rows_of_logits(const char* who, int64_t rows, int64_t inner, int32_t V, int32_t dtype, float scale, const void* logits,
                                 const void* dlogits) {
@@ -575,6 +622,7 @@ int b200gdn_device_status(void) {
       {"dv_local", gdn::dv_local_timeout_flag},   {"scan_bwd", gdn::scan_bwd_timeout_flag}, {"bwd_dqk", gdn::bwd_dqk_timeout_flag},
       {"bwd_wy", gdn::bwd_wy_timeout_flag},       {"bwd_local", gdn::bwd_local_timeout_flag},
             {"selftest", gdn::selftest_timeout_flag},
+      {"linear", gdn::linear_timeout_flag},
       {"decode_stream", gdn::decode_timeout_flag}};
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return gdn::set_error(B200GDN_ERR_CUDA, "device_status: %s", cudaGetErrorString(e));

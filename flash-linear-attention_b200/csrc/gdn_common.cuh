@@ -157,10 +157,13 @@ int launch_gated_recurrence(const b200gdn_gated_recurrence_args& a, cudaStream_t
 int launch_rms_norms(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd);
 int rms_norms_grid(int64_t rows);
 int64_t rms_norms_partials(int64_t rows, int D);
+int launch_linear(const b200gdn_linear_args& a, cudaStream_t st, bool bwd);
+int64_t linear_workspace(const b200gdn_linear_args& a, bool bwd);
 int64_t logprob_workspace(int64_t rows, int V, int dtype, int top_k);
 int launch_logprob(const b200gdn_logprob_args& a, cudaStream_t st, bool bwd);
 int64_t distill_workspace(int64_t rows, int V, int dtype, int K);
 int launch_distill(const b200gdn_distill_args& a, cudaStream_t st, bool bwd);
+int linear_timeout_flag();
 int decode_timeout_flag();
 int intra_fwd_timeout_flag();
 int scan_fwd_timeout_flag();

@@ -1197,6 +1197,102 @@ class NormsFunction : public torch::autograd::Function<NormsFunction> {
   }
 };
 
+// ---- projections -------------------------------------------------------------------------------------------------
+struct LinearForward {
+  Tensor y, x, w, z;
+};
+
+// the call of a pass: its workspace lives as long as its kernels do (freed memory is handed on in the stream's order)
+void linear_call(const char* name, int (*fn)(const b200gdn_linear_args*, void*), b200gdn_linear_args& a, bool bwd, const at::Device& dev) {
+  a.workspace_bytes = b200gdn_linear_workspace_bytes(&a, bwd);
+  Tensor space;
+  if (a.workspace_bytes > 0) {
+    space = new_tensor({a.workspace_bytes}, at::kByte, dev);
+    a.workspace = ptr(space);
+  }
+  call(name, fn, a);
+}
+b200gdn_linear_args linear_args(const Tensor& x, const Tensor& w, int64_t act) {
+  b200gdn_linear_args a{};
+  a.dtype = act_code(x.scalar_type());
+  a.K = (int32_t)x.size(-1);
+  a.N = (int32_t)w.size(0);
+  a.rows = x.numel() / x.size(-1);
+  a.activation = (int32_t)act;
+  a.x = ptr(x);
+  a.weight = ptr(w);
+  return a;
+}
+
+LinearForward linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& residual, int64_t act, bool need_grad) {
+  LinearForward r;
+  const at::Device dev = x.device();
+  c10::cuda::CUDAGuard guard(dev);
+  r.x = dense(x);
+  r.w = dense(w);
+  const Tensor bias = dense(b), res = dense(residual);
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = w.size(0);
+  r.y = new_tensor(sizes, x.scalar_type(), dev);
+  if (act != 0 && need_grad) r.z = new_tensor(sizes, x.scalar_type(), dev);
+  if (r.x.numel() == 0) return r;
+  b200gdn_linear_args a = linear_args(r.x, r.w, act);
+  a.bias = ptr(bias);
+  a.residual = ptr(res);
+  a.y = ptr(r.y);
+  a.z = ptr(r.z);
+  linear_call("b200gdn_linear_fwd", b200gdn_linear_fwd, a, false, dev);
+  return r;
+}
+
+class LinearFunction : public torch::autograd::Function<LinearFunction> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual,
+                        int64_t act) {
+    const Tensor b = val(bias), res = val(residual);
+    auto wanted = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    // what no gradient needs is not kept
+    LinearForward r = linear_forward(x, w, b, res, act, wanted(x) || wanted(w) || wanted(b));
+    ctx->save_for_backward({wanted(w) ? r.x : Tensor(), wanted(x) ? r.w : Tensor(), r.z});
+    ctx->saved_data["s"] = std::vector<int64_t>{act, wanted(x), wanted(w), wanted(b), wanted(res), w.size(0), w.size(1)};
+    ctx->saved_data["x"] = x.sizes().vec();
+    return r.y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &z = saved[2];
+    const auto s = ctx->saved_data["s"].toIntVector();
+    const auto x_sizes = ctx->saved_data["x"].toIntVector();
+    const at::Device dev = grads[0].device();
+    c10::cuda::CUDAGuard guard(dev);
+    const at::ScalarType t = grads[0].scalar_type();
+    const Tensor dy = dense(grads[0]);
+    const int64_t N = s[5], K = s[6], rows = dy.numel() / N;
+    Tensor dx, dw, db;
+    if (s[1]) dx = new_tensor(x_sizes, t, dev);
+    if (s[2]) dw = new_tensor({N, K}, t, dev, rows == 0);
+    if (s[3]) db = new_tensor({N}, t, dev, rows == 0);
+    if (rows > 0 && (s[1] || s[2] || s[3])) {
+      b200gdn_linear_args a{};
+      a.dtype = act_code(t);
+      a.K = (int32_t)K;
+      a.N = (int32_t)N;
+      a.rows = rows;
+      a.activation = (int32_t)s[0];
+      a.x = ptr(x);
+      a.weight = ptr(w);
+      a.z = ptr(z);
+      a.dy = ptr(dy);
+      a.dx = ptr(dx);
+      a.dweight = ptr(dw);
+      a.dbias = ptr(db);
+      linear_call("b200gdn_linear_bwd", b200gdn_linear_bwd, a, true, dev);
+    }
+    return once("fused_linear", {dx, dw, db, s[4] ? grads[0] : Tensor(), Tensor()});
+  }
+};
+
 // ---- rows of logits --------------------------------------------------------------------------------------------
 // The rows as the kernels address them: row r at (r / inner) outer + (r % inner) step.  Slices of a sequence or of a padded
 // vocabulary are read where they lie; what has more levels is copied.
@@ -1660,6 +1756,44 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// fused_linear(x, weight, bias, residual, activation) -> y; NotImplemented while a trace is recorded
+PyObject* py_fused_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(5);
+  if (tracing()) Py_RETURN_NOTIMPLEMENTED;
+  Tensor x, w, b, res;
+  if (!get(args[0], x) || !get(args[1], w) || !get(args[2], b) || !get(args[3], res) || !x.defined() || !w.defined()) {
+    PyErr_SetString(PyExc_TypeError, "fused_linear: a tensor is expected");
+    return nullptr;
+  }
+  const int64_t act = PyLong_AsLongLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  Tensor y;
+  {
+    NoGil nogil;
+    const std::string who = "fused_linear: ";
+    const at::ScalarType t = x.scalar_type();
+    if (t != at::kBFloat16 && t != at::kHalf) raise(who + "dtype " + c10::toString(t) + " is not supported (bf16 or fp16)");
+    if (x.dim() == 0 || x.size(-1) == 0) raise(who + "tokens without features");
+    if (w.dim() != 2 || w.size(1) != x.size(-1) || w.size(0) == 0) raise(who + "weight is [features, " + std::to_string(x.size(-1)) + "]");
+    if (w.size(0) > (1 << 23) || w.size(1) > (1 << 23)) raise(who + "more than 2^23 features");
+    if (x.numel() / x.size(-1) > (1 << 30)) raise(who + "more than 2^30 tokens");
+    if (b.defined() && (b.dim() != 1 || b.size(0) != w.size(0))) raise(who + "bias is a vector of " + std::to_string(w.size(0)));
+    if (res.defined()) {
+      bool same = res.dim() == x.dim() && res.size(-1) == w.size(0);
+      for (int64_t d = 0; same && d + 1 < x.dim(); ++d) same = res.size(d) == x.size(d);
+      if (!same) raise(who + "residual has the shape of the result");
+    }
+    for (const Tensor* p : {&w, &b, &res}) {
+      if (p->defined() && p->scalar_type() != t) raise(who + "weight, bias and residual have the type of x");
+      check("weight, bias or residual", *p, 0, x.device());
+    }
+    y = wants_grad({&x, &w, &b, &res}) ? LinearFunction::apply(x, w, opt(b), opt(res), act) : linear_forward(x, w, b, res, act, false).y;
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 // residual_rms_norm(y, weight, residual, post_weight, gate, scale, flags, alpha, eps) -> (out, z); NotImplemented while a trace is recorded
 PyObject* py_residual_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -1913,6 +2047,7 @@ PyMethodDef methods[] = {
     {"conv", FAST(py_conv), "short causal convolution, differentiable"},
     {"norm_gate", FAST(py_norm_gate), "gated RMS norm, differentiable"},
     {"layer_norm", FAST(py_layer_norm), "layer norm with the residual sum, differentiable"},
+    {"fused_linear", FAST(py_fused_linear), "projection with bias, activation and residual, differentiable"},
     {"residual_rms_norm", FAST(py_residual_rms_norm), "RMS norms either side of a block with gate, scale and residual sum, differentiable"},
     {"gated_recurrence", FAST(py_gated_recurrence), "elementwise gated recurrence, differentiable"},
     {"logprob", FAST(py_logprob), "log probabilities, entropy and top entries of rows of logits, differentiable"},

@@ -1,0 +1,773 @@
+// Projections: y = act(x W^T + b) + residual, and its gradients dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum of dz, in 16-bit types
+// with fp32 sums.
+//
+// All three products run in one persistent kernel on tcgen05 with CTA pairs: a pair forms a 256 x BN tile (128 rows in the tensor memory of
+// each CTA), each CTA brings its 128 rows of A and its half of B by TMA, one thread issues M = 256 instructions that read both CTAs' shared
+// memory.  A single CTA's 128 x 256 tile would need 96 bytes a clock from L2, more than the 64 an SM gets; the pair's 256 x 256 needs 64 a CTA.
+// Warp 4 loads, warp 5 issues, warps 0 to 3 carry finished tiles out of tensor memory while the next tile's sums form in its other half.
+// Operands lie either way: an operand whose contraction runs along its rows in memory is staged as [contraction][64 columns] panels and read
+// as an MN-major operand, so that W and x are never transposed.
+// Few tokens (up to 256): the product is formed the other way round, W's rows as the 256-row side and the tokens as a BN of 32 to 256, so that
+// what is read is W and little else.  Where there are fewer tiles than CTA pairs the contraction is split; the parts are left in fp32 and a
+// second kernel adds them in order and finishes.
+// Up to eight tokens, forward: W passes through registers once, as fast as memory gives it (linear_few_kernel).
+// TMA wants rows 16 bytes apart: operands of other widths are first copied to rows that are.
+#include "gdn_common.cuh"
+#include "rowio.cuh"
+#include "tc5.cuh"
+#include "tma.cuh"
+
+namespace gdn {
+namespace {
+
+__device__ int g_linear_timeout = 0;
+
+// ---- activations -----------------------------------------------------------------------------------------------------------
+enum { NONE = 0, SILU = B200GDN_LINEAR_SILU, SIGMOID = B200GDN_LINEAR_SIGMOID, GELU = B200GDN_LINEAR_GELU };
+
+__device__ __forceinline__ float sigmoid1(float x) { return unpack2(fast_sigmoid2(pack2(x, 0.f))).x; }
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == SILU) return v * sigmoid1(v);
+  if (act == SIGMOID) return sigmoid1(v);
+  if (act == GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  return v;
+}
+__device__ __forceinline__ float slope(float v, int act) {
+  if (act == SILU) {
+    const float s = sigmoid1(v);
+    return s * fmaf(v, 1.f - s, 1.f);
+  }
+  if (act == SIGMOID) {
+    const float s = sigmoid1(v);
+    return s * (1.f - s);
+  }
+  if (act == GELU) return fmaf(v * 0.39894228040143268f, expf(-0.5f * v * v), 0.5f * (1.f + erff(v * 0.70710678118654752f)));
+  return 1.f;
+}
+
+// ---- CTA pairs -------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t leaders(const void* p) {   // the address of the same place in the pair's first CTA
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(a) : "r"(tc5::smem_addr(p)));
+  return a;
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t* slot, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5::smem_addr(slot)), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// a box into this CTA's shared memory; its bytes count on the barrier at `bar` (a cluster address: the pair's first CTA's)
+__device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];\n" ::"r"(
+                   tc5::smem_addr(dst)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+               : "memory");
+}
+// called by a whole converged warp; one lane issues
+__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, e;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// the pair's finished instructions arrive on the barrier at this place in both CTAs
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n.reg .pred e;\n.reg .b16 m;\n"
+      "mov.b16 m, 3;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n}\n" ::"r"(tc5::smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
+}
+// tc5::mbar_wait for a whole warp, for arrivals of either CTA
+__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = tc5::smem_addr(bar);
+  bool done = false;
+  for (uint32_t it = 0; it < (1u << 22) && !done; ++it) {
+    uint32_t d;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(d)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    done = d;
+  }
+  return __all_sync(0xffffffffu, done);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {   // 32 columns of the lane's row
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31}, [%32];\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]),
+        "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]),
+        "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(taddr));
+}
+
+// ---- the product -----------------------------------------------------------------------------------------------------------
+// D[i, j] = sum over k of A(i, k) B(j, k).  `out`, `z` and `residual` are [tokens][features]: token i and feature j, or the other way round.
+struct Product {
+  int rows, cols;             // extents of i and j
+  int steps, splits;          // of 64 along k; parts that are summed apart
+  int tiles_i, tiles_j;
+  int act;
+  int features;               // extent of out's rows, which lie as far apart
+  int wide;                   // out, z and residual: rows on boundaries of 32 or 16 bytes, else 0
+  uint32_t idesc;
+  void *out, *z;              // z: what the activation is applied to, or NULL
+  const void *bias, *residual;
+  float* parts;               // with splits > 1: [splits][tokens][pitch]
+  int64_t tokens, pitch;
+};
+
+constexpr int BK = 64, A_BYTES = 128 * BK * 2, THREADS = 192;
+constexpr int b_bytes(int bn) { return bn / 2 * BK * 2; }
+constexpr int stages_of(int bn) { return bn == 256 ? 6 : bn == 128 ? 8 : bn == 64 ? 10 : 11; }
+constexpr size_t smem_of(int bn) { return (size_t)stages_of(bn) * (A_BYTES + b_bytes(bn)) + 1024; }
+
+struct Tile {
+  int i, j, split, k0, k1;
+};
+// Tiles of eight row blocks, column by column: those at work at one time share their rows of A and B in L2.
+__device__ __forceinline__ Tile tile_of(const Product& p, int t) {
+  const int n = p.tiles_i * p.tiles_j, split = t / n;
+  t -= split * n;
+  const int group = t / (8 * p.tiles_j), first = group * 8, height = min(8, p.tiles_i - first);
+  t -= group * 8 * p.tiles_j;
+  return Tile{first + t % height, t / height, split, (int)((int64_t)p.steps * split / p.splits), (int)((int64_t)p.steps * (split + 1) / p.splits)};
+}
+
+__device__ __forceinline__ void store32(void* p, uint4 a, uint4 b) {   // 32 bytes, on such a boundary
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z),
+               "r"(b.w)
+               : "memory");
+}
+// 32 neighbouring elements of a row of `n` from element j on; `wide`: how the row lies
+template <typename T>
+__device__ __forceinline__ void put_row(void* row, int j, int n, int wide, const float (&v)[32]) {
+  T* p = static_cast<T*>(row) + j;
+  if (wide && j + 32 <= n) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint4 w[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = v[q * 16 + h * 8 + e];
+        w[h] = pack8<T>(x);
+      }
+      if (wide == 32) {
+        store32(p + q * 16, w[0], w[1]);
+      } else {
+        reinterpret_cast<uint4*>(p)[2 * q] = w[0];
+        reinterpret_cast<uint4*>(p)[2 * q + 1] = w[1];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (j + e < n) p[e] = static_cast<T>(v[e]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void add_row(const void* row, int j, int n, int wide, float (&v)[32]) {
+  const T* p = static_cast<const T*>(row) + j;
+  if (wide && j + 32 <= n) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float x[8];
+      unpack8<T>(reinterpret_cast<const uint4*>(p)[q], x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[q * 8 + e] += x[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (j + e < n) v[e] += (float)p[e];
+  }
+}
+
+// SWAPPED: i are features and j tokens
+template <typename T, int BN, bool A_MN, bool B_MN, bool SWAPPED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    linear_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Product p) {
+  constexpr int STAGES = stages_of(BN), STAGE = A_BYTES + b_bytes(BN);
+  constexpr uint32_t COLUMNS = 2 * BN;   // of tensor memory: two tiles
+  extern __shared__ unsigned char raw[];
+  unsigned char* tiles = raw + ((1024 - (tc5::smem_addr(raw) & 1023)) & 1023);
+  __shared__ uint64_t full[STAGES], empty[STAGES], done[2], taken[2];
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cta_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      tc5::mbar_init(&full[s], 1);
+      tc5::mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      tc5::mbar_init(&done[s], 1);
+      tc5::mbar_init(&taken[s], 8);   // the epilogue warps of both CTAs
+    }
+    tc5::fence_mbar_init();
+  }
+  if (warp == 5) pair_tmem_alloc(&tmem_slot, COLUMNS);
+  __syncthreads();
+  tc5::fence_before_sync();
+  cluster_sync();
+  tc5::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const int n_tiles = p.tiles_i * p.tiles_j * p.splits, first = blockIdx.x >> 1, by = gridDim.x >> 1;
+  bool ok = true;
+  if (warp == 4) {
+    if (lane == 0) {
+      tma::prefetch_map(&map_a);
+      tma::prefetch_map(&map_b);
+    }
+    int s = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    for (int t = first; t < n_tiles && ok; t += by) {
+      const Tile at = tile_of(p, t);
+      const int i0 = at.i * 256 + rank * 128, j0 = at.j * BN + rank * (BN / 2);
+      for (int k = at.k0; k < at.k1; ++k) {
+        ok = pair_wait(&empty[s], phase ^ 1u);
+        if (!ok) break;
+        if (lane == 0) {
+          unsigned char* a = tiles + s * STAGE;
+          unsigned char* b = a + A_BYTES;
+          const uint32_t bar = leaders(&full[s]);
+          if (rank == 0) tc5::mbar_expect_tx(&full[s], 2 * STAGE);
+          if constexpr (A_MN) {
+            pair_load(a, &map_a, i0, k * BK, bar);
+            pair_load(a + A_BYTES / 2, &map_a, i0 + 64, k * BK, bar);
+          } else {
+            pair_load(a, &map_a, k * BK, i0, bar);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int c = 0; c < BN / 128; ++c) pair_load(b + c * 64 * BK * 2, &map_b, j0 + c * 64, k * BK, bar);
+          } else {
+            pair_load(b, &map_b, k * BK, j0, bar);
+          }
+        }
+        __syncwarp();
+        issued = min(issued + 1, STAGES);
+        if (++s == STAGES) {
+          s = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    // its copies have landed before a CTA leaves: what was waited for by the other warps in any case, unless a wait ran out
+    if (!ok && rank == 0)
+      for (int i = 0; i < issued; ++i) {
+        if (--s < 0) {
+          s = STAGES - 1;
+          phase ^= 1u;
+        }
+        (void)pair_wait(&full[s], phase);
+      }
+  } else if (warp == 5) {
+    if (rank == 0) {
+      int s = 0, turn = 0;
+      uint32_t phase = 0;
+      for (int t = first; t < n_tiles && ok; t += by, ++turn) {
+        const Tile at = tile_of(p, t);
+        const int half = turn & 1;
+        ok = pair_wait(&taken[half], ((turn >> 1) & 1) ^ 1u);
+        if (!ok) break;
+        tc5::fence_after_sync();
+        const uint32_t acc = tmem + half * BN;
+        for (int k = at.k0; k < at.k1; ++k) {
+          ok = pair_wait(&full[s], phase);
+          if (!ok) break;
+          tc5::fence_after_sync();
+          const uint32_t a = tc5::smem_addr(tiles + s * STAGE), b = a + A_BYTES;
+          const uint64_t da = A_MN ? tc5::smem_desc(a, 64 * BK * 2, 1024) : tc5::smem_desc(a, 16, 1024);
+          const uint64_t db = B_MN ? tc5::smem_desc(b, 64 * BK * 2, 1024) : tc5::smem_desc(b, 16, 1024);
+#pragma unroll
+          for (int q = 0; q < BK / 16; ++q)   // 16 of the contraction: 32 bytes along a row, or 16 rows
+            pair_mma(acc, da + ((A_MN ? q * 2048 : q * 32) >> 4), db + ((B_MN ? q * 2048 : q * 32) >> 4), p.idesc, k > at.k0 || q > 0);
+          pair_commit(&empty[s]);
+          if (++s == STAGES) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) pair_commit(&done[half]);
+      }
+    }
+  } else {
+    int turn = 0;
+    for (int t = first; t < n_tiles && ok; t += by, ++turn) {
+      const Tile at = tile_of(p, t);
+      const int half = turn & 1;
+      ok = pair_wait(&done[half], (turn >> 1) & 1);
+      if (!ok) break;
+      tc5::fence_after_sync();
+      const int i = at.i * 256 + rank * 128 + warp * 32 + lane;
+      const bool live = i < p.rows;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        const int j = at.j * BN + c;
+        if (j >= p.cols) break;   // (the same for all)
+        float v[32];
+        __syncwarp();
+        tmem_ld32(tmem + half * BN + c + ((uint32_t)(warp * 32) << 16), v);
+        tc5::tmem_ld_wait();
+        if (!live) continue;
+        if constexpr (!SWAPPED) {
+          if (p.splits > 1) {
+            float* part = p.parts + ((int64_t)at.split * p.tokens + i) * p.pitch + j;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)   // (the pitch is a multiple of eight)
+              if (j + q * 8 < p.cols)
+                store32(part + q * 8, *reinterpret_cast<const uint4*>(&v[q * 8]), *reinterpret_cast<const uint4*>(&v[q * 8 + 4]));
+            continue;
+          }
+          const int64_t row = (int64_t)i * p.features;
+          if (p.bias) add_row<T>(p.bias, j, p.cols, p.wide, v);
+          if (p.z) put_row<T>(static_cast<T*>(p.z) + row, j, p.cols, p.wide, v);
+          if (p.act != NONE)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = activate(v[e], p.act);
+          if (p.residual) add_row<T>(static_cast<const T*>(p.residual) + row, j, p.cols, p.wide, v);
+          put_row<T>(static_cast<T*>(p.out) + row, j, p.cols, p.wide, v);
+        } else {
+          const float b = p.bias && p.splits == 1 ? (float)static_cast<const T*>(p.bias)[i] : 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            if (j + e >= p.cols) break;
+            if (p.splits > 1) {
+              p.parts[((int64_t)at.split * p.tokens + j + e) * p.pitch + i] = v[e];
+              continue;
+            }
+            const int64_t to = (int64_t)(j + e) * p.features + i;
+            float x = v[e] + b;
+            if (p.z) static_cast<T*>(p.z)[to] = static_cast<T>(x);
+            x = activate(x, p.act);
+            if (p.residual) x += (float)static_cast<const T*>(p.residual)[to];
+            static_cast<T*>(p.out)[to] = static_cast<T>(x);
+          }
+        }
+      }
+      tc5::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_at(leaders(&taken[half]));
+    }
+  }
+  if (!ok && lane == 0) atomicExch(&g_linear_timeout, 1);
+  // neither CTA leaves while the other may still read its tiles or arrive on its barriers
+  __syncthreads();
+  tc5::fence_before_sync();
+  cluster_sync();
+  tc5::fence_after_sync();
+  if (warp == 5) pair_tmem_dealloc(tmem, COLUMNS);
+}
+
+// the parts of a split contraction in their order, and what follows the product
+template <typename T>
+__global__ void __launch_bounds__(256) linear_join_kernel(const Product p) {
+  wait_for_predecessor();
+  const int64_t n = p.tokens * p.features, size = p.tokens * p.pitch;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
+    const int64_t token = at / p.features;
+    const int f = (int)(at - token * p.features);
+    const float* part = p.parts + token * p.pitch + f;
+    float v = part[0];
+    for (int s = 1; s < p.splits; ++s) v += part[s * size];
+    if (p.bias) v += (float)static_cast<const T*>(p.bias)[f];
+    if (p.z) static_cast<T*>(p.z)[at] = static_cast<T>(v);
+    v = activate(v, p.act);
+    if (p.residual) v += (float)static_cast<const T*>(p.residual)[at];
+    static_cast<T*>(p.out)[at] = static_cast<T>(v);
+  }
+}
+
+// ---- up to eight tokens, forward ---------------------------------------------------------------------------------------------
+// A CTA of eight warps forms 8 / WK x R features of all tokens: WK warps share R rows of W, each a part of the contraction, which their lanes walk
+// side by side in 16-byte pieces (one element where rows do not lie so); sums of even and odd elements go together (f32x2).
+constexpr int R = 4;
+template <typename T, int TOKENS, bool WIDE>
+__global__ void __launch_bounds__(256) linear_few_kernel(const Product p, const void* x, const void* w, int K, int WK) {
+  constexpr int E = WIDE ? 8 : 1, P = (E + 1) / 2;
+  __shared__ float sums[8][R * TOKENS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WK;
+  const int f0 = (blockIdx.x * (8 / WK) + warp / WK) * R;
+  const int n_tokens = (int)p.tokens;
+  uint64_t acc[R][TOKENS];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int t = 0; t < TOKENS; ++t) acc[r][t] = 0ull;
+  auto pairs_of = [&](const void* base, int64_t at, uint64_t (&v)[P]) {
+    if constexpr (WIDE) {
+      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(base) + at);
+      v[0] = widen2<T>(u.x), v[1] = widen2<T>(u.y), v[2] = widen2<T>(u.z), v[3] = widen2<T>(u.w);
+    } else {
+      v[0] = pack2((float)static_cast<const T*>(base)[at], 0.f);
+    }
+  };
+  constexpr int U = 2;   // pieces of each row on their way
+  for (int k = (part * 32 + lane) * E; k < K; k += WK * 32 * E * U) {
+    uint64_t a[U][R][P];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int at = k + u * WK * 32 * E;
+        if (f0 + r < p.features && at < K) pairs_of(w, (int64_t)(f0 + r) * K + at, a[u][r]);
+        else
+#pragma unroll
+          for (int i = 0; i < P; ++i) a[u][r][i] = 0ull;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = k + u * WK * 32 * E;
+      if (at >= K) break;
+#pragma unroll
+      for (int t = 0; t < TOKENS; ++t) {
+        if (t >= n_tokens) break;
+        uint64_t b[P];
+        pairs_of(x, (int64_t)t * K + at, b);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < P; ++i) acc[r][t] = fma2(a[u][r][i], b[i], acc[r][t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int t = 0; t < TOKENS; ++t) {
+      const float2 f = unpack2(acc[r][t]);
+      float v = f.x + f.y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) sums[warp][r * TOKENS + t] = v;
+    }
+  __syncthreads();
+  const int at = threadIdx.x, group = at / (R * TOKENS);   // one thread a result: 8 / WK x R x TOKENS of at most 256
+  if (group >= 8 / WK) return;
+  const int r = at % (R * TOKENS) / TOKENS, t = at % TOKENS, f = (blockIdx.x * (8 / WK) + group) * R + r;
+  if (f >= p.features || t >= n_tokens) return;
+  float v = 0.f;
+  for (int i = 0; i < WK; ++i) v += sums[group * WK + i][r * TOKENS + t];
+  if (p.bias) v += (float)static_cast<const T*>(p.bias)[f];
+  const int64_t to = (int64_t)t * p.features + f;
+  if (p.z) static_cast<T*>(p.z)[to] = static_cast<T>(v);
+  v = activate(v, p.act);
+  if (p.residual) v += (float)static_cast<const T*>(p.residual)[to];
+  static_cast<T*>(p.out)[to] = static_cast<T>(v);
+}
+
+// ---- around the gradient's products ------------------------------------------------------------------------------------------
+// rows of `cols` to rows `pitch` apart
+__global__ void __launch_bounds__(256) linear_pad_kernel(const uint16_t* src, uint16_t* dst, int64_t rows, int cols, int pitch) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) dst[r * pitch + c] = src[r * cols + c];
+}
+
+// dz = dy act'(z) (rounded for the products; `dz` NULL: not wanted) and, for db, its sums over the rows of a CTA, unrounded.  Warps take rows in
+// turn, lanes E columns each.
+template <typename T, int E>
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, const T* z, T* dz, float* sums, int64_t rows, int cols, int pitch, int act) {
+  __shared__ float part[8][32 * E];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = (blockIdx.x * 32 + lane) * E;
+  float total[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) total[e] = 0.f;
+  auto get = [&](const T* p, float (&v)[E]) {
+    if constexpr (E == 8) unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
+    else v[0] = (float)*p;
+  };
+  if (c < cols) {
+    constexpr int U = 4;
+    const int64_t step = (int64_t)gridDim.y * 8;
+    for (int64_t r0 = blockIdx.y * 8 + warp; r0 < rows; r0 += step * U) {
+      float d[U][E], v[U][E];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r0 + u * step < rows) {
+          get(dy + (r0 + u * step) * cols + c, d[u]);
+          if (act != NONE) get(z + (r0 + u * step) * cols + c, v[u]);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t r = r0 + u * step;
+        if (r >= rows) break;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (act != NONE) d[u][e] *= slope(v[u][e], act);
+          total[e] += d[u][e];
+        }
+        if (dz) {
+          if constexpr (E == 8) *reinterpret_cast<uint4*>(dz + r * pitch + c) = pack8<T>(d[u]);
+          else dz[r * pitch + c] = static_cast<T>(d[u][0]);
+        }
+      }
+    }
+  }
+  if (sums == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < E; ++e) part[warp][lane * E + e] = total[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * E; i += 256) {
+    const int col = blockIdx.x * 32 * E + i;
+    if (col >= cols) continue;
+    float s = part[0][i];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) s += part[w][i];
+    sums[(int64_t)blockIdx.y * cols + col] = s;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) linear_dbias_kernel(const float* sums, T* dbias, int cols, int n) {
+  wait_for_predecessor();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+  for (int i = 0; i < n; ++i) s += sums[(int64_t)i * cols + c];
+  dbias[c] = static_cast<T>(s);
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+struct Plan {
+  int bn, splits;
+  int64_t parts;   // floats
+};
+// The column tile and the parts of the contraction with the least time by this model: rounds of tiles over the pairs, 0.27 us a step of
+// 256 x 256 (0.17 of 128 columns, 0.12 of fewer: what the loads take), 1.5 us a tile that nothing hides, and 3 us with what the parts move.
+Plan plan_of(int64_t rows, int64_t cols, int64_t depth, bool swapped) {
+  const int pairs = sm_count() / 2, steps = (int)((depth + BK - 1) / BK);
+  Plan best{256, 1, 0};
+  double least = 1e30;
+  for (int bn : {256, 128, 64, 32}) {
+    if (swapped ? (bn < cols && bn < 256) || bn / 2 >= up(cols, 32) : bn < 128) continue;
+    const int64_t tiles = (rows + 255) / 256 * ((cols + bn - 1) / bn);
+    const double step = bn == 256 ? 0.27 : bn == 128 ? 0.17 : 0.12;
+    for (int s = 1; s <= 16 && (s == 1 || steps / s >= 4); ++s) {
+      const double bytes = s > 1 ? 8.0 * s * rows * cols : 0;
+      const double cost = (double)((tiles * s + pairs - 1) / pairs) * ((steps + s - 1) / s * step + 1.5) + (s > 1 ? 3 + bytes / 6e6 : 0);
+      if (cost < least) {
+        least = cost;
+        best = Plan{bn, s, s > 1 ? s * (swapped ? cols * up(rows, 8) : rows * up(cols, 8)) : 0};
+      }
+    }
+  }
+  return best;
+}
+
+struct Operand {
+  const void* base;
+  int64_t rows, cols, pitch;   // as it lies
+};
+template <typename T, int BN, bool A_MN, bool B_MN, bool SWAPPED>
+int launch_tiles(const Operand& a, const Operand& b, Product p, cudaStream_t st) {
+  CUtensorMap ma, mb;
+  if (int e = tma::encode_bf16_2d(&ma, a.base, a.rows, a.cols, a.pitch, A_MN ? 64 : 128)) return set_error(B200GDN_ERR_CUDA, "linear: tensor map of A (%d)", e);
+  if (int e = tma::encode_bf16_2d(&mb, b.base, b.rows, b.cols, b.pitch, B_MN ? 64 : BN / 2)) return set_error(B200GDN_ERR_CUDA, "linear: tensor map of B (%d)", e);
+  p.tiles_i = (p.rows + 255) / 256;
+  p.tiles_j = (p.cols + BN - 1) / BN;
+  const uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
+  p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
+  auto kern = linear_kernel<T, BN, A_MN, B_MN, SWAPPED>;
+  if (int e = ensure_smem(kern, smem_of(BN))) return e;
+  const int64_t tiles = (int64_t)p.tiles_i * p.tiles_j * p.splits;
+  if (tiles > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "linear: more than 2^31 - 1 tiles");
+  const int pairs = (int)(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
+  kern<<<2 * pairs, THREADS, smem_of(BN), st>>>(ma, mb, p);
+  return check_launch("linear");
+}
+
+// A and B as D's rows and columns; `swapped`: D's rows are features
+template <typename T, bool A_MN, bool B_MN>
+int launch_product(const Operand& a, const Operand& b, int64_t depth, Product p, bool swapped, float* parts, cudaStream_t st) {
+  const Plan plan = plan_of(p.rows, p.cols, depth, swapped);
+  p.steps = (int)((depth + BK - 1) / BK);
+  p.splits = plan.splits;
+  p.parts = parts;
+  p.tokens = swapped ? p.cols : p.rows;
+  p.features = swapped ? p.rows : p.cols;
+  p.pitch = up(p.features, 8);
+  uintptr_t bits = reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.z) | reinterpret_cast<uintptr_t>(p.bias) |
+                   reinterpret_cast<uintptr_t>(p.residual) | (uintptr_t)p.features * 2;
+  p.wide = bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 0;
+  int e = B200GDN_ERR_UNSUPPORTED;
+  if (!swapped) {
+    e = plan.bn == 256 ? launch_tiles<T, 256, A_MN, B_MN, false>(a, b, p, st) : launch_tiles<T, 128, A_MN, B_MN, false>(a, b, p, st);
+  } else if constexpr (!B_MN) {
+    e = plan.bn == 256   ? launch_tiles<T, 256, A_MN, false, true>(a, b, p, st)
+        : plan.bn == 128 ? launch_tiles<T, 128, A_MN, false, true>(a, b, p, st)
+        : plan.bn == 64  ? launch_tiles<T, 64, A_MN, false, true>(a, b, p, st)
+                         : launch_tiles<T, 32, A_MN, false, true>(a, b, p, st);
+  }
+  if (e != 0 || plan.splits == 1) return e;
+  const int64_t n = (p.tokens * p.features + 255) / 256, most = 8 * (int64_t)sm_count();
+  launch_overlapped(true, linear_join_kernel<T>, dim3((unsigned)(n < most ? n : most)), 256, 0, st, p);
+  return check_launch("linear_join");
+}
+
+constexpr int64_t FEW = 8, SWAP = 256;   // tokens up to which W's rows pass through registers, and up to which they are the tile's 256
+
+// The workspace, piece by piece on 256-byte boundaries; without a base it only counts.
+struct Space {
+  char* base;
+  int64_t used = 0;
+  void* take(int64_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += up(bytes, 256);
+    return p;
+  }
+};
+bool fits_tma(const void* p, int64_t cols) { return cols % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// the operand itself, or its copy with rows 16 bytes apart
+int operand_of(const void* base, int64_t rows, int64_t cols, Space& space, cudaStream_t st, bool run, Operand& o) {
+  o = Operand{base, rows, cols, cols};
+  if (fits_tma(base, cols)) return 0;
+  o.pitch = up(cols, 8);
+  void* copy = space.take(rows * o.pitch * 2);
+  o.base = copy;
+  if (!run) return 0;
+  const int64_t x = (cols + 255) / 256, most = 16 * (int64_t)sm_count() / x + 1;
+  linear_pad_kernel<<<dim3((unsigned)x, (unsigned)(rows < most ? rows : most)), 256, 0, st>>>(static_cast<const uint16_t*>(base), static_cast<uint16_t*>(copy),
+                                                                                               rows, (int)cols, (int)o.pitch);
+  return check_launch("linear_pad");
+}
+
+template <typename T>
+int forward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool run) {
+  Product p{};
+  p.act = a.activation;
+  p.out = a.y;
+  p.z = a.activation == NONE ? nullptr : a.z;
+  p.bias = a.bias;
+  p.residual = a.residual;
+  if (a.rows <= FEW) {
+    if (!run) return 0;
+    p.tokens = a.rows;
+    p.features = a.N;
+    int wk = 1;
+    while (wk < 8 && (int64_t)a.N * wk / (8 * R) < 3 * sm_count() && wk * 512 <= a.K) wk *= 2;
+    const int grid = (a.N + 8 / wk * R - 1) / (8 / wk * R);
+    const bool wide = fits_tma(a.x, a.K) && fits_tma(a.weight, a.K);
+    auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>(p, a.x, a.weight, a.K, wk); };
+    if (a.rows == 1) wide ? go(linear_few_kernel<T, 1, true>) : go(linear_few_kernel<T, 1, false>);
+    else if (a.rows == 2) wide ? go(linear_few_kernel<T, 2, true>) : go(linear_few_kernel<T, 2, false>);
+    else if (a.rows <= 4) wide ? go(linear_few_kernel<T, 4, true>) : go(linear_few_kernel<T, 4, false>);
+    else wide ? go(linear_few_kernel<T, 8, true>) : go(linear_few_kernel<T, 8, false>);
+    return check_launch("linear_few");
+  }
+  Operand x, w;
+  if (int e = operand_of(a.x, a.rows, a.K, space, st, run, x)) return e;
+  if (int e = operand_of(a.weight, a.N, a.K, space, st, run, w)) return e;
+  const bool swapped = a.rows <= SWAP;
+  p.rows = swapped ? a.N : (int)a.rows;
+  p.cols = swapped ? (int)a.rows : a.N;
+  float* parts = static_cast<float*>(space.take(plan_of(p.rows, p.cols, a.K, swapped).parts * 4));
+  if (!run) return 0;
+  return swapped ? launch_product<T, false, false>(w, x, a.K, p, true, parts, st) : launch_product<T, false, false>(x, w, a.K, p, false, parts, st);
+}
+
+template <typename T>
+int backward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool run) {
+  // dz with rows that TMA reads: dy itself where it is that and lies so
+  const bool apart = (a.dx || a.dweight) && (a.activation != NONE || !fits_tma(a.dy, a.N));
+  Operand dz{a.dy, a.rows, a.N, a.N};
+  T* made = nullptr;
+  if (apart) {
+    dz.pitch = up(a.N, 8);
+    made = static_cast<T*>(space.take(a.rows * dz.pitch * 2));
+    dz.base = made;
+  }
+  const bool wide = fits_tma(a.dy, a.N) && fits_tma(a.z, a.N);
+  const int per = wide ? 256 : 32;
+  const int64_t x = (a.N + per - 1) / per;
+  int64_t y = 8 * (int64_t)sm_count() / x + 1;
+  if (y > (a.rows + 31) / 32) y = (a.rows + 31) / 32;
+  float* sums = a.dbias ? static_cast<float*>(space.take(y * a.N * 4)) : nullptr;
+  if (run && (apart || a.dbias)) {
+    auto go = [&](auto kern) {
+      kern<<<dim3((unsigned)x, (unsigned)y), 256, 0, st>>>(static_cast<const T*>(a.dy), static_cast<const T*>(a.z), made, sums, a.rows, a.N, (int)dz.pitch,
+                                                          a.activation);
+    };
+    wide ? go(linear_dz_kernel<T, 8>) : go(linear_dz_kernel<T, 1>);
+    if (int e = check_launch("linear_dz")) return e;
+    if (a.dbias) {
+      launch_overlapped(true, linear_dbias_kernel<T>, dim3((a.N + 255) / 256), 256, 0, st, (const float*)sums, static_cast<T*>(a.dbias), a.N, (int)y);
+      if (int e = check_launch("linear_dbias")) return e;
+    }
+  }
+  if (a.dx) {
+    Operand w;
+    if (int e = operand_of(a.weight, a.N, a.K, space, st, run, w)) return e;
+    const bool swapped = a.rows <= SWAP;
+    Product p{};
+    p.out = a.dx;
+    p.rows = swapped ? a.K : (int)a.rows;
+    p.cols = swapped ? (int)a.rows : a.K;
+    float* parts = static_cast<float*>(space.take(plan_of(p.rows, p.cols, a.N, swapped).parts * 4));
+    if (run)
+      if (int e = swapped ? launch_product<T, true, false>(w, dz, a.N, p, true, parts, st) : launch_product<T, false, true>(dz, w, a.N, p, false, parts, st)) return e;
+  }
+  if (a.dweight) {
+    Operand in;
+    if (int e = operand_of(a.x, a.rows, a.K, space, st, run, in)) return e;
+    Product p{};
+    p.out = a.dweight;
+    p.rows = a.N;
+    p.cols = a.K;
+    float* parts = static_cast<float*>(space.take(plan_of(p.rows, p.cols, a.rows, false).parts * 4));
+    if (run)
+      if (int e = launch_product<T, true, true>(dz, in, a.rows, p, false, parts, st)) return e;
+  }
+  return 0;
+}
+
+}  // namespace
+
+int64_t linear_workspace(const b200gdn_linear_args& a, bool bwd) {
+  Space space{nullptr};
+  (void)(bwd ? backward<__half>(a, space, nullptr, false) : forward<__half>(a, space, nullptr, false));
+  return space.used;
+}
+
+int launch_linear(const b200gdn_linear_args& a, cudaStream_t st, bool bwd) {
+  Space space{static_cast<char*>(a.workspace)};
+  if (a.dtype == 0) return bwd ? backward<__nv_bfloat16>(a, space, st, true) : forward<__nv_bfloat16>(a, space, st, true);
+  return bwd ? backward<__half>(a, space, st, true) : forward<__half>(a, space, st, true);
+}
+
+int linear_timeout_flag() {
+  int v = 0, zero = 0;
+  cudaMemcpyFromSymbol(&v, g_linear_timeout, sizeof(int));
+  if (v) cudaMemcpyToSymbol(g_linear_timeout, &zero, sizeof(int));
+  return v;
+}
+
+}  // namespace gdn

@@ -495,6 +495,39 @@ int b200gdn_rms_norms_fwd(const b200gdn_rms_norms_args* args, void* stream);
 int b200gdn_rms_norms_bwd(const b200gdn_rms_norms_args* args, void* stream);
 int64_t b200gdn_rms_norms_partials(int64_t rows, int32_t D);
 
+/* Projection of `rows` tokens from K to N features:  z = x weight^T + bias,  y = act(z) + residual, and its gradients
+ *   dz = dy act'(z);  dx = dz weight;  dweight = dz^T x;  dbias = sum of dz   (the residual's is dy)
+ * Sums are held in fp32; dz and the z that is kept for the backward pass are rounded to the tensors' type, which the products read.  act is
+ * B200GDN_LINEAR_SILU, _SIGMOID, _GELU (by the error function) or 0, none.  All tensors are contiguous; where x, weight and dy have rows of a
+ * multiple of 16 bytes on such a boundary they are read in place, else from copies in the workspace.  workspace:
+ * b200gdn_linear_workspace_bytes(args, backward) bytes, with the pointers of `args` set as for the call, on a boundary of 256. */
+#define B200GDN_LINEAR_SILU 1
+#define B200GDN_LINEAR_SIGMOID 2
+#define B200GDN_LINEAR_GELU 3
+typedef struct b200gdn_linear_args {
+  int32_t struct_bytes;
+  int32_t dtype;                 /* 0 = bf16, 1 = fp16: all tensors */
+  int64_t rows;
+  int32_t K, N;
+  int32_t activation;
+  int32_t reserved;
+  const void* x;                 /* [rows, K] (the backward pass reads it for dweight) */
+  const void* weight;            /* [N, K] (the backward pass reads it for dx) */
+  const void* bias;              /* [N] or NULL (forward) */
+  const void* residual;          /* [rows, N] or NULL (forward) */
+  void* y;                       /* [rows, N] (forward) */
+  void* z;                       /* [rows, N], with an activation: written by the forward pass (NULL: not wanted), read by the backward pass */
+  const void* dy;                /* [rows, N] */
+  void* dx;                      /* [rows, K] or NULL, as all gradients */
+  void* dweight;                 /* [N, K] */
+  void* dbias;                   /* [N] */
+  void* workspace;
+  int64_t workspace_bytes;
+} b200gdn_linear_args;
+int b200gdn_linear_fwd(const b200gdn_linear_args* args, void* stream);
+int b200gdn_linear_bwd(const b200gdn_linear_args* args, void* stream);
+int64_t b200gdn_linear_workspace_bytes(const b200gdn_linear_args* args, int32_t backward);
+
 /* Rows of logits over a vocabulary of V.  Row r starts at element (r / inner) stride_outer + (r % inner) stride_inner; the
  * entries of a row lie side by side and need no alignment beyond their own.  scale = 1 / temperature; with m the largest entry:
  *   lp_j = scale (x_j - m) - log(sum exp(scale (x - m)));  p = exp(lp)

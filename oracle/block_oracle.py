@@ -114,3 +114,33 @@ def rms_norms(y, weight, residual, post, post_weight, gate, activation, scale, e
                dpost_weight=(e * c * act * n1).sum(0), dpost_weight_size=(e_size * (c * act_size * n1).abs()).sum(0),
                dscale=(e * act * p).sum(0), dscale_size=(e_size * (act_size * p).abs()).sum(0))
     return out
+
+
+def linear(x, weight, bias, residual, activation, dy=None):
+    """x [M, K], weight [N, K], bias [N], residual [M, N] in their own 16-bit type; `<name>_off`: how far off fp32 sums may be.
+
+    A sum of K products in steps of 16: (K / 16 + 32) units of 2^-23 of the sum of magnitudes.  The gradient reads z and dz rounded to the
+    type (half a step each): the slope changes by at most 0.8 per unit of z."""
+    half = torch.finfo(x.dtype).eps / 2
+
+    def units(n):
+        return (n / 16 + 32) * 2 * U
+    x, w = x.double(), weight.double()
+    b = w.new_zeros(w.shape[0]) if bias is None else bias.double()
+    z, z_size = x @ w.t() + b, x.abs() @ w.abs().t() + b.abs()
+    act, slope, act_size, slope_size = _activation(activation, z)
+    z_off = units(x.shape[1]) * z_size
+    y, y_off = act, 1.2 * z_off + (32 * U * act_size if activation else 0.0)
+    if residual is not None:
+        y, y_off = y + residual.double(), y_off + U * residual.double().abs()
+    out = {'y': y, 'y_off': y_off}
+    if dy is not None:
+        dy = dy.double()
+        dz = dy * slope
+        unrounded = dy.abs() * (0.8 * (half * z.abs() + z_off) + 32 * U * slope_size) if activation else torch.zeros_like(dz)
+        dz_off = unrounded + (half * dz.abs() if activation else 0.0)
+        size = dz.abs() + dz_off
+        out.update(dx=dz @ w, dx_off=dz_off @ w.abs() + units(w.shape[0]) * (size @ w.abs()),
+                   dweight=dz.t() @ x, dweight_off=dz_off.t() @ x.abs() + units(x.shape[0]) * (size.t() @ x.abs()),
+                   dbias=dz.sum(0), dbias_off=unrounded.sum(0) + units(x.shape[0]) * size.sum(0))
+    return out
