@@ -19,7 +19,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int MOST_WARPS = 16, MOST_RANKS = 8;
+constexpr int MOST_RANKS = 16;
 
 // C neighbouring channels of a token, as loaded
 template <typename T, int C>
@@ -32,6 +32,20 @@ struct Piece {
     if constexpr (C == 1) return pack2((float)*reinterpret_cast<const T*>(&u), 0.f);
     else if constexpr (sizeof(T) == 2) return widen2<T>(u);
     else return pack2(__uint_as_float(u.x), __uint_as_float(u.y));
+  }
+  // the pair within [-88, 89]; a NaN stays
+  __device__ __forceinline__ uint64_t gate() const {
+    if constexpr (sizeof(T) == 4 || C == 1) {
+      float2 f = unpack2(pair());
+      asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(f.x));
+      if (C == 2) asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(f.y));
+      return pack2(f.x, f.y);
+    } else {
+      uint32_t w = u;
+      if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %0, %1;\n min.NaN.f16x2 %0, %0, %2;" : "+r"(w) : "r"(0xD580D580u), "r"(0x55905590u));
+      else asm("max.NaN.bf16x2 %0, %0, %1;\n min.NaN.bf16x2 %0, %0, %2;" : "+r"(w) : "r"(0xC2B0C2B0u), "r"(0x42B242B2u));
+      return widen2<T>(w);
+    }
   }
   static __device__ __forceinline__ void store(T* p, uint64_t x) {
     const float2 f = unpack2(x);
@@ -46,11 +60,7 @@ struct Piece {
 // on average where |g| < 1 (beyond, log2 e as a float adds |g| / 4).  The average is what counts here: a
 // channel that remembers a thousand tokens multiplies as many decays, and ex2.approx, which is 0.4 units too small on average (measured),
 // would leave its state off by 2.4e-5.  Below 2^-126.5 the result is zero.
-__device__ __forceinline__ uint64_t decay(uint64_t g) {
-  float2 x = unpack2(g);
-  asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(x.x));   // [-88, 89]: there 2^n is zero, infinity
-  asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(x.y));
-  g = pack2(x.x, x.y);
+__device__ __forceinline__ uint64_t decay(uint64_t g) {   // of a g in [-88, 89]: there 2^n is zero, infinity
   const uint64_t log2e = pack2(1.4426950408889634f, 1.4426950408889634f), bias = pack2(12582912.f, 12582912.f);
   const uint64_t t = fma2(g, log2e, bias);   // 1.5 2^23 + n: n in the lowest bits
   const uint64_t f = fma2(g, log2e, fma2(t, pack2(-1.f, -1.f), bias));
@@ -95,44 +105,51 @@ struct Joined {
 
 // The two buffers of what the warps, and the CTAs of a cluster, leave for one another.  A buffer is written again two steps later, with
 // another barrier in between that everyone passes after reading it.
-template <bool CLUSTER>
+template <int W, bool CLUSTER>
 struct Exchange {
-  ulonglong2 warps[2][MOST_WARPS][32];
+  ulonglong2 warps[2][W][32];
   ulonglong2 ranks[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][32];
 };
 
 // What enters warp `warp` of this CTA, and (in `s`) what leaves the whole step: W warps of each of the cluster's CTAs, from the first
 // one to the last (REVERSE: from the last to the first).
-template <bool CLUSTER, bool REVERSE>
-__device__ __forceinline__ uint64_t join(Exchange<CLUSTER>& x, int turn, int rank, int n_ranks, Joined own, uint64_t& s) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
-  x.warps[turn][warp][lane] = make_ulonglong2(own.a, own.h);
-  __syncthreads();
-  auto warp_at = [&](int i) { return REVERSE ? W - 1 - i : i; };
+template <int W, bool CLUSTER, bool REVERSE>
+__device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int turn, int rank, int n_ranks, Joined own, uint64_t& s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if constexpr (W > 1) {
+    x.warps[turn][warp][lane] = make_ulonglong2(own.a, own.h);
+    __syncthreads();
+  }
   if constexpr (!CLUSTER) {
-    uint64_t mine = 0ull;
-    for (int i = 0; i < W; ++i) {
-      const int w = warp_at(i);
-      const ulonglong2 p = x.warps[turn][w][lane];
-      if (w == warp) mine = s;
-      s = fma2(p.x, s, p.y);
+    uint64_t mine = s;
+    if constexpr (W == 1) {
+      s = fma2(own.a, s, own.h);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const int w = REVERSE ? W - 1 - i : i;
+        const ulonglong2 p = x.warps[turn][w][lane];
+        if (w == warp) mine = s;
+        s = fma2(p.x, s, p.y);
+      }
     }
     return mine;
   } else {
-    Joined ahead = {0, 0}, all = {pack2(1.f, 1.f), 0ull};
+    Joined ahead = {pack2(1.f, 1.f), 0ull}, all = ahead;
+#pragma unroll
     for (int i = 0; i < W; ++i) {
-      const int w = warp_at(i);
+      const int w = REVERSE ? W - 1 - i : i;
       const ulonglong2 p = x.warps[turn][w][lane];
       if (w == warp) ahead = all;
       all.h = fma2(p.x, all.h, p.y);
       all.a = mul2(p.x, all.a);
     }
     cg::cluster_group cluster = cg::this_cluster();
-    if (warp < n_ranks)   // warp i tells CTA i
-      *cluster.map_shared_rank(&x.ranks[turn][rank][lane], warp) = make_ulonglong2(all.a, all.h);
-    for (int i = warp + W; i < n_ranks; i += W) *cluster.map_shared_rank(&x.ranks[turn][rank][lane], i) = make_ulonglong2(all.a, all.h);
+    for (int i = warp; i < n_ranks; i += W)   // to CTA i
+      *cluster.map_shared_rank(&x.ranks[turn][rank][lane], i) = make_ulonglong2(all.a, all.h);
     cluster.sync();
-    uint64_t entering = 0ull;
+    uint64_t entering = s;
+#pragma unroll 4
     for (int i = 0; i < n_ranks; ++i) {
       const int r = REVERSE ? n_ranks - 1 - i : i;
       const ulonglong2 p = x.ranks[turn][r][lane];
@@ -155,12 +172,12 @@ __device__ __forceinline__ Place place_of(const b200gdn_gated_recurrence_args& a
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
-template <typename T, typename G, int C, int R, bool CLUSTER>
-__global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_fwd_kernel(const b200gdn_gated_recurrence_args a) {
-  __shared__ Exchange<CLUSTER> exchange;
+template <typename T, typename G, int C, int R, int W, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2) recurrence_fwd_kernel(const b200gdn_gated_recurrence_args a) {
+  __shared__ Exchange<W, CLUSTER> exchange;
   const Place at = place_of<C, CLUSTER>(a);
   const Span seq = span_of(a, at.seq);
-  const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, step = at.n_ranks * W * R;
+  const int warp = threadIdx.x >> 5, step = at.n_ranks * W * R;
   const bool live = at.channel < a.D, two = C == 2;
   Piece<T, C> x[R];
   Piece<G, C> g[R];
@@ -168,13 +185,21 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_fwd_kernel(cons
   auto fetch = [&](int t) {
     const T* px = static_cast<const T*>(a.x) + (seq.first + t) * a.stride_x + at.channel;
     const G* pg = static_cast<const G*>(a.g) + (seq.first + t) * a.stride_g + at.channel;
+    if (live && t + R <= seq.len) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      x[r].zero();   // past the end: a decay of one, and nothing added
-      g[r].zero();
-      if (live && t + r < seq.len) {
-        x[r].load(px + r * a.stride_x);
-        g[r].load(pg + r * a.stride_g);
+      for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g) {
+        x[r].load(px);
+        g[r].load(pg);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g) {
+        x[r].zero();   // past the end: a decay of one, and nothing added
+        g[r].zero();
+        if (live && t + r < seq.len) {
+          x[r].load(px);
+          g[r].load(pg);
+        }
       }
     }
   };
@@ -185,59 +210,71 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_fwd_kernel(cons
     uint64_t decays[R];
     Piece<T, C> now[R];
     Joined own = {pack2(1.f, 1.f), 0ull};
+    if (t0 < seq.len) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      now[r] = x[r];
-      decays[r] = decay(g[r].pair());
-    }
-    if (i + 1 < n) fetch(t0 + step);
+      for (int r = 0; r < R; ++r) {
+        now[r] = x[r];
+        decays[r] = decay(g[r].gate());
+      }
+      if (i + 1 < n) fetch(t0 + step);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      own.h = fma2(decays[r], own.h, now[r].pair());
-      own.a = mul2(decays[r], own.a);
+      for (int r = 0; r < R; ++r) {
+        own.h = fma2(decays[r], own.h, now[r].pair());
+        own.a = mul2(decays[r], own.a);
+      }
     }
-    uint64_t h = join<CLUSTER, false>(exchange, i & 1, at.rank, at.n_ranks, own, s);
-    if (!live) continue;
-    if (a.states && (t0 & (BT - 1)) == 0 && t0 < seq.len) store_state(a.states, (int64_t)(seq.chunk + t0 / BT) * a.D + at.channel, h, two);
+    uint64_t h = join<W, CLUSTER, false>(exchange, i & 1, at.rank, at.n_ranks, own, s);
+    if (!live || t0 >= seq.len) continue;
+    if (a.states && (t0 & (BT - 1)) == 0) store_state(a.states, (int64_t)(seq.chunk + t0 / BT) * a.D + at.channel, h, two);
     T* ph = static_cast<T*>(a.h) + (seq.first + t0) * a.D + at.channel;
+    const int rows = seq.len - t0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
+    for (int r = 0; r < R; ++r, ph += a.D) {
       h = fma2(decays[r], h, now[r].pair());
-      if (t0 + r < seq.len) Piece<T, C>::store(ph + (int64_t)r * a.D, h);
+      if (r < rows) Piece<T, C>::store(ph, h);
     }
   }
   if (a.ht && live && at.rank == 0 && warp == 0) store_state(a.ht, (int64_t)at.seq * a.D + at.channel, s, two);
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
-template <typename T, typename G, int C, int R, bool CLUSTER>
-__global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_bwd_kernel(const b200gdn_gated_recurrence_args a) {
-  __shared__ Exchange<CLUSTER> exchange;
-  __shared__ ulonglong2 left[2][MOST_WARPS][32];   // (product of decays, tokens' own state) of the warps, from the left
+// A CTA's step is 64 tokens, of which the state ahead is known (or, W = 1, the whole of a sequence of up to R).
+template <typename T, typename G, int C, int R, int W, bool CLUSTER>
+__global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2) recurrence_bwd_kernel(const b200gdn_gated_recurrence_args a) {
+  static_assert(W == 1 || W * R == BT, "a CTA's step is a chunk");
+  __shared__ Exchange<W, CLUSTER> exchange;
+  __shared__ ulonglong2 left[W > 1 ? 2 : 1][W][32];   // (product of decays, tokens' own state) of the warps, from the left
   const Place at = place_of<C, CLUSTER>(a);
   const Span seq = span_of(a, at.seq);
-  const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = at.n_ranks * W * R;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = at.n_ranks * W * R;
   const bool live = at.channel < a.D, two = C == 2;
   Piece<T, C> x[R], dh[R];
   Piece<G, C> g[R];
-  uint64_t start;   // the state ahead of the 64 tokens that this warp's belong to (of one token's warps: ahead of its step)
+  uint64_t start = 0ull;
   const int n = (seq.len + step - 1) / step;
   int t0 = ((n - 1) * at.n_ranks + at.rank) * W * R + warp * R;
-  // a step's 64-token blocks begin with it: W R is a multiple of 64, or a CTA's only step begins at the sequence's first token
-  const int in_block = min(W, BT / R), first_warp = warp / in_block * in_block;
   auto fetch = [&](int t) {
     const T* px = static_cast<const T*>(a.x) + (seq.first + t) * a.stride_x + at.channel;
     const G* pg = static_cast<const G*>(a.g) + (seq.first + t) * a.stride_g + at.channel;
     const T* pd = static_cast<const T*>(a.dh) + (seq.first + t) * a.D + at.channel;
+    if (live && t + R <= seq.len && a.dh) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      x[r].zero();
-      g[r].zero();
-      dh[r].zero();
-      if (live && t + r < seq.len) {
-        x[r].load(px + r * a.stride_x);
-        g[r].load(pg + r * a.stride_g);
-        if (a.dh) dh[r].load(pd + (int64_t)r * a.D);
+      for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g, pd += a.D) {
+        x[r].load(px);
+        g[r].load(pg);
+        dh[r].load(pd);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g, pd += a.D) {
+        x[r].zero();
+        g[r].zero();
+        dh[r].zero();
+        if (live && t + r < seq.len) {
+          x[r].load(px);
+          g[r].load(pg);
+          if (a.dh) dh[r].load(pd);
+        }
       }
     }
     start = load_state(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, live && t < seq.len, two);
@@ -247,12 +284,11 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_bwd_kernel(cons
   for (int i = 0; i < n; ++i, t0 -= step) {
     uint64_t decays[R], kept[R];
     Piece<T, C> up[R];
-    uint64_t h = start;
+    uint64_t h = start, own_left = 0ull;
     Joined own = {pack2(1.f, 1.f), 0ull};
-    uint64_t own_left = 0ull;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      decays[r] = decay(g[r].pair());
+      decays[r] = decay(g[r].gate());
       up[r] = dh[r];
       kept[r] = x[r].pair();
     }
@@ -264,13 +300,16 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_bwd_kernel(cons
       const int q = R - 1 - r;
       own.h = mul2(decays[q], add2(up[q].pair(), own.h));
     }
-    left[i & 1][warp][lane] = make_ulonglong2(own.a, own_left);
-    uint64_t u = join<CLUSTER, true>(exchange, i & 1, at.rank, at.n_ranks, own, s);
-    for (int w = first_warp; w < warp; ++w) {
-      const ulonglong2 p = left[i & 1][w][lane];
-      h = fma2(p.x, h, p.y);
+    if constexpr (W > 1) left[i & 1][warp][lane] = make_ulonglong2(own.a, own_left);
+    uint64_t u = join<W, CLUSTER, true>(exchange, i & 1, at.rank, at.n_ranks, own, s);
+    if constexpr (W > 1) {
+#pragma unroll
+      for (int w = 0; w < W - 1; ++w) {
+        const ulonglong2 p = left[i & 1][w][lane];
+        if (w < warp) h = fma2(p.x, h, p.y);
+      }
     }
-    if (!live) continue;
+    if (!live || t0 >= seq.len) continue;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint64_t from_before = mul2(decays[r], h);
@@ -279,12 +318,13 @@ __global__ void __launch_bounds__(MOST_WARPS * 32, 1) recurrence_bwd_kernel(cons
     }
     T* px = static_cast<T*>(a.dx) + (seq.first + t0) * a.D + at.channel;
     G* pg = static_cast<G*>(a.dg) + (seq.first + t0) * a.D + at.channel;
+    const int rows = seq.len - t0;
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       const int r = R - 1 - q;
       const uint64_t d = add2(up[r].pair(), u);
       u = mul2(decays[r], d);
-      if (t0 + r < seq.len) {
+      if (r < rows) {
         Piece<T, C>::store(px + (int64_t)r * a.D, d);
         if (a.dg) Piece<G, C>::store(pg + (int64_t)r * a.D, mul2(d, kept[r]));
       }
@@ -304,7 +344,7 @@ __global__ void __launch_bounds__(128) recurrence_step_kernel(const b200gdn_gate
     x.load(static_cast<const T*>(a.x) + (int64_t)seq * a.stride_x + d);
     g.load(static_cast<const G*>(a.g) + (int64_t)seq * a.stride_g + d);
     const int64_t at = (int64_t)seq * a.D + d;
-    const uint64_t before = load_state(a.h0, at, true, C == 2), h = fma2(decay(g.pair()), before, x.pair());
+    const uint64_t before = load_state(a.h0, at, true, C == 2), h = fma2(decay(g.gate()), before, x.pair());
     if (a.states) store_state(a.states, at, before, C == 2);
     Piece<T, C>::store(static_cast<T*>(a.h) + at, h);
     if (a.ht) store_state(a.ht, at, h, C == 2);
@@ -312,10 +352,25 @@ __global__ void __launch_bounds__(128) recurrence_step_kernel(const b200gdn_gate
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------------
-template <typename Kern>
-int launch_walk(Kern kern, const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, int C) {
+// clusters of more than eight CTAs have to be asked for, once per thread, kernel and device
+template <auto KERN>
+int allow_large_clusters() {
+  static thread_local uint64_t known = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 64 && (known >> dev & 1)) return 0;
+  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return set_error(B200GDN_ERR_CUDA, "cudaFuncSetAttribute(cluster size): %s", cudaGetErrorString(cudaGetLastError()));
+  if (dev < 64) known |= 1ull << dev;
+  return 0;
+}
+
+template <auto KERN>
+int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, int C) {
   const int64_t ctas = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)) * ranks;
   if (ctas > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 pieces of work", what);
+  if (ranks > 8)
+    if (int e = allow_large_clusters<KERN>()) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(W * 32);
@@ -326,7 +381,7 @@ int launch_walk(Kern kern, const char* what, const b200gdn_gated_recurrence_args
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  (void)cudaLaunchKernelEx(&cfg, kern, a);   // (an error is check_launch's to name)
+  (void)cudaLaunchKernelEx(&cfg, KERN, a);   // (an error is check_launch's to name)
   return check_launch(what);
 }
 
@@ -337,19 +392,20 @@ int launch_c(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd) 
     recurrence_step_kernel<T, G, C><<<dim3((a.D + 128 * C - 1) / (128 * C), n), 128, 0, st>>>(a);
     return check_launch("recurrence_step");
   }
-  constexpr int R = 8;
-  const int64_t tokens = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT / a.n_seq + 1;   // of a sequence, on average
-  int W = 1;
-  while (W < MOST_WARPS && W * R < tokens) W *= 2;
-  if (bwd && a.seq_len == 0 && W * R < BT) W = BT / R;   // a sequence may be longer than the others: its steps begin where chunks do
-  const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)), most = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT;
+  constexpr int W = 8, RB = BT / W, RF = sizeof(T) + sizeof(G) == 4 ? 16 : 8;
+  const int64_t tokens = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT;   // of a sequence, at most
+  if (a.seq_len > 0 && tokens <= (bwd ? RB : RF))
+    return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, 1, false>>("recurrence_bwd", a, st, 1, 1, C)
+               : launch_walk<recurrence_fwd_kernel<T, G, C, RF, 1, false>>("recurrence_fwd", a, st, 1, 1, C);
+  // two CTAs an SM
+  const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)), step = bwd ? BT : W * RF;
   int ranks = 1;
-  while (ranks < MOST_RANKS && work * ranks * 2 <= sm_count() && (int64_t)ranks * 2 * W * R <= most) ranks *= 2;
+  while (ranks < MOST_RANKS && work * ranks * 2 <= 2 * sm_count() && ranks * step < tokens) ranks *= 2;
   if (ranks > 1)
-    return bwd ? launch_walk(recurrence_bwd_kernel<T, G, C, R, true>, "recurrence_bwd", a, st, W, ranks, C)
-               : launch_walk(recurrence_fwd_kernel<T, G, C, R, true>, "recurrence_fwd", a, st, W, ranks, C);
-  return bwd ? launch_walk(recurrence_bwd_kernel<T, G, C, R, false>, "recurrence_bwd", a, st, W, 1, C)
-             : launch_walk(recurrence_fwd_kernel<T, G, C, R, false>, "recurrence_fwd", a, st, W, 1, C);
+    return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, W, true>>("recurrence_bwd", a, st, W, ranks, C)
+               : launch_walk<recurrence_fwd_kernel<T, G, C, RF, W, true>>("recurrence_fwd", a, st, W, ranks, C);
+  return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, W, false>>("recurrence_bwd", a, st, W, 1, C)
+             : launch_walk<recurrence_fwd_kernel<T, G, C, RF, W, false>>("recurrence_fwd", a, st, W, 1, C);
 }
 
 // two channels a thread where every row of every tensor allows it

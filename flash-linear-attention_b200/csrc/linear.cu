@@ -10,7 +10,7 @@
 // Few tokens (up to 256): the product is formed the other way round, W's rows as the 256-row side and the tokens as a BN of 32 to 256, so that
 // what is read is W and little else.  Where there are fewer tiles than CTA pairs the contraction is split; the parts are left in fp32 and a
 // second kernel adds them in order and finishes.
-// Up to eight tokens, forward: W passes through registers once, as fast as memory gives it (linear_few_kernel).
+// Up to 16 tokens, forward: W passes through registers once, as fast as memory gives it (linear_few_kernel).
 // TMA wants rows 16 bytes apart: operands of other widths are first copied to rows that are.
 #include "gdn_common.cuh"
 #include "rowio.cuh"
@@ -161,49 +161,35 @@ __device__ __forceinline__ void store32(void* p, uint4 a, uint4 b) {   // 32 byt
                "r"(b.w)
                : "memory");
 }
-// 32 neighbouring elements of a row of `n` from element j on; `wide`: how the row lies
+// 32 neighbouring elements of a row; `wide`: the boundary it lies on
 template <typename T>
-__device__ __forceinline__ void put_row(void* row, int j, int n, int wide, const float (&v)[32]) {
-  T* p = static_cast<T*>(row) + j;
-  if (wide && j + 32 <= n) {
+__device__ __forceinline__ void put_row(T* p, int wide, const float (&v)[32]) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      uint4 w[2];
+  for (int q = 0; q < 2; ++q) {
+    uint4 w[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x[8];
+    for (int h = 0; h < 2; ++h) {
+      float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = v[q * 16 + h * 8 + e];
-        w[h] = pack8<T>(x);
-      }
-      if (wide == 32) {
-        store32(p + q * 16, w[0], w[1]);
-      } else {
-        reinterpret_cast<uint4*>(p)[2 * q] = w[0];
-        reinterpret_cast<uint4*>(p)[2 * q + 1] = w[1];
-      }
+      for (int e = 0; e < 8; ++e) x[e] = v[q * 16 + h * 8 + e];
+      w[h] = pack8<T>(x);
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (j + e < n) p[e] = static_cast<T>(v[e]);
+    if (wide == 32) {
+      store32(p + q * 16, w[0], w[1]);
+    } else {
+      reinterpret_cast<uint4*>(p)[2 * q] = w[0];
+      reinterpret_cast<uint4*>(p)[2 * q + 1] = w[1];
+    }
   }
 }
 template <typename T>
-__device__ __forceinline__ void add_row(const void* row, int j, int n, int wide, float (&v)[32]) {
-  const T* p = static_cast<const T*>(row) + j;
-  if (wide && j + 32 <= n) {
+__device__ __forceinline__ void add_row(const T* p, float (&v)[32]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float x[8];
-      unpack8<T>(reinterpret_cast<const uint4*>(p)[q], x);
+  for (int q = 0; q < 4; ++q) {
+    float x[8];
+    unpack8<T>(reinterpret_cast<const uint4*>(p)[q], x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[q * 8 + e] += x[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (j + e < n) v[e] += (float)p[e];
+    for (int e = 0; e < 8; ++e) v[q * 8 + e] += x[e];
   }
 }
 
@@ -217,6 +203,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   unsigned char* tiles = raw + ((1024 - (tc5::smem_addr(raw) & 1023)) & 1023);
   __shared__ uint64_t full[STAGES], empty[STAGES], done[2], taken[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ float turned[SWAPPED ? 1 : 4][32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cta_rank();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -334,25 +321,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         __syncwarp();
         tmem_ld32(tmem + half * BN + c + ((uint32_t)(warp * 32) << 16), v);
         tc5::tmem_ld_wait();
-        if (!live) continue;
         if constexpr (!SWAPPED) {
           if (p.splits > 1) {
             float* part = p.parts + ((int64_t)at.split * p.tokens + i) * p.pitch + j;
 #pragma unroll
             for (int q = 0; q < 4; ++q)   // (the pitch is a multiple of eight)
-              if (j + q * 8 < p.cols)
+              if (live && j + q * 8 < p.cols)
                 store32(part + q * 8, *reinterpret_cast<const uint4*>(&v[q * 8]), *reinterpret_cast<const uint4*>(&v[q * 8 + 4]));
-            continue;
-          }
-          const int64_t row = (int64_t)i * p.features;
-          if (p.bias) add_row<T>(p.bias, j, p.cols, p.wide, v);
-          if (p.z) put_row<T>(static_cast<T*>(p.z) + row, j, p.cols, p.wide, v);
-          if (p.act != NONE)
+          } else if (p.wide && j + 32 <= p.cols) {   // a lane writes 64 bytes of its row, whole sectors
+            if (!live) continue;
+            const int64_t to = (int64_t)i * p.features + j;
+            if (p.bias) add_row<T>(static_cast<const T*>(p.bias) + j, v);
+            if (p.z) put_row<T>(static_cast<T*>(p.z) + to, p.wide, v);
+            if (p.act != NONE)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = activate(v[e], p.act);
-          if (p.residual) add_row<T>(static_cast<const T*>(p.residual) + row, j, p.cols, p.wide, v);
-          put_row<T>(static_cast<T*>(p.out) + row, j, p.cols, p.wide, v);
+              for (int e = 0; e < 32; ++e) v[e] = activate(v[e], p.act);
+            if (p.residual) add_row<T>(static_cast<const T*>(p.residual) + to, v);
+            put_row<T>(static_cast<T*>(p.out) + to, p.wide, v);
+          } else {   // rows on any boundary: turned round, so that a warp writes a row's 32 columns at a time
+#pragma unroll
+            for (int e = 0; e < 32; ++e) turned[warp][lane][e] = v[e];
+            __syncwarp();
+            const int col = j + lane, i0 = i - lane;
+            if (col < p.cols) {
+              const float b = p.bias ? (float)static_cast<const T*>(p.bias)[col] : 0.f;
+              int64_t to = (int64_t)i0 * p.features + col;
+#pragma unroll 4
+              for (int r = 0; r < 32 && i0 + r < p.rows; ++r, to += p.features) {
+                float x = turned[warp][r][lane] + b;
+                if (p.z) static_cast<T*>(p.z)[to] = static_cast<T>(x);
+                x = activate(x, p.act);
+                if (p.residual) x += (float)static_cast<const T*>(p.residual)[to];
+                static_cast<T*>(p.out)[to] = static_cast<T>(x);
+              }
+            }
+            __syncwarp();
+          }
         } else {
+          if (!live) continue;
           const float b = p.bias && p.splits == 1 ? (float)static_cast<const T*>(p.bias)[i] : 0.f;
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
@@ -384,154 +390,194 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   if (warp == 5) pair_tmem_dealloc(tmem, COLUMNS);
 }
 
-// the parts of a split contraction in their order, and what follows the product
+// the parts of a split contraction in their order, and what follows the product; four features a thread
 template <typename T>
-__global__ void __launch_bounds__(256) linear_join_kernel(const Product p) {
+__global__ void __launch_bounds__(128) linear_join_kernel(const Product p) {
   wait_for_predecessor();
-  const int64_t n = p.tokens * p.features, size = p.tokens * p.pitch;
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
-    const int64_t token = at / p.features;
-    const int f = (int)(at - token * p.features);
-    const float* part = p.parts + token * p.pitch + f;
-    float v = part[0];
-    for (int s = 1; s < p.splits; ++s) v += part[s * size];
-    if (p.bias) v += (float)static_cast<const T*>(p.bias)[f];
-    if (p.z) static_cast<T*>(p.z)[at] = static_cast<T>(v);
-    v = activate(v, p.act);
-    if (p.residual) v += (float)static_cast<const T*>(p.residual)[at];
-    static_cast<T*>(p.out)[at] = static_cast<T>(v);
+  const int f0 = (blockIdx.x * 128 + threadIdx.x) * 4;
+  if (f0 >= p.features) return;
+  const int64_t size = p.tokens * p.pitch;
+  for (int64_t token = blockIdx.y; token < p.tokens; token += gridDim.y) {
+    const float* part = p.parts + token * p.pitch + f0;   // (the pitch is a multiple of eight)
+    float4 sum = *reinterpret_cast<const float4*>(part);
+#pragma unroll 4
+    for (int s = 1; s < p.splits; ++s) {
+      const float4 q = *reinterpret_cast<const float4*>(part + s * size);
+      sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+    }
+    const float v4[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int f = f0 + e;
+      if (f >= p.features) break;
+      const int64_t at = token * p.features + f;
+      float v = v4[e];
+      if (p.bias) v += (float)static_cast<const T*>(p.bias)[f];
+      if (p.z) static_cast<T*>(p.z)[at] = static_cast<T>(v);
+      v = activate(v, p.act);
+      if (p.residual) v += (float)static_cast<const T*>(p.residual)[at];
+      static_cast<T*>(p.out)[at] = static_cast<T>(v);
+    }
   }
 }
 
-// ---- up to eight tokens, forward ---------------------------------------------------------------------------------------------
-// A CTA of eight warps forms 8 / WK x R features of all tokens: WK warps share R rows of W, each a part of the contraction, which their lanes walk
-// side by side in 16-byte pieces (one element where rows do not lie so); sums of even and odd elements go together (f32x2).
-constexpr int R = 4;
-template <typename T, int TOKENS, bool WIDE>
-__global__ void __launch_bounds__(256) linear_few_kernel(const Product p, const void* x, const void* w, int K, int WK) {
-  constexpr int E = WIDE ? 8 : 1, P = (E + 1) / 2;
-  __shared__ float sums[8][R * TOKENS];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WK;
-  const int f0 = (blockIdx.x * (8 / WK) + warp / WK) * R;
+// ---- few tokens, forward -----------------------------------------------------------------------------------------------------
+// 16 features a CTA, whose warps share the contraction 256 at a time.  What bounds it is W's bytes, so what counts is loads on their way and
+// little else: a lane loads 16 bytes of a row of W, and of x, straight into the registers of mma.sync's operands (which contraction index goes
+// where does not matter as long as it is the same in both), 8 steps of 32 at once; nothing is converted or staged.  tcgen05 would need the
+// bytes to pass through shared memory and a split contraction to occupy every SM.
+constexpr int FEW_STEPS = 8, FEW_WARPS = 16;
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// eight neighbouring elements of a row from k on; zeros past its end, or where there is no row
+template <bool WIDE>
+__device__ __forceinline__ uint4 eight(const uint16_t* row, int k, int K, bool there) {
+  uint4 u = make_uint4(0, 0, 0, 0);
+  if constexpr (WIDE) {
+    if (there && k < K) u = __ldg(reinterpret_cast<const uint4*>(row + k));
+  } else {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (there && k + e < K) w[e >> 1] |= (uint32_t)row[k + e] << (16 * (e & 1));
+    u = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return u;
+}
+template <typename T, int NT, bool WIDE>   // up to 8 NT tokens
+__global__ void __launch_bounds__(FEW_WARPS * 32) linear_few_kernel(const Product p, const uint16_t* x, const uint16_t* w, int K) {
+  __shared__ float sums[FEW_WARPS][16][8 * NT];
+  constexpr int S = NT > 1 ? FEW_STEPS / 2 : FEW_STEPS;   // steps on their way at once
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3, f0 = blockIdx.x * 16;
   const int n_tokens = (int)p.tokens;
-  uint64_t acc[R][TOKENS];
+  const uint16_t* rows[2] = {w + (int64_t)(f0 + g) * K, w + (int64_t)(f0 + g + 8) * K};
+  float acc[NT][4];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+  for (int k0 = warp * S * 32; k0 < K; k0 += warps * S * 32) {
+    uint4 a[S][2], b[S][NT];
 #pragma unroll
-    for (int t = 0; t < TOKENS; ++t) acc[r][t] = 0ull;
-  auto pairs_of = [&](const void* base, int64_t at, uint64_t (&v)[P]) {
-    if constexpr (WIDE) {
-      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(base) + at);
-      v[0] = widen2<T>(u.x), v[1] = widen2<T>(u.y), v[2] = widen2<T>(u.z), v[3] = widen2<T>(u.w);
-    } else {
-      v[0] = pack2((float)static_cast<const T*>(base)[at], 0.f);
+    for (int s = 0; s < S; ++s) {
+      const int k = k0 + s * 32 + t * 8;
+      a[s][0] = eight<WIDE>(rows[0], k, K, f0 + g < p.features);
+      a[s][1] = eight<WIDE>(rows[1], k, K, f0 + g + 8 < p.features);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) b[s][n] = eight<WIDE>(x + (int64_t)(n * 8 + g) * K, k, K, n * 8 + g < n_tokens);
     }
-  };
-  constexpr int U = 2;   // pieces of each row on their way
-  for (int k = (part * 32 + lane) * E; k < K; k += WK * 32 * E * U) {
-    uint64_t a[U][R][P];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int s = 0; s < S; ++s)
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int at = k + u * WK * 32 * E;
-        if (f0 + r < p.features && at < K) pairs_of(w, (int64_t)(f0 + r) * K + at, a[u][r]);
-        else
-#pragma unroll
-          for (int i = 0; i < P; ++i) a[u][r][i] = 0ull;
+      for (int n = 0; n < NT; ++n) {
+        mma_16816<T>(acc[n], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b[s][n].x, b[s][n].y);
+        mma_16816<T>(acc[n], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b[s][n].z, b[s][n].w);
       }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = k + u * WK * 32 * E;
-      if (at >= K) break;
-#pragma unroll
-      for (int t = 0; t < TOKENS; ++t) {
-        if (t >= n_tokens) break;
-        uint64_t b[P];
-        pairs_of(x, (int64_t)t * K + at, b);
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int i = 0; i < P; ++i) acc[r][t] = fma2(a[u][r][i], b[i], acc[r][t]);
-      }
-    }
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int t = 0; t < TOKENS; ++t) {
-      const float2 f = unpack2(acc[r][t]);
-      float v = f.x + f.y;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) sums[warp][r * TOKENS + t] = v;
-    }
+  for (int n = 0; n < NT; ++n) {
+    sums[warp][g][n * 8 + 2 * t] = acc[n][0];
+    sums[warp][g][n * 8 + 2 * t + 1] = acc[n][1];
+    sums[warp][g + 8][n * 8 + 2 * t] = acc[n][2];
+    sums[warp][g + 8][n * 8 + 2 * t + 1] = acc[n][3];
+  }
   __syncthreads();
-  const int at = threadIdx.x, group = at / (R * TOKENS);   // one thread a result: 8 / WK x R x TOKENS of at most 256
-  if (group >= 8 / WK) return;
-  const int r = at % (R * TOKENS) / TOKENS, t = at % TOKENS, f = (blockIdx.x * (8 / WK) + group) * R + r;
-  if (f >= p.features || t >= n_tokens) return;
-  float v = 0.f;
-  for (int i = 0; i < WK; ++i) v += sums[group * WK + i][r * TOKENS + t];
-  if (p.bias) v += (float)static_cast<const T*>(p.bias)[f];
-  const int64_t to = (int64_t)t * p.features + f;
-  if (p.z) static_cast<T*>(p.z)[to] = static_cast<T>(v);
-  v = activate(v, p.act);
-  if (p.residual) v += (float)static_cast<const T*>(p.residual)[to];
-  static_cast<T*>(p.out)[to] = static_cast<T>(v);
+  for (int i = threadIdx.x; i < 16 * 8 * NT; i += blockDim.x) {
+    const int f = f0 + (i & 15), token = i >> 4;
+    if (f >= p.features || token >= n_tokens) continue;
+    float v = 0.f;
+    for (int q = 0; q < warps; ++q) v += sums[q][i & 15][token];
+    if (p.bias) v += (float)static_cast<const T*>(p.bias)[f];
+    const int64_t to = (int64_t)token * p.features + f;
+    if (p.z) static_cast<T*>(p.z)[to] = static_cast<T>(v);
+    v = activate(v, p.act);
+    if (p.residual) v += (float)static_cast<const T*>(p.residual)[to];
+    static_cast<T*>(p.out)[to] = static_cast<T>(v);
+  }
 }
 
 // ---- around the gradient's products ------------------------------------------------------------------------------------------
-// rows of `cols` to rows `pitch` apart
-__global__ void __launch_bounds__(256) linear_pad_kernel(const uint16_t* src, uint16_t* dst, int64_t rows, int cols, int pitch) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) dst[r * pitch + c] = src[r * cols + c];
+// rows of `cols` to rows `pitch` apart, of up to two operands; eight elements a thread
+struct Copies {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int64_t rows[2];
+  int cols[2], pitch[2];
+};
+__global__ void __launch_bounds__(128) linear_pad_kernel(const Copies c) {
+  const int o = blockIdx.z, at = (blockIdx.x * 128 + threadIdx.x) * 8, cols = c.cols[o];
+  if (at >= cols) return;
+  for (int64_t r = blockIdx.y; r < c.rows[o]; r += gridDim.y)
+    *reinterpret_cast<uint4*>(c.dst[o] + r * c.pitch[o] + at) = eight<false>(c.src[o] + r * cols, at, cols, true);
+}
+
+// act'(z) of a pair
+__device__ __forceinline__ uint64_t slope2(uint64_t z, int act) {
+  const uint64_t one = pack2(1.f, 1.f);
+  if (act == GELU) {
+    const float2 f = unpack2(z);
+    return pack2(slope(f.x, GELU), slope(f.y, GELU));
+  }
+  const uint64_t s = fast_sigmoid2(z), rest = fma2(s, pack2(-1.f, -1.f), one);
+  return act == SILU ? mul2(s, fma2(z, rest, one)) : mul2(s, rest);
 }
 
 // dz = dy act'(z) (rounded for the products; `dz` NULL: not wanted) and, for db, its sums over the rows of a CTA, unrounded.  Warps take rows in
-// turn, lanes E columns each.
+// turn, lanes E columns each; four rows are on their way at once.
 template <typename T, int E>
-__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, const T* z, T* dz, float* sums, int64_t rows, int cols, int pitch, int act) {
+__global__ void __launch_bounds__(256, 3) linear_dz_kernel(const T* dy, const T* z, T* dz, float* sums, int64_t rows, int cols, int pitch, int act) {
+  constexpr int P = (E + 1) / 2, U = 4;
+  using Raw = std::conditional_t<E == 8, uint4, uint16_t>;
   __shared__ float part[8][32 * E];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = (blockIdx.x * 32 + lane) * E;
-  float total[E];
+  uint64_t total[P];
 #pragma unroll
-  for (int e = 0; e < E; ++e) total[e] = 0.f;
-  auto get = [&](const T* p, float (&v)[E]) {
-    if constexpr (E == 8) unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
-    else v[0] = (float)*p;
+  for (int i = 0; i < P; ++i) total[i] = 0ull;
+  auto pair = [](const Raw& u, int i) {
+    if constexpr (E == 8) return widen2<T>(reinterpret_cast<const uint32_t*>(&u)[i]);
+    else return pack2((float)*reinterpret_cast<const T*>(&u), 0.f);
   };
   if (c < cols) {
-    constexpr int U = 4;
     const int64_t step = (int64_t)gridDim.y * 8;
     for (int64_t r0 = blockIdx.y * 8 + warp; r0 < rows; r0 += step * U) {
-      float d[U][E], v[U][E];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (r0 + u * step < rows) {
-          get(dy + (r0 + u * step) * cols + c, d[u]);
-          if (act != NONE) get(z + (r0 + u * step) * cols + c, v[u]);
-        }
+      Raw d[U], v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t r = r0 + u * step;
-        if (r >= rows) break;
+        d[u] = v[u] = Raw{};
+        if (r0 + u * step < rows) {
+          d[u] = *reinterpret_cast<const Raw*>(dy + (r0 + u * step) * cols + c);
+          if (act != NONE) v[u] = *reinterpret_cast<const Raw*>(z + (r0 + u * step) * cols + c);
+        }
+      }
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if (act != NONE) d[u][e] *= slope(v[u][e], act);
-          total[e] += d[u][e];
+      for (int u = 0; u < U; ++u) {
+        Raw out;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          uint64_t g = pair(d[u], i);
+          if (act != NONE) g = mul2(g, slope2(pair(v[u], i), act));
+          total[i] = add2(total[i], g);   // (a row past the end adds zeros)
+          if constexpr (E == 8) reinterpret_cast<uint32_t*>(&out)[i] = narrow2<T>(g);
+          else *reinterpret_cast<T*>(&out) = static_cast<T>(unpack2(g).x);
         }
-        if (dz) {
-          if constexpr (E == 8) *reinterpret_cast<uint4*>(dz + r * pitch + c) = pack8<T>(d[u]);
-          else dz[r * pitch + c] = static_cast<T>(d[u][0]);
-        }
+        if (dz && r0 + u * step < rows) *reinterpret_cast<Raw*>(dz + (r0 + u * step) * pitch + c) = out;
       }
     }
   }
   if (sums == nullptr) return;
 #pragma unroll
-  for (int e = 0; e < E; ++e) part[warp][lane * E + e] = total[e];
+  for (int i = 0; i < P; ++i) {
+    const float2 f = unpack2(total[i]);
+    part[warp][lane * E + 2 * i] = f.x;
+    if (E > 1) part[warp][lane * E + 2 * i + 1] = f.y;
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < 32 * E; i += 256) {
     const int col = blockIdx.x * 32 * E + i;
@@ -627,12 +673,12 @@ int launch_product(const Operand& a, const Operand& b, int64_t depth, Product p,
                          : launch_tiles<T, 32, A_MN, false, true>(a, b, p, st);
   }
   if (e != 0 || plan.splits == 1) return e;
-  const int64_t n = (p.tokens * p.features + 255) / 256, most = 8 * (int64_t)sm_count();
-  launch_overlapped(true, linear_join_kernel<T>, dim3((unsigned)(n < most ? n : most)), 256, 0, st, p);
+  const int64_t x = (p.features + 511) / 512, most = 16 * (int64_t)sm_count() / x + 1;
+  launch_overlapped(true, linear_join_kernel<T>, dim3((unsigned)x, (unsigned)(p.tokens < most ? p.tokens : most)), 128, 0, st, p);
   return check_launch("linear_join");
 }
 
-constexpr int64_t FEW = 8, SWAP = 256;   // tokens up to which W's rows pass through registers, and up to which they are the tile's 256
+constexpr int64_t FEW = 16, SWAP = 256;   // tokens up to which W passes through registers, and up to which its rows are the tile's 256
 
 // The workspace, piece by piece on 256-byte boundaries; without a base it only counts.
 struct Space {
@@ -646,17 +692,28 @@ struct Space {
 };
 bool fits_tma(const void* p, int64_t cols) { return cols % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// the operand itself, or its copy with rows 16 bytes apart
-int operand_of(const void* base, int64_t rows, int64_t cols, Space& space, cudaStream_t st, bool run, Operand& o) {
-  o = Operand{base, rows, cols, cols};
-  if (fits_tma(base, cols)) return 0;
-  o.pitch = up(cols, 8);
-  void* copy = space.take(rows * o.pitch * 2);
-  o.base = copy;
-  if (!run) return 0;
-  const int64_t x = (cols + 255) / 256, most = 16 * (int64_t)sm_count() / x + 1;
-  linear_pad_kernel<<<dim3((unsigned)x, (unsigned)(rows < most ? rows : most)), 256, 0, st>>>(static_cast<const uint16_t*>(base), static_cast<uint16_t*>(copy),
-                                                                                               rows, (int)cols, (int)o.pitch);
+// Two operands, each itself or its copy with rows 16 bytes apart (a base of NULL: no such operand).
+int operands_of(Operand& a, Operand& b, Space& space, cudaStream_t st, bool run) {
+  Copies c{};
+  int n = 0;
+  int64_t x = 1, y = 1;
+  for (Operand* o : {&a, &b}) {
+    if (o->base == nullptr || fits_tma(o->base, o->cols)) continue;
+    o->pitch = up(o->cols, 8);
+    void* copy = space.take(o->rows * o->pitch * 2);
+    c.src[n] = static_cast<const uint16_t*>(o->base);
+    c.dst[n] = static_cast<uint16_t*>(copy);
+    c.rows[n] = o->rows;
+    c.cols[n] = (int)o->cols;
+    c.pitch[n] = (int)o->pitch;
+    o->base = copy;
+    x = x > (o->cols + 1023) / 1024 ? x : (o->cols + 1023) / 1024;
+    y = y > o->rows ? y : o->rows;
+    ++n;
+  }
+  if (n == 0 || !run) return 0;
+  const int64_t most = 16 * (int64_t)sm_count() / x + 1;
+  linear_pad_kernel<<<dim3((unsigned)x, (unsigned)(y < most ? y : most), n), 128, 0, st>>>(c);
   return check_launch("linear_pad");
 }
 
@@ -672,20 +729,16 @@ int forward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool ru
     if (!run) return 0;
     p.tokens = a.rows;
     p.features = a.N;
-    int wk = 1;
-    while (wk < 8 && (int64_t)a.N * wk / (8 * R) < 3 * sm_count() && wk * 512 <= a.K) wk *= 2;
-    const int grid = (a.N + 8 / wk * R - 1) / (8 / wk * R);
+    // sixteen warps a CTA where features are few and the contraction long, else eight
+    const int grid = (a.N + 15) / 16, warps = grid < 2 * sm_count() && a.K > 8 * FEW_STEPS * 32 ? 16 : 8;
     const bool wide = fits_tma(a.x, a.K) && fits_tma(a.weight, a.K);
-    auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>(p, a.x, a.weight, a.K, wk); };
-    if (a.rows == 1) wide ? go(linear_few_kernel<T, 1, true>) : go(linear_few_kernel<T, 1, false>);
-    else if (a.rows == 2) wide ? go(linear_few_kernel<T, 2, true>) : go(linear_few_kernel<T, 2, false>);
-    else if (a.rows <= 4) wide ? go(linear_few_kernel<T, 4, true>) : go(linear_few_kernel<T, 4, false>);
-    else wide ? go(linear_few_kernel<T, 8, true>) : go(linear_few_kernel<T, 8, false>);
+    auto go = [&](auto kern) { kern<<<grid, warps * 32, 0, st>>>(p, static_cast<const uint16_t*>(a.x), static_cast<const uint16_t*>(a.weight), a.K); };
+    if (a.rows <= 8) wide ? go(linear_few_kernel<T, 1, true>) : go(linear_few_kernel<T, 1, false>);
+    else wide ? go(linear_few_kernel<T, 2, true>) : go(linear_few_kernel<T, 2, false>);
     return check_launch("linear_few");
   }
-  Operand x, w;
-  if (int e = operand_of(a.x, a.rows, a.K, space, st, run, x)) return e;
-  if (int e = operand_of(a.weight, a.N, a.K, space, st, run, w)) return e;
+  Operand x{a.x, a.rows, a.K, a.K}, w{a.weight, a.N, a.K, a.K};
+  if (int e = operands_of(x, w, space, st, run)) return e;
   const bool swapped = a.rows <= SWAP;
   p.rows = swapped ? a.N : (int)a.rows;
   p.cols = swapped ? (int)a.rows : a.N;
@@ -707,13 +760,13 @@ int backward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool r
   }
   const bool wide = fits_tma(a.dy, a.N) && fits_tma(a.z, a.N);
   const int per = wide ? 256 : 32;
-  const int64_t x = (a.N + per - 1) / per;
-  int64_t y = 8 * (int64_t)sm_count() / x + 1;
+  const int64_t columns = (a.N + per - 1) / per;
+  int64_t y = 6 * (int64_t)sm_count() / columns + 1;
   if (y > (a.rows + 31) / 32) y = (a.rows + 31) / 32;
   float* sums = a.dbias ? static_cast<float*>(space.take(y * a.N * 4)) : nullptr;
   if (run && (apart || a.dbias)) {
     auto go = [&](auto kern) {
-      kern<<<dim3((unsigned)x, (unsigned)y), 256, 0, st>>>(static_cast<const T*>(a.dy), static_cast<const T*>(a.z), made, sums, a.rows, a.N, (int)dz.pitch,
+      kern<<<dim3((unsigned)columns, (unsigned)y), 256, 0, st>>>(static_cast<const T*>(a.dy), static_cast<const T*>(a.z), made, sums, a.rows, a.N, (int)dz.pitch,
                                                           a.activation);
     };
     wide ? go(linear_dz_kernel<T, 8>) : go(linear_dz_kernel<T, 1>);
@@ -723,9 +776,9 @@ int backward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool r
       if (int e = check_launch("linear_dbias")) return e;
     }
   }
+  Operand x{a.dweight ? a.x : nullptr, a.rows, a.K, a.K}, w{a.dx ? a.weight : nullptr, a.N, a.K, a.K};
+  if (int e = operands_of(x, w, space, st, run)) return e;
   if (a.dx) {
-    Operand w;
-    if (int e = operand_of(a.weight, a.N, a.K, space, st, run, w)) return e;
     const bool swapped = a.rows <= SWAP;
     Product p{};
     p.out = a.dx;
@@ -736,15 +789,13 @@ int backward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool r
       if (int e = swapped ? launch_product<T, true, false>(w, dz, a.N, p, true, parts, st) : launch_product<T, false, true>(dz, w, a.N, p, false, parts, st)) return e;
   }
   if (a.dweight) {
-    Operand in;
-    if (int e = operand_of(a.x, a.rows, a.K, space, st, run, in)) return e;
     Product p{};
     p.out = a.dweight;
     p.rows = a.N;
     p.cols = a.K;
     float* parts = static_cast<float*>(space.take(plan_of(p.rows, p.cols, a.rows, false).parts * 4));
     if (run)
-      if (int e = launch_product<T, true, true>(dz, in, a.rows, p, false, parts, st)) return e;
+      if (int e = launch_product<T, true, true>(dz, x, a.rows, p, false, parts, st)) return e;
   }
   return 0;
 }
