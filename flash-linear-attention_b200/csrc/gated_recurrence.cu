@@ -9,15 +9,15 @@
 // sequence: step by step each takes its turn of W R tokens, and their joined pairs go to one another's shared memory.
 // The backward pass does not read h, which is rounded to its type, but forms it again from x in fp32; the forward pass leaves the state
 // ahead of every 64 tokens (a 32nd of x's bytes in bf16) so that this needs no pass of its own from the left.
-#include <cooperative_groups.h>
-
 #include "gdn_common.cuh"
 #include "rowio.cuh"
+#include "tc5.cuh"
+#include "tma.cuh"
 
 namespace gdn {
 namespace {
 
-namespace cg = cooperative_groups;
+__device__ int g_recurrence_timeout = 0;
 
 constexpr int MOST_RANKS = 16;
 
@@ -28,6 +28,7 @@ struct Piece {
   Raw u;
   __device__ __forceinline__ void zero() { u = Raw{}; }
   __device__ __forceinline__ void load(const T* p) { u = __ldcs(reinterpret_cast<const Raw*>(p)); }
+  __device__ __forceinline__ void take(const void* shared) { u = *static_cast<const Raw*>(shared); }
   __device__ __forceinline__ uint64_t pair() const {   // of one channel: the second half is zero
     if constexpr (C == 1) return pack2((float)*reinterpret_cast<const T*>(&u), 0.f);
     else if constexpr (sizeof(T) == 2) return widen2<T>(u);
@@ -103,31 +104,80 @@ struct Joined {
   uint64_t a, h;
 };
 
-// The two buffers of what the warps, and the CTAs of a cluster, leave for one another.  A buffer is written again two steps later, with
-// another barrier in between that everyone passes after reading it.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {   // the same place in another CTA of the cluster
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(tc5::smem_addr(p)), "r"(rank));
+  return a;
+}
+// 16 bytes into another CTA's shared memory, which count on its barrier
+__device__ __forceinline__ void send16(uint32_t to, uint32_t bar, uint64_t lo, uint64_t hi) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];\n" ::"r"(to), "l"(lo), "l"(hi), "r"(bar) : "memory");
+}
+
+// A wait that has run out is told at the end and not repeated: what follows is invalid, but every thread still comes to the end.
+struct Patience {
+  bool ok = true;
+  __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
+    if (ok) ok = tc5::mbar_wait_warp(bar, parity);
+  }
+};
+
+// The two buffers of what the warps, and the CTAs of a cluster, leave for one another.  A buffer is written again two steps later: by then
+// every warp has passed the barrier of the step between, and so has every CTA of the cluster, whose joined pair of that step has come in.
 template <int W, bool CLUSTER>
 struct Exchange {
   ulonglong2 warps[2][W][32];
   ulonglong2 ranks[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][32];
+  uint64_t came[2];   // the joined pairs of all CTAs
+
+  __device__ __forceinline__ void init() {
+    if constexpr (CLUSTER) {
+      if (threadIdx.x == 0) {
+        tc5::mbar_init(&came[0], 1);
+        tc5::mbar_init(&came[1], 1);
+        tc5::fence_mbar_init();
+      }
+      __syncthreads();
+      cluster_sync();
+    }
+  }
+  __device__ __forceinline__ void leave() {   // no CTA ends while another one may still send to it
+    if constexpr (CLUSTER) cluster_sync();
+  }
 };
 
-// What enters warp `warp` of this CTA, and (in `s`) what leaves the whole step: W warps of each of the cluster's CTAs, from the first
-// one to the last (REVERSE: from the last to the first).
-template <int W, bool CLUSTER, bool REVERSE>
-__device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int turn, int rank, int n_ranks, Joined own, uint64_t& s) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// What enters warp `warp` of this CTA at step `i`, and (in `s`) what leaves the whole step: W warps of each of the cluster's CTAs, from the
+// first one to the last (REVERSE: from the last to the first).  `meanwhile` runs once all warps have their tokens in registers.
+template <int W, bool CLUSTER, bool REVERSE, typename F>
+__device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int i, int warp, int rank, int n_ranks, Joined own, uint64_t& s, Patience& patience,
+                                         F meanwhile) {
+  const int lane = threadIdx.x & 31, turn = i & 1;
   if constexpr (W > 1) {
     x.warps[turn][warp][lane] = make_ulonglong2(own.a, own.h);
     __syncthreads();
   }
+  meanwhile();
   if constexpr (!CLUSTER) {
     uint64_t mine = s;
     if constexpr (W == 1) {
       s = fma2(own.a, s, own.h);
     } else {
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const int w = REVERSE ? W - 1 - i : i;
+      for (int q = 0; q < W; ++q) {
+        const int w = REVERSE ? W - 1 - q : q;
         const ulonglong2 p = x.warps[turn][w][lane];
         if (w == warp) mine = s;
         s = fma2(p.x, s, p.y);
@@ -137,21 +187,20 @@ __device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int turn, int 
   } else {
     Joined ahead = {pack2(1.f, 1.f), 0ull}, all = ahead;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const int w = REVERSE ? W - 1 - i : i;
+    for (int q = 0; q < W; ++q) {
+      const int w = REVERSE ? W - 1 - q : q;
       const ulonglong2 p = x.warps[turn][w][lane];
       if (w == warp) ahead = all;
       all.h = fma2(p.x, all.h, p.y);
       all.a = mul2(p.x, all.a);
     }
-    cg::cluster_group cluster = cg::this_cluster();
-    for (int i = warp; i < n_ranks; i += W)   // to CTA i
-      *cluster.map_shared_rank(&x.ranks[turn][rank][lane], i) = make_ulonglong2(all.a, all.h);
-    cluster.sync();
+    if (threadIdx.x == 0) tc5::mbar_expect_tx(&x.came[turn], n_ranks * 32 * 16);
+    for (int r = warp; r < n_ranks; r += W) send16(at_rank(&x.ranks[turn][rank][lane], r), at_rank(&x.came[turn], r), all.a, all.h);
+    patience.wait(&x.came[turn], (i >> 1) & 1);
     uint64_t entering = s;
 #pragma unroll 4
-    for (int i = 0; i < n_ranks; ++i) {
-      const int r = REVERSE ? n_ranks - 1 - i : i;
+    for (int q = 0; q < n_ranks; ++q) {
+      const int r = REVERSE ? n_ranks - 1 - q : q;
       const ulonglong2 p = x.ranks[turn][r][lane];
       if (r == rank) entering = s;
       s = fma2(p.x, s, p.y);
@@ -160,177 +209,294 @@ __device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int turn, int 
   }
 }
 
-struct Place {   // of a CTA
-  int seq, channel, rank, n_ranks;
+struct Place {   // of a CTA: its sequence, the lane's first channel and the tile's
+  int seq, channel, tile, rank, n_ranks;
 };
 template <int C, bool CLUSTER>
 __device__ __forceinline__ Place place_of(const b200gdn_gated_recurrence_args& a) {
   const int tiles = (a.D + 32 * C - 1) / (32 * C);
-  const int n = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
-  const int i = blockIdx.x / n, seq = i / tiles;
-  return Place{a.seq_order ? a.seq_order[seq] : seq, (i % tiles) * 32 * C + (int)(threadIdx.x & 31) * C, CLUSTER ? (int)(blockIdx.x % n) : 0, n};
+  const int n = CLUSTER ? (int)cluster_size() : 1;
+  const int i = blockIdx.x / n, seq = i / tiles, first = (i % tiles) * 32 * C;
+  return Place{a.seq_order ? a.seq_order[seq] : seq, first + (int)(threadIdx.x & 31) * C, first, CLUSTER ? (int)cluster_rank() : 0, n};
 }
 
+// The tensors that a step reads, in tiles of [W R tokens][32 C channels], STAGES steps deep, by TMA: `full` counts a stage's bytes.  Tokens
+// past the end of the tensor and channels past its last one arrive as zeros, tokens past the sequence's end are another sequence's.
+template <int N, int ROWS, int STAGES>
+struct Tiles {
+  unsigned char* base;
+  uint64_t* full;
+  int bytes[N];    // of a row
+  int offset[N + 1];   // within a stage
+
+  __device__ __forceinline__ void init(unsigned char* shared, uint64_t* bars, const int (&row_bytes)[N]) {
+    base = shared;
+    full = bars;
+    offset[0] = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      bytes[i] = row_bytes[i];
+      offset[i + 1] = offset[i] + row_bytes[i] * ROWS;
+    }
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < STAGES; ++s) tc5::mbar_init(&full[s], 1);
+      tc5::fence_mbar_init();
+    }
+    __syncthreads();
+  }
+  // one thread
+  __device__ __forceinline__ void load(int stage, const CUtensorMap* const (&maps)[N], int channel, int row) const {
+    tc5::mbar_expect_tx(&full[stage], offset[N]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) tma::load_2d(base + stage * offset[N] + offset[i], maps[i], channel, row, &full[stage]);
+  }
+  __device__ __forceinline__ const unsigned char* row(int stage, int i, int r) const { return base + stage * offset[N] + offset[i] + r * bytes[i]; }
+};
+constexpr int stages_of(int stage_bytes) { return stage_bytes * 4 <= 100 * 1024 ? 4 : stage_bytes * 3 <= 100 * 1024 ? 3 : 2; }   // two CTAs an SM
+
 // ---- forward -------------------------------------------------------------------------------------------------------------
-template <typename T, typename G, int C, int R, int W, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2) recurrence_fwd_kernel(const b200gdn_gated_recurrence_args a) {
+// TMA: the tokens come by way of shared memory, several steps ahead; else (odd widths and boundaries) straight to registers, one step ahead.
+template <typename T, typename G, int C, int R, int W, bool CLUSTER, bool TMA>
+__global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
+    recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, const b200gdn_gated_recurrence_args a) {
+  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * 32 * C * (int)(sizeof(T) + sizeof(G)));
   __shared__ Exchange<W, CLUSTER> exchange;
+  __shared__ uint64_t full[STAGES];
+  extern __shared__ __align__(128) unsigned char shared_tiles[];
   const Place at = place_of<C, CLUSTER>(a);
   const Span seq = span_of(a, at.seq);
-  const int warp = threadIdx.x >> 5, step = at.n_ranks * W * R;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, step = at.n_ranks * ROWS;
   const bool live = at.channel < a.D, two = C == 2;
+  const int n = (seq.len + step - 1) / step, in_step = warp * R;
+  int t0 = at.rank * ROWS + in_step;
   Piece<T, C> x[R];
   Piece<G, C> g[R];
-  int t0 = (at.rank * W + warp) * R;
+  Tiles<2, ROWS, STAGES> tiles;
+  const CUtensorMap* const maps[2] = {&map_x, &map_g};
+  Patience patience;
   auto fetch = [&](int t) {
     const T* px = static_cast<const T*>(a.x) + (seq.first + t) * a.stride_x + at.channel;
     const G* pg = static_cast<const G*>(a.g) + (seq.first + t) * a.stride_g + at.channel;
-    if (live && t + R <= seq.len) {
 #pragma unroll
-      for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g) {
+    for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g) {
+      x[r].zero();   // past the end: a decay of one, and nothing added
+      g[r].zero();
+      if (live && t + r < seq.len) {
         x[r].load(px);
         g[r].load(pg);
       }
-    } else {
-#pragma unroll
-      for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g) {
-        x[r].zero();   // past the end: a decay of one, and nothing added
-        g[r].zero();
-        if (live && t + r < seq.len) {
-          x[r].load(px);
-          g[r].load(pg);
-        }
-      }
     }
   };
+  exchange.init();
+  if constexpr (TMA) {
+    const int row_bytes[2] = {32 * C * (int)sizeof(T), 32 * C * (int)sizeof(G)};
+    tiles.init(shared_tiles, full, row_bytes);
+    if (threadIdx.x == 0)
+      for (int i = 0; i < STAGES && i < n; ++i) tiles.load(i, maps, at.tile, (int)seq.first + i * step + at.rank * ROWS);
+  } else {
+    fetch(t0);
+  }
   uint64_t s = load_state(a.h0, (int64_t)at.seq * a.D + at.channel, live, two);
-  fetch(t0);
-  const int n = (seq.len + step - 1) / step;
+  int stage = 0;
+  uint32_t phase = 0;
   for (int i = 0; i < n; ++i, t0 += step) {
     uint64_t decays[R];
     Piece<T, C> now[R];
     Joined own = {pack2(1.f, 1.f), 0ull};
-    if (t0 < seq.len) {
+    const int rows = seq.len - t0;
+    if constexpr (TMA) {
+      patience.wait(&full[stage], phase);
+      const unsigned char *px = tiles.row(stage, 0, in_step) + lane * C * sizeof(T), *pg = tiles.row(stage, 1, in_step) + lane * C * sizeof(G);
+      if (rows >= R) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        now[r] = x[r];
-        decays[r] = decay(g[r].gate());
+        for (int r = 0; r < R; ++r) {
+          now[r].take(px + r * 32 * C * sizeof(T));
+          g[r].take(pg + r * 32 * C * sizeof(G));
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          now[r].zero();
+          g[r].zero();
+          if (r < rows) {
+            now[r].take(px + r * 32 * C * sizeof(T));
+            g[r].take(pg + r * 32 * C * sizeof(G));
+          }
+        }
       }
-      if (i + 1 < n) fetch(t0 + step);
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) now[r] = x[r];
+    }
+    if (rows > 0) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        decays[r] = decay(g[r].gate());
         own.h = fma2(decays[r], own.h, now[r].pair());
         own.a = mul2(decays[r], own.a);
       }
     }
-    uint64_t h = join<W, CLUSTER, false>(exchange, i & 1, at.rank, at.n_ranks, own, s);
-    if (!live || t0 >= seq.len) continue;
+    if (!TMA && i + 1 < n) fetch(t0 + step);
+    uint64_t h = join<W, CLUSTER, false>(exchange, i, warp, at.rank, at.n_ranks, own, s, patience, [&] {
+      if (TMA && threadIdx.x == 0 && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + (i + STAGES) * step + at.rank * ROWS);
+    });
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    if (!live || rows <= 0) continue;
     if (a.states && (t0 & (BT - 1)) == 0) store_state(a.states, (int64_t)(seq.chunk + t0 / BT) * a.D + at.channel, h, two);
     T* ph = static_cast<T*>(a.h) + (seq.first + t0) * a.D + at.channel;
-    const int rows = seq.len - t0;
+    if (rows >= R) {
 #pragma unroll
-    for (int r = 0; r < R; ++r, ph += a.D) {
-      h = fma2(decays[r], h, now[r].pair());
-      if (r < rows) Piece<T, C>::store(ph, h);
+      for (int r = 0; r < R; ++r) {
+        h = fma2(decays[r], h, now[r].pair());
+        Piece<T, C>::store(ph + (int64_t)r * a.D, h);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        h = fma2(decays[r], h, now[r].pair());
+        if (r < rows) Piece<T, C>::store(ph + (int64_t)r * a.D, h);
+      }
     }
   }
   if (a.ht && live && at.rank == 0 && warp == 0) store_state(a.ht, (int64_t)at.seq * a.D + at.channel, s, two);
+  if (!patience.ok && lane == 0) atomicExch(&g_recurrence_timeout, 1);
+  exchange.leave();
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
 // A CTA's step is 64 tokens, of which the state ahead is known (or, W = 1, the whole of a sequence of up to R).
-template <typename T, typename G, int C, int R, int W, bool CLUSTER>
-__global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2) recurrence_bwd_kernel(const b200gdn_gated_recurrence_args a) {
+template <typename T, typename G, int C, int R, int W, bool CLUSTER, bool TMA>
+__global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
+    recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_dh,
+                          const b200gdn_gated_recurrence_args a) {
   static_assert(W == 1 || W * R == BT, "a CTA's step is a chunk");
+  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * 32 * C * (int)(2 * sizeof(T) + sizeof(G)));
   __shared__ Exchange<W, CLUSTER> exchange;
   __shared__ ulonglong2 left[W > 1 ? 2 : 1][W][32];   // (product of decays, tokens' own state) of the warps, from the left
+  __shared__ uint64_t full[STAGES];
+  extern __shared__ __align__(128) unsigned char shared_tiles[];
   const Place at = place_of<C, CLUSTER>(a);
   const Span seq = span_of(a, at.seq);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = at.n_ranks * W * R;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, step = at.n_ranks * ROWS;
   const bool live = at.channel < a.D, two = C == 2;
+  const int n = (seq.len + step - 1) / step, in_step = warp * R;
+  const int last = (n - 1) * step + at.rank * ROWS;   // where this CTA's last (first to be taken) tokens begin
+  int t0 = last + in_step;
   Piece<T, C> x[R], dh[R];
   Piece<G, C> g[R];
+  Tiles<3, ROWS, STAGES> tiles;
+  const CUtensorMap* const maps[3] = {&map_x, &map_g, &map_dh};
+  Patience patience;
   uint64_t start = 0ull;
-  const int n = (seq.len + step - 1) / step;
-  int t0 = ((n - 1) * at.n_ranks + at.rank) * W * R + warp * R;
+  auto fetch_start = [&](int t) { start = load_state(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, live && t < seq.len, two); };
   auto fetch = [&](int t) {
     const T* px = static_cast<const T*>(a.x) + (seq.first + t) * a.stride_x + at.channel;
     const G* pg = static_cast<const G*>(a.g) + (seq.first + t) * a.stride_g + at.channel;
     const T* pd = static_cast<const T*>(a.dh) + (seq.first + t) * a.D + at.channel;
-    if (live && t + R <= seq.len && a.dh) {
 #pragma unroll
-      for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g, pd += a.D) {
+    for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g, pd += a.D) {
+      x[r].zero();
+      g[r].zero();
+      dh[r].zero();
+      if (live && t + r < seq.len) {
         x[r].load(px);
         g[r].load(pg);
-        dh[r].load(pd);
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < R; ++r, px += a.stride_x, pg += a.stride_g, pd += a.D) {
-        x[r].zero();
-        g[r].zero();
-        dh[r].zero();
-        if (live && t + r < seq.len) {
-          x[r].load(px);
-          g[r].load(pg);
-          if (a.dh) dh[r].load(pd);
-        }
+        if (a.dh) dh[r].load(pd);
       }
     }
-    start = load_state(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, live && t < seq.len, two);
   };
+  exchange.init();
+  if constexpr (TMA) {
+    const int row_bytes[3] = {32 * C * (int)sizeof(T), 32 * C * (int)sizeof(G), 32 * C * (int)sizeof(T)};
+    tiles.init(shared_tiles, full, row_bytes);
+    if (threadIdx.x == 0)
+      for (int i = 0; i < STAGES && i < n; ++i) tiles.load(i, maps, at.tile, (int)seq.first + last - i * step);
+  } else if (n > 0) {
+    fetch(t0);
+  }
+  if (n > 0) fetch_start(t0);
   uint64_t s = load_state(a.dht, (int64_t)at.seq * a.D + at.channel, live, two);
-  if (n > 0) fetch(t0);
+  int stage = 0;
+  uint32_t phase = 0;
   for (int i = 0; i < n; ++i, t0 -= step) {
     uint64_t decays[R], kept[R];
     Piece<T, C> up[R];
     uint64_t h = start, own_left = 0ull;
     Joined own = {pack2(1.f, 1.f), 0ull};
+    const int rows = seq.len - t0;
+    if constexpr (TMA) {
+      patience.wait(&full[stage], phase);
+      const unsigned char *px = tiles.row(stage, 0, in_step) + lane * C * sizeof(T), *pg = tiles.row(stage, 1, in_step) + lane * C * sizeof(G),
+                          *pd = tiles.row(stage, 2, in_step) + lane * C * sizeof(T);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      decays[r] = decay(g[r].gate());
-      up[r] = dh[r];
-      kept[r] = x[r].pair();
+      for (int r = 0; r < R; ++r) {
+        x[r].zero();
+        g[r].zero();
+        up[r].zero();
+        if (r < rows) {
+          x[r].take(px + r * 32 * C * sizeof(T));
+          g[r].take(pg + r * 32 * C * sizeof(G));
+          up[r].take(pd + r * 32 * C * sizeof(T));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) up[r] = dh[r];
     }
-    if (i + 1 < n) fetch(t0 - step);
+    if (rows > 0) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      own_left = fma2(decays[r], own_left, kept[r]);
-      own.a = mul2(decays[r], own.a);
-      const int q = R - 1 - r;
-      own.h = mul2(decays[q], add2(up[q].pair(), own.h));
+      for (int r = 0; r < R; ++r) {
+        decays[r] = decay(g[r].gate());
+        kept[r] = x[r].pair();
+        own_left = fma2(decays[r], own_left, kept[r]);
+        own.a = mul2(decays[r], own.a);
+      }
+#pragma unroll
+      for (int q = R - 1; q >= 0; --q) own.h = mul2(decays[q], add2(up[q].pair(), own.h));
+    }
+    if (i + 1 < n) {
+      if (!TMA) fetch(t0 - step);
+      fetch_start(t0 - step);
     }
     if constexpr (W > 1) left[i & 1][warp][lane] = make_ulonglong2(own.a, own_left);
-    uint64_t u = join<W, CLUSTER, true>(exchange, i & 1, at.rank, at.n_ranks, own, s);
+    uint64_t u = join<W, CLUSTER, true>(exchange, i, warp, at.rank, at.n_ranks, own, s, patience, [&] {
+      if (TMA && threadIdx.x == 0 && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + last - (i + STAGES) * step);
+    });
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1u;
+    }
+    if (!live || rows <= 0) continue;
     if constexpr (W > 1) {
-#pragma unroll
-      for (int w = 0; w < W - 1; ++w) {
+      for (int w = 0; w < warp; ++w) {
         const ulonglong2 p = left[i & 1][w][lane];
-        if (w < warp) h = fma2(p.x, h, p.y);
+        h = fma2(p.x, h, p.y);
       }
     }
-    if (!live || t0 >= seq.len) continue;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint64_t from_before = mul2(decays[r], h);
       h = fma2(decays[r], h, kept[r]);
       kept[r] = from_before;
     }
-    T* px = static_cast<T*>(a.dx) + (seq.first + t0) * a.D + at.channel;
-    G* pg = static_cast<G*>(a.dg) + (seq.first + t0) * a.D + at.channel;
-    const int rows = seq.len - t0;
+    T* const to_dx = static_cast<T*>(a.dx) + (seq.first + t0) * a.D + at.channel;
+    G* const to_dg = static_cast<G*>(a.dg) + (seq.first + t0) * a.D + at.channel;
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const int r = R - 1 - q;
+    for (int r = R - 1; r >= 0; --r) {
       const uint64_t d = add2(up[r].pair(), u);
       u = mul2(decays[r], d);
       if (r < rows) {
-        Piece<T, C>::store(px + (int64_t)r * a.D, d);
-        if (a.dg) Piece<G, C>::store(pg + (int64_t)r * a.D, mul2(d, kept[r]));
+        Piece<T, C>::store(to_dx + (int64_t)r * a.D, d);
+        if (a.dg) Piece<G, C>::store(to_dg + (int64_t)r * a.D, mul2(d, kept[r]));
       }
     }
   }
   if (a.dh0 && live && at.rank == 0 && warp == 0) store_state(a.dh0, (int64_t)at.seq * a.D + at.channel, s, two);
+  if (!patience.ok && lane == 0) atomicExch(&g_recurrence_timeout, 1);
+  exchange.leave();
 }
 
 // ---- one token a sequence ------------------------------------------------------------------------------------------------
@@ -365,15 +531,18 @@ int allow_large_clusters() {
   return 0;
 }
 
-template <auto KERN>
-int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, int C) {
+template <auto KERN, typename... M>
+int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, int C, size_t smem, const M&... maps) {
   const int64_t ctas = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)) * ranks;
   if (ctas > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 pieces of work", what);
   if (ranks > 8)
     if (int e = allow_large_clusters<KERN>()) return e;
+  if (smem > 0)
+    if (int e = ensure_smem(KERN, smem)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(W * 32);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -381,12 +550,29 @@ int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaSt
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  (void)cudaLaunchKernelEx(&cfg, KERN, a);   // (an error is check_launch's to name)
+  (void)cudaLaunchKernelEx(&cfg, KERN, maps..., a);   // (an error is check_launch's to name)
   return check_launch(what);
 }
 
+template <typename T, typename G, int C, int W, bool CLUSTER, bool TMA>
+int launch_pass(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, int ranks) {
+  constexpr int RB = BT / 8, RF = sizeof(T) + sizeof(G) == 4 ? 16 : 8;
+  CUtensorMap x{}, g{}, dh{};
+  const int rows = W * (bwd ? RB : RF), stage = rows * 32 * C * (int)(sizeof(T) * (bwd ? 2 : 1) + sizeof(G));
+  if (TMA) {
+    bind_context();
+    int e = tma::encode_plain_2d(&x, a.x, sizeof(T), a.rows, a.D, a.stride_x, 32 * C, rows);
+    if (e == 0) e = tma::encode_plain_2d(&g, a.g, sizeof(G), a.rows, a.D, a.stride_g, 32 * C, rows);
+    if (e == 0 && bwd) e = tma::encode_plain_2d(&dh, a.dh, sizeof(T), a.rows, a.D, a.D, 32 * C, rows);
+    if (e != 0) return set_error(B200GDN_ERR_CUDA, "gated_recurrence: tensor map (%d)", e);
+  }
+  const size_t smem = TMA ? (size_t)stage * stages_of(stage) : 0;
+  return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, W, CLUSTER, TMA>>("recurrence_bwd", a, st, W, ranks, C, smem, x, g, dh)
+             : launch_walk<recurrence_fwd_kernel<T, G, C, RF, W, CLUSTER, TMA>>("recurrence_fwd", a, st, W, ranks, C, smem, x, g);
+}
+
 template <typename T, typename G, int C>
-int launch_c(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd) {
+int launch_c(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, bool tiles) {
   if (!bwd && a.seq_len == 1) {
     const int n = a.n_seq < 65535 ? a.n_seq : 65535;
     recurrence_step_kernel<T, G, C><<<dim3((a.D + 128 * C - 1) / (128 * C), n), 128, 0, st>>>(a);
@@ -394,21 +580,17 @@ int launch_c(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd) 
   }
   constexpr int W = 8, RB = BT / W, RF = sizeof(T) + sizeof(G) == 4 ? 16 : 8;
   const int64_t tokens = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT;   // of a sequence, at most
-  if (a.seq_len > 0 && tokens <= (bwd ? RB : RF))
-    return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, 1, false>>("recurrence_bwd", a, st, 1, 1, C)
-               : launch_walk<recurrence_fwd_kernel<T, G, C, RF, 1, false>>("recurrence_fwd", a, st, 1, 1, C);
+  if (a.seq_len > 0 && tokens <= (bwd ? RB : RF)) return launch_pass<T, G, C, 1, false, false>(a, st, bwd, 1);
   // two CTAs an SM
   const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)), step = bwd ? BT : W * RF;
   int ranks = 1;
   while (ranks < MOST_RANKS && work * ranks * 2 <= 2 * sm_count() && ranks * step < tokens) ranks *= 2;
-  if (ranks > 1)
-    return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, W, true>>("recurrence_bwd", a, st, W, ranks, C)
-               : launch_walk<recurrence_fwd_kernel<T, G, C, RF, W, true>>("recurrence_fwd", a, st, W, ranks, C);
-  return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, W, false>>("recurrence_bwd", a, st, W, 1, C)
-             : launch_walk<recurrence_fwd_kernel<T, G, C, RF, W, false>>("recurrence_fwd", a, st, W, 1, C);
+  if constexpr (C == 2)
+    if (tiles) return ranks > 1 ? launch_pass<T, G, C, W, true, true>(a, st, bwd, ranks) : launch_pass<T, G, C, W, false, true>(a, st, bwd, 1);
+  return ranks > 1 ? launch_pass<T, G, C, W, true, false>(a, st, bwd, ranks) : launch_pass<T, G, C, W, false, false>(a, st, bwd, 1);
 }
 
-// two channels a thread where every row of every tensor allows it
+// two channels a thread where every row of every tensor allows it; by TMA where rows are a multiple of 16 bytes on such boundaries
 template <typename T, typename G>
 int launch_tg(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd) {
   auto bits = [](std::initializer_list<const void*> all) {
@@ -418,7 +600,8 @@ int launch_tg(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd)
   };
   const bool pairs = ((a.D | a.stride_x | a.stride_g) & 1) == 0 && bits({a.x, a.h, a.dh, a.dx}) % (2 * sizeof(T)) == 0 &&
                      bits({a.g, a.dg}) % (2 * sizeof(G)) == 0;
-  return pairs ? launch_c<T, G, 2>(a, st, bwd) : launch_c<T, G, 1>(a, st, bwd);
+  const bool tiles = (a.D * sizeof(T) | a.stride_x * sizeof(T) | a.stride_g * sizeof(G) | bits({a.x, a.g, a.dh})) % 16 == 0 && (!bwd || a.dh != nullptr);
+  return pairs ? launch_c<T, G, 2>(a, st, bwd, tiles) : launch_c<T, G, 1>(a, st, bwd, false);
 }
 
 }  // namespace
@@ -428,6 +611,13 @@ int launch_gated_recurrence(const b200gdn_gated_recurrence_args& a, cudaStream_t
   if (a.dtype == 2) return launch_tg<float, float>(a, st, bwd);
   if (a.dtype == 0) return wide ? launch_tg<__nv_bfloat16, float>(a, st, bwd) : launch_tg<__nv_bfloat16, __nv_bfloat16>(a, st, bwd);
   return wide ? launch_tg<__half, float>(a, st, bwd) : launch_tg<__half, __half>(a, st, bwd);
+}
+
+int recurrence_timeout_flag() {
+  int v = 0, zero = 0;
+  cudaMemcpyFromSymbol(&v, g_recurrence_timeout, sizeof(int));
+  if (v) cudaMemcpyToSymbol(g_recurrence_timeout, &zero, sizeof(int));
+  return v;
 }
 
 }  // namespace gdn

@@ -164,6 +164,7 @@ int launch_logprob(const b200gdn_logprob_args& a, cudaStream_t st, bool bwd);
 int64_t distill_workspace(int64_t rows, int V, int dtype, int K);
 int launch_distill(const b200gdn_distill_args& a, cudaStream_t st, bool bwd);
 int linear_timeout_flag();
+int recurrence_timeout_flag();
 int decode_timeout_flag();
 int intra_fwd_timeout_flag();
 int scan_fwd_timeout_flag();
@@ -227,6 +228,13 @@ void launch_overlapped(bool overlap, void (*kern)(P...), dim3 grid, int threads,
   cfg.attrs = &attr;
   cfg.numAttrs = overlap ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
+// A thread that has made no CUDA call yet, as autograd's are, has no context, which the driver's own calls (tensor maps) need.
+inline void bind_context() {
+  static thread_local bool bound = false;
+  int dev = 0;
+  if (!bound && cudaGetDevice(&dev) == cudaSuccess) bound = cudaSetDevice(dev) == cudaSuccess;
 }
 
 // Streaming multiprocessors of the current device (148 where there is none to ask), looked up once per device.

@@ -635,6 +635,7 @@ struct Operand {
 template <typename T, int BN, bool A_MN, bool B_MN, bool SWAPPED>
 int launch_tiles(const Operand& a, const Operand& b, Product p, cudaStream_t st) {
   CUtensorMap ma, mb;
+  bind_context();
   if (int e = tma::encode_bf16_2d(&ma, a.base, a.rows, a.cols, a.pitch, A_MN ? 64 : 128)) return set_error(B200GDN_ERR_CUDA, "linear: tensor map of A (%d)", e);
   if (int e = tma::encode_bf16_2d(&mb, b.base, b.rows, b.cols, b.pitch, B_MN ? 64 : BN / 2)) return set_error(B200GDN_ERR_CUDA, "linear: tensor map of B (%d)", e);
   p.tiles_i = (p.rows + 255) / 256;
