@@ -19,7 +19,7 @@ namespace {
 
 __device__ int g_recurrence_timeout = 0;
 
-constexpr int MOST_RANKS = 16;
+constexpr int MOST_RANKS = 16;   // CTAs of a cluster
 
 // C neighbouring channels of a token, as loaded
 template <typename T, int C>
@@ -122,9 +122,10 @@ __device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {   // the 
   asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(tc5::smem_addr(p)), "r"(rank));
   return a;
 }
-// 16 bytes into another CTA's shared memory, which count on its barrier
-__device__ __forceinline__ void send16(uint32_t to, uint32_t bar, uint64_t lo, uint64_t hi) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];\n" ::"r"(to), "l"(lo), "l"(hi), "r"(bar) : "memory");
+// from this CTA's shared memory into another's, counted on its barrier
+__device__ __forceinline__ void send(uint32_t to, uint32_t from, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(to), "r"(from), "r"(bytes), "r"(bar)
+               : "memory");
 }
 
 // A wait that has run out is told at the end and not repeated: what follows is invalid, but every thread still comes to the end.
@@ -135,13 +136,16 @@ struct Patience {
   }
 };
 
-// The two buffers of what the warps, and the CTAs of a cluster, leave for one another.  A buffer is written again two steps later: by then
-// every warp has passed the barrier of the step between, and so has every CTA of the cluster, whose joined pair of that step has come in.
+// What the warps of a CTA, and the CTAs of a cluster, leave for one another.  A buffer is written again two steps later: by then every warp has
+// passed the barrier of the step between, and so has every CTA of the cluster, whose joined pair of that step has come in.
+// Between CTAs 512 bytes go as one copy: stores that count on the other's barrier lane by lane cost 0.28 us a CTA of the cluster, a
+// barrier of the whole cluster more, since it waits for every store on its way to memory.
 template <int W, bool CLUSTER>
 struct Exchange {
   ulonglong2 warps[2][W][32];
-  ulonglong2 ranks[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][32];
-  uint64_t came[2];   // the joined pairs of all CTAs
+  uint64_t carry[2][32];   // what leaves the step, without a cluster
+  ulonglong2 ranks[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][32], mine[CLUSTER ? 2 : 1][32];
+  uint64_t came[2];        // the joined pairs of all CTAs
 
   __device__ __forceinline__ void init() {
     if constexpr (CLUSTER) {
@@ -159,55 +163,76 @@ struct Exchange {
   }
 };
 
-// What enters warp `warp` of this CTA at step `i`, and (in `s`) what leaves the whole step: W warps of each of the cluster's CTAs, from the
-// first one to the last (REVERSE: from the last to the first).  `meanwhile` runs once all warps have their tokens in registers.
+// What enters warp `warp` of this CTA at step `i`: W warps of each of the cluster's CTAs, from the first one to the last (REVERSE: from the last to
+// the first).  s: what enters the step, then what leaves it (of a CTA without a cluster only the last warp knows, and tells the others at
+// the next step).  `meanwhile` runs once all warps have their tokens in registers.
 template <int W, bool CLUSTER, bool REVERSE, typename F>
 __device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int i, int warp, int rank, int n_ranks, Joined own, uint64_t& s, Patience& patience,
                                          F meanwhile) {
-  const int lane = threadIdx.x & 31, turn = i & 1;
-  if constexpr (W > 1) {
-    x.warps[turn][warp][lane] = make_ulonglong2(own.a, own.h);
-    __syncthreads();
-  }
-  meanwhile();
-  if constexpr (!CLUSTER) {
-    uint64_t mine = s;
-    if constexpr (W == 1) {
-      s = fma2(own.a, s, own.h);
-    } else {
-#pragma unroll
-      for (int q = 0; q < W; ++q) {
-        const int w = REVERSE ? W - 1 - q : q;
-        const ulonglong2 p = x.warps[turn][w][lane];
-        if (w == warp) mine = s;
-        s = fma2(p.x, s, p.y);
-      }
-    }
+  const int lane = threadIdx.x & 31, turn = i & 1, ahead_of = REVERSE ? W - 1 - warp : warp;   // warps ahead of this one
+  if constexpr (W == 1) {
+    const uint64_t mine = s;
+    s = fma2(own.a, s, own.h);
     return mine;
   } else {
-    Joined ahead = {pack2(1.f, 1.f), 0ull}, all = ahead;
+    x.warps[turn][warp][lane] = make_ulonglong2(own.a, own.h);
+    __syncthreads();
+    meanwhile();
+    if constexpr (!CLUSTER) {
+      uint64_t mine = i == 0 ? s : x.carry[turn][lane];
 #pragma unroll
-    for (int q = 0; q < W; ++q) {
-      const int w = REVERSE ? W - 1 - q : q;
-      const ulonglong2 p = x.warps[turn][w][lane];
-      if (w == warp) ahead = all;
-      all.h = fma2(p.x, all.h, p.y);
-      all.a = mul2(p.x, all.a);
-    }
-    if (threadIdx.x == 0) tc5::mbar_expect_tx(&x.came[turn], n_ranks * 32 * 16);
-    for (int r = warp; r < n_ranks; r += W) send16(at_rank(&x.ranks[turn][rank][lane], r), at_rank(&x.came[turn], r), all.a, all.h);
-    patience.wait(&x.came[turn], (i >> 1) & 1);
-    uint64_t entering = s;
+      for (int q = 0; q < W - 1; ++q)
+        if (q < ahead_of) {
+          const ulonglong2 p = x.warps[turn][REVERSE ? W - 1 - q : q][lane];
+          mine = fma2(p.x, mine, p.y);
+        }
+      s = fma2(own.a, mine, own.h);
+      if (ahead_of == W - 1) x.carry[turn ^ 1][lane] = s;
+      return mine;
+    } else {
+      // warp 0 joins all of them, to tell the other CTAs
+      const int n = warp == 0 ? W : ahead_of;
+      Joined ahead = {pack2(1.f, 1.f), 0ull};
+#pragma unroll
+      for (int q = 0; q < W; ++q)
+        if (q < n) {
+          const ulonglong2 p = x.warps[turn][REVERSE ? W - 1 - q : q][lane];
+          ahead.h = fma2(p.x, ahead.h, p.y);
+          ahead.a = mul2(p.x, ahead.a);
+        }
+      if (warp == 0) {
+        x.mine[turn][lane] = make_ulonglong2(ahead.a, ahead.h);
+        tc5::fence_async_smem();
+        if (lane == 0) tc5::mbar_expect_tx(&x.came[turn], n_ranks * 512);
+        __syncwarp();
+        if (lane < n_ranks) send(at_rank(&x.ranks[turn][rank][0], lane), tc5::smem_addr(&x.mine[turn][0]), 512, at_rank(&x.came[turn], lane));
+        // ahead of warp 0: nothing, or (REVERSE) the others
+        ahead = {pack2(1.f, 1.f), 0ull};
+        if constexpr (REVERSE) {
+#pragma unroll
+          for (int q = 0; q < W - 1; ++q) {
+            const ulonglong2 p = x.warps[turn][W - 1 - q][lane];
+            ahead.h = fma2(p.x, ahead.h, p.y);
+            ahead.a = mul2(p.x, ahead.a);
+          }
+        }
+      }
+      patience.wait(&x.came[turn], (i >> 1) & 1);
+      uint64_t entering = s;
 #pragma unroll 4
-    for (int q = 0; q < n_ranks; ++q) {
-      const int r = REVERSE ? n_ranks - 1 - q : q;
-      const ulonglong2 p = x.ranks[turn][r][lane];
-      if (r == rank) entering = s;
-      s = fma2(p.x, s, p.y);
+      for (int q = 0; q < n_ranks; ++q) {
+        const int r = REVERSE ? n_ranks - 1 - q : q;
+        const ulonglong2 p = x.ranks[turn][r][lane];
+        if (r == rank) entering = s;
+        s = fma2(p.x, s, p.y);
+      }
+      return fma2(ahead.a, entering, ahead.h);
     }
-    return fma2(ahead.a, entering, ahead.h);
   }
 }
+// the warp that knows what leaves the last step
+template <int W, bool CLUSTER, bool REVERSE>
+__device__ __forceinline__ bool knows_the_end(int n, int warp, int rank) { return rank == 0 && warp == (CLUSTER || REVERSE || n == 0 ? 0 : W - 1); }
 
 struct Place {   // of a CTA: its sequence, the lane's first channel and the tile's
   int seq, channel, tile, rank, n_ranks;
@@ -252,14 +277,17 @@ struct Tiles {
   }
   __device__ __forceinline__ const unsigned char* row(int stage, int i, int r) const { return base + stage * offset[N] + offset[i] + r * bytes[i]; }
 };
-constexpr int stages_of(int stage_bytes) { return stage_bytes * 4 <= 100 * 1024 ? 4 : stage_bytes * 3 <= 100 * 1024 ? 3 : 2; }   // two CTAs an SM
+constexpr int stages_of(int stage_bytes, bool cluster) {   // two CTAs an SM
+  const int room = (cluster ? 76 : 95) * 1024 / stage_bytes;
+  return room > 4 ? 4 : room < 1 ? 1 : room;
+}
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
 // TMA: the tokens come by way of shared memory, several steps ahead; else (odd widths and boundaries) straight to registers, one step ahead.
 template <typename T, typename G, int C, int R, int W, bool CLUSTER, bool TMA>
 __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, const b200gdn_gated_recurrence_args a) {
-  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * 32 * C * (int)(sizeof(T) + sizeof(G)));
+  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * 32 * C * (int)(sizeof(T) + sizeof(G)), CLUSTER);
   __shared__ Exchange<W, CLUSTER> exchange;
   __shared__ uint64_t full[STAGES];
   extern __shared__ __align__(128) unsigned char shared_tiles[];
@@ -299,11 +327,12 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
   uint64_t s = load_state(a.h0, (int64_t)at.seq * a.D + at.channel, live, two);
   int stage = 0;
   uint32_t phase = 0;
-  for (int i = 0; i < n; ++i, t0 += step) {
-    uint64_t decays[R];
-    Piece<T, C> now[R];
+  uint64_t decays[R];
+  Piece<T, C> now[R];
+  // the warp's tokens of step i, from t on: their decays, and the pair that they come to
+  auto begin = [&](int i, int t) {
+    const int rows = seq.len - t;
     Joined own = {pack2(1.f, 1.f), 0ull};
-    const int rows = seq.len - t0;
     if constexpr (TMA) {
       patience.wait(&full[stage], phase);
       const unsigned char *px = tiles.row(stage, 0, in_step) + lane * C * sizeof(T), *pg = tiles.row(stage, 1, in_step) + lane * C * sizeof(G);
@@ -336,44 +365,56 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
         own.a = mul2(decays[r], own.a);
       }
     }
-    if (!TMA && i + 1 < n) fetch(t0 + step);
-    uint64_t h = join<W, CLUSTER, false>(exchange, i, warp, at.rank, at.n_ranks, own, s, patience, [&] {
-      if (TMA && threadIdx.x == 0 && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + (i + STAGES) * step + at.rank * ROWS);
-    });
+    if (!TMA && i + 1 < n) fetch(t + step);
+    return own;
+  };
+  // once all warps have step i in registers
+  auto next = [&](int i) {
+    if (TMA && threadIdx.x == 0 && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + (i + STAGES) * step + at.rank * ROWS);
     if (++stage == STAGES) {
       stage = 0;
       phase ^= 1u;
     }
-    if (!live || rows <= 0) continue;
-    if (a.states && (t0 & (BT - 1)) == 0) store_state(a.states, (int64_t)(seq.chunk + t0 / BT) * a.D + at.channel, h, two);
-    T* ph = static_cast<T*>(a.h) + (seq.first + t0) * a.D + at.channel;
+  };
+  // the tokens from t on, entered with h
+  auto finish = [&](int t, uint64_t h) {
+    const int rows = seq.len - t;
+    if (!live || rows <= 0) return;
+    if (a.states && (t & (BT - 1)) == 0) store_state(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, h, two);
+    T* const to = static_cast<T*>(a.h) + (seq.first + t) * a.D + at.channel;
     if (rows >= R) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         h = fma2(decays[r], h, now[r].pair());
-        Piece<T, C>::store(ph + (int64_t)r * a.D, h);
+        Piece<T, C>::store(to + (int64_t)r * a.D, h);
       }
     } else {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         h = fma2(decays[r], h, now[r].pair());
-        if (r < rows) Piece<T, C>::store(ph + (int64_t)r * a.D, h);
+        if (r < rows) Piece<T, C>::store(to + (int64_t)r * a.D, h);
       }
     }
+  };
+  for (int i = 0; i < n; ++i, t0 += step) {
+    const Joined own = begin(i, t0);
+    const uint64_t h = join<W, CLUSTER, false>(exchange, i, warp, at.rank, at.n_ranks, own, s, patience, [&] { next(i); });
+    finish(t0, h);
   }
-  if (a.ht && live && at.rank == 0 && warp == 0) store_state(a.ht, (int64_t)at.seq * a.D + at.channel, s, two);
+  if (a.ht && live && knows_the_end<W, CLUSTER, false>(n, warp, at.rank)) store_state(a.ht, (int64_t)at.seq * a.D + at.channel, s, two);
   if (!patience.ok && lane == 0) atomicExch(&g_recurrence_timeout, 1);
   exchange.leave();
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
-// A CTA's step is 64 tokens, of which the state ahead is known (or, W = 1, the whole of a sequence of up to R).
+// A CTA's step is one or more chunks, ahead of which the state is known (or, W = 1, the whole of a sequence of up to R).
 template <typename T, typename G, int C, int R, int W, bool CLUSTER, bool TMA>
 __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_dh,
                           const b200gdn_gated_recurrence_args a) {
-  static_assert(W == 1 || W * R == BT, "a CTA's step is a chunk");
-  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * 32 * C * (int)(2 * sizeof(T) + sizeof(G)));
+  static_assert(W == 1 || (W * R) % BT == 0, "a CTA's step begins where a chunk does");
+  constexpr int IN_CHUNK = BT / R;   // warps
+  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * 32 * C * (int)(2 * sizeof(T) + sizeof(G)), CLUSTER);
   __shared__ Exchange<W, CLUSTER> exchange;
   __shared__ ulonglong2 left[W > 1 ? 2 : 1][W][32];   // (product of decays, tokens' own state) of the warps, from the left
   __shared__ uint64_t full[STAGES];
@@ -431,15 +472,24 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
       patience.wait(&full[stage], phase);
       const unsigned char *px = tiles.row(stage, 0, in_step) + lane * C * sizeof(T), *pg = tiles.row(stage, 1, in_step) + lane * C * sizeof(G),
                           *pd = tiles.row(stage, 2, in_step) + lane * C * sizeof(T);
+      if (rows >= R) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        x[r].zero();
-        g[r].zero();
-        up[r].zero();
-        if (r < rows) {
+        for (int r = 0; r < R; ++r) {
           x[r].take(px + r * 32 * C * sizeof(T));
           g[r].take(pg + r * 32 * C * sizeof(G));
           up[r].take(pd + r * 32 * C * sizeof(T));
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          x[r].zero();
+          g[r].zero();
+          up[r].zero();
+          if (r < rows) {
+            x[r].take(px + r * 32 * C * sizeof(T));
+            g[r].take(pg + r * 32 * C * sizeof(G));
+            up[r].take(pd + r * 32 * C * sizeof(T));
+          }
         }
       }
     } else {
@@ -462,19 +512,23 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
       fetch_start(t0 - step);
     }
     if constexpr (W > 1) left[i & 1][warp][lane] = make_ulonglong2(own.a, own_left);
-    uint64_t u = join<W, CLUSTER, true>(exchange, i, warp, at.rank, at.n_ranks, own, s, patience, [&] {
+    auto next = [&] {
       if (TMA && threadIdx.x == 0 && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + last - (i + STAGES) * step);
-    });
+    };
+    uint64_t u = join<W, CLUSTER, true>(exchange, i, warp, at.rank, at.n_ranks, own, s, patience, next);
     if (++stage == STAGES) {
       stage = 0;
       phase ^= 1u;
     }
     if (!live || rows <= 0) continue;
     if constexpr (W > 1) {
-      for (int w = 0; w < warp; ++w) {
-        const ulonglong2 p = left[i & 1][w][lane];
-        h = fma2(p.x, h, p.y);
-      }
+      const int before = warp % IN_CHUNK;
+#pragma unroll
+      for (int w = 0; w < IN_CHUNK - 1; ++w)
+        if (w < before) {
+          const ulonglong2 p = left[i & 1][warp - before + w][lane];
+          h = fma2(p.x, h, p.y);
+        }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -484,17 +538,21 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     }
     T* const to_dx = static_cast<T*>(a.dx) + (seq.first + t0) * a.D + at.channel;
     G* const to_dg = static_cast<G*>(a.dg) + (seq.first + t0) * a.D + at.channel;
+    auto finish = [&](auto full) {
 #pragma unroll
-    for (int r = R - 1; r >= 0; --r) {
-      const uint64_t d = add2(up[r].pair(), u);
-      u = mul2(decays[r], d);
-      if (r < rows) {
-        Piece<T, C>::store(to_dx + (int64_t)r * a.D, d);
-        if (a.dg) Piece<G, C>::store(to_dg + (int64_t)r * a.D, mul2(d, kept[r]));
+      for (int r = R - 1; r >= 0; --r) {
+        const uint64_t d = add2(up[r].pair(), u);
+        u = mul2(decays[r], d);
+        if (decltype(full)::value || r < rows) {
+          Piece<T, C>::store(to_dx + (int64_t)r * a.D, d);
+          if (a.dg) Piece<G, C>::store(to_dg + (int64_t)r * a.D, mul2(d, kept[r]));
+        }
       }
-    }
+    };
+    if (rows >= R) finish(std::true_type());
+    else finish(std::false_type());
   }
-  if (a.dh0 && live && at.rank == 0 && warp == 0) store_state(a.dh0, (int64_t)at.seq * a.D + at.channel, s, two);
+  if (a.dh0 && live && knows_the_end<W, CLUSTER, true>(n, warp, at.rank)) store_state(a.dh0, (int64_t)at.seq * a.D + at.channel, s, two);
   if (!patience.ok && lane == 0) atomicExch(&g_recurrence_timeout, 1);
   exchange.leave();
 }
@@ -531,32 +589,67 @@ int allow_large_clusters() {
   return 0;
 }
 
+// How many clusters of `ranks` CTAs are resident at once: fewer than the SMs suggest, since a cluster lies within one of the chip's parts.
+template <auto KERN>
+int resident_clusters(cudaLaunchConfig_t cfg, int ranks) {
+  static std::atomic<int> known[64][MOST_RANKS + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = known[dev][ranks].load(std::memory_order_relaxed);
+  if (n > 0) return n - 1;
+  cfg.gridDim = dim3(ranks);
+  if (cudaOccupancyMaxActiveClusters(&n, KERN, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    n = 0;
+  }
+  known[dev][ranks].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
+// `ranks`: the most CTAs a cluster may have.  As many are taken as let every sequence's cluster work at the same time (131072 tokens of 1024
+// channels, bf16 with fp32 gates: 358 us with 12, 484 with 16, of which 14 clusters are resident where 16 are wanted), in sizes that pack well
+// (8191 x 1003 fp32 backward: 62 us with 8, 89 with 9).
 template <auto KERN, typename... M>
 int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, int C, size_t smem, const M&... maps) {
-  const int64_t ctas = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)) * ranks;
-  if (ctas > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 pieces of work", what);
-  if (ranks > 8)
-    if (int e = allow_large_clusters<KERN>()) return e;
+  const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C));
   if (smem > 0)
     if (int e = ensure_smem(KERN, smem)) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ranks;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  if (ranks > 1) {
+    if (int e = allow_large_clusters<KERN>()) return e;
+    cfg.numAttrs = 1;
+    const int most = ranks;
+    ranks = 1;
+    for (int r : {16, 12, 8, 6, 4, 3, 2}) {
+      attr.val.clusterDim.x = r;
+      if (r > most || work * r > 2 * sm_count() || resident_clusters<KERN>(cfg, r) < work) continue;
+      ranks = r;
+      break;
+    }
+    attr.val.clusterDim.x = ranks;
+  }
+  if (work * ranks > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 pieces of work", what);
+  cfg.gridDim = dim3((unsigned)(work * ranks));
   (void)cudaLaunchKernelEx(&cfg, KERN, maps..., a);   // (an error is check_launch's to name)
   return check_launch(what);
 }
 
+// tokens of a warp at a time
+template <typename T, typename G>
+constexpr int rows_fwd(bool tma) { return sizeof(T) + sizeof(G) <= (tma ? 6 : 4) ? 16 : 8; }
+template <typename T, typename G>
+constexpr int rows_bwd(bool tma) { return tma && sizeof(T) + sizeof(G) == 4 ? 16 : 8; }
+
 template <typename T, typename G, int C, int W, bool CLUSTER, bool TMA>
 int launch_pass(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, int ranks) {
-  constexpr int RB = BT / 8, RF = sizeof(T) + sizeof(G) == 4 ? 16 : 8;
+  constexpr int RB = rows_bwd<T, G>(TMA), RF = rows_fwd<T, G>(TMA);
   CUtensorMap x{}, g{}, dh{};
   const int rows = W * (bwd ? RB : RF), stage = rows * 32 * C * (int)(sizeof(T) * (bwd ? 2 : 1) + sizeof(G));
   if (TMA) {
@@ -566,7 +659,7 @@ int launch_pass(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bw
     if (e == 0 && bwd) e = tma::encode_plain_2d(&dh, a.dh, sizeof(T), a.rows, a.D, a.D, 32 * C, rows);
     if (e != 0) return set_error(B200GDN_ERR_CUDA, "gated_recurrence: tensor map (%d)", e);
   }
-  const size_t smem = TMA ? (size_t)stage * stages_of(stage) : 0;
+  const size_t smem = TMA ? (size_t)stage * stages_of(stage, CLUSTER) : 0;
   return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, W, CLUSTER, TMA>>("recurrence_bwd", a, st, W, ranks, C, smem, x, g, dh)
              : launch_walk<recurrence_fwd_kernel<T, G, C, RF, W, CLUSTER, TMA>>("recurrence_fwd", a, st, W, ranks, C, smem, x, g);
 }
@@ -578,16 +671,13 @@ int launch_c(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, 
     recurrence_step_kernel<T, G, C><<<dim3((a.D + 128 * C - 1) / (128 * C), n), 128, 0, st>>>(a);
     return check_launch("recurrence_step");
   }
-  constexpr int W = 8, RB = BT / W, RF = sizeof(T) + sizeof(G) == 4 ? 16 : 8;
   const int64_t tokens = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT;   // of a sequence, at most
-  if (a.seq_len > 0 && tokens <= (bwd ? RB : RF)) return launch_pass<T, G, C, 1, false, false>(a, st, bwd, 1);
-  // two CTAs an SM
-  const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)), step = bwd ? BT : W * RF;
-  int ranks = 1;
-  while (ranks < MOST_RANKS && work * ranks * 2 <= 2 * sm_count() && ranks * step < tokens) ranks *= 2;
+  if (a.seq_len > 0 && tokens <= (bwd ? rows_bwd<T, G>(false) : rows_fwd<T, G>(false))) return launch_pass<T, G, C, 1, false, false>(a, st, bwd, 1);
+  const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)), most = (tokens + BT - 1) / BT;
+  const bool alone = work > sm_count() || most < 2;
   if constexpr (C == 2)
-    if (tiles) return ranks > 1 ? launch_pass<T, G, C, W, true, true>(a, st, bwd, ranks) : launch_pass<T, G, C, W, false, true>(a, st, bwd, 1);
-  return ranks > 1 ? launch_pass<T, G, C, W, true, false>(a, st, bwd, ranks) : launch_pass<T, G, C, W, false, false>(a, st, bwd, 1);
+    if (tiles) return alone ? launch_pass<T, G, C, 8, false, true>(a, st, bwd, 1) : launch_pass<T, G, C, 8, true, true>(a, st, bwd, (int)(most < MOST_RANKS ? most : MOST_RANKS));
+  return alone ? launch_pass<T, G, C, 8, false, false>(a, st, bwd, 1) : launch_pass<T, G, C, 8, true, false>(a, st, bwd, (int)(most < MOST_RANKS ? most : MOST_RANKS));
 }
 
 // two channels a thread where every row of every tensor allows it; by TMA where rows are a multiple of 16 bytes on such boundaries

@@ -106,10 +106,10 @@ def test_slices_are_read_where_they_lie(dtype, gtype):
         sg.copy_(g)
         leaves = [sx.detach().requires_grad_(True), sg.detach().requires_grad_(True)]
         h, ht = gated_recurrence(*leaves, initial_state=h0, output_final_state=True)
-        want, want_t = gated_recurrence(x, g, initial_state=h0, output_final_state=True)
-        close('h', h.detach(), want.double(), 0)
-        close('ht', ht.detach(), want_t.double(), 8 * O.U * want_t.abs().double())
+        # (not against a call on contiguous tensors, whose steps may be others: two roundings of what differs in fp32 may be a whole step apart)
         r = O.recurrence(x.view(-1, D), g.view(-1, D), h0, O.dense_bounds(B, T), dh.view(-1, D))
+        close('h', h.detach().reshape(-1, D), r['h'], r['h_off'])
+        close('ht', ht.detach(), r['ht'], r['ht_off'])
         for name, t in zip(('dx', 'dg'), torch.autograd.grad(h, leaves, dh)):
             close(name, t.reshape(-1, D), r[name], r[name + '_off'])
     # neither slices nor rows: what cannot be read in place is copied
