@@ -622,7 +622,7 @@ int b200gdn_device_status(void) {
       {"dv_local", gdn::dv_local_timeout_flag},   {"scan_bwd", gdn::scan_bwd_timeout_flag}, {"bwd_dqk", gdn::bwd_dqk_timeout_flag},
       {"bwd_wy", gdn::bwd_wy_timeout_flag},       {"bwd_local", gdn::bwd_local_timeout_flag},
             {"selftest", gdn::selftest_timeout_flag},
-      {"linear", gdn::linear_timeout_flag},     {"gated_recurrence", gdn::recurrence_timeout_flag},
+      {"linear", gdn::linear_timeout_flag},     {"gated_recurrence", gdn::recurrence_timeout_flag}, {"rms_norms", gdn::norms_timeout_flag},
       {"decode_stream", gdn::decode_timeout_flag}};
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return gdn::set_error(B200GDN_ERR_CUDA, "device_status: %s", cudaGetErrorString(e));

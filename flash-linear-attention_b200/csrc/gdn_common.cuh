@@ -165,6 +165,7 @@ int64_t distill_workspace(int64_t rows, int V, int dtype, int K);
 int launch_distill(const b200gdn_distill_args& a, cudaStream_t st, bool bwd);
 int linear_timeout_flag();
 int recurrence_timeout_flag();
+int norms_timeout_flag();
 int decode_timeout_flag();
 int intra_fwd_timeout_flag();
 int scan_fwd_timeout_flag();

@@ -5,21 +5,127 @@
 //     dw = sum of dout z r2;  t = sum of e act y r1:  dw1 = alpha scale t,  dscale = alpha w1 t
 // z is normalised as it is summed, in fp32; only what is handed on is rounded.  The backward pass forms z again from the inputs, which it
 // reads in any case but for the residual, so that z need not be kept.
-// HBM streaming, in the manner of layer_norm.cu: a row lies in the registers of TPR threads in NV pieces of N elements, CTAs walk the rows
-// with the next one on its way, a thread's columns stay its own and so the parameters' gradients are sums in registers, which a second
-// kernel joins in a fixed order.  The second norm needs what the first one gives: two barriers a row, forward as well as backward.
+// HBM streaming, in the manner of layer_norm.cu: the threads of a group share a row, E elements each, which are worked on as E / 2 fp32 pairs;
+// groups walk the rows, so that a thread's columns stay its own: parameters are read once, their gradients are sums in registers, which a
+// second kernel joins in a fixed order.  The second norm needs what the first one gives: two barriers a row, forward as well as backward.
+// Rows of a multiple of 16 bytes come by bulk copies into a ring of shared memory, two to four rows ahead; of other rows the next one is
+// on its way to registers.
 #include "gdn_common.cuh"
 #include "row_pieces.cuh"
+#include "tc5.cuh"
+#include "tma.cuh"
 
 namespace gdn {
 namespace {
 
+__device__ int g_norms_timeout = 0;
+
 constexpr uint32_t POST = B200GDN_NORMS_POST, SIGMOID = B200GDN_NORMS_SIGMOID, SILU = B200GDN_NORMS_SILU;
-constexpr int threads_of(int tpr) { return tpr > 32 ? tpr : 128; }
+constexpr int threads_of(int tpr) { return tpr > 32 ? tpr : 128; }   // rows of several warps have a CTA to themselves
 
 // down: a power of two, down^2 in [1 / 4 D, 1 / D]: a sum of squares of elements times `down` is within range wherever their mean is, which
 // is that sum times `up`
 __device__ __forceinline__ float down_of(int D) { return __int_as_float((127 - (33 - __clz(D - 1)) / 2) << 23); }
+
+// A thread's E elements of a row, as loaded: pieces of N neighbouring ones, TPR pieces apart; a pair is two neighbours, or (N = 1) an
+// element and the one TPR further on.
+template <typename T, int N, int TPR, int E>
+struct Part {
+  static constexpr int WORDS = E * (int)sizeof(T) / 4, BYTES = N * (int)sizeof(T);
+  uint32_t w[WORDS];
+
+  static __device__ __forceinline__ int column(int sub, int e) { return ((e / N) * TPR + sub) * N + e % N; }
+  // `row`: in global or shared memory
+  __device__ __forceinline__ void load(const T* row, int sub, int D) {
+    if constexpr (BYTES == 16) {
+#pragma unroll
+      for (int v = 0; v < E / N; ++v) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (column(sub, v * N) < D) u = *reinterpret_cast<const uint4*>(row + column(sub, v * N));
+        w[4 * v] = u.x, w[4 * v + 1] = u.y, w[4 * v + 2] = u.z, w[4 * v + 3] = u.w;
+      }
+    } else if constexpr (BYTES == 4) {
+#pragma unroll
+      for (int v = 0; v < WORDS; ++v) w[v] = column(sub, v * N) < D ? *reinterpret_cast<const uint32_t*>(row + column(sub, v * N)) : 0u;
+    } else {
+#pragma unroll
+      for (int v = 0; v < WORDS; ++v) {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+        const uint32_t lo = column(sub, 2 * v) < D ? p[column(sub, 2 * v)] : 0, hi = column(sub, 2 * v + 1) < D ? p[column(sub, 2 * v + 1)] : 0;
+        w[v] = lo | hi << 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int sub, int D) const {
+    if constexpr (BYTES == 16) {
+#pragma unroll
+      for (int v = 0; v < E / N; ++v)
+        if (column(sub, v * N) < D) *reinterpret_cast<uint4*>(row + column(sub, v * N)) = make_uint4(w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
+    } else if constexpr (BYTES == 4) {
+#pragma unroll
+      for (int v = 0; v < WORDS; ++v)
+        if (column(sub, v * N) < D) *reinterpret_cast<uint32_t*>(row + column(sub, v * N)) = w[v];
+    } else {
+#pragma unroll
+      for (int v = 0; v < WORDS; ++v) {
+        uint16_t* p = reinterpret_cast<uint16_t*>(row);
+        if (column(sub, 2 * v) < D) p[column(sub, 2 * v)] = (uint16_t)w[v];
+        if (column(sub, 2 * v + 1) < D) p[column(sub, 2 * v + 1)] = (uint16_t)(w[v] >> 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int v = 0; v < WORDS; ++v) w[v] = 0u;
+  }
+  __device__ __forceinline__ uint64_t pair(int i) const {
+    if constexpr (sizeof(T) == 2) return widen2<T>(w[i]);
+    else return pack2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  }
+  __device__ __forceinline__ void set(int i, uint64_t x) {
+    if constexpr (sizeof(T) == 2) {
+      w[i] = narrow2<T>(x);
+    } else {
+      const float2 f = unpack2(x);
+      w[2 * i] = __float_as_uint(f.x);
+      w[2 * i + 1] = __float_as_uint(f.y);
+    }
+  }
+  // a parameter's pair i; `absent` where there is none, zero past the row's end
+  static __device__ __forceinline__ uint64_t param(const void* p, int dtype, int sub, int D, int i, float absent) {
+    const int a = column(sub, 2 * i), b = column(sub, 2 * i + 1);
+    return pack2(a < D ? (p ? ld_param(p, a, dtype) : absent) : 0.f, b < D ? (p ? ld_param(p, b, dtype) : absent) : 0.f);
+  }
+};
+
+// The tensors of a row, those that are there, side by side in a ring of SLOTS rows, as bulk copies; each group has its own.
+template <int SLOTS>
+struct Ring {
+  unsigned char* base;
+  uint64_t* full;
+  int slot = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+
+  // one thread of the group
+  __device__ __forceinline__ void fill(int at, const void* const* tensors, int n, int64_t row, int row_bytes) const {
+    tc5::mbar_expect_tx(&full[at], n * row_bytes);
+    for (int i = 0; i < n; ++i) tma::load_1d(base + (at * n + i) * row_bytes, static_cast<const char*>(tensors[i]) + row * row_bytes, row_bytes, &full[at]);
+  }
+  __device__ __forceinline__ void wait() {   // (a wait that has run out is told at the end and not repeated)
+    if (ok) ok = tc5::mbar_wait_warp(&full[slot], phase);
+  }
+  __device__ __forceinline__ void next() {
+    if (++slot == SLOTS) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+constexpr int slots_of(int n_tensors, int tpr, int e, int size) {   // 54 KB for 128 threads
+  const int room = 54 * 1024 * threads_of(tpr) / 128 / (threads_of(tpr) / tpr) / (n_tensors * tpr * e * size);
+  return room > 4 ? 4 : room < 1 ? 1 : room;
+}
 
 // act(gate) and, where asked for, act'(gate)
 template <bool SLOPE>
@@ -39,271 +145,298 @@ __device__ __forceinline__ uint64_t activation(uint64_t g, uint32_t flags, uint6
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
-template <typename T, int N, int TPR, int NV>
+template <typename T, int N, int TPR, int E, bool RING>
 __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_norms_fwd_kernel(const b200gdn_rms_norms_args a) {
-  constexpr int RPC = threads_of(TPR) / TPR, NW = TPR > 32 ? TPR / 32 : 1, P = pairs(N);
-  constexpr bool HELD = NV * N <= 8;   // the parameters as fp32 pairs in registers; else they come from the cache with every row
+  using Row = Part<T, N, TPR, E>;
+  constexpr int RPC = threads_of(TPR) / TPR, NW = TPR > 32 ? TPR / 32 : 1, P = E / 2, SLOTS = RING ? slots_of(3, TPR, E, sizeof(T)) : 1;
   __shared__ float scratch[2][2][NW];
+  __shared__ uint64_t full[RING ? RPC * SLOTS : 1];
+  extern __shared__ __align__(128) unsigned char ring_bytes[];
   const int sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const bool post = a.flags & POST;
   const float inv = 1.f / a.D, down = down_of(a.D), up = inv / (down * down);
-  const uint64_t by = spread<N>(down);
-  uint64_t c[HELD ? NV : 1][P], w[HELD ? NV : 1][P];
-  auto params = [&](int d, uint64_t (&c)[P], uint64_t (&w)[P]) {   // what p's normalised elements are multiplied with, and z's
-    load_params<N>(a.scale, a.param_dtype, d, 1.f, c);
-    load_params<N>(post ? a.post_weight : nullptr, a.param_dtype, d, 1.f, w);
+  const uint64_t by = pack2(down, down);
+  uint64_t c[P], w[P];   // what the normalised p is multiplied with, and z
 #pragma unroll
-    for (int i = 0; i < P; ++i) c[i] = mul2(mul2(c[i], spread<N>(a.alpha)), w[i]);
-    load_params<N>(a.weight, a.param_dtype, d, 1.f, w);
-  };
-  if constexpr (HELD) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) c[v][i] = w[v][i] = 0ull;
-      if ((v * TPR + sub) * N < a.D) params((v * TPR + sub) * N, c[v], w[v]);
-    }
+  for (int i = 0; i < P; ++i) {
+    c[i] = mul2(Row::param(a.scale, a.param_dtype, sub, a.D, i, 1.f), pack2(a.alpha, a.alpha));
+    if (post) c[i] = mul2(c[i], Row::param(a.post_weight, a.param_dtype, sub, a.D, i, 1.f));
+    w[i] = Row::param(a.weight, a.param_dtype, sub, a.D, i, 1.f);
   }
-  Vec<T, N> y[NV], res[NV], gate[NV];
-  auto fetch = [&](int64_t row) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int d = (v * TPR + sub) * N;
-      y[v].u = res[v].u = gate[v].u = decltype(y[v].u){};
-      if (row < a.rows && d < a.D) {
-        y[v].load(a.y, row * a.D + d);
-        if (a.residual) res[v].load(a.residual, row * a.D + d);
-        if (a.gate) gate[v].load(a.gate, row * a.D + d);
-      }
-    }
-  };
   const int64_t step = (int64_t)gridDim.x * RPC;
   int64_t row = (int64_t)blockIdx.x * RPC + group;
-  fetch(row);
+  const int row_bytes = a.D * (int)sizeof(T), n_tensors = 1 + (a.residual != nullptr) + (a.gate != nullptr);
+  const void* tensors[3] = {a.y, a.residual ? a.residual : a.gate, a.gate};
+  Ring<SLOTS> ring{ring_bytes + group * SLOTS * n_tensors * row_bytes, full + group * SLOTS};
+  Row y, res, gate;
+  auto fetch = [&](int64_t row) {
+    y.zero(), res.zero(), gate.zero();
+    if (row >= a.rows) return;
+    y.load(static_cast<const T*>(a.y) + row * a.D, sub, a.D);
+    if (a.residual) res.load(static_cast<const T*>(a.residual) + row * a.D, sub, a.D);
+    if (a.gate) gate.load(static_cast<const T*>(a.gate) + row * a.D, sub, a.D);
+  };
+  if constexpr (RING) {
+    if (sub == 0) {
+      for (int i = 0; i < SLOTS; ++i) tc5::mbar_init(&ring.full[i], 1);
+      tc5::fence_mbar_init();
+      for (int i = 0; i < SLOTS && row + i * step < a.rows; ++i) ring.fill(i, tensors, n_tensors, row + i * step, row_bytes);
+    }
+    __syncthreads();
+  } else {
+    fetch(row);
+  }
   for (int turn = 0; row - group < a.rows; turn ^= 1, row += step) {
+    if constexpr (RING) {
+      if (row < a.rows) ring.wait();
+      const T* at = reinterpret_cast<const T*>(ring.base + ring.slot * n_tensors * row_bytes);
+      y.load(at, sub, a.D);
+      if (a.residual) res.load(at += a.D, sub, a.D);
+      else res.zero();
+      if (a.gate) gate.load(at += a.D, sub, a.D);
+    }
     float s[1] = {0.f}, r1 = 1.f;
     if (post) {
       uint64_t sum = 0ull;
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const uint64_t x = mul2(y[v].pair(i), by);
-          sum = fma2(x, x, sum);
-        }
+      for (int i = 0; i < P; ++i) {
+        const uint64_t x = mul2(y.pair(i), by);
+        sum = fma2(x, x, sum);
+      }
       s[0] = both(sum);
       row_sums<TPR>(s, scratch[turn][0]);
       r1 = __frsqrt_rn(s[0] * up + a.eps);
     }
-    uint64_t z[NV][P], sum = 0ull;
-    const uint64_t by_r1 = spread<N>(r1);
+    uint64_t z[P], sum = 0ull;
+    const uint64_t by_r1 = pack2(r1, r1);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int d = (v * TPR + sub) * N;
-      if constexpr (!HELD) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) c[0][i] = 0ull;
-        if (d < a.D) params(d, c[0], w[0]);
-      }
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        uint64_t none, k = mul2(c[HELD ? v : 0][i], by_r1);
-        if (a.gate) k = mul2(k, activation<false>(gate[v].pair(i), a.flags, none));
-        z[v][i] = fma2(y[v].pair(i), k, res[v].pair(i));
-        const uint64_t x = mul2(z[v][i], by);
-        sum = fma2(x, x, sum);
-      }
+    for (int i = 0; i < P; ++i) {
+      uint64_t none, k = mul2(c[i], by_r1);
+      if (a.gate) k = mul2(k, activation<false>(gate.pair(i), a.flags, none));
+      z[i] = fma2(y.pair(i), k, res.pair(i));
+      const uint64_t x = mul2(z[i], by);
+      sum = fma2(x, x, sum);
     }
-    fetch(row + step);
+    if constexpr (!RING) fetch(row + step);
     s[0] = both(sum);
     row_sums<TPR>(s, scratch[turn][1]);
-    const float r2 = __frsqrt_rn(s[0] * up + a.eps);
-    const uint64_t by_r2 = spread<N>(r2);
-    if (row >= a.rows) continue;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int d = (v * TPR + sub) * N;
-      if (d >= a.D) continue;
-      if constexpr (!HELD) load_params<N>(a.weight, a.param_dtype, d, 1.f, w[0]);
-      Vec<T, N> o;
-      if (a.z) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) o.set(i, z[v][i]);
-        o.store(a.z, row * a.D + d);
-      }
-#pragma unroll
-      for (int i = 0; i < P; ++i) o.set(i, mul2(mul2(z[v][i], by_r2), w[HELD ? v : 0][i]));
-      o.store(a.out, row * a.D + d);
+    if constexpr (RING) {   // (the whole group has passed: what it read is in registers)
+      if (TPR == 32) __syncwarp();
+      if (sub == 0 && row + SLOTS * step < a.rows) ring.fill(ring.slot, tensors, n_tensors, row + SLOTS * step, row_bytes);
+      ring.next();
     }
+    const float r2 = __frsqrt_rn(s[0] * up + a.eps);
+    const uint64_t by_r2 = pack2(r2, r2);
+    if (row >= a.rows) continue;
+    Row o;
+    if (a.z) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) o.set(i, z[i]);
+      o.store(static_cast<T*>(a.z) + row * a.D, sub, a.D);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) o.set(i, mul2(mul2(z[i], by_r2), w[i]));
+    o.store(static_cast<T*>(a.out) + row * a.D, sub, a.D);
     if (sub == 0 && a.rstd_z) {
       a.rstd_y[row] = r1;
       a.rstd_z[row] = r2;
     }
   }
+  if (RING && !ring.ok && sub == 0) atomicExch(&g_norms_timeout, 1);
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
-constexpr int bwd_ctas(int tpr) { return tpr <= 128 ? 4 : tpr == 256 ? 2 : 1; }
-
-template <typename T, int N, int TPR, int NV>
-__global__ void __launch_bounds__(threads_of(TPR), bwd_ctas(TPR)) rms_norms_bwd_kernel(const b200gdn_rms_norms_args a) {
-  constexpr int RPC = threads_of(TPR) / TPR, NW = TPR > 32 ? TPR / 32 : 1, P = pairs(N);
-  constexpr bool HELD = NV * N <= 8;
+template <typename T, int N, int TPR, int E, bool RING>
+__global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_norms_bwd_kernel(const b200gdn_rms_norms_args a) {
+  using Row = Part<T, N, TPR, E>;
+  constexpr int RPC = threads_of(TPR) / TPR, NW = TPR > 32 ? TPR / 32 : 1, P = E / 2, SLOTS = RING ? slots_of(5, TPR, E, sizeof(T)) : 1;
+  constexpr bool AHEAD = !RING && E * sizeof(T) <= 16;   // registers for the next row
   __shared__ float scratch[2][2][NW];
-  __shared__ float part[RPC > 1 ? RPC * 2 * TPR * NV * N : 1];
+  __shared__ float part[RPC > 1 ? RPC * 2 * TPR * E : 1];
+  __shared__ uint64_t full[RING ? RPC * SLOTS : 1];
+  extern __shared__ __align__(128) unsigned char ring_bytes[];
   const int sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const bool post = a.flags & POST;
   const float inv = 1.f / a.D;
-  uint64_t c[HELD ? NV : 1][P], w1[HELD ? NV : 1][P], w[HELD ? NV : 1][P];
-  auto params = [&](int d, uint64_t (&c)[P], uint64_t (&w1)[P], uint64_t (&w)[P]) {   // alpha scale, and the norms' weights
-    load_params<N>(a.scale, a.param_dtype, d, 1.f, c);
+  uint64_t c[P], w[P], dw[P], dt[P];   // alpha scale post_weight, weight; the columns' sums
 #pragma unroll
-    for (int i = 0; i < P; ++i) c[i] = mul2(c[i], spread<N>(a.alpha));
-    load_params<N>(post ? a.post_weight : nullptr, a.param_dtype, d, 1.f, w1);
-    load_params<N>(a.weight, a.param_dtype, d, 1.f, w);
-  };
-  uint64_t dw[NV][P], dt[NV][P];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) dw[v][i] = dt[v][i] = 0ull;
-    if constexpr (HELD) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) c[v][i] = w1[v][i] = w[v][i] = 0ull;
-      if ((v * TPR + sub) * N < a.D) params((v * TPR + sub) * N, c[v], w1[v], w[v]);
-    }
+  for (int i = 0; i < P; ++i) {
+    c[i] = mul2(Row::param(a.scale, a.param_dtype, sub, a.D, i, 1.f), pack2(a.alpha, a.alpha));
+    if (post) c[i] = mul2(c[i], Row::param(a.post_weight, a.param_dtype, sub, a.D, i, 1.f));
+    w[i] = Row::param(a.weight, a.param_dtype, sub, a.D, i, 1.f);
+    dw[i] = dt[i] = 0ull;
   }
-  struct Row {
-    Vec<T, N> y[NV], res[NV], gate[NV], dout[NV], dz[NV];
-    float r1, r2;
-  };
-  Row next;
-  auto fetch = [&](int64_t row) {
-    const bool live = row < a.rows;   // (a row past the end adds zeros to every sum)
-    next.r1 = live ? a.rstd_y[row] : 0.f;
-    next.r2 = live ? a.rstd_z[row] : 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int d = (v * TPR + sub) * N;
-      next.y[v].u = next.res[v].u = next.gate[v].u = next.dout[v].u = next.dz[v].u = decltype(next.y[v].u){};
-      if (live && d < a.D) {
-        next.y[v].load(a.y, row * a.D + d);
-        if (a.residual) next.res[v].load(a.residual, row * a.D + d);
-        if (a.gate) next.gate[v].load(a.gate, row * a.D + d);
-        if (a.dout) next.dout[v].load(a.dout, row * a.D + d);
-        if (a.dz) next.dz[v].load(a.dz, row * a.D + d);
-      }
-    }
-  };
   const int64_t step = (int64_t)gridDim.x * RPC;
   int64_t row = (int64_t)blockIdx.x * RPC + group;
-  fetch(row);
+  const int row_bytes = a.D * (int)sizeof(T);
+  const void* tensors[5];
+  int n_tensors = 0;
+  for (const void* p : {a.y, a.residual, a.gate, a.dout, a.dz})
+    if (p) tensors[n_tensors++] = p;
+  Ring<SLOTS> ring{ring_bytes + group * SLOTS * n_tensors * row_bytes, full + group * SLOTS};
+  struct Rows {
+    Row y, res, gate, dout, dz;
+    float r1, r2;
+  };
+  Rows next;
+  auto fetch_sums = [&](int64_t row) {   // (a row past the end adds zeros to every sum)
+    next.r1 = row < a.rows ? a.rstd_y[row] : 0.f;
+    next.r2 = row < a.rows ? a.rstd_z[row] : 0.f;
+  };
+  auto fetch = [&](Rows& to, int64_t row) {
+    to.y.zero(), to.res.zero(), to.gate.zero(), to.dout.zero(), to.dz.zero();
+    if (row >= a.rows) return;
+    to.y.load(static_cast<const T*>(a.y) + row * a.D, sub, a.D);
+    if (a.residual) to.res.load(static_cast<const T*>(a.residual) + row * a.D, sub, a.D);
+    if (a.gate) to.gate.load(static_cast<const T*>(a.gate) + row * a.D, sub, a.D);
+    if (a.dout) to.dout.load(static_cast<const T*>(a.dout) + row * a.D, sub, a.D);
+    if (a.dz) to.dz.load(static_cast<const T*>(a.dz) + row * a.D, sub, a.D);
+  };
+  if constexpr (RING) {
+    if (sub == 0) {
+      for (int i = 0; i < SLOTS; ++i) tc5::mbar_init(&ring.full[i], 1);
+      tc5::fence_mbar_init();
+      for (int i = 0; i < SLOTS && row + i * step < a.rows; ++i) ring.fill(i, tensors, n_tensors, row + i * step, row_bytes);
+    }
+    __syncthreads();
+  } else if constexpr (AHEAD) {
+    fetch(next, row);
+  }
+  fetch_sums(row);
+  // By chunks: from the ring a chunk is read where it is used, and again after the barrier, rather than held.
+  constexpr int CHUNK = N == 1 ? 2 : N, CHUNKS = E / CHUNK, CP = CHUNK / 2;
+  using Chunk = Part<T, N, TPR, CHUNK>;
   for (int turn = 0; row - group < a.rows; turn ^= 1, row += step) {
-    Row cur = next;
-    fetch(row + step);
-    const uint64_t r1 = spread<N>(cur.r1), r2 = spread<N>(cur.r2);
-    uint64_t z[NV][P], sum = 0ull;   // z, then e
+    Rows cur;
+    const T *at_y = nullptr, *at_res = nullptr, *at_gate = nullptr, *at_dout = nullptr, *at_dz = nullptr;
+    const bool live = row < a.rows;
+    const float r1f = next.r1, r2f = next.r2;
+    if constexpr (RING) {
+      if (live) ring.wait();
+      const T* at = reinterpret_cast<const T*>(ring.base + ring.slot * n_tensors * row_bytes);
+      at_y = at;
+      if (a.residual) at_res = at += a.D;
+      if (a.gate) at_gate = at += a.D;
+      if (a.dout) at_dout = at += a.D;
+      if (a.dz) at_dz = at += a.D;
+    } else if constexpr (AHEAD) {
+      cur = next;
+      fetch(next, row + step);
+    } else {
+      fetch(cur, row);
+    }
+    auto chunk = [&](const T* at, const Row& held, int v) {
+      Chunk q;
+      if constexpr (RING) {
+        if (live && at) q.load(at + v * TPR * CHUNK, sub, a.D - v * TPR * CHUNK);
+        else q.zero();
+      } else {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int d = (v * TPR + sub) * N;
-      if constexpr (!HELD) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) c[0][i] = w1[0][i] = w[0][i] = 0ull;
-        if (d < a.D) params(d, c[0], w1[0], w[0]);
+        for (int i = 0; i < Chunk::WORDS; ++i) q.w[i] = held.w[v * Chunk::WORDS + i];
       }
-      const int q = HELD ? v : 0;
+      return q;
+    };
+    fetch_sums(row + step);
+    const uint64_t r1 = pack2(r1f, r1f), r2 = pack2(r2f, r2f);
+    uint64_t z[P], sum = 0ull;   // z r2, then f times what dy has of it
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        uint64_t none, k = mul2(mul2(c[q][i], w1[q][i]), r1);
-        if (a.gate) k = mul2(k, activation<false>(cur.gate[v].pair(i), a.flags, none));
-        z[v][i] = fma2(cur.y[v].pair(i), k, cur.res[v].pair(i));
-        const uint64_t g = cur.dout[v].pair(i), n = mul2(z[v][i], r2);
-        sum = fma2(mul2(g, w[q][i]), n, sum);
-        dw[v][i] = fma2(g, n, dw[v][i]);
+    for (int v = 0; v < CHUNKS; ++v) {
+      const Chunk y = chunk(at_y, cur.y, v), res = chunk(at_res, cur.res, v), dout = chunk(at_dout, cur.dout, v);
+      Chunk gate;
+      if (a.gate) gate = chunk(at_gate, cur.gate, v);
+#pragma unroll
+      for (int q = 0; q < CP; ++q) {
+        const int i = v * CP + q;
+        uint64_t none, k = mul2(c[i], r1);
+        if (a.gate) k = mul2(k, activation<false>(gate.pair(q), a.flags, none));
+        z[i] = mul2(fma2(y.pair(q), k, res.pair(q)), r2);
+        const uint64_t g = dout.pair(q);
+        sum = fma2(mul2(g, w[i]), z[i], sum);
+        dw[i] = fma2(g, z[i], dw[i]);
       }
     }
     float s[1] = {both(sum)};
     row_sums<TPR>(s, scratch[turn][0]);
-    const uint64_t back = spread<N>(-s[0] * inv);   // of n = z r2
-    const bool live = row < a.rows;
+    const uint64_t back = pack2(-s[0] * inv, -s[0] * inv);
     sum = 0ull;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int d = (v * TPR + sub) * N;
-      if constexpr (!HELD) {
-        if (d < a.D) params(d, c[0], w1[0], w[0]);
-        else {
+    for (int v = 0; v < CHUNKS; ++v) {
+      const Chunk y = chunk(at_y, cur.y, v), dout = chunk(at_dout, cur.dout, v), dz = chunk(at_dz, cur.dz, v);
+      Chunk gate, dgate, dres;
+      if (a.gate) gate = chunk(at_gate, cur.gate, v);
 #pragma unroll
-          for (int i = 0; i < P; ++i) c[0][i] = w1[0][i] = w[0][i] = 0ull;
-        }
-      }
-      const int q = HELD ? v : 0;
-      Vec<T, N> dgate;
-      dgate.u = decltype(dgate.u){};
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const uint64_t h = fma2(mul2(z[v][i], r2), back, mul2(cur.dout[v].pair(i), w[q][i]));
-        const uint64_t e = fma2(h, r2, cur.dz[v].pair(i)), n1 = mul2(cur.y[v].pair(i), r1);
-        uint64_t slope, act = spread<N>(1.f);
+      for (int q = 0; q < CP; ++q) {
+        const int i = v * CP + q;
+        const uint64_t h = fma2(z[i], back, mul2(dout.pair(q), w[i]));
+        const uint64_t e = fma2(h, r2, dz.pair(q)), n1 = mul2(y.pair(q), r1), ec = mul2(e, c[i]);
+        dres.set(q, e);
         if (a.gate) {
-          act = activation<true>(cur.gate[v].pair(i), a.flags, slope);
-          if (a.dgate) dgate.set(i, mul2(mul2(mul2(e, c[q][i]), mul2(n1, w1[q][i])), slope));
+          uint64_t slope;
+          const uint64_t act = activation<true>(gate.pair(q), a.flags, slope);
+          if (a.dgate) dgate.set(q, mul2(mul2(ec, n1), slope));
+          dt[i] = fma2(mul2(e, act), n1, dt[i]);
+          z[i] = mul2(ec, act);
+        } else {
+          dt[i] = fma2(e, n1, dt[i]);
+          z[i] = ec;
         }
-        const uint64_t f = mul2(e, act);
-        dt[v][i] = fma2(f, n1, dt[v][i]);
-        z[v][i] = mul2(f, mul2(c[q][i], w1[q][i]));
-        sum = fma2(z[v][i], n1, sum);
-        cur.res[v].set(i, e);
+        sum = fma2(z[i], n1, sum);
       }
-      if (live && d < a.D) {
-        if (a.dgate) dgate.store(a.dgate, row * a.D + d);
-        if (a.dresidual) cur.res[v].store(a.dresidual, row * a.D + d);
+      if (live) {
+        const int64_t to = row * a.D + v * TPR * CHUNK;
+        if (a.dgate) dgate.store(static_cast<T*>(a.dgate) + to, sub, a.D - v * TPR * CHUNK);
+        if (a.dresidual) dres.store(static_cast<T*>(a.dresidual) + to, sub, a.D - v * TPR * CHUNK);
       }
     }
     uint64_t mean = 0ull;
-    if (post) {
+    Row y;   // the row as it was, before its place in the ring is filled again
+#pragma unroll
+    for (int v = 0; v < CHUNKS; ++v) {
+      const Chunk q = chunk(at_y, cur.y, v);
+#pragma unroll
+      for (int i = 0; i < Chunk::WORDS; ++i) y.w[v * Chunk::WORDS + i] = q.w[i];
+    }
+    if (post || RING) {   // (with a ring for its barrier: the row has been read)
       s[0] = both(sum);
       row_sums<TPR>(s, scratch[turn][1]);
-      mean = spread<N>(-s[0] * inv);
+      if (post) mean = pack2(-s[0] * inv, -s[0] * inv);
+    }
+    if constexpr (RING) {
+      if (TPR == 32) __syncwarp();
+      if (sub == 0 && row + SLOTS * step < a.rows) ring.fill(ring.slot, tensors, n_tensors, row + SLOTS * step, row_bytes);
+      ring.next();
     }
     if (!live || !a.dy) continue;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int d = (v * TPR + sub) * N;
-      if (d >= a.D) continue;
-#pragma unroll
-      for (int i = 0; i < P; ++i) cur.y[v].set(i, mul2(fma2(mul2(cur.y[v].pair(i), r1), mean, z[v][i]), r1));   // (r1 is one without the first norm)
-      cur.y[v].store(a.dy, row * a.D + d);
-    }
+    for (int i = 0; i < P; ++i) y.set(i, mul2(fma2(mul2(y.pair(i), r1), mean, z[i]), r1));   // (r1 is one without the first norm)
+    y.store(static_cast<T*>(a.dy) + row * a.D, sub, a.D);
   }
+  if (RING && !ring.ok && sub == 0) atomicExch(&g_norms_timeout, 1);
   if (a.partials == nullptr) return;
-  constexpr int C = TPR * NV * N;
-  auto leave = [&](int which, int d, uint64_t x) {   // a pair of columns
+  constexpr int COLUMNS = TPR * E;
+  auto leave = [&](int which, int i, uint64_t x) {
     const float2 f = unpack2(x);
-    if constexpr (RPC == 1) {
-      float* at = a.partials + ((int64_t)blockIdx.x * 2 + which) * a.D;
-      if (d < a.D) at[d] = f.x;
-      if (N > 1 && d + 1 < a.D) at[d + 1] = f.y;
-    } else {
-      part[(group * 2 + which) * C + d] = f.x;
-      if (N > 1) part[(group * 2 + which) * C + d + 1] = f.y;
+    const int at[2] = {Row::column(sub, 2 * i), Row::column(sub, 2 * i + 1)};
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float v = q ? f.y : f.x;
+      if constexpr (RPC > 1) part[(group * 2 + which) * COLUMNS + at[q]] = v;
+      else if (at[q] < a.D) a.partials[((int64_t)blockIdx.x * 2 + which) * a.D + at[q]] = v;
     }
   };
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      leave(0, (v * TPR + sub) * N + 2 * i, dw[v][i]);
-      leave(1, (v * TPR + sub) * N + 2 * i, dt[v][i]);
-    }
+  for (int i = 0; i < P; ++i) {
+    leave(0, i, dw[i]);
+    leave(1, i, dt[i]);
+  }
   if constexpr (RPC > 1) {   // the groups' sums in their order
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * C; i += threads_of(TPR)) {
-      const int which = i / C, d = i % C;
+    for (int i = threadIdx.x; i < 2 * COLUMNS; i += threads_of(TPR)) {
+      const int which = i / COLUMNS, d = i % COLUMNS;
       if (d >= a.D) continue;
       float s = 0.f;
 #pragma unroll
-      for (int g = 0; g < RPC; ++g) s += part[(g * 2 + which) * C + d];
+      for (int g = 0; g < RPC; ++g) s += part[(g * 2 + which) * COLUMNS + d];
       a.partials[((int64_t)blockIdx.x * 2 + which) * a.D + d] = s;
     }
   }
@@ -461,16 +594,21 @@ int grid_of(int64_t rows, int each, int per_sm) {   // CTAs that take `each` row
   const int64_t want = (rows + each - 1) / each, most = (int64_t)per_sm * sm_count();
   return (int)(want < most ? want : most);
 }
-template <typename T, int N, int TPR, int NV>
-int launch_fwd(const b200gdn_rms_norms_args& a, cudaStream_t st) {
-  rms_norms_fwd_kernel<T, N, TPR, NV><<<grid_of(a.rows, threads_of(TPR) / TPR, 512 / threads_of(TPR)), threads_of(TPR), 0, st>>>(a);
-  return check_launch("rms_norms_fwd");
-}
-template <typename T, int N, int TPR, int NV>
-int launch_bwd(const b200gdn_rms_norms_args& a, cudaStream_t st) {
-  const int n = grid_of(a.rows, threads_of(TPR) / TPR, bwd_ctas(TPR));
-  rms_norms_bwd_kernel<T, N, TPR, NV><<<n, threads_of(TPR), 0, st>>>(a);
-  if (int e = check_launch("rms_norms_bwd")) return e;
+template <typename T, int N, int TPR, int E, bool RING>
+int launch_rows(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
+  constexpr int threads = threads_of(TPR), RPC = threads / TPR;
+  const int n = grid_of(a.rows, RPC, 512 / threads);
+  auto go = [&](auto kern, int most) {
+    int tensors = 0;
+    for (const void* p : {a.y, a.residual, a.gate, bwd ? a.dout : nullptr, bwd ? a.dz : nullptr}) tensors += p != nullptr;
+    const size_t smem = RING ? (size_t)RPC * slots_of(most, TPR, E, sizeof(T)) * tensors * a.D * sizeof(T) : 0;
+    if (RING)   // (what a row may take at most: the limit is set once)
+      if (int e = ensure_smem(kern, (size_t)RPC * slots_of(most, TPR, E, sizeof(T)) * most * TPR * E * sizeof(T))) return e;
+    kern<<<n, threads, smem, st>>>(a);
+    return check_launch(bwd ? "rms_norms_bwd" : "rms_norms_fwd");
+  };
+  if (!bwd) return go(rms_norms_fwd_kernel<T, N, TPR, E, RING>, 3);
+  if (int e = go(rms_norms_bwd_kernel<T, N, TPR, E, RING>, 5)) return e;
   return a.partials ? reduce_partials(a, n, st) : 0;
 }
 
@@ -491,29 +629,24 @@ int launch_wide(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
   return reduce_partials(joined, n, st);
 }
 
-// Eight elements a thread and, where that is more threads than a CTA has registers for, more.
+// Sixteen elements a thread where rows come by the ring, else eight; where that is more threads than a CTA has registers for, sixteen.
 template <typename T, int N>
 int launch_n(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
-  const int pieces = (a.D + N - 1) / N;
-  constexpr int V = 8 / N;   // pieces that make eight elements
-  if (!bwd) {
-    if (pieces <= 8) return launch_fwd<T, N, 8, 1>(a, st);
-    if (pieces <= 32) return launch_fwd<T, N, 32, 1>(a, st);
-    if (pieces <= 32 * V) return launch_fwd<T, N, 32, V>(a, st);
-    if (pieces <= 64 * V) return launch_fwd<T, N, 64, V>(a, st);
-    if (pieces <= 128 * V) return launch_fwd<T, N, 128, V>(a, st);
-    if (pieces <= 256 * V) return launch_fwd<T, N, 128, 2 * V>(a, st);
-    if (pieces <= 512 * V) return launch_fwd<T, N, 256, 2 * V>(a, st);
-    if (pieces <= 1024 * V) return launch_fwd<T, N, 512, 2 * V>(a, st);
+  if (a.D <= 64) return launch_rows<T, N, 8, 8, false>(a, st, bwd);
+  if (a.D <= 128) return launch_rows<T, N, 16, 8, false>(a, st, bwd);
+  if (a.D <= 256) return launch_rows<T, N, 32, 8, false>(a, st, bwd);
+  if constexpr (N * sizeof(T) == 16) {
+    if (a.D <= 512) return launch_rows<T, N, 64, 8, true>(a, st, bwd);
+    if (a.D <= 1024) return launch_rows<T, N, 64, 16, true>(a, st, bwd);
+    if (a.D <= 2048) return launch_rows<T, N, 128, 16, true>(a, st, bwd);
+    if (a.D <= 4096) return launch_rows<T, N, 256, 16, true>(a, st, bwd);
+    if (a.D <= 8192) return launch_rows<T, N, 512, 16, true>(a, st, bwd);
   } else {
-    if (pieces <= 8) return launch_bwd<T, N, 8, 1>(a, st);
-    if (pieces <= 32) return launch_bwd<T, N, 32, 1>(a, st);
-    if (pieces <= 32 * V) return launch_bwd<T, N, 32, V>(a, st);
-    if (pieces <= 64 * V) return launch_bwd<T, N, 64, V>(a, st);
-    if (pieces <= 128 * V) return launch_bwd<T, N, 128, V>(a, st);
-    if (pieces <= 256 * V) return launch_bwd<T, N, 256, V>(a, st);
-    if (pieces <= 512 * V) return launch_bwd<T, N, 512, V>(a, st);
-    if (pieces <= 1024 * V) return launch_bwd<T, N, 512, 2 * V>(a, st);
+    if (a.D <= 512) return launch_rows<T, N, 64, 8, false>(a, st, bwd);
+    if (a.D <= 1024) return launch_rows<T, N, 128, 8, false>(a, st, bwd);
+    if (a.D <= 2048) return launch_rows<T, N, 256, 8, false>(a, st, bwd);
+    if (a.D <= 4096) return launch_rows<T, N, 512, 8, false>(a, st, bwd);
+    if (a.D <= 8192) return launch_rows<T, N, 512, 16, false>(a, st, bwd);
   }
   return launch_wide<T>(a, st, bwd);
 }
@@ -550,6 +683,13 @@ int64_t rms_norms_partials(int64_t rows, int D) { return (rows + 3) / 4 * 4 + (i
 
 int launch_rms_norms(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
   return a.dtype == 0 ? launch_t<__nv_bfloat16>(a, st, bwd) : a.dtype == 1 ? launch_t<__half>(a, st, bwd) : launch_t<float>(a, st, bwd);
+}
+
+int norms_timeout_flag() {
+  int v = 0, zero = 0;
+  cudaMemcpyFromSymbol(&v, g_norms_timeout, sizeof(int));
+  if (v) cudaMemcpyToSymbol(g_norms_timeout, &zero, sizeof(int));
+  return v;
 }
 
 }  // namespace gdn
