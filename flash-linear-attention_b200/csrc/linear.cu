@@ -4,12 +4,12 @@
 // All three products run in one persistent kernel on tcgen05 with CTA pairs: a pair forms a 256 x BN tile (128 rows in the tensor memory of
 // each CTA), each CTA brings its 128 rows of A and its half of B by TMA, one thread issues M = 256 instructions that read both CTAs' shared
 // memory.  A single CTA's 128 x 256 tile would need 96 bytes a clock from L2, more than the 64 an SM gets; the pair's 256 x 256 needs 64 a CTA.
-// Warp 4 loads, warp 5 issues, warps 0 to 3 carry finished tiles out of tensor memory while the next tile's sums form in its other half.
+// Two warps load and issue, eight carry finished tiles out of tensor memory while the next tile's sums form in its other half.
 // Operands lie either way: an operand whose contraction runs along its rows in memory is staged as [contraction][64 columns] panels and read
 // as an MN-major operand, so that W and x are never transposed.
 // Few tokens (up to 256): the product is formed the other way round, W's rows as the 256-row side and the tokens as a BN of 32 to 256, so that
 // what is read is W and little else.  Where there are fewer tiles than CTA pairs the contraction is split; the parts are left in fp32 and a
-// second kernel adds them in order and finishes.
+// second kernel adds them in order and finishes; so is that of the tiles of the last round, where they leave pairs without work.
 // Up to 16 tokens, forward: W passes through registers once, as fast as memory gives it (linear_few_kernel).
 // TMA wants rows 16 bytes apart: operands of other widths are first copied to rows that are.
 #include "gdn_common.cuh"
@@ -31,6 +31,15 @@ __device__ __forceinline__ float activate(float v, int act) {
   if (act == SIGMOID) return sigmoid1(v);
   if (act == GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
   return v;
+}
+__device__ __forceinline__ void activate2(float& a, float& b, int act) {   // of a pair: two results from one reciprocal each
+  if (act == SILU || act == SIGMOID) {
+    const uint64_t v = pack2(a, b), s = fast_sigmoid2(v);
+    const float2 r = unpack2(act == SILU ? mul2(v, s) : s);
+    a = r.x, b = r.y;
+  } else {
+    a = activate(a, act), b = activate(b, act);
+  }
 }
 __device__ __forceinline__ float slope(float v, int act) {
   if (act == SILU) {
@@ -127,33 +136,38 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {   //
 // D[i, j] = sum over k of A(i, k) B(j, k).  `out`, `z` and `residual` are [tokens][features]: token i and feature j, or the other way round.
 struct Product {
   int rows, cols;             // extents of i and j
-  int steps, splits;          // of 64 along k; parts that are summed apart
+  int steps;                  // of 64 along k
   int tiles_i, tiles_j;
+  int whole, splits;          // tiles that are formed whole, and the parts along k of each of the others
   int act;
   int features;               // extent of out's rows, which lie as far apart
   int wide;                   // out, z and residual: rows on boundaries of 32 or 16 bytes, else 0
   uint32_t idesc;
   void *out, *z;              // z: what the activation is applied to, or NULL
   const void *bias, *residual;
-  float* parts;               // with splits > 1: [splits][tokens][pitch]
-  int64_t tokens, pitch;
+  float* parts;               // of the tiles that are not formed whole: [tile][part][256 x BN], features side by side
+  int64_t tokens;
 };
 
-constexpr int BK = 64, A_BYTES = 128 * BK * 2, THREADS = 192;
+constexpr int BK = 64, A_BYTES = 128 * BK * 2, EPILOGUE = 8, THREADS = 32 * (EPILOGUE + 2);   // warps that carry tiles out, and two more
 constexpr int b_bytes(int bn) { return bn / 2 * BK * 2; }
 constexpr int stages_of(int bn) { return bn == 256 ? 6 : bn == 128 ? 8 : bn == 64 ? 10 : 11; }
 constexpr size_t smem_of(int bn) { return (size_t)stages_of(bn) * (A_BYTES + b_bytes(bn)) + 1024; }
 
 struct Tile {
-  int i, j, split, k0, k1;
+  int i, j, part, k0, k1;   // part: of the tiles that are not formed whole, else -1
 };
 // Tiles of eight row blocks, column by column: those at work at one time share their rows of A and B in L2.
 __device__ __forceinline__ Tile tile_of(const Product& p, int t) {
-  const int n = p.tiles_i * p.tiles_j, split = t / n;
-  t -= split * n;
-  const int group = t / (8 * p.tiles_j), first = group * 8, height = min(8, p.tiles_i - first);
+  int part = -1, q = 0;
+  if (t >= p.whole) {
+    part = t - p.whole;
+    t = p.whole + part / p.splits;
+    q = part % p.splits;
+  }
+  const int n = part < 0 ? 1 : p.splits, group = t / (8 * p.tiles_j), first = group * 8, height = min(8, p.tiles_i - first);
   t -= group * 8 * p.tiles_j;
-  return Tile{first + t % height, t / height, split, (int)((int64_t)p.steps * split / p.splits), (int)((int64_t)p.steps * (split + 1) / p.splits)};
+  return Tile{first + t % height, t / height, part, (int)((int64_t)p.steps * q / n), (int)((int64_t)p.steps * (q + 1) / n)};
 }
 
 __device__ __forceinline__ void store32(void* p, uint4 a, uint4 b) {   // 32 bytes, on such a boundary
@@ -203,7 +217,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   unsigned char* tiles = raw + ((1024 - (tc5::smem_addr(raw) & 1023)) & 1023);
   __shared__ uint64_t full[STAGES], empty[STAGES], done[2], taken[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ float turned[SWAPPED ? 1 : 4][32][33];
+  __shared__ float turned[SWAPPED ? 1 : EPILOGUE][32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cta_rank();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -212,19 +226,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     for (int s = 0; s < 2; ++s) {
       tc5::mbar_init(&done[s], 1);
-      tc5::mbar_init(&taken[s], 8);   // the epilogue warps of both CTAs
+      tc5::mbar_init(&taken[s], 2 * EPILOGUE);   // the epilogue warps of both CTAs
     }
     tc5::fence_mbar_init();
   }
-  if (warp == 5) pair_tmem_alloc(&tmem_slot, COLUMNS);
+  if (warp == EPILOGUE + 1) pair_tmem_alloc(&tmem_slot, COLUMNS);
   __syncthreads();
   tc5::fence_before_sync();
   cluster_sync();
   tc5::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const int n_tiles = p.tiles_i * p.tiles_j * p.splits, first = blockIdx.x >> 1, by = gridDim.x >> 1;
+  const int n_tiles = p.whole + (p.tiles_i * p.tiles_j - p.whole) * p.splits, first = blockIdx.x >> 1, by = gridDim.x >> 1;
   bool ok = true;
-  if (warp == 4) {
+  if (warp == EPILOGUE) {
     if (lane == 0) {
       tma::prefetch_map(&map_a);
       tma::prefetch_map(&map_b);
@@ -273,7 +287,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         (void)pair_wait(&full[s], phase);
       }
-  } else if (warp == 5) {
+  } else if (warp == EPILOGUE + 1) {
     if (rank == 0) {
       int s = 0, turn = 0;
       uint32_t phase = 0;
@@ -311,62 +325,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       ok = pair_wait(&done[half], (turn >> 1) & 1);
       if (!ok) break;
       tc5::fence_after_sync();
-      const int i = at.i * 256 + rank * 128 + warp * 32 + lane;
+      // a warp reads its quarter of the lanes; warps four apart share it column block by column block
+      const int local = rank * 128 + (warp & 3) * 32 + lane, i = at.i * 256 + local;
       const bool live = i < p.rows;
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
+      for (int c = warp / 4 * 32; c < BN; c += EPILOGUE / 4 * 32) {
         const int j = at.j * BN + c;
         if (j >= p.cols) break;   // (the same for all)
         float v[32];
         __syncwarp();
-        tmem_ld32(tmem + half * BN + c + ((uint32_t)(warp * 32) << 16), v);
+        tmem_ld32(tmem + half * BN + c + ((uint32_t)((warp & 3) * 32) << 16), v);
         tc5::tmem_ld_wait();
-        if constexpr (!SWAPPED) {
-          if (p.splits > 1) {
-            float* part = p.parts + ((int64_t)at.split * p.tokens + i) * p.pitch + j;
+        if (at.part >= 0) {
+          float* part = p.parts + (int64_t)at.part * 256 * BN;
+          if constexpr (!SWAPPED) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)   // (the pitch is a multiple of eight)
-              if (live && j + q * 8 < p.cols)
-                store32(part + q * 8, *reinterpret_cast<const uint4*>(&v[q * 8]), *reinterpret_cast<const uint4*>(&v[q * 8 + 4]));
-          } else if (p.wide && j + 32 <= p.cols) {   // a lane writes 64 bytes of its row, whole sectors
-            if (!live) continue;
-            const int64_t to = (int64_t)i * p.features + j;
-            if (p.bias) add_row<T>(static_cast<const T*>(p.bias) + j, v);
-            if (p.z) put_row<T>(static_cast<T*>(p.z) + to, p.wide, v);
-            if (p.act != NONE)
+            for (int q = 0; q < 4; ++q)
+              store32(part + local * BN + c + q * 8, *reinterpret_cast<const uint4*>(&v[q * 8]), *reinterpret_cast<const uint4*>(&v[q * 8 + 4]));
+          } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = activate(v[e], p.act);
-            if (p.residual) add_row<T>(static_cast<const T*>(p.residual) + to, v);
-            put_row<T>(static_cast<T*>(p.out) + to, p.wide, v);
-          } else {   // rows on any boundary: turned round, so that a warp writes a row's 32 columns at a time
-#pragma unroll
-            for (int e = 0; e < 32; ++e) turned[warp][lane][e] = v[e];
-            __syncwarp();
-            const int col = j + lane, i0 = i - lane;
-            if (col < p.cols) {
-              const float b = p.bias ? (float)static_cast<const T*>(p.bias)[col] : 0.f;
-              int64_t to = (int64_t)i0 * p.features + col;
-#pragma unroll 4
-              for (int r = 0; r < 32 && i0 + r < p.rows; ++r, to += p.features) {
-                float x = turned[warp][r][lane] + b;
-                if (p.z) static_cast<T*>(p.z)[to] = static_cast<T>(x);
-                x = activate(x, p.act);
-                if (p.residual) x += (float)static_cast<const T*>(p.residual)[to];
-                static_cast<T*>(p.out)[to] = static_cast<T>(x);
-              }
-            }
-            __syncwarp();
+            for (int e = 0; e < 32; ++e) part[(c + e) * 256 + local] = v[e];
           }
-        } else {
+        } else if constexpr (SWAPPED) {
           if (!live) continue;
-          const float b = p.bias && p.splits == 1 ? (float)static_cast<const T*>(p.bias)[i] : 0.f;
+          const float b = p.bias ? (float)static_cast<const T*>(p.bias)[i] : 0.f;
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             if (j + e >= p.cols) break;
-            if (p.splits > 1) {
-              p.parts[((int64_t)at.split * p.tokens + j + e) * p.pitch + i] = v[e];
-              continue;
-            }
             const int64_t to = (int64_t)(j + e) * p.features + i;
             float x = v[e] + b;
             if (p.z) static_cast<T*>(p.z)[to] = static_cast<T>(x);
@@ -374,6 +359,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             if (p.residual) x += (float)static_cast<const T*>(p.residual)[to];
             static_cast<T*>(p.out)[to] = static_cast<T>(x);
           }
+        } else if (p.wide && j + 32 <= p.cols) {   // a lane writes 64 bytes of its row, whole sectors
+          if (!live) continue;
+          const int64_t to = (int64_t)i * p.features + j;
+          if (p.bias) add_row<T>(static_cast<const T*>(p.bias) + j, v);
+          if (p.z) put_row<T>(static_cast<T*>(p.z) + to, p.wide, v);
+          if (p.act != NONE)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) activate2(v[e], v[e + 1], p.act);
+          if (p.residual) add_row<T>(static_cast<const T*>(p.residual) + to, v);
+          put_row<T>(static_cast<T*>(p.out) + to, p.wide, v);
+        } else {   // rows on any boundary: turned round, so that a warp writes a row's 32 columns at a time
+          const int col = j + lane, i0 = i - lane, rows = min(32, p.rows - i0);
+          const bool here = col < p.cols;
+          T res[32];   // (all on their way at once)
+#pragma unroll
+          for (int r = 0; r < 32; ++r)
+            if (p.residual) res[r] = here && r < rows ? static_cast<const T*>(p.residual)[(int64_t)(i0 + r) * p.features + col] : static_cast<T>(0.f);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) turned[warp][lane][e] = v[e];
+          __syncwarp();
+          const float b = p.bias && here ? (float)static_cast<const T*>(p.bias)[col] : 0.f;
+#pragma unroll
+          for (int r = 0; r < 32; ++r) v[r] = turned[warp][r][lane] + b;
+          __syncwarp();
+          if (!here) continue;
+          const int64_t to = (int64_t)i0 * p.features + col;
+          if (p.z)
+#pragma unroll
+            for (int r = 0; r < 32; ++r)
+              if (r < rows) static_cast<T*>(p.z)[to + (int64_t)r * p.features] = static_cast<T>(v[r]);
+          if (p.act != NONE)
+#pragma unroll
+            for (int r = 0; r < 32; r += 2) activate2(v[r], v[r + 1], p.act);
+#pragma unroll
+          for (int r = 0; r < 32; ++r)
+            if (r < rows) static_cast<T*>(p.out)[to + (int64_t)r * p.features] = static_cast<T>(p.residual ? v[r] + (float)res[r] : v[r]);
         }
       }
       tc5::fence_before_sync();
@@ -387,37 +408,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   tc5::fence_before_sync();
   cluster_sync();
   tc5::fence_after_sync();
-  if (warp == 5) pair_tmem_dealloc(tmem, COLUMNS);
+  if (warp == EPILOGUE + 1) pair_tmem_dealloc(tmem, COLUMNS);
 }
 
-// the parts of a split contraction in their order, and what follows the product; four features a thread
-template <typename T>
-__global__ void __launch_bounds__(128) linear_join_kernel(const Product p) {
+// Tiles that were formed in parts: the parts in their order, and what follows the product; four features a thread.
+template <typename T, int BN, bool SWAPPED>
+__global__ void __launch_bounds__(256) linear_join_kernel(const Product p) {
+  constexpr int SIZE = 256 * BN, WIDTH = SWAPPED ? 256 : BN;   // features of a tile
   wait_for_predecessor();
-  const int f0 = (blockIdx.x * 128 + threadIdx.x) * 4;
-  if (f0 >= p.features) return;
-  const int64_t size = p.tokens * p.pitch;
-  for (int64_t token = blockIdx.y; token < p.tokens; token += gridDim.y) {
-    const float* part = p.parts + token * p.pitch + f0;   // (the pitch is a multiple of eight)
-    float4 sum = *reinterpret_cast<const float4*>(part);
+  const int tile = blockIdx.y, at = (blockIdx.x * 256 + threadIdx.x) * 4, f_local = at % WIDTH, t_local = at / WIDTH;
+  Product whole = p;
+  whole.whole = p.tiles_i * p.tiles_j;
+  const Tile where = tile_of(whole, p.whole + tile);
+  const int f0 = (SWAPPED ? where.i * 256 : where.j * BN) + f_local, token = (SWAPPED ? where.j * BN : where.i * 256) + t_local;
+  if (at >= SIZE || f0 >= p.features || token >= p.tokens) return;
+  const float* part = p.parts + (int64_t)tile * p.splits * SIZE + at;
+  float4 sum = *reinterpret_cast<const float4*>(part);
 #pragma unroll 4
-    for (int s = 1; s < p.splits; ++s) {
-      const float4 q = *reinterpret_cast<const float4*>(part + s * size);
-      sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
-    }
-    const float v4[4] = {sum.x, sum.y, sum.z, sum.w};
+  for (int s = 1; s < p.splits; ++s) {
+    const float4 q = *reinterpret_cast<const float4*>(part + (int64_t)s * SIZE);
+    sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+  }
+  const float v4[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int f = f0 + e;
-      if (f >= p.features) break;
-      const int64_t at = token * p.features + f;
-      float v = v4[e];
-      if (p.bias) v += (float)static_cast<const T*>(p.bias)[f];
-      if (p.z) static_cast<T*>(p.z)[at] = static_cast<T>(v);
-      v = activate(v, p.act);
-      if (p.residual) v += (float)static_cast<const T*>(p.residual)[at];
-      static_cast<T*>(p.out)[at] = static_cast<T>(v);
-    }
+  for (int e = 0; e < 4; ++e) {
+    const int f = f0 + e;
+    if (f >= p.features) break;
+    const int64_t to = (int64_t)token * p.features + f;
+    float v = v4[e];
+    if (p.bias) v += (float)static_cast<const T*>(p.bias)[f];
+    if (p.z) static_cast<T*>(p.z)[to] = static_cast<T>(v);
+    v = activate(v, p.act);
+    if (p.residual) v += (float)static_cast<const T*>(p.residual)[to];
+    static_cast<T*>(p.out)[to] = static_cast<T>(v);
   }
 }
 
@@ -603,25 +626,26 @@ __global__ void __launch_bounds__(256) linear_dbias_kernel(const float* sums, T*
 constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 struct Plan {
-  int bn, splits;
+  int bn, whole, splits;
   int64_t parts;   // floats
 };
-// The column tile and the parts of the contraction with the least time by this model: rounds of tiles over the pairs, 0.27 us a step of
-// 256 x 256 (0.17 of 128 columns, 0.12 of fewer: what the loads take), 1.5 us a tile that nothing hides, and 3 us with what the parts move.
+// The column tile, and the parts that the tiles of the last, incomplete round are formed in, with the least time by this model: 0.32 us a step
+// of 256 x 256 (0.28 of 128 columns, 0.2 of fewer: what the loads take), 2 us a tile that nothing hides, and 3 us with what the parts move.
+// (8192 x 2048 from 16384 tokens, 256 tiles on 74 pairs: 408 us in whole tiles, 362 with the last 34 in two parts each.)
 Plan plan_of(int64_t rows, int64_t cols, int64_t depth, bool swapped) {
   const int pairs = sm_count() / 2, steps = (int)((depth + BK - 1) / BK);
-  Plan best{256, 1, 0};
+  Plan best{256, 0, 1, 0};
   double least = 1e30;
   for (int bn : {256, 128, 64, 32}) {
     if (swapped ? (bn < cols && bn < 256) || bn / 2 >= up(cols, 32) : bn < 128) continue;
-    const int64_t tiles = (rows + 255) / 256 * ((cols + bn - 1) / bn);
-    const double step = bn == 256 ? 0.27 : bn == 128 ? 0.17 : 0.12;
-    for (int s = 1; s <= 16 && (s == 1 || steps / s >= 4); ++s) {
-      const double bytes = s > 1 ? 8.0 * s * rows * cols : 0;
-      const double cost = (double)((tiles * s + pairs - 1) / pairs) * ((steps + s - 1) / s * step + 1.5) + (s > 1 ? 3 + bytes / 6e6 : 0);
+    const int64_t tiles = (rows + 255) / 256 * ((cols + bn - 1) / bn), whole = tiles / pairs * pairs, rest = tiles - whole;
+    const double step = bn == 256 ? 0.32 : bn == 128 ? 0.28 : 0.2;
+    for (int s = 1; s <= 16 && (s == 1 || (rest > 0 && rest * s <= pairs && steps / s >= 4)); ++s) {
+      const double moved = s > 1 ? 8.0 * rest * s * 256 * bn : 0;
+      const double cost = (double)whole / pairs * (steps * step + 2) + (rest > 0 ? (steps + s - 1) / s * step + 2 : 0) + (s > 1 ? 3 + moved / 6e6 : 0);
       if (cost < least) {
         least = cost;
-        best = Plan{bn, s, s > 1 ? s * (swapped ? cols * up(rows, 8) : rows * up(cols, 8)) : 0};
+        best = s > 1 ? Plan{bn, (int)whole, s, rest * s * 256 * bn} : Plan{bn, (int)tiles, 1, 0};
       }
     }
   }
@@ -644,39 +668,38 @@ int launch_tiles(const Operand& a, const Operand& b, Product p, cudaStream_t st)
   p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
   auto kern = linear_kernel<T, BN, A_MN, B_MN, SWAPPED>;
   if (int e = ensure_smem(kern, smem_of(BN))) return e;
-  const int64_t tiles = (int64_t)p.tiles_i * p.tiles_j * p.splits;
-  if (tiles > INT32_MAX) return set_error(B200GDN_ERR_UNSUPPORTED, "linear: more than 2^31 - 1 tiles");
+  const int rest = p.tiles_i * p.tiles_j - p.whole;   // (checked to be within an int)
+  const int64_t tiles = p.whole + (int64_t)rest * p.splits;
   const int pairs = (int)(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
   kern<<<2 * pairs, THREADS, smem_of(BN), st>>>(ma, mb, p);
-  return check_launch("linear");
+  if (int e = check_launch("linear")) return e;
+  if (rest == 0) return 0;
+  launch_overlapped(true, linear_join_kernel<T, BN, SWAPPED>, dim3(256 * BN / 1024, rest), 256, 0, st, p);
+  return check_launch("linear_join");
 }
 
 // A and B as D's rows and columns; `swapped`: D's rows are features
 template <typename T, bool A_MN, bool B_MN>
 int launch_product(const Operand& a, const Operand& b, int64_t depth, Product p, bool swapped, float* parts, cudaStream_t st) {
+  const int64_t most = ((int64_t)p.rows + 255) / 256 * (((int64_t)p.cols + 31) / 32);
+  if (most > INT32_MAX / 16) return set_error(B200GDN_ERR_UNSUPPORTED, "linear: a result of more than 2^27 tiles");
   const Plan plan = plan_of(p.rows, p.cols, depth, swapped);
+  p.whole = plan.whole;
   p.steps = (int)((depth + BK - 1) / BK);
   p.splits = plan.splits;
   p.parts = parts;
   p.tokens = swapped ? p.cols : p.rows;
   p.features = swapped ? p.rows : p.cols;
-  p.pitch = up(p.features, 8);
   uintptr_t bits = reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.z) | reinterpret_cast<uintptr_t>(p.bias) |
                    reinterpret_cast<uintptr_t>(p.residual) | (uintptr_t)p.features * 2;
   p.wide = bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 0;
-  int e = B200GDN_ERR_UNSUPPORTED;
-  if (!swapped) {
-    e = plan.bn == 256 ? launch_tiles<T, 256, A_MN, B_MN, false>(a, b, p, st) : launch_tiles<T, 128, A_MN, B_MN, false>(a, b, p, st);
-  } else if constexpr (!B_MN) {
-    e = plan.bn == 256   ? launch_tiles<T, 256, A_MN, false, true>(a, b, p, st)
-        : plan.bn == 128 ? launch_tiles<T, 128, A_MN, false, true>(a, b, p, st)
-        : plan.bn == 64  ? launch_tiles<T, 64, A_MN, false, true>(a, b, p, st)
-                         : launch_tiles<T, 32, A_MN, false, true>(a, b, p, st);
-  }
-  if (e != 0 || plan.splits == 1) return e;
-  const int64_t x = (p.features + 511) / 512, most = 16 * (int64_t)sm_count() / x + 1;
-  launch_overlapped(true, linear_join_kernel<T>, dim3((unsigned)x, (unsigned)(p.tokens < most ? p.tokens : most)), 128, 0, st, p);
-  return check_launch("linear_join");
+  if (!swapped) return plan.bn == 256 ? launch_tiles<T, 256, A_MN, B_MN, false>(a, b, p, st) : launch_tiles<T, 128, A_MN, B_MN, false>(a, b, p, st);
+  if constexpr (!B_MN)
+    return plan.bn == 256   ? launch_tiles<T, 256, A_MN, false, true>(a, b, p, st)
+           : plan.bn == 128 ? launch_tiles<T, 128, A_MN, false, true>(a, b, p, st)
+           : plan.bn == 64  ? launch_tiles<T, 64, A_MN, false, true>(a, b, p, st)
+                            : launch_tiles<T, 32, A_MN, false, true>(a, b, p, st);
+  return B200GDN_ERR_UNSUPPORTED;
 }
 
 constexpr int64_t FEW = 16, SWAP = 256;   // tokens up to which W passes through registers, and up to which its rows are the tile's 256

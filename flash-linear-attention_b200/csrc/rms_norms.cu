@@ -91,10 +91,25 @@ struct Part {
       w[2 * i + 1] = __float_as_uint(f.y);
     }
   }
-  // a parameter's pair i; `absent` where there is none, zero past the row's end
-  static __device__ __forceinline__ uint64_t param(const void* p, int dtype, int sub, int D, int i, float absent) {
-    const int a = column(sub, 2 * i), b = column(sub, 2 * i + 1);
-    return pack2(a < D ? (p ? ld_param(p, a, dtype) : absent) : 0.f, b < D ? (p ? ld_param(p, b, dtype) : absent) : 0.f);
+  // a parameter's pairs; `absent` where there is none, zero past the row's end
+  static __device__ __forceinline__ void params(const void* p, int dtype, int sub, int D, float absent, uint64_t (&x)[E / 2]) {
+    if constexpr (N == 1) {
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        const int a = column(sub, 2 * i), b = column(sub, 2 * i + 1);
+        x[i] = pack2(a < D ? (p ? ld_param(p, a, dtype) : absent) : 0.f, b < D ? (p ? ld_param(p, b, dtype) : absent) : 0.f);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < E / N; ++v) {
+        uint64_t q[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) q[i] = 0ull;
+        if (column(sub, v * N) < D) load_params<N>(p, dtype, column(sub, v * N), absent, q);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) x[v * N / 2 + i] = q[i];
+      }
+    }
   }
 };
 
@@ -156,13 +171,6 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
   const bool post = a.flags & POST;
   const float inv = 1.f / a.D, down = down_of(a.D), up = inv / (down * down);
   const uint64_t by = pack2(down, down);
-  uint64_t c[P], w[P];   // what the normalised p is multiplied with, and z
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    c[i] = mul2(Row::param(a.scale, a.param_dtype, sub, a.D, i, 1.f), pack2(a.alpha, a.alpha));
-    if (post) c[i] = mul2(c[i], Row::param(a.post_weight, a.param_dtype, sub, a.D, i, 1.f));
-    w[i] = Row::param(a.weight, a.param_dtype, sub, a.D, i, 1.f);
-  }
   const int64_t step = (int64_t)gridDim.x * RPC;
   int64_t row = (int64_t)blockIdx.x * RPC + group;
   const int row_bytes = a.D * (int)sizeof(T), n_tensors = 1 + (a.residual != nullptr) + (a.gate != nullptr);
@@ -186,6 +194,12 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
   } else {
     fetch(row);
   }
+  uint64_t c[P], w[P];   // what the normalised p is multiplied with, and z
+  Row::params(post ? a.post_weight : nullptr, a.param_dtype, sub, a.D, 1.f, c);
+  Row::params(a.scale, a.param_dtype, sub, a.D, 1.f, w);
+#pragma unroll
+  for (int i = 0; i < P; ++i) c[i] = mul2(mul2(w[i], pack2(a.alpha, a.alpha)), c[i]);
+  Row::params(a.weight, a.param_dtype, sub, a.D, 1.f, w);
   for (int turn = 0; row - group < a.rows; turn ^= 1, row += step) {
     if constexpr (RING) {
       if (row < a.rows) ring.wait();
@@ -258,14 +272,6 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
   const int sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const bool post = a.flags & POST;
   const float inv = 1.f / a.D;
-  uint64_t c[P], w[P], dw[P], dt[P];   // alpha scale post_weight, weight; the columns' sums
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    c[i] = mul2(Row::param(a.scale, a.param_dtype, sub, a.D, i, 1.f), pack2(a.alpha, a.alpha));
-    if (post) c[i] = mul2(c[i], Row::param(a.post_weight, a.param_dtype, sub, a.D, i, 1.f));
-    w[i] = Row::param(a.weight, a.param_dtype, sub, a.D, i, 1.f);
-    dw[i] = dt[i] = 0ull;
-  }
   const int64_t step = (int64_t)gridDim.x * RPC;
   int64_t row = (int64_t)blockIdx.x * RPC + group;
   const int row_bytes = a.D * (int)sizeof(T);
@@ -303,6 +309,15 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     fetch(next, row);
   }
   fetch_sums(row);
+  uint64_t c[P], w[P], dw[P], dt[P];   // alpha scale post_weight, weight; the columns' sums
+  Row::params(post ? a.post_weight : nullptr, a.param_dtype, sub, a.D, 1.f, c);
+  Row::params(a.scale, a.param_dtype, sub, a.D, 1.f, w);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    c[i] = mul2(mul2(w[i], pack2(a.alpha, a.alpha)), c[i]);
+    dw[i] = dt[i] = 0ull;
+  }
+  Row::params(a.weight, a.param_dtype, sub, a.D, 1.f, w);
   // By chunks: from the ring a chunk is read where it is used, and again after the barrier, rather than held.
   constexpr int CHUNK = N == 1 ? 2 : N, CHUNKS = E / CHUNK, CP = CHUNK / 2;
   using Chunk = Part<T, N, TPR, CHUNK>;
