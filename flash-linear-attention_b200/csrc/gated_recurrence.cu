@@ -2,7 +2,7 @@
 //     forward   over R tokens of a warp with a = exp(g): h' = their recurrence from 0 and A = their product of a; entered with s they leave
 //               A s + h'
 //     backward  u_t = a_t (dh_t + u_{t+1}) from the right in the same way; dx_t = dh_t + u_{t+1}, dg_t = dx_t a_t h_{t-1}
-// HBM streaming: what counts is that every tensor is read once.  A CTA owns 32 C neighbouring channels of a sequence and walks it in steps
+// HBM streaming: what counts is that every tensor is read once.  A CTA owns 64 neighbouring channels of a sequence, two a lane, and walks it in steps
 // of W R tokens, R for each of its W warps, which hold them in registers (the next step's are on their way meanwhile): each warp joins its
 // own tokens, leaves (A, h') in shared memory, and after one barrier a step goes through the warps ahead of it for the state its first
 // token sees, then through its tokens again.  Where sequences x channels give fewer CTAs than there are SMs, CTAs of a cluster share a
@@ -21,25 +21,41 @@ __device__ int g_recurrence_timeout = 0;
 
 constexpr int MOST_RANKS = 16;   // CTAs of a cluster
 
-// C neighbouring channels of a token, as loaded
-template <typename T, int C>
+// A lane's two channels of a token, as loaded: neighbours in one access (APART 1), or 32 apart where rows do not allow that (APART 32).  `two`:
+// there is a second one.
+constexpr int WIDTH = 64;   // channels of a CTA
+template <int APART>
+__device__ __forceinline__ int channel_of(int lane) { return APART == 1 ? 2 * lane : lane; }
+
+template <typename T, int APART>
 struct Piece {
-  using Raw = std::conditional_t<sizeof(T) * C == 8, uint2, std::conditional_t<sizeof(T) * C == 4, uint32_t, uint16_t>>;
+  using Raw = std::conditional_t<sizeof(T) == 4, uint2, uint32_t>;
   Raw u;
   __device__ __forceinline__ void zero() { u = Raw{}; }
-  __device__ __forceinline__ void load(const T* p) { u = __ldcs(reinterpret_cast<const Raw*>(p)); }
-  __device__ __forceinline__ void take(const void* shared) { u = *static_cast<const Raw*>(shared); }
-  __device__ __forceinline__ uint64_t pair() const {   // of one channel: the second half is zero
-    if constexpr (C == 1) return pack2((float)*reinterpret_cast<const T*>(&u), 0.f);
-    else if constexpr (sizeof(T) == 2) return widen2<T>(u);
+  __device__ __forceinline__ void load(const T* p, bool two) {
+    if constexpr (APART == 1) {
+      u = __ldcs(reinterpret_cast<const Raw*>(p));
+    } else if constexpr (sizeof(T) == 4) {
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+      u.x = __ldcs(q);
+      u.y = two ? __ldcs(q + APART) : 0u;
+    } else {
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+      const uint32_t lo = __ldcs(q), hi = two ? __ldcs(q + APART) : 0;
+      u = lo | hi << 16;
+    }
+  }
+  __device__ __forceinline__ void take(const void* shared) { u = *static_cast<const Raw*>(shared); }   // (neighbours)
+  __device__ __forceinline__ uint64_t pair() const {
+    if constexpr (sizeof(T) == 2) return widen2<T>(u);
     else return pack2(__uint_as_float(u.x), __uint_as_float(u.y));
   }
   // the pair within [-88, 89]; a NaN stays
   __device__ __forceinline__ uint64_t gate() const {
-    if constexpr (sizeof(T) == 4 || C == 1) {
+    if constexpr (sizeof(T) == 4) {
       float2 f = unpack2(pair());
       asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(f.x));
-      if (C == 2) asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(f.y));
+      asm("max.NaN.f32 %0, %0, 0fC2B00000;\n min.NaN.f32 %0, %0, 0f42B20000;" : "+f"(f.y));
       return pack2(f.x, f.y);
     } else {
       uint32_t w = u;
@@ -48,11 +64,15 @@ struct Piece {
       return widen2<T>(w);
     }
   }
-  static __device__ __forceinline__ void store(T* p, uint64_t x) {
-    const float2 f = unpack2(x);
-    if constexpr (C == 1) *p = static_cast<T>(f.x);
-    else if constexpr (sizeof(T) == 2) __stcs(reinterpret_cast<uint32_t*>(p), narrow2<T>(x));
-    else __stcs(reinterpret_cast<float2*>(p), f);
+  static __device__ __forceinline__ void store(T* p, uint64_t x, bool two) {
+    if constexpr (APART == 1) {
+      if constexpr (sizeof(T) == 2) __stcs(reinterpret_cast<uint32_t*>(p), narrow2<T>(x));
+      else __stcs(reinterpret_cast<float2*>(p), unpack2(x));
+    } else {
+      const float2 f = unpack2(x);
+      p[0] = static_cast<T>(f.x);
+      if (two) p[APART] = static_cast<T>(f.y);
+    }
   }
 };
 
@@ -89,14 +109,16 @@ __device__ __forceinline__ Span span_of(const b200gdn_gated_recurrence_args& a, 
   return Span{head.row, tail.row + tail.len - head.row, c};
 }
 
+template <int APART>
 __device__ __forceinline__ uint64_t load_state(const float* p, int64_t at, bool there, bool two) {
   if (p == nullptr || !there) return 0ull;
-  return pack2(p[at], two ? p[at + 1] : 0.f);
+  return pack2(p[at], two ? p[at + APART] : 0.f);
 }
+template <int APART>
 __device__ __forceinline__ void store_state(float* p, int64_t at, uint64_t x, bool two) {
   const float2 f = unpack2(x);
   p[at] = f.x;
-  if (two) p[at + 1] = f.y;
+  if (two) p[at + APART] = f.y;
 }
 
 // [0]: the product of the decays, [1]: what the tokens leave of themselves
@@ -237,15 +259,15 @@ __device__ __forceinline__ bool knows_the_end(int n, int warp, int rank) { retur
 struct Place {   // of a CTA: its sequence, the lane's first channel and the tile's
   int seq, channel, tile, rank, n_ranks;
 };
-template <int C, bool CLUSTER>
+template <int APART, bool CLUSTER>
 __device__ __forceinline__ Place place_of(const b200gdn_gated_recurrence_args& a) {
-  const int tiles = (a.D + 32 * C - 1) / (32 * C);
+  const int tiles = (a.D + WIDTH - 1) / WIDTH;
   const int n = CLUSTER ? (int)cluster_size() : 1;
-  const int i = blockIdx.x / n, seq = i / tiles, first = (i % tiles) * 32 * C;
-  return Place{a.seq_order ? a.seq_order[seq] : seq, first + (int)(threadIdx.x & 31) * C, first, CLUSTER ? (int)cluster_rank() : 0, n};
+  const int i = blockIdx.x / n, seq = i / tiles, first = (i % tiles) * WIDTH;
+  return Place{a.seq_order ? a.seq_order[seq] : seq, first + channel_of<APART>(threadIdx.x & 31), first, CLUSTER ? (int)cluster_rank() : 0, n};
 }
 
-// The tensors that a step reads, in tiles of [W R tokens][32 C channels], STAGES steps deep, by TMA: `full` counts a stage's bytes.  Tokens
+// The tensors that a step reads, in tiles of [W R tokens][64 channels], STAGES steps deep, by TMA: `full` counts a stage's bytes.  Tokens
 // past the end of the tensor and channels past its last one arrive as zeros, tokens past the sequence's end are another sequence's.
 template <int N, int ROWS, int STAGES>
 struct Tiles {
@@ -284,21 +306,21 @@ constexpr int stages_of(int stage_bytes, bool cluster) {   // two CTAs an SM
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
 // TMA: the tokens come by way of shared memory, several steps ahead; else (odd widths and boundaries) straight to registers, one step ahead.
-template <typename T, typename G, int C, int R, int W, bool CLUSTER, bool TMA>
+template <typename T, typename G, int APART, int R, int W, bool CLUSTER, bool TMA>
 __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, const b200gdn_gated_recurrence_args a) {
-  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * 32 * C * (int)(sizeof(T) + sizeof(G)), CLUSTER);
+  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * WIDTH * (int)(sizeof(T) + sizeof(G)), CLUSTER);
   __shared__ Exchange<W, CLUSTER> exchange;
   __shared__ uint64_t full[STAGES];
   extern __shared__ __align__(128) unsigned char shared_tiles[];
-  const Place at = place_of<C, CLUSTER>(a);
+  const Place at = place_of<APART, CLUSTER>(a);
   const Span seq = span_of(a, at.seq);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, step = at.n_ranks * ROWS;
-  const bool live = at.channel < a.D, two = C == 2;
+  const bool live = at.channel < a.D, two = APART == 1 || at.channel + APART < a.D;
   const int n = (seq.len + step - 1) / step, in_step = warp * R;
   int t0 = at.rank * ROWS + in_step;
-  Piece<T, C> x[R];
-  Piece<G, C> g[R];
+  Piece<T, APART> x[R];
+  Piece<G, APART> g[R];
   Tiles<2, ROWS, STAGES> tiles;
   const CUtensorMap* const maps[2] = {&map_x, &map_g};
   Patience patience;
@@ -310,37 +332,37 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
       x[r].zero();   // past the end: a decay of one, and nothing added
       g[r].zero();
       if (live && t + r < seq.len) {
-        x[r].load(px);
-        g[r].load(pg);
+        x[r].load(px, two);
+        g[r].load(pg, two);
       }
     }
   };
   exchange.init();
   if constexpr (TMA) {
-    const int row_bytes[2] = {32 * C * (int)sizeof(T), 32 * C * (int)sizeof(G)};
+    const int row_bytes[2] = {WIDTH * (int)sizeof(T), WIDTH * (int)sizeof(G)};
     tiles.init(shared_tiles, full, row_bytes);
     if (threadIdx.x == 0)
       for (int i = 0; i < STAGES && i < n; ++i) tiles.load(i, maps, at.tile, (int)seq.first + i * step + at.rank * ROWS);
   } else {
     fetch(t0);
   }
-  uint64_t s = load_state(a.h0, (int64_t)at.seq * a.D + at.channel, live, two);
+  uint64_t s = load_state<APART>(a.h0, (int64_t)at.seq * a.D + at.channel, live, two);
   int stage = 0;
   uint32_t phase = 0;
   uint64_t decays[R];
-  Piece<T, C> now[R];
+  Piece<T, APART> now[R];
   // the warp's tokens of step i, from t on: their decays, and the pair that they come to
   auto begin = [&](int i, int t) {
     const int rows = seq.len - t;
     Joined own = {pack2(1.f, 1.f), 0ull};
     if constexpr (TMA) {
       patience.wait(&full[stage], phase);
-      const unsigned char *px = tiles.row(stage, 0, in_step) + lane * C * sizeof(T), *pg = tiles.row(stage, 1, in_step) + lane * C * sizeof(G);
+      const unsigned char *px = tiles.row(stage, 0, in_step) + 2 * lane * sizeof(T), *pg = tiles.row(stage, 1, in_step) + 2 * lane * sizeof(G);
       if (rows >= R) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          now[r].take(px + r * 32 * C * sizeof(T));
-          g[r].take(pg + r * 32 * C * sizeof(G));
+          now[r].take(px + r * WIDTH * sizeof(T));
+          g[r].take(pg + r * WIDTH * sizeof(G));
         }
       } else {
 #pragma unroll
@@ -348,8 +370,8 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
           now[r].zero();
           g[r].zero();
           if (r < rows) {
-            now[r].take(px + r * 32 * C * sizeof(T));
-            g[r].take(pg + r * 32 * C * sizeof(G));
+            now[r].take(px + r * WIDTH * sizeof(T));
+            g[r].take(pg + r * WIDTH * sizeof(G));
           }
         }
       }
@@ -380,19 +402,19 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
   auto finish = [&](int t, uint64_t h) {
     const int rows = seq.len - t;
     if (!live || rows <= 0) return;
-    if (a.states && (t & (BT - 1)) == 0) store_state(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, h, two);
+    if (a.states && (t & (BT - 1)) == 0) store_state<APART>(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, h, two);
     T* const to = static_cast<T*>(a.h) + (seq.first + t) * a.D + at.channel;
     if (rows >= R) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         h = fma2(decays[r], h, now[r].pair());
-        Piece<T, C>::store(to + (int64_t)r * a.D, h);
+        Piece<T, APART>::store(to + (int64_t)r * a.D, h, two);
       }
     } else {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         h = fma2(decays[r], h, now[r].pair());
-        if (r < rows) Piece<T, C>::store(to + (int64_t)r * a.D, h);
+        if (r < rows) Piece<T, APART>::store(to + (int64_t)r * a.D, h, two);
       }
     }
   };
@@ -401,38 +423,38 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     const uint64_t h = join<W, CLUSTER, false>(exchange, i, warp, at.rank, at.n_ranks, own, s, patience, [&] { next(i); });
     finish(t0, h);
   }
-  if (a.ht && live && knows_the_end<W, CLUSTER, false>(n, warp, at.rank)) store_state(a.ht, (int64_t)at.seq * a.D + at.channel, s, two);
+  if (a.ht && live && knows_the_end<W, CLUSTER, false>(n, warp, at.rank)) store_state<APART>(a.ht, (int64_t)at.seq * a.D + at.channel, s, two);
   if (!patience.ok && lane == 0) atomicExch(&g_recurrence_timeout, 1);
   exchange.leave();
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
 // A CTA's step is one or more chunks, ahead of which the state is known (or, W = 1, the whole of a sequence of up to R).
-template <typename T, typename G, int C, int R, int W, bool CLUSTER, bool TMA>
+template <typename T, typename G, int APART, int R, int W, bool CLUSTER, bool TMA>
 __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     recurrence_bwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_dh,
                           const b200gdn_gated_recurrence_args a) {
   static_assert(W == 1 || (W * R) % BT == 0, "a CTA's step begins where a chunk does");
   constexpr int IN_CHUNK = BT / R;   // warps
-  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * 32 * C * (int)(2 * sizeof(T) + sizeof(G)), CLUSTER);
+  constexpr int ROWS = W * R, STAGES = stages_of(ROWS * WIDTH * (int)(2 * sizeof(T) + sizeof(G)), CLUSTER);
   __shared__ Exchange<W, CLUSTER> exchange;
   __shared__ ulonglong2 left[W > 1 ? 2 : 1][W][32];   // (product of decays, tokens' own state) of the warps, from the left
   __shared__ uint64_t full[STAGES];
   extern __shared__ __align__(128) unsigned char shared_tiles[];
-  const Place at = place_of<C, CLUSTER>(a);
+  const Place at = place_of<APART, CLUSTER>(a);
   const Span seq = span_of(a, at.seq);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, step = at.n_ranks * ROWS;
-  const bool live = at.channel < a.D, two = C == 2;
+  const bool live = at.channel < a.D, two = APART == 1 || at.channel + APART < a.D;
   const int n = (seq.len + step - 1) / step, in_step = warp * R;
   const int last = (n - 1) * step + at.rank * ROWS;   // where this CTA's last (first to be taken) tokens begin
   int t0 = last + in_step;
-  Piece<T, C> x[R], dh[R];
-  Piece<G, C> g[R];
+  Piece<T, APART> x[R], dh[R];
+  Piece<G, APART> g[R];
   Tiles<3, ROWS, STAGES> tiles;
   const CUtensorMap* const maps[3] = {&map_x, &map_g, &map_dh};
   Patience patience;
   uint64_t start = 0ull;
-  auto fetch_start = [&](int t) { start = load_state(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, live && t < seq.len, two); };
+  auto fetch_start = [&](int t) { start = load_state<APART>(a.states, (int64_t)(seq.chunk + t / BT) * a.D + at.channel, live && t < seq.len, two); };
   auto fetch = [&](int t) {
     const T* px = static_cast<const T*>(a.x) + (seq.first + t) * a.stride_x + at.channel;
     const G* pg = static_cast<const G*>(a.g) + (seq.first + t) * a.stride_g + at.channel;
@@ -443,15 +465,15 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
       g[r].zero();
       dh[r].zero();
       if (live && t + r < seq.len) {
-        x[r].load(px);
-        g[r].load(pg);
-        if (a.dh) dh[r].load(pd);
+        x[r].load(px, two);
+        g[r].load(pg, two);
+        if (a.dh) dh[r].load(pd, two);
       }
     }
   };
   exchange.init();
   if constexpr (TMA) {
-    const int row_bytes[3] = {32 * C * (int)sizeof(T), 32 * C * (int)sizeof(G), 32 * C * (int)sizeof(T)};
+    const int row_bytes[3] = {WIDTH * (int)sizeof(T), WIDTH * (int)sizeof(G), WIDTH * (int)sizeof(T)};
     tiles.init(shared_tiles, full, row_bytes);
     if (threadIdx.x == 0)
       for (int i = 0; i < STAGES && i < n; ++i) tiles.load(i, maps, at.tile, (int)seq.first + last - i * step);
@@ -459,25 +481,25 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     fetch(t0);
   }
   if (n > 0) fetch_start(t0);
-  uint64_t s = load_state(a.dht, (int64_t)at.seq * a.D + at.channel, live, two);
+  uint64_t s = load_state<APART>(a.dht, (int64_t)at.seq * a.D + at.channel, live, two);
   int stage = 0;
   uint32_t phase = 0;
   for (int i = 0; i < n; ++i, t0 -= step) {
     uint64_t decays[R], kept[R];
-    Piece<T, C> up[R];
+    Piece<T, APART> up[R];
     uint64_t h = start, own_left = 0ull;
     Joined own = {pack2(1.f, 1.f), 0ull};
     const int rows = seq.len - t0;
     if constexpr (TMA) {
       patience.wait(&full[stage], phase);
-      const unsigned char *px = tiles.row(stage, 0, in_step) + lane * C * sizeof(T), *pg = tiles.row(stage, 1, in_step) + lane * C * sizeof(G),
-                          *pd = tiles.row(stage, 2, in_step) + lane * C * sizeof(T);
+      const unsigned char *px = tiles.row(stage, 0, in_step) + 2 * lane * sizeof(T), *pg = tiles.row(stage, 1, in_step) + 2 * lane * sizeof(G),
+                          *pd = tiles.row(stage, 2, in_step) + 2 * lane * sizeof(T);
       if (rows >= R) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          x[r].take(px + r * 32 * C * sizeof(T));
-          g[r].take(pg + r * 32 * C * sizeof(G));
-          up[r].take(pd + r * 32 * C * sizeof(T));
+          x[r].take(px + r * WIDTH * sizeof(T));
+          g[r].take(pg + r * WIDTH * sizeof(G));
+          up[r].take(pd + r * WIDTH * sizeof(T));
         }
       } else {
 #pragma unroll
@@ -486,9 +508,9 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
           g[r].zero();
           up[r].zero();
           if (r < rows) {
-            x[r].take(px + r * 32 * C * sizeof(T));
-            g[r].take(pg + r * 32 * C * sizeof(G));
-            up[r].take(pd + r * 32 * C * sizeof(T));
+            x[r].take(px + r * WIDTH * sizeof(T));
+            g[r].take(pg + r * WIDTH * sizeof(G));
+            up[r].take(pd + r * WIDTH * sizeof(T));
           }
         }
       }
@@ -544,34 +566,35 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
         const uint64_t d = add2(up[r].pair(), u);
         u = mul2(decays[r], d);
         if (decltype(full)::value || r < rows) {
-          Piece<T, C>::store(to_dx + (int64_t)r * a.D, d);
-          if (a.dg) Piece<G, C>::store(to_dg + (int64_t)r * a.D, mul2(d, kept[r]));
+          Piece<T, APART>::store(to_dx + (int64_t)r * a.D, d, two);
+          if (a.dg) Piece<G, APART>::store(to_dg + (int64_t)r * a.D, mul2(d, kept[r]), two);
         }
       }
     };
     if (rows >= R) finish(std::true_type());
     else finish(std::false_type());
   }
-  if (a.dh0 && live && knows_the_end<W, CLUSTER, true>(n, warp, at.rank)) store_state(a.dh0, (int64_t)at.seq * a.D + at.channel, s, two);
+  if (a.dh0 && live && knows_the_end<W, CLUSTER, true>(n, warp, at.rank)) store_state<APART>(a.dh0, (int64_t)at.seq * a.D + at.channel, s, two);
   if (!patience.ok && lane == 0) atomicExch(&g_recurrence_timeout, 1);
   exchange.leave();
 }
 
 // ---- one token a sequence ------------------------------------------------------------------------------------------------
-template <typename T, typename G, int C>
+template <typename T, typename G, int APART>
 __global__ void __launch_bounds__(128) recurrence_step_kernel(const b200gdn_gated_recurrence_args a) {
-  const int d = (blockIdx.x * 128 + threadIdx.x) * C;
+  const int i = blockIdx.x * 128 + threadIdx.x, d = i / 32 * WIDTH + channel_of<APART>(i & 31);
   if (d >= a.D) return;
+  const bool two = APART == 1 || d + APART < a.D;
   for (int seq = blockIdx.y; seq < a.n_seq; seq += gridDim.y) {
-    Piece<T, C> x;
-    Piece<G, C> g;
-    x.load(static_cast<const T*>(a.x) + (int64_t)seq * a.stride_x + d);
-    g.load(static_cast<const G*>(a.g) + (int64_t)seq * a.stride_g + d);
+    Piece<T, APART> x;
+    Piece<G, APART> g;
+    x.load(static_cast<const T*>(a.x) + (int64_t)seq * a.stride_x + d, two);
+    g.load(static_cast<const G*>(a.g) + (int64_t)seq * a.stride_g + d, two);
     const int64_t at = (int64_t)seq * a.D + d;
-    const uint64_t before = load_state(a.h0, at, true, C == 2), h = fma2(decay(g.gate()), before, x.pair());
-    if (a.states) store_state(a.states, at, before, C == 2);
-    Piece<T, C>::store(static_cast<T*>(a.h) + at, h);
-    if (a.ht) store_state(a.ht, at, h, C == 2);
+    const uint64_t before = load_state<APART>(a.h0, at, true, two), h = fma2(decay(g.gate()), before, x.pair());
+    if (a.states) store_state<APART>(a.states, at, before, two);
+    Piece<T, APART>::store(static_cast<T*>(a.h) + at, h, two);
+    if (a.ht) store_state<APART>(a.ht, at, h, two);
   }
 }
 
@@ -610,8 +633,8 @@ int resident_clusters(cudaLaunchConfig_t cfg, int ranks) {
 // channels, bf16 with fp32 gates: 358 us with 12, 484 with 16, of which 14 clusters are resident where 16 are wanted), in sizes that pack well
 // (8191 x 1003 fp32 backward: 62 us with 8, 89 with 9).
 template <auto KERN, typename... M>
-int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, int C, size_t smem, const M&... maps) {
-  const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C));
+int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, size_t smem, const M&... maps) {
+  const int64_t work = (int64_t)a.n_seq * ((a.D + WIDTH - 1) / WIDTH);
   if (smem > 0)
     if (int e = ensure_smem(KERN, smem)) return e;
   cudaLaunchConfig_t cfg = {};
@@ -647,40 +670,47 @@ constexpr int rows_fwd(bool tma) { return sizeof(T) + sizeof(G) <= (tma ? 6 : 4)
 template <typename T, typename G>
 constexpr int rows_bwd(bool tma) { return tma && sizeof(T) + sizeof(G) == 4 ? 16 : 8; }
 
-template <typename T, typename G, int C, int W, bool CLUSTER, bool TMA>
+template <typename T, typename G, int APART, int W, bool CLUSTER, bool TMA>
 int launch_pass(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, int ranks) {
   constexpr int RB = rows_bwd<T, G>(TMA), RF = rows_fwd<T, G>(TMA);
   CUtensorMap x{}, g{}, dh{};
-  const int rows = W * (bwd ? RB : RF), stage = rows * 32 * C * (int)(sizeof(T) * (bwd ? 2 : 1) + sizeof(G));
+  const int rows = W * (bwd ? RB : RF), stage = rows * WIDTH * (int)(sizeof(T) * (bwd ? 2 : 1) + sizeof(G));
   if (TMA) {
     bind_context();
-    int e = tma::encode_plain_2d(&x, a.x, sizeof(T), a.rows, a.D, a.stride_x, 32 * C, rows);
-    if (e == 0) e = tma::encode_plain_2d(&g, a.g, sizeof(G), a.rows, a.D, a.stride_g, 32 * C, rows);
-    if (e == 0 && bwd) e = tma::encode_plain_2d(&dh, a.dh, sizeof(T), a.rows, a.D, a.D, 32 * C, rows);
+    int e = tma::encode_plain_2d(&x, a.x, sizeof(T), a.rows, a.D, a.stride_x, WIDTH, rows);
+    if (e == 0) e = tma::encode_plain_2d(&g, a.g, sizeof(G), a.rows, a.D, a.stride_g, WIDTH, rows);
+    if (e == 0 && bwd) e = tma::encode_plain_2d(&dh, a.dh, sizeof(T), a.rows, a.D, a.D, WIDTH, rows);
     if (e != 0) return set_error(B200GDN_ERR_CUDA, "gated_recurrence: tensor map (%d)", e);
   }
   const size_t smem = TMA ? (size_t)stage * stages_of(stage, CLUSTER) : 0;
-  return bwd ? launch_walk<recurrence_bwd_kernel<T, G, C, RB, W, CLUSTER, TMA>>("recurrence_bwd", a, st, W, ranks, C, smem, x, g, dh)
-             : launch_walk<recurrence_fwd_kernel<T, G, C, RF, W, CLUSTER, TMA>>("recurrence_fwd", a, st, W, ranks, C, smem, x, g);
+  return bwd ? launch_walk<recurrence_bwd_kernel<T, G, APART, RB, W, CLUSTER, TMA>>("recurrence_bwd", a, st, W, ranks, smem, x, g, dh)
+             : launch_walk<recurrence_fwd_kernel<T, G, APART, RF, W, CLUSTER, TMA>>("recurrence_fwd", a, st, W, ranks, smem, x, g);
 }
 
-template <typename T, typename G, int C>
+template <typename T, typename G, int APART>
 int launch_c(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, bool tiles) {
   if (!bwd && a.seq_len == 1) {
     const int n = a.n_seq < 65535 ? a.n_seq : 65535;
-    recurrence_step_kernel<T, G, C><<<dim3((a.D + 128 * C - 1) / (128 * C), n), 128, 0, st>>>(a);
+    recurrence_step_kernel<T, G, APART><<<dim3((a.D + 255) / 256, n), 128, 0, st>>>(a);
     return check_launch("recurrence_step");
   }
   const int64_t tokens = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT;   // of a sequence, at most
-  if (a.seq_len > 0 && tokens <= (bwd ? rows_bwd<T, G>(false) : rows_fwd<T, G>(false))) return launch_pass<T, G, C, 1, false, false>(a, st, bwd, 1);
-  const int64_t work = (int64_t)a.n_seq * ((a.D + 32 * C - 1) / (32 * C)), most = (tokens + BT - 1) / BT;
-  const bool alone = work > sm_count() || most < 2;
-  if constexpr (C == 2)
-    if (tiles) return alone ? launch_pass<T, G, C, 8, false, true>(a, st, bwd, 1) : launch_pass<T, G, C, 8, true, true>(a, st, bwd, (int)(most < MOST_RANKS ? most : MOST_RANKS));
-  return alone ? launch_pass<T, G, C, 8, false, false>(a, st, bwd, 1) : launch_pass<T, G, C, 8, true, false>(a, st, bwd, (int)(most < MOST_RANKS ? most : MOST_RANKS));
+  if (a.seq_len > 0 && tokens <= (bwd ? rows_bwd<T, G>(false) : rows_fwd<T, G>(false))) return launch_pass<T, G, APART, 1, false, false>(a, st, bwd, 1);
+  // Alone, a CTA takes a sequence's 64 channels; with fewer of these than SMs (forward, where a step costs less than what CTAs tell one another,
+  // than three quarters) clusters share them: 4 x 4096 x 2048 bf16, 128 pieces of work, forward 45 us alone and 51 by twos, backward 106 and 72.
+  const int64_t work = (int64_t)a.n_seq * ((a.D + WIDTH - 1) / WIDTH);
+  auto go = [&](auto tma) {
+    constexpr bool TMA = decltype(tma)::value;
+    const int64_t step = 8 * (bwd ? rows_bwd<T, G>(TMA) : rows_fwd<T, G>(TMA)), steps = (tokens + step - 1) / step;
+    if (steps < 2 || work > (bwd ? 4 : 3) * sm_count() / 4) return launch_pass<T, G, APART, 8, false, TMA>(a, st, bwd, 1);
+    return launch_pass<T, G, APART, 8, true, TMA>(a, st, bwd, (int)(steps < MOST_RANKS ? steps : MOST_RANKS));
+  };
+  if constexpr (APART == 1)
+    if (tiles) return go(std::true_type());
+  return go(std::false_type());
 }
 
-// two channels a thread where every row of every tensor allows it; by TMA where rows are a multiple of 16 bytes on such boundaries
+// two channels in one access where every row of every tensor allows it; by TMA where rows are a multiple of 16 bytes on such boundaries
 template <typename T, typename G>
 int launch_tg(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd) {
   auto bits = [](std::initializer_list<const void*> all) {
@@ -691,7 +721,7 @@ int launch_tg(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd)
   const bool pairs = ((a.D | a.stride_x | a.stride_g) & 1) == 0 && bits({a.x, a.h, a.dh, a.dx}) % (2 * sizeof(T)) == 0 &&
                      bits({a.g, a.dg}) % (2 * sizeof(G)) == 0;
   const bool tiles = (a.D * sizeof(T) | a.stride_x * sizeof(T) | a.stride_g * sizeof(G) | bits({a.x, a.g, a.dh})) % 16 == 0 && (!bwd || a.dh != nullptr);
-  return pairs ? launch_c<T, G, 2>(a, st, bwd, tiles) : launch_c<T, G, 1>(a, st, bwd, false);
+  return pairs ? launch_c<T, G, 1>(a, st, bwd, tiles) : launch_c<T, G, 32>(a, st, bwd, false);
 }
 
 }  // namespace
