@@ -785,7 +785,8 @@ int backward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool r
   const bool wide = fits_tma(a.dy, a.N) && fits_tma(a.z, a.N);
   const int per = wide ? 256 : 32;
   const int64_t columns = (a.N + per - 1) / per;
-  int64_t y = 6 * (int64_t)sm_count() / columns + 1;
+  int64_t y = 3 * (int64_t)sm_count() / columns;   // one round of CTAs
+  if (y < 1) y = 1;
   if (y > (a.rows + 31) / 32) y = (a.rows + 31) / 32;
   float* sums = a.dbias ? static_cast<float*>(space.take(y * a.N * 4)) : nullptr;
   if (run && (apart || a.dbias)) {

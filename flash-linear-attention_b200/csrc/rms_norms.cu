@@ -142,21 +142,33 @@ constexpr int slots_of(int n_tensors, int tpr, int e, int size) {   // 54 KB for
   return room > 4 ? 4 : room < 1 ? 1 : room;
 }
 
-// act(gate) and, where asked for, act'(gate)
-template <bool SLOPE>
-__device__ __forceinline__ uint64_t activation(uint64_t g, uint32_t flags, uint64_t& slope) {
+// act(gate) and, where asked for, act'(gate).  What the gate is (NO_GATE, or AS_IT_IS, SIGMOID, SILU) is known where a row's loop begins: a
+// question asked pair by pair costs a branch each and moves where its ways meet again.
+constexpr uint32_t NO_GATE = ~0u, AS_IT_IS = 0u;
+template <uint32_t ACT, bool SLOPE>
+__device__ __forceinline__ uint64_t activation(uint64_t g, uint64_t& slope) {
   const uint64_t one = pack2(1.f, 1.f);
-  if (!(flags & (SIGMOID | SILU))) {
-    if (SLOPE) slope = one;
+  if constexpr (ACT == AS_IT_IS) {
+    slope = one;
     return g;
+  } else {
+    const uint64_t s = fast_sigmoid2(g);
+    if constexpr (ACT == SIGMOID) {
+      if (SLOPE) slope = fma2(mul2(s, s), pack2(-1.f, -1.f), s);
+      return s;
+    } else {
+      if (SLOPE) slope = mul2(s, fma2(g, fma2(s, pack2(-1.f, -1.f), one), one));
+      return mul2(g, s);
+    }
   }
-  const uint64_t s = fast_sigmoid2(g), ns = mul2(s, pack2(-1.f, -1.f)), rest = add2(one, ns);   // 1 - sigmoid
-  if (flags & SIGMOID) {
-    if (SLOPE) slope = mul2(s, rest);
-    return s;
-  }
-  if (SLOPE) slope = mul2(s, fma2(g, rest, one));
-  return mul2(g, s);
+}
+template <uint32_t V> struct Constant { static constexpr uint32_t value = V; };
+template <typename F>
+__device__ __forceinline__ void with_gate(const b200gdn_rms_norms_args& a, F f) {
+  if (!a.gate) f(Constant<NO_GATE>());
+  else if (a.flags & SIGMOID) f(Constant<SIGMOID>());
+  else if (a.flags & SILU) f(Constant<SILU>());
+  else f(Constant<AS_IT_IS>());
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
@@ -223,14 +235,17 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     }
     uint64_t z[P], sum = 0ull;
     const uint64_t by_r1 = pack2(r1, r1);
+    with_gate(a, [&](auto act) {
+      constexpr uint32_t ACT = decltype(act)::value;
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      uint64_t none, k = mul2(c[i], by_r1);
-      if (a.gate) k = mul2(k, activation<false>(gate.pair(i), a.flags, none));
-      z[i] = fma2(y.pair(i), k, res.pair(i));
-      const uint64_t x = mul2(z[i], by);
-      sum = fma2(x, x, sum);
-    }
+      for (int i = 0; i < P; ++i) {
+        uint64_t none, k = mul2(c[i], by_r1);
+        if constexpr (ACT != NO_GATE) k = mul2(k, activation<ACT, false>(gate.pair(i), none));
+        z[i] = fma2(y.pair(i), k, res.pair(i));
+        const uint64_t x = mul2(z[i], by);
+        sum = fma2(x, x, sum);
+      }
+    });
     if constexpr (!RING) fetch(row + step);
     s[0] = both(sum);
     row_sums<TPR>(s, scratch[turn][1]);
@@ -354,55 +369,61 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     fetch_sums(row + step);
     const uint64_t r1 = pack2(r1f, r1f), r2 = pack2(r2f, r2f);
     uint64_t z[P], sum = 0ull;   // z r2, then f times what dy has of it
+    with_gate(a, [&](auto act) {
+      constexpr uint32_t ACT = decltype(act)::value;
 #pragma unroll
-    for (int v = 0; v < CHUNKS; ++v) {
-      const Chunk y = chunk(at_y, cur.y, v), res = chunk(at_res, cur.res, v), dout = chunk(at_dout, cur.dout, v);
-      Chunk gate;
-      if (a.gate) gate = chunk(at_gate, cur.gate, v);
+      for (int v = 0; v < CHUNKS; ++v) {
+        const Chunk y = chunk(at_y, cur.y, v), res = chunk(at_res, cur.res, v), dout = chunk(at_dout, cur.dout, v);
+        Chunk gate;
+        if constexpr (ACT != NO_GATE) gate = chunk(at_gate, cur.gate, v);
 #pragma unroll
-      for (int q = 0; q < CP; ++q) {
-        const int i = v * CP + q;
-        uint64_t none, k = mul2(c[i], r1);
-        if (a.gate) k = mul2(k, activation<false>(gate.pair(q), a.flags, none));
-        z[i] = mul2(fma2(y.pair(q), k, res.pair(q)), r2);
-        const uint64_t g = dout.pair(q);
-        sum = fma2(mul2(g, w[i]), z[i], sum);
-        dw[i] = fma2(g, z[i], dw[i]);
+        for (int q = 0; q < CP; ++q) {
+          const int i = v * CP + q;
+          uint64_t none, k = mul2(c[i], r1);
+          if constexpr (ACT != NO_GATE) k = mul2(k, activation<ACT, false>(gate.pair(q), none));
+          z[i] = mul2(fma2(y.pair(q), k, res.pair(q)), r2);
+          const uint64_t g = dout.pair(q);
+          sum = fma2(mul2(g, w[i]), z[i], sum);
+          dw[i] = fma2(g, z[i], dw[i]);
+        }
       }
-    }
+    });
     float s[1] = {both(sum)};
     row_sums<TPR>(s, scratch[turn][0]);
     const uint64_t back = pack2(-s[0] * inv, -s[0] * inv);
     sum = 0ull;
+    with_gate(a, [&](auto act) {
+      constexpr uint32_t ACT = decltype(act)::value;
 #pragma unroll
-    for (int v = 0; v < CHUNKS; ++v) {
-      const Chunk y = chunk(at_y, cur.y, v), dout = chunk(at_dout, cur.dout, v), dz = chunk(at_dz, cur.dz, v);
-      Chunk gate, dgate, dres;
-      if (a.gate) gate = chunk(at_gate, cur.gate, v);
+      for (int v = 0; v < CHUNKS; ++v) {
+        const Chunk y = chunk(at_y, cur.y, v), dout = chunk(at_dout, cur.dout, v), dz = chunk(at_dz, cur.dz, v);
+        Chunk gate, dgate, dres;
+        if constexpr (ACT != NO_GATE) gate = chunk(at_gate, cur.gate, v);
 #pragma unroll
-      for (int q = 0; q < CP; ++q) {
-        const int i = v * CP + q;
-        const uint64_t h = fma2(z[i], back, mul2(dout.pair(q), w[i]));
-        const uint64_t e = fma2(h, r2, dz.pair(q)), n1 = mul2(y.pair(q), r1), ec = mul2(e, c[i]);
-        dres.set(q, e);
-        if (a.gate) {
-          uint64_t slope;
-          const uint64_t act = activation<true>(gate.pair(q), a.flags, slope);
-          if (a.dgate) dgate.set(q, mul2(mul2(ec, n1), slope));
-          dt[i] = fma2(mul2(e, act), n1, dt[i]);
-          z[i] = mul2(ec, act);
-        } else {
-          dt[i] = fma2(e, n1, dt[i]);
-          z[i] = ec;
+        for (int q = 0; q < CP; ++q) {
+          const int i = v * CP + q;
+          const uint64_t h = fma2(z[i], back, mul2(dout.pair(q), w[i]));
+          const uint64_t e = fma2(h, r2, dz.pair(q)), n1 = mul2(y.pair(q), r1), ec = mul2(e, c[i]);
+          dres.set(q, e);
+          if constexpr (ACT != NO_GATE) {
+            uint64_t slope;
+            const uint64_t act = activation<ACT, true>(gate.pair(q), slope);
+            dgate.set(q, ACT == AS_IT_IS ? mul2(ec, n1) : mul2(mul2(ec, n1), slope));
+            dt[i] = fma2(mul2(e, act), n1, dt[i]);
+            z[i] = mul2(ec, act);
+          } else {
+            dt[i] = fma2(e, n1, dt[i]);
+            z[i] = ec;
+          }
+          sum = fma2(z[i], n1, sum);
         }
-        sum = fma2(z[i], n1, sum);
+        if (live) {
+          const int64_t to = row * a.D + v * TPR * CHUNK;
+          if (ACT != NO_GATE && a.dgate) dgate.store(static_cast<T*>(a.dgate) + to, sub, a.D - v * TPR * CHUNK);
+          if (a.dresidual) dres.store(static_cast<T*>(a.dresidual) + to, sub, a.D - v * TPR * CHUNK);
+        }
       }
-      if (live) {
-        const int64_t to = row * a.D + v * TPR * CHUNK;
-        if (a.dgate) dgate.store(static_cast<T*>(a.dgate) + to, sub, a.D - v * TPR * CHUNK);
-        if (a.dresidual) dres.store(static_cast<T*>(a.dresidual) + to, sub, a.D - v * TPR * CHUNK);
-      }
-    }
+    });
     uint64_t mean = 0ull;
     Row y;   // the row as it was, before its place in the ring is filled again
 #pragma unroll
@@ -503,12 +524,14 @@ struct Element {   // of column d: what the passes over a wide row form again ea
     w1 = (a.flags & POST) && a.post_weight ? ld_param(a.post_weight, d, a.param_dtype) : 1.f;
     p = y * r1 * w1;
     act = slope = 1.f;
-    if (a.gate) {
-      const float g = Io<T>::ld(a.gate, row + d);
-      uint64_t s;
-      act = unpack2(activation<true>(pack2(g, 0.f), a.flags, s)).x;
-      slope = unpack2(s).x;
-    }
+    with_gate(a, [&](auto which) {
+      constexpr uint32_t ACT = decltype(which)::value;
+      if constexpr (ACT != NO_GATE) {
+        uint64_t s;
+        act = unpack2(activation<ACT, true>(pack2(Io<T>::ld(a.gate, row + d), 0.f), s)).x;
+        slope = unpack2(s).x;
+      }
+    });
     z = fmaf(p, c * act, a.residual ? Io<T>::ld(a.residual, row + d) : 0.f);
   }
 };
