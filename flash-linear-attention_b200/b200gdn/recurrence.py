@@ -33,7 +33,7 @@ def gated_recurrence(
 
     x, g ``[B,T,D]`` in bf16, fp16 or fp32 (``B == 1`` with ``cu_seqlens [N+1]``, whose sequences lie one behind the other); slices of a
     wider projection are read where they lie.  g is the logarithm of a decay, as the mixers' gates are: 0 keeps, minus infinity forgets.
-    (Above 0 a state grows; products of ``exp(g)`` over up to 1024 neighbouring tokens must stay within fp32's range then.)  A g that has
+    (Above 0 a state grows; products of ``exp(g)`` over up to 2048 neighbouring tokens must stay within fp32's range then.)  A g that has
     neither the type of x nor fp32 is cast to fp32.
 
     ``initial_state [N,D]`` (zeros where absent) and ``final_state [N,D]`` in fp32; everything in between is held in fp32 too, and
@@ -43,6 +43,8 @@ def gated_recurrence(
     """
     if not x.is_cuda:
         raise _lib.B200GDNError('gated_recurrence runs on a CUDA device only (no CPU path)')
+    if x.dim() != 3:
+        raise _lib.B200GDNError(f'gated_recurrence: x is [batch, tokens, channels], got {tuple(x.shape)}')
     if cu_seqlens is not None and x.shape[0] != 1:
         raise ValueError(f"The batch size is expected to be 1 rather than {x.shape[0]} when using `cu_seqlens`.")
     if inplace_state and not output_final_state:

@@ -236,6 +236,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync();
   tc5::fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  wait_for_predecessor();   // nothing global is touched before
   const int n_tiles = p.whole + (p.tiles_i * p.tiles_j - p.whole) * p.splits, first = blockIdx.x >> 1, by = gridDim.x >> 1;
   bool ok = true;
   if (warp == EPILOGUE) {
@@ -447,9 +448,9 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const Product p) {
 // ---- few tokens, forward -----------------------------------------------------------------------------------------------------
 // 16 features a CTA, whose warps share the contraction 256 at a time.  What bounds it is W's bytes, so what counts is loads on their way and
 // little else: a lane loads 16 bytes of a row of W, and of x, straight into the registers of mma.sync's operands (which contraction index goes
-// where does not matter as long as it is the same in both), 8 steps of 32 at once; nothing is converted or staged.  tcgen05 would need the
+// where does not matter as long as it is the same in both), four steps of 32 at once; nothing is converted or staged.  tcgen05 would need the
 // bytes to pass through shared memory and a split contraction to occupy every SM.
-constexpr int FEW_STEPS = 8, FEW_WARPS = 16;
+constexpr int FEW_STEPS = 4, FEW_WARPS = 16;
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
@@ -477,12 +478,13 @@ __device__ __forceinline__ uint4 eight(const uint16_t* row, int k, int K, bool t
   return u;
 }
 template <typename T, int NT, bool WIDE>   // up to 8 NT tokens
-__global__ void __launch_bounds__(FEW_WARPS * 32) linear_few_kernel(const Product p, const uint16_t* x, const uint16_t* w, int K) {
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) linear_few_kernel(const Product p, const uint16_t* x, const uint16_t* w, int K) {
   __shared__ float sums[FEW_WARPS][16][8 * NT];
-  constexpr int S = NT > 1 ? FEW_STEPS / 2 : FEW_STEPS;   // steps on their way at once
+  constexpr int S = NT > 1 ? FEW_STEPS / 2 : FEW_STEPS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3, f0 = blockIdx.x * 16;
   const int n_tokens = (int)p.tokens;
   const uint16_t* rows[2] = {w + (int64_t)(f0 + g) * K, w + (int64_t)(f0 + g + 8) * K};
+  wait_for_predecessor();
   float acc[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
@@ -537,8 +539,16 @@ struct Copies {
 __global__ void __launch_bounds__(128) linear_pad_kernel(const Copies c) {
   const int o = blockIdx.z, at = (blockIdx.x * 128 + threadIdx.x) * 8, cols = c.cols[o];
   if (at >= cols) return;
-  for (int64_t r = blockIdx.y; r < c.rows[o]; r += gridDim.y)
-    *reinterpret_cast<uint4*>(c.dst[o] + r * c.pitch[o] + at) = eight<false>(c.src[o] + r * cols, at, cols, true);
+  constexpr int U = 4;   // rows on their way at once
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // (these wait for the whole of it before they touch anything)
+  for (int64_t r0 = (int64_t)blockIdx.y * U; r0 < c.rows[o]; r0 += (int64_t)gridDim.y * U) {
+    uint4 u[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) u[i] = eight<false>(c.src[o] + (r0 + i) * cols, at, cols, r0 + i < c.rows[o]);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (r0 + i < c.rows[o]) *reinterpret_cast<uint4*>(c.dst[o] + (r0 + i) * c.pitch[o] + at) = u[i];
+  }
 }
 
 // act'(z) of a pair
@@ -557,14 +567,14 @@ __device__ __forceinline__ uint64_t slope2(uint64_t z, int act) {
 template <typename T, int E>
 __global__ void __launch_bounds__(256, 3) linear_dz_kernel(const T* dy, const T* z, T* dz, float* sums, int64_t rows, int cols, int pitch, int act) {
   constexpr int P = (E + 1) / 2, U = 4;
-  using Raw = std::conditional_t<E == 8, uint4, uint16_t>;
+  using Raw = std::conditional_t<E == 8, uint4, std::conditional_t<E == 2, uint32_t, uint16_t>>;
   __shared__ float part[8][32 * E];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = (blockIdx.x * 32 + lane) * E;
   uint64_t total[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) total[i] = 0ull;
   auto pair = [](const Raw& u, int i) {
-    if constexpr (E == 8) return widen2<T>(reinterpret_cast<const uint32_t*>(&u)[i]);
+    if constexpr (E > 1) return widen2<T>(reinterpret_cast<const uint32_t*>(&u)[i]);
     else return pack2((float)*reinterpret_cast<const T*>(&u), 0.f);
   };
   if (c < cols) {
@@ -587,7 +597,7 @@ __global__ void __launch_bounds__(256, 3) linear_dz_kernel(const T* dy, const T*
           uint64_t g = pair(d[u], i);
           if (act != NONE) g = mul2(g, slope2(pair(v[u], i), act));
           total[i] = add2(total[i], g);   // (a row past the end adds zeros)
-          if constexpr (E == 8) reinterpret_cast<uint32_t*>(&out)[i] = narrow2<T>(g);
+          if constexpr (E > 1) reinterpret_cast<uint32_t*>(&out)[i] = narrow2<T>(g);
           else *reinterpret_cast<T*>(&out) = static_cast<T>(unpack2(g).x);
         }
         if (dz && r0 + u * step < rows) *reinterpret_cast<Raw*>(dz + (r0 + u * step) * pitch + c) = out;
@@ -668,10 +678,11 @@ int launch_tiles(const Operand& a, const Operand& b, Product p, cudaStream_t st)
   p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) | ((uint32_t)(BN >> 3) << 17) | ((256u >> 4) << 24);
   auto kern = linear_kernel<T, BN, A_MN, B_MN, SWAPPED>;
   if (int e = ensure_smem(kern, smem_of(BN))) return e;
+  // With one round of tiles a good part of the time is the launch, barriers and tensor memory: that begins while the kernel ahead finishes.
   const int rest = p.tiles_i * p.tiles_j - p.whole;   // (checked to be within an int)
   const int64_t tiles = p.whole + (int64_t)rest * p.splits;
   const int pairs = (int)(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
-  kern<<<2 * pairs, THREADS, smem_of(BN), st>>>(ma, mb, p);
+  launch_overlapped(tiles <= pairs, kern, dim3(2 * pairs), THREADS, smem_of(BN), st, ma, mb, p);
   if (int e = check_launch("linear")) return e;
   if (rest == 0) return 0;
   launch_overlapped(true, linear_join_kernel<T, BN, SWAPPED>, dim3(256 * BN / 1024, rest), 256, 0, st, p);
@@ -737,6 +748,7 @@ int operands_of(Operand& a, Operand& b, Space& space, cudaStream_t st, bool run)
   }
   if (n == 0 || !run) return 0;
   const int64_t most = 16 * (int64_t)sm_count() / x + 1;
+  y = (y + 3) / 4;
   linear_pad_kernel<<<dim3((unsigned)x, (unsigned)(y < most ? y : most), n), 128, 0, st>>>(c);
   return check_launch("linear_pad");
 }
@@ -754,9 +766,11 @@ int forward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool ru
     p.tokens = a.rows;
     p.features = a.N;
     // sixteen warps a CTA where features are few and the contraction long, else eight
-    const int grid = (a.N + 15) / 16, warps = grid < 2 * sm_count() && a.K > 8 * FEW_STEPS * 32 ? 16 : 8;
+    const int grid = (a.N + 15) / 16, warps = grid < 2 * sm_count() && a.K > 2048 ? 16 : 8;
     const bool wide = fits_tma(a.x, a.K) && fits_tma(a.weight, a.K);
-    auto go = [&](auto kern) { kern<<<grid, warps * 32, 0, st>>>(p, static_cast<const uint16_t*>(a.x), static_cast<const uint16_t*>(a.weight), a.K); };
+    auto go = [&](auto kern) {
+      launch_overlapped(true, kern, dim3(grid), warps * 32, 0, st, p, static_cast<const uint16_t*>(a.x), static_cast<const uint16_t*>(a.weight), a.K);
+    };
     if (a.rows <= 8) wide ? go(linear_few_kernel<T, 1, true>) : go(linear_few_kernel<T, 1, false>);
     else wide ? go(linear_few_kernel<T, 2, true>) : go(linear_few_kernel<T, 2, false>);
     return check_launch("linear_few");
@@ -782,8 +796,9 @@ int backward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool r
     made = static_cast<T*>(space.take(a.rows * dz.pitch * 2));
     dz.base = made;
   }
-  const bool wide = fits_tma(a.dy, a.N) && fits_tma(a.z, a.N);
-  const int per = wide ? 256 : 32;
+  // columns of a thread: 16 bytes of them, two, or one, as width and boundaries allow
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.z) | (uintptr_t)a.N * 2;
+  const int each = bits % 16 == 0 ? 8 : bits % 4 == 0 ? 2 : 1, per = 32 * each;
   const int64_t columns = (a.N + per - 1) / per;
   int64_t y = 3 * (int64_t)sm_count() / columns;   // one round of CTAs
   if (y < 1) y = 1;
@@ -794,7 +809,7 @@ int backward(const b200gdn_linear_args& a, Space& space, cudaStream_t st, bool r
       kern<<<dim3((unsigned)columns, (unsigned)y), 256, 0, st>>>(static_cast<const T*>(a.dy), static_cast<const T*>(a.z), made, sums, a.rows, a.N, (int)dz.pitch,
                                                           a.activation);
     };
-    wide ? go(linear_dz_kernel<T, 8>) : go(linear_dz_kernel<T, 1>);
+    each == 8 ? go(linear_dz_kernel<T, 8>) : each == 2 ? go(linear_dz_kernel<T, 2>) : go(linear_dz_kernel<T, 1>);
     if (int e = check_launch("linear_dz")) return e;
     if (a.dbias) {
       launch_overlapped(true, linear_dbias_kernel<T>, dim3((a.N + 255) / 256), 256, 0, st, (const float*)sums, static_cast<T*>(a.dbias), a.N, (int)y);
