@@ -301,7 +301,7 @@ struct Tiles {
 };
 constexpr int stages_of(int stage_bytes, bool cluster) {   // two CTAs an SM
   const int room = (cluster ? 76 : 95) * 1024 / stage_bytes;
-  return room > 4 ? 4 : room < 1 ? 1 : room;
+  return room >= 2 ? 2 : 1;   // (four are no faster)
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------

@@ -8,8 +8,8 @@
 // HBM streaming, in the manner of layer_norm.cu: the threads of a group share a row, E elements each, which are worked on as E / 2 fp32 pairs;
 // groups walk the rows, so that a thread's columns stay its own: parameters are read once, their gradients are sums in registers, which a
 // second kernel joins in a fixed order.  The second norm needs what the first one gives: two barriers a row, forward as well as backward.
-// Rows of a multiple of 16 bytes come by bulk copies into a ring of shared memory, two to four rows ahead; of other rows the next one is
-// on its way to registers.
+// Rows of a multiple of 16 bytes come by bulk copies into a ring of shared memory, two rows ahead; of other rows the next one is on its way
+// to registers.
 #include "gdn_common.cuh"
 #include "row_pieces.cuh"
 #include "tc5.cuh"
@@ -137,9 +137,10 @@ struct Ring {
     }
   }
 };
-constexpr int slots_of(int n_tensors, int tpr, int e, int size) {   // 54 KB for 128 threads
-  const int room = 54 * 1024 * threads_of(tpr) / 128 / (threads_of(tpr) / tpr) / (n_tensors * tpr * e * size);
-  return room > 4 ? 4 : room < 1 ? 1 : room;
+// Two rows are enough, and more are worse: reads run so far ahead of the writes that memory changes between them more often (65536 x 4096 bf16
+// forward: 330 us with two, 373 with three or four).
+constexpr int slots_of(int n_tensors, int tpr, int e, int size) {   // of 54 KB for 128 threads
+  return 54 * 1024 * threads_of(tpr) / 128 / (threads_of(tpr) / tpr) / (n_tensors * tpr * e * size) > 1 ? 2 : 1;
 }
 
 // act(gate) and, where asked for, act'(gate).  What the gate is (NO_GATE, or AS_IT_IS, SIGMOID, SILU) is known where a row's loop begins: a
@@ -163,16 +164,18 @@ __device__ __forceinline__ uint64_t activation(uint64_t g, uint64_t& slope) {
   }
 }
 template <uint32_t V> struct Constant { static constexpr uint32_t value = V; };
-template <typename F>
+enum Gates { WITHOUT, WITH, EITHER };   // of a kernel: large ones that need not look are a twentieth faster
+template <Gates GATE, typename F>
 __device__ __forceinline__ void with_gate(const b200gdn_rms_norms_args& a, F f) {
-  if (!a.gate) f(Constant<NO_GATE>());
+  if (GATE == WITHOUT || (GATE == EITHER && !a.gate)) f(Constant<NO_GATE>());
+  else if constexpr (GATE == WITHOUT) return;
   else if (a.flags & SIGMOID) f(Constant<SIGMOID>());
   else if (a.flags & SILU) f(Constant<SILU>());
   else f(Constant<AS_IT_IS>());
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
-template <typename T, int N, int TPR, int E, bool RING>
+template <typename T, int N, int TPR, int E, bool RING, Gates GATE>
 __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_norms_fwd_kernel(const b200gdn_rms_norms_args a) {
   using Row = Part<T, N, TPR, E>;
   constexpr int RPC = threads_of(TPR) / TPR, NW = TPR > 32 ? TPR / 32 : 1, P = E / 2, SLOTS = RING ? slots_of(3, TPR, E, sizeof(T)) : 1;
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
   const uint64_t by = pack2(down, down);
   const int64_t step = (int64_t)gridDim.x * RPC;
   int64_t row = (int64_t)blockIdx.x * RPC + group;
-  const int row_bytes = a.D * (int)sizeof(T), n_tensors = 1 + (a.residual != nullptr) + (a.gate != nullptr);
+  const int row_bytes = a.D * (int)sizeof(T), n_tensors = 1 + (a.residual != nullptr) + (GATE != WITHOUT && a.gate != nullptr);
   const void* tensors[3] = {a.y, a.residual ? a.residual : a.gate, a.gate};
   Ring<SLOTS> ring{ring_bytes + group * SLOTS * n_tensors * row_bytes, full + group * SLOTS};
   Row y, res, gate;
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     if (row >= a.rows) return;
     y.load(static_cast<const T*>(a.y) + row * a.D, sub, a.D);
     if (a.residual) res.load(static_cast<const T*>(a.residual) + row * a.D, sub, a.D);
-    if (a.gate) gate.load(static_cast<const T*>(a.gate) + row * a.D, sub, a.D);
+    if (GATE != WITHOUT && a.gate) gate.load(static_cast<const T*>(a.gate) + row * a.D, sub, a.D);
   };
   if constexpr (RING) {
     if (sub == 0) {
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
       y.load(at, sub, a.D);
       if (a.residual) res.load(at += a.D, sub, a.D);
       else res.zero();
-      if (a.gate) gate.load(at += a.D, sub, a.D);
+      if (GATE != WITHOUT && a.gate) gate.load(at += a.D, sub, a.D);
     }
     float s[1] = {0.f}, r1 = 1.f;
     if (post) {
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     }
     uint64_t z[P], sum = 0ull;
     const uint64_t by_r1 = pack2(r1, r1);
-    with_gate(a, [&](auto act) {
+    with_gate<GATE>(a, [&](auto act) {
       constexpr uint32_t ACT = decltype(act)::value;
 #pragma unroll
       for (int i = 0; i < P; ++i) {
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
-template <typename T, int N, int TPR, int E, bool RING>
+template <typename T, int N, int TPR, int E, bool RING, Gates GATE>
 __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_norms_bwd_kernel(const b200gdn_rms_norms_args a) {
   using Row = Part<T, N, TPR, E>;
   constexpr int RPC = threads_of(TPR) / TPR, NW = TPR > 32 ? TPR / 32 : 1, P = E / 2, SLOTS = RING ? slots_of(5, TPR, E, sizeof(T)) : 1;
@@ -309,7 +312,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     if (row >= a.rows) return;
     to.y.load(static_cast<const T*>(a.y) + row * a.D, sub, a.D);
     if (a.residual) to.res.load(static_cast<const T*>(a.residual) + row * a.D, sub, a.D);
-    if (a.gate) to.gate.load(static_cast<const T*>(a.gate) + row * a.D, sub, a.D);
+    if (GATE != WITHOUT && a.gate) to.gate.load(static_cast<const T*>(a.gate) + row * a.D, sub, a.D);
     if (a.dout) to.dout.load(static_cast<const T*>(a.dout) + row * a.D, sub, a.D);
     if (a.dz) to.dz.load(static_cast<const T*>(a.dz) + row * a.D, sub, a.D);
   };
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
       const T* at = reinterpret_cast<const T*>(ring.base + ring.slot * n_tensors * row_bytes);
       at_y = at;
       if (a.residual) at_res = at += a.D;
-      if (a.gate) at_gate = at += a.D;
+      if (GATE != WITHOUT && a.gate) at_gate = at += a.D;
       if (a.dout) at_dout = at += a.D;
       if (a.dz) at_dz = at += a.D;
     } else if constexpr (AHEAD) {
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     fetch_sums(row + step);
     const uint64_t r1 = pack2(r1f, r1f), r2 = pack2(r2f, r2f);
     uint64_t z[P], sum = 0ull;   // z r2, then f times what dy has of it
-    with_gate(a, [&](auto act) {
+    with_gate<GATE>(a, [&](auto act) {
       constexpr uint32_t ACT = decltype(act)::value;
 #pragma unroll
       for (int v = 0; v < CHUNKS; ++v) {
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     row_sums<TPR>(s, scratch[turn][0]);
     const uint64_t back = pack2(-s[0] * inv, -s[0] * inv);
     sum = 0ull;
-    with_gate(a, [&](auto act) {
+    with_gate<GATE>(a, [&](auto act) {
       constexpr uint32_t ACT = decltype(act)::value;
 #pragma unroll
       for (int v = 0; v < CHUNKS; ++v) {
@@ -524,7 +527,7 @@ struct Element {   // of column d: what the passes over a wide row form again ea
     w1 = (a.flags & POST) && a.post_weight ? ld_param(a.post_weight, d, a.param_dtype) : 1.f;
     p = y * r1 * w1;
     act = slope = 1.f;
-    with_gate(a, [&](auto which) {
+    with_gate<EITHER>(a, [&](auto which) {
       constexpr uint32_t ACT = decltype(which)::value;
       if constexpr (ACT != NO_GATE) {
         uint64_t s;
@@ -632,22 +635,28 @@ int grid_of(int64_t rows, int each, int per_sm) {   // CTAs that take `each` row
   const int64_t want = (rows + each - 1) / each, most = (int64_t)per_sm * sm_count();
   return (int)(want < most ? want : most);
 }
-template <typename T, int N, int TPR, int E, bool RING>
-int launch_rows(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
-  constexpr int threads = threads_of(TPR), RPC = threads / TPR;
+template <typename T, int N, int TPR, int E, bool RING, bool BWD>
+int launch_rows(const b200gdn_rms_norms_args& a, cudaStream_t st) {
+  constexpr int threads = threads_of(TPR), RPC = threads / TPR, MOST = BWD ? 5 : 3;   // tensors of a row
   const int n = grid_of(a.rows, RPC, 512 / threads);
-  auto go = [&](auto kern, int most) {
+  auto go = [&](auto kern) {
     int tensors = 0;
-    for (const void* p : {a.y, a.residual, a.gate, bwd ? a.dout : nullptr, bwd ? a.dz : nullptr}) tensors += p != nullptr;
-    const size_t smem = RING ? (size_t)RPC * slots_of(most, TPR, E, sizeof(T)) * tensors * a.D * sizeof(T) : 0;
+    for (const void* p : {a.y, a.residual, a.gate, BWD ? a.dout : nullptr, BWD ? a.dz : nullptr}) tensors += p != nullptr;
+    const size_t smem = RING ? (size_t)RPC * slots_of(MOST, TPR, E, sizeof(T)) * tensors * a.D * sizeof(T) : 0;
     if (RING)   // (what a row may take at most: the limit is set once)
-      if (int e = ensure_smem(kern, (size_t)RPC * slots_of(most, TPR, E, sizeof(T)) * most * TPR * E * sizeof(T))) return e;
+      if (int e = ensure_smem(kern, (size_t)RPC * slots_of(MOST, TPR, E, sizeof(T)) * MOST * TPR * E * sizeof(T))) return e;
     kern<<<n, threads, smem, st>>>(a);
-    return check_launch(bwd ? "rms_norms_bwd" : "rms_norms_fwd");
+    return check_launch(BWD ? "rms_norms_bwd" : "rms_norms_fwd");
   };
-  if (!bwd) return go(rms_norms_fwd_kernel<T, N, TPR, E, RING>, 3);
-  if (int e = go(rms_norms_bwd_kernel<T, N, TPR, E, RING>, 5)) return e;
-  return a.partials ? reduce_partials(a, n, st) : 0;
+  auto pass = [&](auto gates) {
+    constexpr Gates GATE = decltype(gates)::value;
+    if constexpr (BWD) return go(rms_norms_bwd_kernel<T, N, TPR, E, RING, GATE>);
+    else return go(rms_norms_fwd_kernel<T, N, TPR, E, RING, GATE>);
+  };
+  int e;
+  if constexpr (RING) e = a.gate ? pass(std::integral_constant<Gates, WITH>()) : pass(std::integral_constant<Gates, WITHOUT>());
+  else e = pass(std::integral_constant<Gates, EITHER>());
+  return e == 0 && BWD && a.partials ? reduce_partials(a, n, st) : e;
 }
 
 template <typename T>
@@ -668,25 +677,26 @@ int launch_wide(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
 }
 
 // Sixteen elements a thread where rows come by the ring, else eight; where that is more threads than a CTA has registers for, sixteen.
-template <typename T, int N>
-int launch_n(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
-  if (a.D <= 64) return launch_rows<T, N, 8, 8, false>(a, st, bwd);
-  if (a.D <= 128) return launch_rows<T, N, 16, 8, false>(a, st, bwd);
-  if (a.D <= 256) return launch_rows<T, N, 32, 8, false>(a, st, bwd);
+// (Backward, sixteen in one warp spill: 16384 x 512 bf16 gated 66 us, 47 with eight in two.)
+template <typename T, int N, bool BWD>
+int launch_n(const b200gdn_rms_norms_args& a, cudaStream_t st) {
+  if (a.D <= 64) return launch_rows<T, N, 8, 8, false, BWD>(a, st);
+  if (a.D <= 128) return launch_rows<T, N, 16, 8, false, BWD>(a, st);
+  if (a.D <= 256) return launch_rows<T, N, 32, 8, false, BWD>(a, st);
   if constexpr (N * sizeof(T) == 16) {
-    if (a.D <= 512) return launch_rows<T, N, 64, 8, true>(a, st, bwd);
-    if (a.D <= 1024) return launch_rows<T, N, 64, 16, true>(a, st, bwd);
-    if (a.D <= 2048) return launch_rows<T, N, 128, 16, true>(a, st, bwd);
-    if (a.D <= 4096) return launch_rows<T, N, 256, 16, true>(a, st, bwd);
-    if (a.D <= 8192) return launch_rows<T, N, 512, 16, true>(a, st, bwd);
+    if (a.D <= 512) return launch_rows<T, N, BWD ? 64 : 32, BWD ? 8 : 16, true, BWD>(a, st);
+    if (a.D <= 1024) return launch_rows<T, N, 64, 16, true, BWD>(a, st);
+    if (a.D <= 2048) return launch_rows<T, N, 128, 16, true, BWD>(a, st);
+    if (a.D <= 4096) return launch_rows<T, N, 256, 16, true, BWD>(a, st);
+    if (a.D <= 8192) return launch_rows<T, N, 512, 16, true, BWD>(a, st);
   } else {
-    if (a.D <= 512) return launch_rows<T, N, 64, 8, false>(a, st, bwd);
-    if (a.D <= 1024) return launch_rows<T, N, 128, 8, false>(a, st, bwd);
-    if (a.D <= 2048) return launch_rows<T, N, 256, 8, false>(a, st, bwd);
-    if (a.D <= 4096) return launch_rows<T, N, 512, 8, false>(a, st, bwd);
-    if (a.D <= 8192) return launch_rows<T, N, 512, 16, false>(a, st, bwd);
+    if (a.D <= 512) return launch_rows<T, N, 64, 8, false, BWD>(a, st);
+    if (a.D <= 1024) return launch_rows<T, N, 128, 8, false, BWD>(a, st);
+    if (a.D <= 2048) return launch_rows<T, N, 256, 8, false, BWD>(a, st);
+    if (a.D <= 4096) return launch_rows<T, N, 512, 8, false, BWD>(a, st);
+    if (a.D <= 8192) return launch_rows<T, N, 512, 16, false, BWD>(a, st);
   }
-  return launch_wide<T>(a, st, bwd);
+  return launch_wide<T>(a, st, BWD);
 }
 
 // 16 bytes of the rows' elements, of 16-bit ones else two, else one: what divides the width and what every tensor that is read or written
@@ -704,13 +714,17 @@ int piece_of(const b200gdn_rms_norms_args& a) {
   return fits(16 / size) ? 16 / size : size == 2 && fits(2) ? 2 : 1;
 }
 
-template <typename T>
-int launch_t(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
+template <typename T, bool BWD>
+int launch_t(const b200gdn_rms_norms_args& a, cudaStream_t st) {
   const int n = piece_of<T>(a);
-  if (n == 16 / sizeof(T)) return launch_n<T, 16 / sizeof(T)>(a, st, bwd);
+  if (n == 16 / sizeof(T)) return launch_n<T, 16 / sizeof(T), BWD>(a, st);
   if constexpr (sizeof(T) == 2)
-    if (n == 2) return launch_n<T, 2>(a, st, bwd);
-  return launch_n<T, 1>(a, st, bwd);
+    if (n == 2) return launch_n<T, 2, BWD>(a, st);
+  return launch_n<T, 1, BWD>(a, st);
+}
+template <bool BWD>
+int launch(const b200gdn_rms_norms_args& a, cudaStream_t st) {
+  return a.dtype == 0 ? launch_t<__nv_bfloat16, BWD>(a, st) : a.dtype == 1 ? launch_t<__half, BWD>(a, st) : launch_t<float, BWD>(a, st);
 }
 
 }  // namespace
@@ -720,7 +734,7 @@ int rms_norms_grid(int64_t rows) { return (int)(rows < 1 ? 1 : rows < most_ctas(
 int64_t rms_norms_partials(int64_t rows, int D) { return (rows + 3) / 4 * 4 + (int64_t)rms_norms_grid(rows) * 2 * D; }
 
 int launch_rms_norms(const b200gdn_rms_norms_args& a, cudaStream_t st, bool bwd) {
-  return a.dtype == 0 ? launch_t<__nv_bfloat16>(a, st, bwd) : a.dtype == 1 ? launch_t<__half>(a, st, bwd) : launch_t<float>(a, st, bwd);
+  return bwd ? launch<true>(a, st) : launch<false>(a, st);
 }
 
 int norms_timeout_flag() {
