@@ -131,7 +131,7 @@ class RmsNormsArgs(C.Structure):
 class GatedRecurrenceArgs(C.Structure):
     _fields_ = [
         ('struct_bytes', C.c_int32), ('D', C.c_int32), ('rows', C.c_int64), ('n_seq', C.c_int32), ('seq_len', C.c_int32), ('n_chunks', C.c_int32),
-        ('dtype', C.c_int32), ('gate_dtype', C.c_int32), ('reserved', C.c_int32), ('stride_x', C.c_int64), ('stride_g', C.c_int64),
+        ('dtype', C.c_int32), ('gate_dtype', C.c_int32), ('longest', C.c_int32), ('stride_x', C.c_int64), ('stride_g', C.c_int64),
         ('chunk_meta', _p), ('seq_meta', _p), ('seq_order', _p), ('x', _p), ('g', _p), ('h0', _p), ('h', _p), ('ht', _p), ('states', _p),
         ('dh', _p), ('dht', _p), ('dx', _p), ('dg', _p), ('dh0', _p),
     ]

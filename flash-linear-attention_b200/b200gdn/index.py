@@ -23,6 +23,7 @@ class Tables(tuple):
     empty_seqs = False   # some sequence has no token (and so no tile)
     stream = 0           # the stream whose memory the tables are
     order = None      # int32 [n_seq]: sequences by falling length, None when all are of one length
+    longest = 0       # chunks of the longest sequence
     _native = None
 
     def native(self):
@@ -60,6 +61,7 @@ def device_tables(bounds, device) -> Tables:
     if out[0].is_cuda:
         out.stream = torch.cuda.current_stream(out[0].device).cuda_stream
     out.empty_seqs = bool((sm[:, 1] == 0).any())
+    out.longest = int(sm[:, 1].max()) if len(sm) else 0
     if len(sm) > 1 and (sm[:, 1] != sm[0, 1]).any():
         out.order = torch.from_numpy(np.argsort(-sm[:, 1], kind='stable').astype(np.int32)).to(device)
     return out

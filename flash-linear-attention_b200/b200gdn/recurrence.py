@@ -16,8 +16,10 @@ from .recorded import RecordedCall, recorded
 
 
 def _native(x, g, initial_state, output_final_state, inplace_state, cu_seqlens, cu_seqlens_cpu):
-    plan = None if cu_seqlens is None else tables_for(x.shape[0], x.shape[1], cu_seqlens, cu_seqlens_cpu, x.device).native()
-    return _lib.host().gated_recurrence(x, g, initial_state, output_final_state, inplace_state, plan)
+    if cu_seqlens is None:
+        return _lib.host().gated_recurrence(x, g, initial_state, output_final_state, inplace_state, None, 0)
+    tables = tables_for(x.shape[0], x.shape[1], cu_seqlens, cu_seqlens_cpu, x.device)
+    return _lib.host().gated_recurrence(x, g, initial_state, output_final_state, inplace_state, tables.native(), tables.longest)
 
 
 def gated_recurrence(

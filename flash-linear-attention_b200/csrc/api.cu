@@ -390,7 +390,7 @@ static int check_gated_recurrence_args(const b200gdn_gated_recurrence_args* a, c
   if (a->struct_bytes != (int32_t)sizeof(b200gdn_gated_recurrence_args))
     return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: struct_bytes %d != %zu (ABI mismatch)", who, a->struct_bytes,
                      sizeof(b200gdn_gated_recurrence_args));
-  if (a->rows <= 0 || a->D <= 0 || a->n_seq <= 0 || a->seq_len < 0 || (a->seq_len == 0 && a->n_chunks < 0))
+  if (a->rows <= 0 || a->D <= 0 || a->n_seq <= 0 || a->seq_len < 0 || (a->seq_len == 0 && (a->n_chunks < 0 || a->longest < 0)))
     return set_error(B200GDN_ERR_BAD_ARGUMENT, "%s: empty problem (rows=%lld D=%d n_seq=%d seq_len=%d n_chunks=%d)", who, (long long)a->rows, a->D,
                      a->n_seq, a->seq_len, a->n_chunks);
   if (a->rows > (1 << 30)) return set_error(B200GDN_ERR_UNSUPPORTED, "%s: more than 2^30 rows", who);

@@ -629,11 +629,11 @@ int resident_clusters(cudaLaunchConfig_t cfg, int ranks) {
   return n;
 }
 
-// `ranks`: the most CTAs a cluster may have.  As many are taken as let every sequence's cluster work at the same time (131072 tokens of 1024
+// `ranks`: the most CTAs a cluster may have.  Unless it is wanted `exactly`, as many are taken as let every sequence's cluster work at once (131072 tokens of 1024
 // channels, bf16 with fp32 gates: 358 us with 12, 484 with 16, of which 14 clusters are resident where 16 are wanted), in sizes that pack well
 // (8191 x 1003 fp32 backward: 62 us with 8, 89 with 9).
 template <auto KERN, typename... M>
-int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, size_t smem, const M&... maps) {
+int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaStream_t st, int W, int ranks, bool exactly, size_t smem, const M&... maps) {
   const int64_t work = (int64_t)a.n_seq * ((a.D + WIDTH - 1) / WIDTH);
   if (smem > 0)
     if (int e = ensure_smem(KERN, smem)) return e;
@@ -652,7 +652,7 @@ int launch_walk(const char* what, const b200gdn_gated_recurrence_args& a, cudaSt
     ranks = 1;
     for (int r : {16, 12, 8, 6, 4, 3, 2}) {
       attr.val.clusterDim.x = r;
-      if (r > most || work * r > 2 * sm_count() || resident_clusters<KERN>(cfg, r) < work) continue;
+      if (r > most || (!exactly && (work * r > 2 * sm_count() || resident_clusters<KERN>(cfg, r) < work))) continue;
       ranks = r;
       break;
     }
@@ -671,7 +671,7 @@ template <typename T, typename G>
 constexpr int rows_bwd(bool tma) { return tma && sizeof(T) + sizeof(G) == 4 ? 16 : 8; }
 
 template <typename T, typename G, int APART, int W, bool CLUSTER, bool TMA>
-int launch_pass(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, int ranks) {
+int launch_pass(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, int ranks, bool exactly) {
   constexpr int RB = rows_bwd<T, G>(TMA), RF = rows_fwd<T, G>(TMA);
   CUtensorMap x{}, g{}, dh{};
   const int rows = W * (bwd ? RB : RF), stage = rows * WIDTH * (int)(sizeof(T) * (bwd ? 2 : 1) + sizeof(G));
@@ -683,8 +683,8 @@ int launch_pass(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bw
     if (e != 0) return set_error(B200GDN_ERR_CUDA, "gated_recurrence: tensor map (%d)", e);
   }
   const size_t smem = TMA ? (size_t)stage * stages_of(stage, CLUSTER) : 0;
-  return bwd ? launch_walk<recurrence_bwd_kernel<T, G, APART, RB, W, CLUSTER, TMA>>("recurrence_bwd", a, st, W, ranks, smem, x, g, dh)
-             : launch_walk<recurrence_fwd_kernel<T, G, APART, RF, W, CLUSTER, TMA>>("recurrence_fwd", a, st, W, ranks, smem, x, g);
+  return bwd ? launch_walk<recurrence_bwd_kernel<T, G, APART, RB, W, CLUSTER, TMA>>("recurrence_bwd", a, st, W, ranks, exactly, smem, x, g, dh)
+             : launch_walk<recurrence_fwd_kernel<T, G, APART, RF, W, CLUSTER, TMA>>("recurrence_fwd", a, st, W, ranks, exactly, smem, x, g);
 }
 
 template <typename T, typename G, int APART>
@@ -694,16 +694,20 @@ int launch_c(const b200gdn_gated_recurrence_args& a, cudaStream_t st, bool bwd, 
     recurrence_step_kernel<T, G, APART><<<dim3((a.D + 255) / 256, n), 128, 0, st>>>(a);
     return check_launch("recurrence_step");
   }
-  const int64_t tokens = a.seq_len > 0 ? a.seq_len : (int64_t)a.n_chunks * BT;   // of a sequence, at most
-  if (a.seq_len > 0 && tokens <= (bwd ? rows_bwd<T, G>(false) : rows_fwd<T, G>(false))) return launch_pass<T, G, APART, 1, false, false>(a, st, bwd, 1);
+  const int64_t tokens = a.seq_len > 0 ? a.seq_len : (int64_t)(a.longest > 0 ? a.longest : a.n_chunks) * BT;   // of a sequence, at most
+  if (a.seq_len > 0 && tokens <= (bwd ? rows_bwd<T, G>(false) : rows_fwd<T, G>(false))) return launch_pass<T, G, APART, 1, false, false>(a, st, bwd, 1, false);
   // Alone, a CTA takes a sequence's 64 channels; with fewer of these than SMs (forward, where a step costs less than what CTAs tell one another,
   // than three quarters) clusters share them: 4 x 4096 x 2048 bf16, 128 pieces of work, forward 45 us alone and 51 by twos, backward 106 and 72.
   const int64_t work = (int64_t)a.n_seq * ((a.D + WIDTH - 1) / WIDTH);
   auto go = [&](auto tma) {
     constexpr bool TMA = decltype(tma)::value;
     const int64_t step = 8 * (bwd ? rows_bwd<T, G>(TMA) : rows_fwd<T, G>(TMA)), steps = (tokens + step - 1) / step;
-    if (steps < 2 || work > (bwd ? 4 : 3) * sm_count() / 4) return launch_pass<T, G, APART, 8, false, TMA>(a, st, bwd, 1);
-    return launch_pass<T, G, APART, 8, true, TMA>(a, st, bwd, (int)(steps < MOST_RANKS ? steps : MOST_RANKS));
+    // packed: as many CTAs a cluster as leave the longest sequence no more steps than all SMs take for all of them
+    const int64_t all = (int64_t)a.n_chunks * BT / step * (work / a.n_seq) + 1, wanted = a.longest > 0 ? steps * 2 * sm_count() / all : 0;
+    if (steps < 2 || (wanted < 2 && work > (bwd ? 4 : 3) * sm_count() / 4)) return launch_pass<T, G, APART, 8, false, TMA>(a, st, bwd, 1, false);
+    const bool enough = wanted > 1 && work > sm_count() / 2;
+    const int64_t most = enough ? (wanted < 8 ? wanted : 8) : MOST_RANKS;
+    return launch_pass<T, G, APART, 8, true, TMA>(a, st, bwd, (int)(steps < most ? steps : most), enough);
   };
   if constexpr (APART == 1)
     if (tiles) return go(std::true_type());

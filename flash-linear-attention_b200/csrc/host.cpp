@@ -925,6 +925,7 @@ class LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
 // ---- gated recurrence ------------------------------------------------------------------------------------------
 struct RecurrenceSaved : torch::CustomClassHolder {
   PlanPtr plan;   // null: sequences of one length
+  int64_t longest = 0;
   bool has_h0 = false, want_x = false, want_g = false, want_h0 = false;
   at::ScalarType gt = at::kFloat, ht = at::kFloat;
 };
@@ -943,13 +944,14 @@ Tensor token_rows(const Tensor& x, int64_t& stride) {
   return x.contiguous();
 }
 
-b200gdn_gated_recurrence_args recurrence_args(const Tensor& x, const Tensor& g, int64_t n_seq, const Plan* plan) {
+b200gdn_gated_recurrence_args recurrence_args(const Tensor& x, const Tensor& g, int64_t n_seq, const Plan* plan, int64_t longest) {
   b200gdn_gated_recurrence_args a{};
   a.D = (int32_t)x.size(2);
   a.rows = x.size(0) * x.size(1);
   a.n_seq = (int32_t)n_seq;
   if (plan) {
     a.n_chunks = plan->n_chunks;
+    a.longest = (int32_t)longest;
     a.chunk_meta = iptr(plan->chunk_meta);
     a.seq_meta = iptr(plan->seq_meta);
     a.seq_order = iptr(plan->seq_order);
@@ -967,7 +969,7 @@ b200gdn_gated_recurrence_args recurrence_args(const Tensor& x, const Tensor& g, 
 }
 
 RecurrenceForward recurrence_forward(const Tensor& x_in, const Tensor& g_in, const Tensor& initial_state, bool output_final_state, bool inplace_state,
-                                     const PlanPtr& plan, bool need_grad) {
+                                     const PlanPtr& plan, int64_t longest, bool need_grad) {
   RecurrenceForward r;
   const at::Device dev = x_in.device();
   c10::cuda::CUDAGuard guard(dev);
@@ -996,7 +998,7 @@ RecurrenceForward recurrence_forward(const Tensor& x_in, const Tensor& g_in, con
     }
     return r;
   }
-  b200gdn_gated_recurrence_args a = recurrence_args(r.x, r.g, n_seq, plan.get());
+  b200gdn_gated_recurrence_args a = recurrence_args(r.x, r.g, n_seq, plan.get(), longest);
   a.h0 = fptr(h0);
   a.h = ptr(r.h);
   a.ht = fptr(r.final_state);
@@ -1009,11 +1011,12 @@ RecurrenceForward recurrence_forward(const Tensor& x_in, const Tensor& g_in, con
 class RecurrenceFunction : public torch::autograd::Function<RecurrenceFunction> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const std::optional<Tensor>& initial_state,
-                               bool output_final_state, const PlanPtr& plan) {
+                               bool output_final_state, const PlanPtr& plan, int64_t longest) {
     const Tensor h0 = val(initial_state);
-    RecurrenceForward r = recurrence_forward(x, g, h0, output_final_state, false, plan, true);
+    RecurrenceForward r = recurrence_forward(x, g, h0, output_final_state, false, plan, longest, true);
     auto s = c10::make_intrusive<RecurrenceSaved>();
     s->plan = plan;
+    s->longest = longest;
     s->has_h0 = h0.defined();
     s->want_x = x.requires_grad();
     s->want_g = g.requires_grad();
@@ -1048,7 +1051,7 @@ class RecurrenceFunction : public torch::autograd::Function<RecurrenceFunction> 
         else dh0.zero_();
       }
     } else {
-      b200gdn_gated_recurrence_args a = recurrence_args(x, g, n_seq, s.plan.get());
+      b200gdn_gated_recurrence_args a = recurrence_args(x, g, n_seq, s.plan.get(), s.longest);
       a.states = fptr(states);
       a.dh = ptr(dh);
       a.dht = fptr(dht);
@@ -1058,7 +1061,7 @@ class RecurrenceFunction : public torch::autograd::Function<RecurrenceFunction> 
       if (s.plan) in_use(s.plan);
       call("b200gdn_gated_recurrence_bwd", b200gdn_gated_recurrence_bwd, a);
     }
-    return once("gated_recurrence", {s.want_x ? dx : Tensor(), cast(dg, s.gt), dh0.defined() ? cast(dh0, s.ht) : Tensor(), Tensor(), Tensor()});
+    return once("gated_recurrence", {s.want_x ? dx : Tensor(), cast(dg, s.gt), dh0.defined() ? cast(dh0, s.ht) : Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -1837,11 +1840,11 @@ PyObject* py_residual_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t narg
   END_HANDLE_TH_ERRORS
 }
 
-// gated_recurrence(x, g, initial_state, output_final_state, inplace_state, plan or None) -> (h, final_state); NotImplemented while a
-// trace is recorded
+// gated_recurrence(x, g, initial_state, output_final_state, inplace_state, plan or None, chunks of the longest sequence) -> (h, final_state);
+// NotImplemented while a trace is recorded
 PyObject* py_gated_recurrence(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  NEED_ARGS(6);
+  NEED_ARGS(7);
   if (tracing()) Py_RETURN_NOTIMPLEMENTED;
   Tensor x, g, h0;
   if (!get(args[0], x) || !get(args[1], g) || !get(args[2], h0) || !x.defined() || !g.defined()) {
@@ -1849,6 +1852,7 @@ PyObject* py_gated_recurrence(PyObject*, PyObject* const* args, Py_ssize_t nargs
     return nullptr;
   }
   const bool out_state = truth(args[3]), inplace = truth(args[4]);
+  const int64_t longest = PyLong_AsLongLong(args[6]);
   if (PyErr_Occurred()) return nullptr;
   PlanPtr plan;
   if (args[5] != Py_None) plan = plan_of(args[5]);
@@ -1867,11 +1871,11 @@ PyObject* py_gated_recurrence(PyObject*, PyObject* const* args, Py_ssize_t nargs
     check("initial_state", h0, 0, x.device());
     if (wants_grad({&x, &g, &h0})) {
       if (inplace && out_state) raise("gated_recurrence: inplace_state where gradients are asked for");
-      variable_list out = RecurrenceFunction::apply(x, g, opt(h0), out_state, plan);
+      variable_list out = RecurrenceFunction::apply(x, g, opt(h0), out_state, plan, longest);
       h = out[0];
       if (out.size() > 1) fin = out[1];
     } else {
-      RecurrenceForward r = recurrence_forward(x, g, h0, out_state, inplace, plan, false);
+      RecurrenceForward r = recurrence_forward(x, g, h0, out_state, inplace, plan, longest, false);
       if (inplace && out_state && !r.final_state.is_inference()) torch::autograd::impl::bump_version(r.final_state);
       h = r.h;
       fin = r.final_state;

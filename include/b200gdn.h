@@ -431,7 +431,7 @@ typedef struct b200gdn_gated_recurrence_args {
   int32_t n_seq, seq_len, n_chunks;
   int32_t dtype;                 /* 0 = bf16, 1 = fp16, 2 = fp32: x, h, dh, dx */
   int32_t gate_dtype;            /* the same codes: g, dg; that of x, or 2 */
-  int32_t reserved;
+  int32_t longest;               /* 64-token chunks of the longest sequence, with tables (0: not known; it goes into the launch alone) */
   int64_t stride_x, stride_g;    /* elements from one row of x (of g) to the next; all else is contiguous */
   const int32_t* chunk_meta;     /* with seq_len = 0 */
   const int32_t* seq_meta;
