@@ -12,6 +12,9 @@
 // second kernel adds them in order and finishes; so is that of the tiles of the last round, where they leave pairs without work.
 // Up to 16 tokens, forward: W passes through registers once, as fast as memory gives it (linear_few_kernel).
 // TMA wants rows 16 bytes apart: operands of other widths are first copied to rows that are.
+// Bound by the tensor pipe (88 to 92 % of its cycles) and the clock it is left: 16384 x 2048 -> 8192 bf16 with bias and SiLU, z kept, 343 us
+// (1.60 PFLOP/s; 1.64 is the library's burst), dx 345, dW 366, dz with db 135 (123 at copy rate).  Small products: 2 us until the first operands are there,
+// 0.3 us a step of 64, 2 us for the last epilogue and the end.  4 tokens, 2048 -> 8192: 7.9 us a call (5.1 for W at copy rate).
 #include "gdn_common.cuh"
 #include "rowio.cuh"
 #include "tc5.cuh"

@@ -10,6 +10,10 @@
 // second kernel joins in a fixed order.  The second norm needs what the first one gives: two barriers a row, forward as well as backward.
 // Rows of a multiple of 16 bytes come by bulk copies into a ring of shared memory, two rows ahead; of other rows the next one is on its way
 // to registers.
+// Measured, bf16: 65536 x 4096 with both norms and a scale forward 330 us (328 at copy rate), backward 525 (492); 16384 x 2048 with a sigmoid gate as
+// well 62 (51) and 119 (82), where instructions count: 28 and 57 an element; 8191 x 1003 fp32 39 (25) and 58 (40), 8191 x 1002 bf16 29 and 45 (13 and 20).
+// Rows of other widths than multiples of 16 bytes beyond 4096 elements spill backward (260 to 576 bytes a thread); beyond 8192 elements a
+// row is looked at several times.
 #include "gdn_common.cuh"
 #include "row_pieces.cuh"
 #include "tc5.cuh"

@@ -84,6 +84,14 @@ def test_packed(cu, rows, D, dtype):
             assert (t[0, :cu[0]] == 0).all() and (t[0, cu[-1]:] == 0).all()
 
 
+@pytest.mark.parametrize('D,dtype,gtype', [(1280, BF, BF), (1290, BF, F), (1283, F, F), (1280, HF, F)])
+def test_one_sequence_much_longer_than_the_others(D, dtype, gtype):
+    """More pieces of work than SMs, and yet the longest sequence is shared by CTAs."""
+    cu = [0, 5, 10, 20, 60, 64, 2000, 2010, 2100]
+    args = make(1, 2100, D, 8, dtype, gtype, True, seed=20)
+    run_and_check(*args, O.packed_bounds(cu), cu=torch.tensor(cu, dtype=torch.int32, device='cuda'))
+
+
 def test_gradients_of_one_result_only():
     for grads in (('h',), ('ht',)):
         for B, T, D in ((2, 1, 8), (2, 70, 34), (1, 1400, 64)):
