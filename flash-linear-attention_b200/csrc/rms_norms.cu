@@ -8,10 +8,10 @@
 // HBM streaming, in the manner of layer_norm.cu: the threads of a group share a row, E elements each, which are worked on as E / 2 fp32 pairs;
 // groups walk the rows, so that a thread's columns stay its own: parameters are read once, their gradients are sums in registers, which a
 // second kernel joins in a fixed order.  The second norm needs what the first one gives: two barriers a row, forward as well as backward.
-// Rows of a multiple of 16 bytes come by bulk copies into a ring of shared memory, two rows ahead; of other rows the next one is on its way
-// to registers.
+// Rows of more than 256 elements come by bulk copies into a ring of shared memory, two rows ahead; shorter ones, of tensors that do not begin on
+// 16 bytes, and backward those whose width is no multiple of 16 bytes, to registers, one row ahead.
 // Measured, bf16: 65536 x 4096 with both norms and a scale forward 330 us (328 at copy rate), backward 525 (492); 16384 x 2048 with a sigmoid gate as
-// well 62 (51) and 119 (82), where instructions count: 28 and 57 an element; 8191 x 1003 fp32 39 (25) and 58 (40), 8191 x 1002 bf16 29 and 45 (13 and 20).
+// well 62 (51) and 119 (82), where instructions count: 28 and 57 an element; 8191 x 1003 fp32 38 (25) and 58 (40), 8191 x 1002 bf16 25 and 45 (13 and 20).
 // Rows of other widths than multiples of 16 bytes beyond 4096 elements spill backward (260 to 576 bytes a thread); beyond 8192 elements a
 // row is looked at several times.
 #include "gdn_common.cuh"
@@ -117,7 +117,10 @@ struct Part {
   }
 };
 
-// The tensors of a row, those that are there, side by side in a ring of SLOTS rows, as bulk copies; each group has its own.
+// The tensors of a row, those that are there, side by side in a ring of SLOTS rows, as bulk copies; each group has its own.  A copy begins on 16
+// bytes: of a row that does not, it begins with the end of the row ahead, and ends with the beginning of the next one.  (The tensors themselves
+// begin on 16 bytes, so all rows of a number lie alike.)
+__host__ __device__ constexpr int room_of(int row_bytes) { return row_bytes % 16 == 0 ? row_bytes : (row_bytes + 31) / 16 * 16; }
 template <int SLOTS>
 struct Ring {
   unsigned char* base;
@@ -127,9 +130,25 @@ struct Ring {
   bool ok = true;
 
   // one thread of the group
-  __device__ __forceinline__ void fill(int at, const void* const* tensors, int n, int64_t row, int row_bytes) const {
-    tc5::mbar_expect_tx(&full[at], n * row_bytes);
-    for (int i = 0; i < n; ++i) tma::load_1d(base + (at * n + i) * row_bytes, static_cast<const char*>(tensors[i]) + row * row_bytes, row_bytes, &full[at]);
+  template <typename T>
+  __device__ __forceinline__ void fill(int at, const void* const* tensors, int n, int64_t row, int64_t rows, int row_bytes) const {
+    const int ahead = (int)(row * row_bytes & 15), end = ahead + row_bytes;
+    int bytes = (end + 15) / 16 * 16;
+    unsigned char* to = base + at * n * room_of(row_bytes);
+    if (row * row_bytes - ahead + bytes > rows * row_bytes) {   // the tensor ends within the last 16 bytes: what is there comes by itself
+      bytes = end / 16 * 16;
+      for (int i = 0; i < n; ++i)
+        for (int e = bytes; e < end; e += (int)sizeof(T))
+          *reinterpret_cast<T*>(to + i * room_of(row_bytes) + e) =
+              *reinterpret_cast<const T*>(static_cast<const char*>(tensors[i]) + (row * row_bytes - ahead + e));
+    }
+    tc5::mbar_expect_tx(&full[at], n * bytes);
+    for (int i = 0; i < n; ++i)
+      tma::load_1d(to + i * room_of(row_bytes), static_cast<const char*>(tensors[i]) + (row * row_bytes - ahead), bytes, &full[at]);
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* first(int n, int64_t row, int row_bytes) const {   // of the tensors of the row that is there now
+    return reinterpret_cast<const T*>(base + slot * n * room_of(row_bytes) + (row * row_bytes & 15));
   }
   __device__ __forceinline__ void wait() {   // (a wait that has run out is told at the end and not repeated)
     if (ok) ok = tc5::mbar_wait_warp(&full[slot], phase);
@@ -144,7 +163,7 @@ struct Ring {
 // Two rows are enough, and more are worse: reads run so far ahead of the writes that memory changes between them more often (65536 x 4096 bf16
 // forward: 330 us with two, 373 with three or four).
 constexpr int slots_of(int n_tensors, int tpr, int e, int size) {   // of 54 KB for 128 threads
-  return 54 * 1024 * threads_of(tpr) / 128 / (threads_of(tpr) / tpr) / (n_tensors * tpr * e * size) > 1 ? 2 : 1;
+  return 54 * 1024 * threads_of(tpr) / 128 / (threads_of(tpr) / tpr) / (n_tensors * room_of(tpr * e * size)) > 1 ? 2 : 1;
 }
 
 // act(gate) and, where asked for, act'(gate).  What the gate is (NO_GATE, or AS_IT_IS, SIGMOID, SILU) is known where a row's loop begins: a
@@ -194,7 +213,8 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
   int64_t row = (int64_t)blockIdx.x * RPC + group;
   const int row_bytes = a.D * (int)sizeof(T), n_tensors = 1 + (a.residual != nullptr) + (GATE != WITHOUT && a.gate != nullptr);
   const void* tensors[3] = {a.y, a.residual ? a.residual : a.gate, a.gate};
-  Ring<SLOTS> ring{ring_bytes + group * SLOTS * n_tensors * row_bytes, full + group * SLOTS};
+  Ring<SLOTS> ring{ring_bytes + group * SLOTS * n_tensors * room_of(row_bytes), full + group * SLOTS};
+  const int room = room_of(row_bytes) / (int)sizeof(T);
   Row y, res, gate;
   auto fetch = [&](int64_t row) {
     y.zero(), res.zero(), gate.zero();
@@ -207,7 +227,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     if (sub == 0) {
       for (int i = 0; i < SLOTS; ++i) tc5::mbar_init(&ring.full[i], 1);
       tc5::fence_mbar_init();
-      for (int i = 0; i < SLOTS && row + i * step < a.rows; ++i) ring.fill(i, tensors, n_tensors, row + i * step, row_bytes);
+      for (int i = 0; i < SLOTS && row + i * step < a.rows; ++i) ring.template fill<T>(i, tensors, n_tensors, row + i * step, a.rows, row_bytes);
     }
     __syncthreads();
   } else {
@@ -222,11 +242,11 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
   for (int turn = 0; row - group < a.rows; turn ^= 1, row += step) {
     if constexpr (RING) {
       if (row < a.rows) ring.wait();
-      const T* at = reinterpret_cast<const T*>(ring.base + ring.slot * n_tensors * row_bytes);
+      const T* at = ring.template first<T>(n_tensors, row, row_bytes);
       y.load(at, sub, a.D);
-      if (a.residual) res.load(at += a.D, sub, a.D);
+      if (a.residual) res.load(at += room, sub, a.D);
       else res.zero();
-      if (GATE != WITHOUT && a.gate) gate.load(at += a.D, sub, a.D);
+      if (GATE != WITHOUT && a.gate) gate.load(at += room, sub, a.D);
     }
     float s[1] = {0.f}, r1 = 1.f;
     if (post) {
@@ -258,7 +278,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     row_sums<TPR>(s, scratch[turn][1]);
     if constexpr (RING) {   // (the whole group has passed: what it read is in registers)
       if (TPR == 32) __syncwarp();
-      if (sub == 0 && row + SLOTS * step < a.rows) ring.fill(ring.slot, tensors, n_tensors, row + SLOTS * step, row_bytes);
+      if (sub == 0 && row + SLOTS * step < a.rows) ring.template fill<T>(ring.slot, tensors, n_tensors, row + SLOTS * step, a.rows, row_bytes);
       ring.next();
     }
     const float r2 = __frsqrt_rn(s[0] * up + a.eps);
@@ -301,7 +321,8 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
   int n_tensors = 0;
   for (const void* p : {a.y, a.residual, a.gate, a.dout, a.dz})
     if (p) tensors[n_tensors++] = p;
-  Ring<SLOTS> ring{ring_bytes + group * SLOTS * n_tensors * row_bytes, full + group * SLOTS};
+  Ring<SLOTS> ring{ring_bytes + group * SLOTS * n_tensors * room_of(row_bytes), full + group * SLOTS};
+  const int room = room_of(row_bytes) / (int)sizeof(T);
   struct Rows {
     Row y, res, gate, dout, dz;
     float r1, r2;
@@ -324,7 +345,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     if (sub == 0) {
       for (int i = 0; i < SLOTS; ++i) tc5::mbar_init(&ring.full[i], 1);
       tc5::fence_mbar_init();
-      for (int i = 0; i < SLOTS && row + i * step < a.rows; ++i) ring.fill(i, tensors, n_tensors, row + i * step, row_bytes);
+      for (int i = 0; i < SLOTS && row + i * step < a.rows; ++i) ring.template fill<T>(i, tensors, n_tensors, row + i * step, a.rows, row_bytes);
     }
     __syncthreads();
   } else if constexpr (AHEAD) {
@@ -350,12 +371,12 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     const float r1f = next.r1, r2f = next.r2;
     if constexpr (RING) {
       if (live) ring.wait();
-      const T* at = reinterpret_cast<const T*>(ring.base + ring.slot * n_tensors * row_bytes);
+      const T* at = ring.template first<T>(n_tensors, row, row_bytes);
       at_y = at;
-      if (a.residual) at_res = at += a.D;
-      if (GATE != WITHOUT && a.gate) at_gate = at += a.D;
-      if (a.dout) at_dout = at += a.D;
-      if (a.dz) at_dz = at += a.D;
+      if (a.residual) at_res = at += room;
+      if (GATE != WITHOUT && a.gate) at_gate = at += room;
+      if (a.dout) at_dout = at += room;
+      if (a.dz) at_dz = at += room;
     } else if constexpr (AHEAD) {
       cur = next;
       fetch(next, row + step);
@@ -446,7 +467,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     }
     if constexpr (RING) {
       if (TPR == 32) __syncwarp();
-      if (sub == 0 && row + SLOTS * step < a.rows) ring.fill(ring.slot, tensors, n_tensors, row + SLOTS * step, row_bytes);
+      if (sub == 0 && row + SLOTS * step < a.rows) ring.template fill<T>(ring.slot, tensors, n_tensors, row + SLOTS * step, a.rows, row_bytes);
       ring.next();
     }
     if (!live || !a.dy) continue;
@@ -646,9 +667,9 @@ int launch_rows(const b200gdn_rms_norms_args& a, cudaStream_t st) {
   auto go = [&](auto kern) {
     int tensors = 0;
     for (const void* p : {a.y, a.residual, a.gate, BWD ? a.dout : nullptr, BWD ? a.dz : nullptr}) tensors += p != nullptr;
-    const size_t smem = RING ? (size_t)RPC * slots_of(MOST, TPR, E, sizeof(T)) * tensors * a.D * sizeof(T) : 0;
+    const size_t smem = RING ? (size_t)RPC * slots_of(MOST, TPR, E, sizeof(T)) * tensors * room_of(a.D * (int)sizeof(T)) : 0;
     if (RING)   // (what a row may take at most: the limit is set once)
-      if (int e = ensure_smem(kern, (size_t)RPC * slots_of(MOST, TPR, E, sizeof(T)) * MOST * TPR * E * sizeof(T))) return e;
+      if (int e = ensure_smem(kern, (size_t)RPC * slots_of(MOST, TPR, E, sizeof(T)) * MOST * (TPR * E * sizeof(T) + 16))) return e;
     kern<<<n, threads, smem, st>>>(a);
     return check_launch(BWD ? "rms_norms_bwd" : "rms_norms_fwd");
   };
@@ -658,7 +679,7 @@ int launch_rows(const b200gdn_rms_norms_args& a, cudaStream_t st) {
     else return go(rms_norms_fwd_kernel<T, N, TPR, E, RING, GATE>);
   };
   int e;
-  if constexpr (RING) e = a.gate ? pass(std::integral_constant<Gates, WITH>()) : pass(std::integral_constant<Gates, WITHOUT>());
+  if constexpr (RING && N * sizeof(T) == 16) e = a.gate ? pass(std::integral_constant<Gates, WITH>()) : pass(std::integral_constant<Gates, WITHOUT>());
   else e = pass(std::integral_constant<Gates, EITHER>());
   return e == 0 && BWD && a.partials ? reduce_partials(a, n, st) : e;
 }
@@ -687,13 +708,20 @@ int launch_n(const b200gdn_rms_norms_args& a, cudaStream_t st) {
   if (a.D <= 64) return launch_rows<T, N, 8, 8, false, BWD>(a, st);
   if (a.D <= 128) return launch_rows<T, N, 16, 8, false, BWD>(a, st);
   if (a.D <= 256) return launch_rows<T, N, 32, 8, false, BWD>(a, st);
-  if constexpr (N * sizeof(T) == 16) {
-    if (a.D <= 512) return launch_rows<T, N, BWD ? 64 : 32, BWD ? 8 : 16, true, BWD>(a, st);
-    if (a.D <= 1024) return launch_rows<T, N, 64, 16, true, BWD>(a, st);
-    if (a.D <= 2048) return launch_rows<T, N, 128, 16, true, BWD>(a, st);
-    if (a.D <= 4096) return launch_rows<T, N, 256, 16, true, BWD>(a, st);
-    if (a.D <= 8192) return launch_rows<T, N, 512, 16, true, BWD>(a, st);
-  } else {
+  // by the ring: rows in pieces of 16 bytes, and forward narrower ones too, where the tensors begin on 16 (8191 x 1002 bf16 forward 25 us, 30 by
+  // registers; backward 51 and 45)
+  if constexpr (N * sizeof(T) == 16 || !BWD) {
+    uintptr_t begin = 0;
+    for (const void* p : {a.y, a.residual, a.gate, BWD ? a.dout : nullptr, BWD ? a.dz : nullptr}) begin |= reinterpret_cast<uintptr_t>(p);
+    if (begin % 16 == 0) {
+      if (a.D <= 512) return launch_rows<T, N, BWD ? 64 : 32, BWD ? 8 : 16, true, BWD>(a, st);
+      if (a.D <= 1024) return launch_rows<T, N, 64, 16, true, BWD>(a, st);
+      if (a.D <= 2048) return launch_rows<T, N, 128, 16, true, BWD>(a, st);
+      if (a.D <= 4096) return launch_rows<T, N, 256, 16, true, BWD>(a, st);
+      if (a.D <= 8192) return launch_rows<T, N, 512, 16, true, BWD>(a, st);
+    }
+  }
+  if constexpr (N * sizeof(T) != 16) {
     if (a.D <= 512) return launch_rows<T, N, 64, 8, false, BWD>(a, st);
     if (a.D <= 1024) return launch_rows<T, N, 128, 8, false, BWD>(a, st);
     if (a.D <= 2048) return launch_rows<T, N, 256, 8, false, BWD>(a, st);
