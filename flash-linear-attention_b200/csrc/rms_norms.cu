@@ -11,7 +11,7 @@
 // Rows of more than 256 elements come by bulk copies into a ring of shared memory, two rows ahead; shorter ones, of tensors that do not begin on
 // 16 bytes, and backward those whose width is no multiple of 16 bytes, to registers, one row ahead.
 // Measured, bf16: 65536 x 4096 with both norms and a scale forward 330 us (328 at copy rate), backward 525 (492); 16384 x 2048 with a sigmoid gate as
-// well 62 (51) and 119 (82), where instructions count: 28 and 57 an element; 8191 x 1003 fp32 38 (25) and 58 (40), 8191 x 1002 bf16 25 and 45 (13 and 20).
+// well 62 (51) and 119 (82), where instructions count: 28 and 57 an element; 8191 x 1003 fp32 37 (25) and 58 (40), 8191 x 1002 bf16 25 and 45 (13 and 20).
 // Rows of other widths than multiples of 16 bytes beyond 4096 elements spill backward (260 to 576 bytes a thread); beyond 8192 elements a
 // row is looked at several times.
 #include "gdn_common.cuh"
@@ -709,7 +709,7 @@ int launch_n(const b200gdn_rms_norms_args& a, cudaStream_t st) {
   if (a.D <= 128) return launch_rows<T, N, 16, 8, false, BWD>(a, st);
   if (a.D <= 256) return launch_rows<T, N, 32, 8, false, BWD>(a, st);
   // by the ring: rows in pieces of 16 bytes, and forward narrower ones too, where the tensors begin on 16 (8191 x 1002 bf16 forward 25 us, 30 by
-  // registers; backward 51 and 45)
+  // registers; backward 54 and 45, 8191 x 1003 fp32 83 and 58)
   if constexpr (N * sizeof(T) == 16 || !BWD) {
     uintptr_t begin = 0;
     for (const void* p : {a.y, a.residual, a.gate, BWD ? a.dout : nullptr, BWD ? a.dz : nullptr}) begin |= reinterpret_cast<uintptr_t>(p);
