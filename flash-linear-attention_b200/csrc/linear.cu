@@ -465,12 +465,13 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// eight neighbouring elements of a row from k on; zeros past its end, or where there is no row
+// eight neighbouring elements of a row from k on; zeros past its end, or where there is no row.  By ordinary loads: the kernel ahead may still
+// write x, or W, when this one begins, and only of these is it known that they see what was written before wait_for_predecessor.
 template <bool WIDE>
 __device__ __forceinline__ uint4 eight(const uint16_t* row, int k, int K, bool there) {
   uint4 u = make_uint4(0, 0, 0, 0);
   if constexpr (WIDE) {
-    if (there && k < K) u = __ldg(reinterpret_cast<const uint4*>(row + k));
+    if (there && k < K) u = *reinterpret_cast<const uint4*>(row + k);
   } else {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll

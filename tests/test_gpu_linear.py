@@ -183,3 +183,32 @@ def test_refusals():
     dx, = torch.autograd.grad(fused_linear(leaf, w).float().square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match='no second derivative'):
         dx.sum().backward()
+
+
+def test_calls_of_few_tokens_in_a_row():
+    """Each call reads what the one ahead has just written, and begins before it ends: in a captured graph, on changing data, against calls
+    between which the device is waited for."""
+    from b200gdn import fused_linear
+    for M, D in ((1, 1024), (4, 2048), (16, 520), (9, 96)):
+        gen = torch.Generator(device='cuda').manual_seed(M)
+        layers = [(torch.randn(D, D, device='cuda', generator=gen) * D ** -0.5).to(BF) for _ in range(6)]
+        data = [torch.randn(M, D, device='cuda', generator=gen).to(BF) for _ in range(8)]
+
+        def chain(x, wait):
+            out = []
+            for w in layers:
+                x = fused_linear(x, w, None, x, 'silu')
+                out.append(x)
+                if wait:
+                    torch.cuda.synchronize()
+            return out
+        want = [chain(x, True) for x in data]
+        held, graph = data[0].clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = chain(held, False)
+        for _ in range(3):
+            for x, w in zip(data, want):
+                held.copy_(x)
+                graph.replay()
+                assert all(torch.equal(p, q) for p, q in zip(got, w))
+                assert all(torch.equal(p, q) for p, q in zip(chain(x, False), w))
