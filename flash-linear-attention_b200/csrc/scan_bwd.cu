@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(NTHREADS, DK == 64 && PRE ? 2 : 1)
       uint32_t odd = 0;
 #pragma unroll 8
       for (int r = row0; r < rows; r += NTHREADS / 8) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(d_o + (int64_t)r * a.HV * DV));
+        const uint4 w = *reinterpret_cast<const uint4*>(d_o + (int64_t)r * a.HV * DV);   // (not __ldg: the kernel ahead may be what writes it)
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd |= ((u[e] & 0x7f800000u) == 0x7f800000u) | ((u[e] & 0x7f80u) == 0x7f80u);

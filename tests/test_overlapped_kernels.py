@@ -19,7 +19,17 @@ def source(name):
 NOT_COHERENT = re.compile(r'__ldg\b|\bld\.global(\.\w+)*\.nc\b|__restrict__')
 
 
-@pytest.mark.parametrize('name', ['linear.cu'])
+def overlapped():
+    names = [os.path.basename(p) for p in sorted(glob.glob(os.path.join(CSRC, '*.cu')))]
+    return [n for n in names if 'wait_for_predecessor();' in source(n)]
+
+
+@pytest.mark.parametrize('name', overlapped())
 def test_what_the_kernel_ahead_writes_is_not_read_by_the_non_coherent_path(name):
-    text = source(name)
-    assert 'wait_for_predecessor();' in text and not NOT_COHERENT.findall(text)
+    assert not NOT_COHERENT.findall(source(name))
+
+
+def test_the_sources_are_found():
+    assert {'linear.cu', 'scan_bwd.cu', 'rms_norms.cu'} <= set(overlapped())
+    for header in glob.glob(os.path.join(CSRC, '*.cuh')):   # what they include
+        assert not NOT_COHERENT.findall(source(os.path.basename(header))), header
