@@ -233,13 +233,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     tc5::fence_mbar_init();
   }
+  wait_for_predecessor();   // (no tensor memory is held meanwhile: a kernel ahead that still has its own to come by would wait for this one)
   if (warp == EPILOGUE + 1) pair_tmem_alloc(&tmem_slot, COLUMNS);
   __syncthreads();
   tc5::fence_before_sync();
   cluster_sync();
   tc5::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  wait_for_predecessor();   // nothing global is touched before
   const int n_tiles = p.whole + (p.tiles_i * p.tiles_j - p.whole) * p.splits, first = blockIdx.x >> 1, by = gridDim.x >> 1;
   bool ok = true;
   if (warp == EPILOGUE) {

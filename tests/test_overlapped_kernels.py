@@ -33,3 +33,11 @@ def test_the_sources_are_found():
     assert {'linear.cu', 'scan_bwd.cu', 'rms_norms.cu'} <= set(overlapped())
     for header in glob.glob(os.path.join(CSRC, '*.cuh')):   # what they include
         assert not NOT_COHERENT.findall(source(os.path.basename(header))), header
+
+
+@pytest.mark.parametrize('name', overlapped())
+def test_no_tensor_memory_is_held_while_the_kernel_ahead_is_waited_for(name):
+    """That kernel releases its successor's launch before it allocates its own: on one SM each would wait for the other, without an end."""
+    for body in source(name).split('__global__')[1:]:
+        wait, alloc = body.find('wait_for_predecessor();'), re.search(r'tmem_alloc\(', body)
+        assert wait < 0 or alloc is None or wait < alloc.start(), body[:200]
