@@ -566,6 +566,15 @@ __device__ __forceinline__ uint64_t slope2(uint64_t z, int act) {
   return act == SILU ? mul2(s, fma2(z, rest, one)) : mul2(s, rest);
 }
 
+// Two elements of the kept z within their type's finite values (a NaN stays).  z was rounded to be kept: what left the type's range there is infinite,
+// and infinity times the slope's zero would be NaN.  The activation saw the number itself, whose slope is that of the type's largest: 0 or 1.
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %0, %1;\n min.NaN.f16x2 %0, %0, %2;" : "+r"(w) : "r"(0xFBFFFBFFu), "r"(0x7BFF7BFFu));
+  else asm("max.NaN.bf16x2 %0, %0, %1;\n min.NaN.bf16x2 %0, %0, %2;" : "+r"(w) : "r"(0xFF7FFF7Fu), "r"(0x7F7F7F7Fu));
+  return w;
+}
+
 // dz = dy act'(z) (rounded for the products; `dz` NULL: not wanted) and, for db, its sums over the rows of a CTA, unrounded.  Warps take rows in
 // turn, lanes E columns each; four rows are on their way at once.
 template <typename T, int E>
@@ -577,9 +586,9 @@ __global__ void __launch_bounds__(256, 3) linear_dz_kernel(const T* dy, const T*
   uint64_t total[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) total[i] = 0ull;
-  auto pair = [](const Raw& u, int i) {
-    if constexpr (E > 1) return widen2<T>(reinterpret_cast<const uint32_t*>(&u)[i]);
-    else return pack2((float)*reinterpret_cast<const T*>(&u), 0.f);
+  auto word = [](const Raw& u, int i) -> uint32_t {   // two elements; of one alone the second is zero
+    if constexpr (E > 1) return reinterpret_cast<const uint32_t*>(&u)[i];
+    else return u;
   };
   if (c < cols) {
     const int64_t step = (int64_t)gridDim.y * 8;
@@ -598,8 +607,8 @@ __global__ void __launch_bounds__(256, 3) linear_dz_kernel(const T* dy, const T*
         Raw out;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          uint64_t g = pair(d[u], i);
-          if (act != NONE) g = mul2(g, slope2(pair(v[u], i), act));
+          uint64_t g = widen2<T>(word(d[u], i));
+          if (act != NONE) g = mul2(g, slope2(widen2<T>(finite2<T>(word(v[u], i))), act));
           total[i] = add2(total[i], g);   // (a row past the end adds zeros)
           if constexpr (E > 1) reinterpret_cast<uint32_t*>(&out)[i] = narrow2<T>(g);
           else *reinterpret_cast<T*>(&out) = static_cast<T>(unpack2(g).x);

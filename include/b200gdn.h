@@ -497,7 +497,8 @@ int64_t b200gdn_rms_norms_partials(int64_t rows, int32_t D);
 
 /* Projection of `rows` tokens from K to N features:  z = x weight^T + bias,  y = act(z) + residual, and its gradients
  *   dz = dy act'(z);  dx = dz weight;  dweight = dz^T x;  dbias = sum of dz   (the residual's is dy)
- * Sums are held in fp32; dz and the z that is kept for the backward pass are rounded to the tensors' type, which the products read.  act is
+ * Sums are held in fp32; dz and the z that is kept for the backward pass are rounded to the tensors' type, which the products read; a z beyond that
+ * type's range is kept as an infinity and has the slope of the type's largest value, a dz beyond it is infinite.  act is
  * B200GDN_LINEAR_SILU, _SIGMOID, _GELU (by the error function) or 0, none.  All tensors are contiguous; where x, weight and dy have rows of a
  * multiple of 16 bytes on such a boundary they are read in place, else from copies in the workspace.  workspace:
  * b200gdn_linear_workspace_bytes(args, backward) bytes, with the pointers of `args` set as for the call, on a boundary of 256. */

@@ -212,3 +212,33 @@ def test_calls_of_few_tokens_in_a_row():
                 graph.replay()
                 assert all(torch.equal(p, q) for p, q in zip(got, w))
                 assert all(torch.equal(p, q) for p, q in zip(chain(x, False), w))
+
+
+@pytest.mark.parametrize('act', ['silu', 'gelu', 'sigmoid'])
+@pytest.mark.parametrize('M', [7, 100, 600])
+def test_gradients_where_the_activations_input_leaves_the_types_range(M, act):
+    """fp16: feature 0 has z = -80000, feature 1 z = 70000, beyond 65504, where the activation is applied all the same: their slopes are 0 and 1 (of the sigmoid 0 and
+    0).  Feature 1's y comes back into range by the residual."""
+    from b200gdn import fused_linear
+    for K, N in ((64, 64), (72, 50), (33, 35)):   # dz by eight, two and one element a thread
+        x, w, b, r, dy = make(M, K, N, HF, seed=N)
+        x[:, 0] = 250
+        w[:, 0] = 0
+        w[:2] = 0
+        w[0, 0], w[1, 0] = -320, 280
+        b[:2], r[:, 1] = 0, -40000 if act != 'sigmoid' else 0
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+        y = fused_linear(*leaves, activation=act)
+        want = O.linear(x, w[1:], b[1:], r[:, 1:], act, dy[:, 1:])   # feature 0 adds nothing to any gradient
+        close('y', y.detach()[:, 1:], want['y'], want['y_off'])
+        assert torch.equal(y.detach()[:, 0], r[:, 0])
+        dx, dw, db, _ = torch.autograd.grad(y, leaves, dy)
+        close('dx', dx, want['dx'], want['dx_off'])
+        assert (dw[0] == 0).all() and db[0] == 0
+        close('dweight', dw[2:], want['dweight'][1:], want['dweight_off'][1:])
+        close('dbias', db[2:], want['dbias'][1:], want['dbias_off'][1:])
+        # (the oracle lets a slope be off by z's rounding, which here it is not)
+        up = dy[:, 1].double() * (act != 'sigmoid')
+        units = (M / 16 + 32) * 2 * O.U
+        close('dweight', dw[1], up @ x.double(), units * (up.abs() @ x.double().abs()))
+        close('dbias', db[1], up.sum(), units * up.abs().sum())
