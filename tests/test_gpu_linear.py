@@ -242,3 +242,23 @@ def test_gradients_where_the_activations_input_leaves_the_types_range(M, act):
         units = (M / 16 + 32) * 2 * O.U
         close('dweight', dw[1], up @ x.double(), units * (up.abs() @ x.double().abs()))
         close('dbias', db[1], up.sum(), units * up.abs().sum())
+
+
+@pytest.mark.parametrize('M', [9, 250, 1000])
+@pytest.mark.parametrize('dtype', [BF, HF])
+def test_gelu_where_little_is_left_of_it(dtype, M):
+    """Far below zero, z exact (the weight is the identity).  A result is off by half a step of its type (denormal ones by half of the smallest, 2^-25 in
+    fp16) and by what fp32 leaves of erfc: 16 units for the functions and v^2 for the argument's rounding, by their size."""
+    from b200gdn import fused_linear
+    K = 40
+    x = -torch.linspace(0.0, 12.0 if dtype == BF else 5.6, M * K, device='cuda').to(dtype).view(M, K)
+    eye = torch.eye(K, device='cuda', dtype=dtype)
+    leaf = x.clone().requires_grad_(True)
+    y = fused_linear(leaf, eye, activation='gelu')
+    dx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    v = x.double()
+    cdf, pdf = 0.5 * torch.special.erfc(-v * 0.5 ** 0.5), torch.exp(-0.5 * v * v) / (2 * torch.pi) ** 0.5
+    for name, got, want, size in (('y', y.detach(), v * cdf, v.abs() * cdf), ('dx', dx, cdf + v * pdf, cdf + v.abs() * pdf)):
+        limit = EPS[dtype] * want.abs() + (v * v + 16) * 2 * O.U * size + (2.0 ** -25 if dtype == HF else 1e-38)
+        far = ((got.double() - want).abs() / limit).max().item()
+        assert far <= 1.0, f'{name}: {far:.2f} of what is allowed'
