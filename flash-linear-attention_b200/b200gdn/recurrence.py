@@ -35,8 +35,8 @@ def gated_recurrence(
 
     x, g ``[B,T,D]`` in bf16, fp16 or fp32 (``B == 1`` with ``cu_seqlens [N+1]``, whose sequences lie one behind the other); slices of a
     wider projection are read where they lie.  g is the logarithm of a decay, as the mixers' gates are: 0 keeps, minus infinity forgets.
-    (Above 0 a state grows; products of ``exp(g)`` over up to 2048 neighbouring tokens must stay within fp32's range then.)  A g that has
-    neither the type of x nor fp32 is cast to fp32.
+    (Above 0 a state grows; products of ``exp(g)`` over up to 2048 neighbouring tokens must stay below 2^127 then.)  A decay below 2^-126.5 counts
+    as zero; while decays are not zero an infinite state stays infinite.  A g that has neither the type of x nor fp32 is cast to fp32.
 
     ``initial_state [N,D]`` (zeros where absent) and ``final_state [N,D]`` in fp32; everything in between is held in fp32 too, and
     gradients, which reach x, g and initial_state from both results, are formed from states that were not rounded.  A sequence without

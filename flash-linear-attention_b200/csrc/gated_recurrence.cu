@@ -130,6 +130,38 @@ struct Joined {
   uint64_t a, h;
 };
 
+// A state that is infinite stays so for as long as decays are not zero, but their product over many tokens may leave fp32's range.  Such a product is
+// kept as -0, one of decays of which one is zero as +0: a finite state they carry alike (a decay is never negative), and where a joined state
+// comes out as NaN it is formed again by `carry`, which tells them apart.
+__device__ __forceinline__ bool any_zero(uint64_t a) {
+  const float2 f = unpack2(a);
+  return f.x == 0.f || f.y == 0.f;
+}
+__device__ __forceinline__ bool any_nan(uint64_t a) {
+  const float2 f = unpack2(a);
+  return f.x != f.x || f.y != f.y;
+}
+__device__ __forceinline__ float carry(float a, float s, float h) {   // a s + h
+  return __float_as_uint(a) == 0x80000000u && isinf(s) ? s + h : fmaf(a, s, h);
+}
+template <int R>
+__device__ __forceinline__ uint64_t signed_product(uint64_t product, const uint64_t (&decays)[R]) {
+  if (!any_zero(product)) return product;
+  float2 least = unpack2(decays[0]);
+#pragma unroll
+  for (int r = 1; r < R; ++r) {
+    const float2 f = unpack2(decays[r]);
+    least.x = fminf(least.x, f.x);
+    least.y = fminf(least.y, f.y);
+  }
+  const float2 p = unpack2(product);
+  return pack2(p.x == 0.f && least.x > 0.f ? -0.f : p.x, p.y == 0.f && least.y > 0.f ? -0.f : p.y);
+}
+__device__ __forceinline__ uint64_t carry(uint64_t a, uint64_t s, uint64_t h) {
+  const float2 u = unpack2(a), v = unpack2(s), w = unpack2(h);
+  return pack2(carry(u.x, v.x, w.x), carry(u.y, v.y, w.y));
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
@@ -169,7 +201,7 @@ struct Patience {
 template <int W, bool CLUSTER>
 struct Exchange {
   ulonglong2 warps[2][W][32];
-  uint64_t carry[2][32];   // what leaves the step, without a cluster
+  uint64_t carry[2][32];   // what enters the step, and what leaves it, without a cluster
   ulonglong2 ranks[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][32], mine[CLUSTER ? 2 : 1][32];
   uint64_t came[2];        // the joined pairs of all CTAs
 
@@ -183,6 +215,9 @@ struct Exchange {
       __syncthreads();
       cluster_sync();
     }
+  }
+  __device__ __forceinline__ void enter(uint64_t s) {   // what enters the first step
+    if (W > 1 && !CLUSTER && threadIdx.x < 32) carry[0][threadIdx.x] = s;
   }
   __device__ __forceinline__ void leave() {   // no CTA ends while another one may still send to it
     if constexpr (CLUSTER) cluster_sync();
@@ -199,51 +234,87 @@ __device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int i, int war
   if constexpr (W == 1) {
     const uint64_t mine = s;
     s = fma2(own.a, s, own.h);
+    if (any_nan(s)) s = carry(own.a, mine, own.h);
     return mine;
   } else {
     x.warps[turn][warp][lane] = make_ulonglong2(own.a, own.h);
     __syncthreads();
     meanwhile();
+    auto at = [&](int q) { return x.warps[turn][REVERSE ? W - 1 - q : q][lane]; };
     if constexpr (!CLUSTER) {
-      uint64_t mine = i == 0 ? s : x.carry[turn][lane];
+      uint64_t mine = x.carry[turn][lane];
 #pragma unroll
       for (int q = 0; q < W - 1; ++q)
         if (q < ahead_of) {
-          const ulonglong2 p = x.warps[turn][REVERSE ? W - 1 - q : q][lane];
+          const ulonglong2 p = at(q);
           mine = fma2(p.x, mine, p.y);
         }
       s = fma2(own.a, mine, own.h);
+      if (any_nan(s)) {
+        mine = x.carry[turn][lane];
+#pragma unroll 1
+        for (int q = 0; q < ahead_of; ++q) mine = carry(at(q).x, mine, at(q).y);
+        const ulonglong2 p = at(ahead_of);
+        s = carry(p.x, mine, p.y);
+      }
       if (ahead_of == W - 1) x.carry[turn ^ 1][lane] = s;
       return mine;
     } else {
-      // warp 0 joins all of them, to tell the other CTAs
-      const int n = warp == 0 ? W : ahead_of;
-      Joined ahead = {pack2(1.f, 1.f), 0ull};
+      auto ahead_at = [&](int n) {   // what the first n warps come to
+        Joined ahead = {pack2(1.f, 1.f), 0ull};
 #pragma unroll
-      for (int q = 0; q < W; ++q)
-        if (q < n) {
-          const ulonglong2 p = x.warps[turn][REVERSE ? W - 1 - q : q][lane];
-          ahead.h = fma2(p.x, ahead.h, p.y);
-          ahead.a = mul2(p.x, ahead.a);
+        for (int q = 0; q < W; ++q)
+          if (q < n) {
+            const ulonglong2 p = at(q);
+            ahead.h = fma2(p.x, ahead.h, p.y);
+            ahead.a = mul2(p.x, ahead.a);
+          }
+        return ahead;
+      };
+      auto with_sign = [](uint64_t product, uint32_t least_x, uint32_t least_y) {   // by the least of the factors' bits
+        const float2 p = unpack2(product);
+        return pack2(p.x == 0.f ? least_x == 0u ? 0.f : -0.f : p.x, p.y == 0.f ? least_y == 0u ? 0.f : -0.f : p.y);
+      };
+      auto carefully = [&](Joined ahead, int n) {
+        uint32_t least_x = ~0u, least_y = ~0u;
+        ahead.h = 0ull;
+#pragma unroll 1
+        for (int q = 0; q < n; ++q) {
+          const ulonglong2 p = at(q);
+          const float2 f = unpack2(p.x);
+          least_x = min(least_x, __float_as_uint(f.x));
+          least_y = min(least_y, __float_as_uint(f.y));
+          ahead.h = carry(p.x, ahead.h, p.y);
         }
+        ahead.a = with_sign(ahead.a, least_x, least_y);
+        return ahead;
+      };
+      // warp 0 joins all of them, to tell the other CTAs
+      Joined ahead = ahead_at(warp == 0 ? W : ahead_of);
       if (warp == 0) {
+        if (any_nan(ahead.h)) {
+          ahead = carefully(ahead, W);
+        } else if (any_zero(ahead.a)) {   // (common where channels forget, and on the way from CTA to CTA: no loop)
+          uint32_t least_x = ~0u, least_y = ~0u;
+#pragma unroll
+          for (int q = 0; q < W; ++q) {
+            const float2 f = unpack2(at(q).x);
+            least_x = min(least_x, __float_as_uint(f.x));
+            least_y = min(least_y, __float_as_uint(f.y));
+          }
+          ahead.a = with_sign(ahead.a, least_x, least_y);
+        }
         x.mine[turn][lane] = make_ulonglong2(ahead.a, ahead.h);
         tc5::fence_async_smem();
         if (lane == 0) tc5::mbar_expect_tx(&x.came[turn], n_ranks * 512);
         __syncwarp();
         if (lane < n_ranks) send(at_rank(&x.ranks[turn][rank][0], lane), tc5::smem_addr(&x.mine[turn][0]), 512, at_rank(&x.came[turn], lane));
         // ahead of warp 0: nothing, or (REVERSE) the others
-        ahead = {pack2(1.f, 1.f), 0ull};
-        if constexpr (REVERSE) {
-#pragma unroll
-          for (int q = 0; q < W - 1; ++q) {
-            const ulonglong2 p = x.warps[turn][W - 1 - q][lane];
-            ahead.h = fma2(p.x, ahead.h, p.y);
-            ahead.a = mul2(p.x, ahead.a);
-          }
-        }
+        if constexpr (REVERSE) ahead = ahead_at(W - 1);
+        else ahead = {pack2(1.f, 1.f), 0ull};
       }
       patience.wait(&x.came[turn], (i >> 1) & 1);
+      const uint64_t first = s;
       uint64_t entering = s;
 #pragma unroll 4
       for (int q = 0; q < n_ranks; ++q) {
@@ -252,7 +323,20 @@ __device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int i, int war
         if (r == rank) entering = s;
         s = fma2(p.x, s, p.y);
       }
-      return fma2(ahead.a, entering, ahead.h);
+      uint64_t mine = fma2(ahead.a, entering, ahead.h);
+      if (any_nan(add2(s, mine))) {   // (a sum of infinities of both signs too: no harm)
+        s = first;
+#pragma unroll 1
+        for (int q = 0; q < n_ranks; ++q) {
+          const int r = REVERSE ? n_ranks - 1 - q : q;
+          const ulonglong2 p = x.ranks[turn][r][lane];
+          if (r == rank) entering = s;
+          s = carry(p.x, s, p.y);
+        }
+        ahead = carefully(ahead, ahead_of);
+        mine = carry(ahead.a, entering, ahead.h);
+      }
+      return mine;
     }
   }
 }
@@ -351,6 +435,7 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     fetch(t0);
   }
   uint64_t s = load_state<APART>(a.h0, (int64_t)at.seq * a.D + at.channel, live, two);
+  exchange.enter(s);
   int stage = 0;
   uint32_t phase = 0;
   uint64_t decays[R];
@@ -390,6 +475,7 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
         own.h = fma2(decays[r], own.h, now[r].pair());
         own.a = mul2(decays[r], own.a);
       }
+      own.a = signed_product(own.a, decays);
     }
     if (!TMA && i + 1 < n) fetch(t + step);
     return own;
@@ -486,6 +572,7 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
   }
   if (n > 0) fetch_start(t0);
   uint64_t s = load_state<APART>(a.dht, (int64_t)at.seq * a.D + at.channel, live, two);
+  exchange.enter(s);
   int stage = 0;
   uint32_t phase = 0;
   for (int i = 0; i < n; ++i, t0 -= step) {
@@ -532,6 +619,7 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
       }
 #pragma unroll
       for (int q = R - 1; q >= 0; --q) own.h = mul2(decays[q], add2(up[q].pair(), own.h));
+      own.a = signed_product(own.a, decays);
     }
     if (i + 1 < n) {
       if (!TMA) fetch(t0 - step);
@@ -555,6 +643,14 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
           const ulonglong2 p = left[i & 1][warp - before + w][lane];
           h = fma2(p.x, h, p.y);
         }
+      if (any_nan(h)) {
+        h = load_state<APART>(a.states, (int64_t)(seq.chunk + t0 / BT) * a.D + at.channel, true, two);
+#pragma unroll 1
+        for (int w = 0; w < before; ++w) {
+          const ulonglong2 p = left[i & 1][warp - before + w][lane];
+          h = carry(p.x, h, p.y);
+        }
+      }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {

@@ -421,7 +421,8 @@ int b200gdn_layer_norm_ctas(int64_t rows);
  *   h_t = exp(g_t) h_{t-1} + x_t,   h_{-1} = h0 (or 0)
  * and, with dh the upstream gradient of h and dht that of the last state of each sequence,
  *   dx_t = dh_t + exp(g_{t+1}) dx_{t+1} (+ dht at the last token),   dg_t = dx_t exp(g_t) h_{t-1},   dh0 = exp(g_0) dx_0
- * g is a logarithm of a decay; above 0 the products of exp(g) over neighbouring tokens have to stay within fp32's range.  States are fp32.
+ * g is a logarithm of a decay; above 0 the products of exp(g) over up to 2048 neighbouring tokens have to stay below 2^127.  A decay below 2^-126.5
+ * counts as zero; while decays are not zero an infinite state stays infinite.  States are fp32.
  * Sequences: seq_len > 0: n_seq of that many tokens, one behind the other, without tables; else the tables of the chunk passes, whose
  * 64-token chunks n_chunks counts.  Rows that no sequence covers are neither read nor written.  ht may be h0 itself. */
 typedef struct b200gdn_gated_recurrence_args {

@@ -325,3 +325,42 @@ def test_refusals():
     dx, = torch.autograd.grad(gated_recurrence(leaf, x)[0].square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match='no second derivative'):
         dx.sum().backward()
+
+
+def _token_by_token(x, g, h0, dh, dht):
+    """h, the last state, dx, dg and dh0 of sequences [B, T, D], in 64 bits and in the definition's order."""
+    a = torch.exp(g.double())
+    x, dh, h, u = x.double(), dh.double(), h0.double(), dht.double()
+    hs, before, dx, dg = [], [], [None] * x.shape[1], [None] * x.shape[1]
+    for t in range(x.shape[1]):
+        before.append(h)
+        h = a[:, t] * h + x[:, t]
+        hs.append(h)
+    for t in range(x.shape[1] - 1, -1, -1):
+        dx[t] = dh[:, t] + u
+        dg[t] = dx[t] * (a[:, t] * before[t])
+        u = a[:, t] * dx[t]
+    return torch.stack(hs, 1), h, torch.stack(dx, 1), torch.stack(dg, 1), u
+
+
+@pytest.mark.parametrize('B,T,D', [(1, 7, 32), (2, 100, 64), (1, 700, 64), (1, 700, 35), (1, 5000, 64), (8, 400, 1280), (8, 400, 1283), (2, 300, 1280)])
+@pytest.mark.parametrize('dtype,gtype', [(BF, BF), (HF, F), (F, F)])
+def test_a_state_that_is_infinite_stays_so(B, T, D, dtype, gtype):
+    """While no decay is zero, however far their product over many tokens falls below fp32's range: where the definition has an infinity or NaN, there
+    it is, of the same sign, and nowhere else."""
+    from b200gdn import gated_recurrence
+    inf = float('inf')
+    for gate in (-1.5, -12.0):   # the product leaves the range over 64 tokens, over eight
+        x, _, h0, dh, dht = make(B, T, D, B, dtype, gtype, True, seed=T)
+        g = torch.full((B, T, D), gate, device='cuda').to(gtype)
+        h0[:, 0], h0[:, 1], x[:, T // 3, 2], x[:, T // 4, 3], x[:, T // 2, 3] = inf, -inf, inf, inf, -inf
+        x[:, 2, 4], g[:, T // 2, 4] = -inf, -inf          # a decay of zero: NaN from there on
+        dht[:, 5], dht[:, 6], dh[:, T // 2, 7], dh[:, T - 1, 8], dh[:, T // 2, 8] = inf, -inf, inf, -inf, inf
+        dh[:, T // 2, 9], g[:, T // 3, 9] = inf, -inf
+        leaves = [t.clone().requires_grad_(True) for t in (x, g, h0)]
+        h, ht = gated_recurrence(*leaves, output_final_state=True)
+        got = [h.detach(), ht.detach(), *torch.autograd.grad([h, ht], leaves, [dh, dht])]
+        for name, p, q in zip(('h', 'ht', 'dx', 'dg', 'dh0'), got, _token_by_token(x, g, h0, dh, dht)):
+            p = p.double()
+            assert torch.equal(torch.isnan(p), torch.isnan(q)), (name, gate)
+            assert torch.equal(p[torch.isinf(p)], q[torch.isinf(p)]) and torch.equal(torch.isinf(p), torch.isinf(q)), (name, gate)
