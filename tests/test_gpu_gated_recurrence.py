@@ -364,3 +364,64 @@ def test_a_state_that_is_infinite_stays_so(B, T, D, dtype, gtype):
             p = p.double()
             assert torch.equal(torch.isnan(p), torch.isnan(q)), (name, gate)
             assert torch.equal(p[torch.isinf(p)], q[torch.isinf(p)]) and torch.equal(torch.isinf(p), torch.isinf(q)), (name, gate)
+
+
+def side_by_side(t):
+    """[B, T, ...] as [T, B ...]: sequences of one length as channels of one, which the oracle walks in T steps"""
+    return t.transpose(0, 1).reshape(t.shape[1], -1)
+
+
+def run_side_by_side(x, g, h0, dh, dht):
+    from b200gdn import gated_recurrence
+    leaves = [t if t is None else t.clone().requires_grad_(True) for t in (x, g, h0)]
+    h, ht = gated_recurrence(*leaves, output_final_state=True)
+    r = O.recurrence(side_by_side(x), side_by_side(g), None if h0 is None else h0.reshape(1, -1), [(0, x.shape[1])], side_by_side(dh), dht.reshape(1, -1))
+    got = torch.autograd.grad([h, ht], [t for t in leaves if t is not None], [dh, dht])
+    for name, t in (('h', h.detach()), ('dx', got[0]), ('dg', got[1])):
+        close(name, side_by_side(t), r[name], r[name + '_off'])
+    close('ht', ht.detach().reshape(1, -1), r['ht'], r['ht_off'])
+    if h0 is not None:
+        close('dh0', got[2].reshape(1, -1), r['dh0'], r['dh0_off'])
+
+
+@pytest.mark.parametrize('B,T,D', [(8, 700, 1280), (8, 641, 1290), (8, 700, 1283), (5, 1300, 2056), (1, 6000, 64), (1, 6100, 33), (3, 3000, 130)])
+@pytest.mark.parametrize('dtype,gtype', [(BF, BF), (BF, F), (HF, HF), (F, F)])
+def test_many_steps(B, T, D, dtype, gtype):
+    """More pieces of work than SMs, where a CTA has its sequence alone and walks it in many steps (by TMA, by pairs, by single elements); and
+    few channels in clusters, three and more steps of the largest."""
+    for h0 in (True, False):
+        run_side_by_side(*make(B, T, D, B, dtype, gtype, h0, seed=T))
+
+
+@pytest.mark.parametrize('B,T,D,most', [(2, 40, 64, 0.5), (2, 1, 8, 3.0), (1, 3000, 64, 0.03), (1, 2500, 35, 0.03), (8, 400, 1280, 0.1), (3, 7, 5, 2.0)])
+@pytest.mark.parametrize('dtype,gtype', [(BF, BF), (BF, F), (F, F)])
+def test_gates_above_zero(B, T, D, most, dtype, gtype):
+    """States that grow, by up to e^45 over a sequence, beside channels that forget."""
+    x, _, h0, dh, dht = make(B, T, D, B, dtype, gtype, True, seed=D)
+    g = most * torch.rand(B, T, D, device='cuda')
+    g[..., 1::3] *= -1
+    g[..., 2::3] -= most / 2
+    run_side_by_side(x, g.to(gtype), h0, dh, dht)
+
+
+def test_the_gradient_of_a_long_sequence_of_many_rows():
+    """Offsets beyond 2^31 elements, backward: the last rows' gradients are those of a short call from the state before them."""
+    from b200gdn import gated_recurrence
+    T, D, n = 300000, 8192, 200
+    x = torch.full((1, T, D), 0.5, dtype=BF, device='cuda')
+    g = torch.full((1, T, D), -0.125, dtype=BF, device='cuda')
+    dh = torch.zeros(1, T, D, dtype=BF, device='cuda')
+    for t in (x, dh):
+        t[:, -n:] = torch.randn(1, n, D, device='cuda').to(BF)
+    dht = torch.randn(1, D, device='cuda')
+    leaves = [x.requires_grad_(True), g.requires_grad_(True)]
+    h, ht = gated_recurrence(*leaves, output_final_state=True)
+    dx, dg = torch.autograd.grad([h, ht], leaves, [dh, dht])
+    before = torch.full((1, D), 0.5 / (1 - 2.718281828459045 ** -0.125), device='cuda')
+    r = O.recurrence(x.detach()[0, -n:], g.detach()[0, -n:], before, [(0, n)], dh[0, -n:], dht)
+    close('dx', dx[0, -n:], r['dx'], r['dx_off'])
+    # (the state before the tail is off by up to 16 U x its size / (1 - decay), and what is left of it multiplies dx)
+    left = torch.exp(-0.125 * torch.arange(1, n + 1, device='cuda').double())[:, None]
+    off = 16 * O.U * before.double() / (1 - 2.718281828459045 ** -0.125)
+    close('dg', dg[0, -n:], r['dg'], r['dg_off'] + r['dx'].abs() * left * off)
+    assert (dx[0, :1000] == 0).all() and (dg[0, :1000] == 0).all()   # what is left so far ahead is below any digit

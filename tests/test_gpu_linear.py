@@ -262,3 +262,33 @@ def test_gelu_where_little_is_left_of_it(dtype, M):
         limit = EPS[dtype] * want.abs() + (v * v + 16) * 2 * O.U * size + (2.0 ** -25 if dtype == HF else 1e-38)
         far = ((got.double() - want).abs() / limit).max().item()
         assert far <= 1.0, f'{name}: {far:.2f} of what is allowed'
+
+
+def test_results_of_many_rows():
+    """Offsets beyond 2^31 elements, forward and backward: the last rows' results are those of a short call; where the others' upstream gradient is zero, so are
+    the sums over all rows."""
+    from b200gdn import fused_linear
+    M, K, N, n = 300000, 72, 8192, 300
+    x, w, b, r, dy = make(n, K, N, BF, seed=6)
+    want = O.linear(x, w, b, r, 'silu', dy)
+
+    def behind(v):
+        big = torch.zeros(M, v.shape[1], dtype=BF, device='cuda')
+        big[-n:] = v
+        return big
+    leaves = [behind(x).requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True), behind(r)]
+    y = fused_linear(*leaves, activation='silu')
+    close('y', y.detach()[-n:], want['y'], want['y_off'])
+    got = torch.autograd.grad(y, leaves[:3], behind(dy))
+    del y
+    for name, g in zip(NAMES, got):
+        close('d' + name, g[-n:] if name == 'x' else g, want['d' + name], want['d' + name + '_off'])
+    assert (got[0][:-n] == 0).all()
+    del got, leaves
+    x, w, b, r, dy = make(n, N, K, BF, seed=7)   # x and dx of so many elements
+    want = O.linear(x, w, b, r, None, dy)
+    leaves = [behind(x).requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)]
+    y = fused_linear(*leaves, behind(r))
+    close('y', y.detach()[-n:], want['y'], want['y_off'])
+    for name, g in zip(NAMES, torch.autograd.grad(y, leaves, behind(dy))):
+        close('d' + name, g[-n:] if name == 'x' else g, want['d' + name], want['d' + name + '_off'])

@@ -266,3 +266,22 @@ def test_refusals():
     dx, = torch.autograd.grad(residual_rms_norm(leaf)[0].square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match='no second derivative'):
         dx.sum().backward()
+
+
+def test_the_gradient_of_many_rows():
+    """Offsets beyond 2^31 elements, backward."""
+    from b200gdn import residual_rms_norm
+    rows, D, n = 300000, 8192, 64
+    t, dout, dz = make(n, D, BF, F, seed=5)
+
+    def behind(v):   # the last rows of a large tensor
+        big = torch.ones(rows, D, dtype=BF, device='cuda')
+        big[-n:] = v
+        return big
+    big = {k: behind(t[k]).requires_grad_(True) for k in ('y', 'residual', 'gate')}
+    out, z = residual_rms_norm(big['y'], t['weight'], big['residual'], True, t['post_weight'], big['gate'], 'silu')
+    del out
+    got = dict(zip(big, torch.autograd.grad([z], list(big.values()), [behind(dz)])))
+    want = O.rms_norms(t['y'], t['weight'], t['residual'], True, t['post_weight'], t['gate'], 'silu', None, 1e-6, None, dz)
+    for k, v in got.items():
+        close('d' + k, v[-n:], want['d' + k], want['d' + k + '_size'])
