@@ -6,13 +6,14 @@
 // steps of W R tokens, R for each of its W = 8 warps: each warp joins its own tokens, leaves (A, h') in shared memory, and after one barrier
 // a step goes through the warps ahead of it for the state its first token sees, then through its tokens again.  Where there are fewer
 // sequences x channel tiles than SMs (or some sequences are much longer than others), CTAs of a cluster share a sequence: step by step each
-// takes its turn of W R tokens, and their joined pairs go to one another's shared memory.  Tokens come by TMA two steps ahead; where rows are not a multiple of
-// 16 bytes, to registers one step ahead.
+// takes its turn of W R tokens, and their joined pairs go to one another's shared memory.  Tokens come by TMA, two steps ahead where a step's tiles are
+// 32 KB (forward with gates of x's type, backward of 16-bit x with fp32 gates), one where they are 48 (the others); where rows are not a multiple of 16 bytes, to
+// registers one step ahead.
 // The backward pass does not read h, which is rounded to its type, but forms it again from x in fp32; the forward pass leaves the state
 // ahead of every 64 tokens (a 32nd of x's bytes in bf16) so that this needs no pass of its own from the left.
 // Bound by instructions where warps are few (39 a row of 64 channels forward, 17 of them the decays), by memory where they are many.  Measured: 16 x 1024 x 8192
-// bf16 forward 135 us (123 at copy rate), backward 242 (205); 4 x 4096 x 2048, 128 pieces of work, 49 and 72 (31 and 51); 131072 x 1024 with
-// fp32 decays, 16 pieces in clusters of 12, 280 (164); 8191 x 1003 fp32, 16 pieces, 39 and 58 (15 and 25).
+// bf16 forward 139 us (123 at copy rate), backward 242 (205); 4 x 4096 x 2048, 128 pieces of work, 52 and 73 (31 and 51); 131072 x 1024 with
+// fp32 decays, 16 pieces in clusters of 12, 272 (164); 8191 x 1003 fp32, 16 pieces, 40 and 59 (15 and 25).
 #include "gdn_common.cuh"
 #include "rowio.cuh"
 #include "tc5.cuh"
@@ -81,7 +82,7 @@ struct Piece {
 };
 
 // exp of a pair: 2^n 2^f with n the nearest integer to g log2 e and a polynomial of degree six for 2^f on [-1/2, 1/2] (least squares of the
-// relative error, 2e-9), in pairs of operations.  Off by 1.5 units of 2^-24 at most and 0.1
+// relative error: 6e-9 root mean square, 1.6e-8 at most), in pairs of operations.  Off by 1.5 units of 2^-24 at most and 0.1
 // on average where |g| < 1 (beyond, log2 e as a float adds |g| / 4).  The average is what counts here: a
 // channel that remembers a thousand tokens multiplies as many decays, and ex2.approx, which is 0.4 units too small on average (measured),
 // would leave its state off by 2.4e-5.  Below 2^-126.5 the result is zero.
@@ -393,7 +394,7 @@ constexpr int stages_of(int stage_bytes, bool cluster) {   // two CTAs an SM
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
-// TMA: the tokens come by way of shared memory, several steps ahead; else (odd widths and boundaries) straight to registers, one step ahead.
+// TMA: the tokens come by way of shared memory, one or two steps ahead; else (odd widths and boundaries) straight to registers, one step ahead.
 template <typename T, typename G, int APART, int R, int W, bool CLUSTER, bool TMA>
 __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     recurrence_fwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, const b200gdn_gated_recurrence_args a) {

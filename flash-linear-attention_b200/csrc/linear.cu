@@ -14,7 +14,9 @@
 // TMA wants rows 16 bytes apart: operands of other widths are first copied to rows that are.
 // Bound by the tensor pipe (88 to 92 % of its cycles) and the clock it is left: 16384 x 2048 -> 8192 bf16 with bias and SiLU, z kept, 343 us
 // (1.60 PFLOP/s; 1.64 is the library's burst), dx 345, dW 366, dz with db 135 (123 at copy rate).  Small products: 2 us until the first operands are there,
-// 0.3 us a step of 64, 2 us for the last epilogue and the end.  4 tokens, 2048 -> 8192: 7.9 us a call (5.1 for W at copy rate).
+// 0.3 us a step of 64, 2 us for the last epilogue and the end.  4 tokens, 2048 -> 8192: 7.8 us a call (5.1 for W at copy rate).
+// Rounded to 16 bits beside the results: dz, since the products read 16 bits (bf16 dx and dW are off by 0.0024 of their size against 64 bits, 0.0017 of it by
+// their own rounding), and the z kept for the backward pass, which in 32 would take as many bytes again as y: the slope changes by at most 0.8 of what z does.
 #include "gdn_common.cuh"
 #include "rowio.cuh"
 #include "tc5.cuh"
@@ -31,7 +33,7 @@ enum { NONE = 0, SILU = B200GDN_LINEAR_SILU, SIGMOID = B200GDN_LINEAR_SIGMOID, G
 // The normal distribution's function of a pair, and e = exp(-v^2 / 2).  Of -|v| it is e t Q(t) with t = 1 / (1 + 0.24 |v|), Q of degree seven by least squares of the
 // relative error (4.3e-7; 7.5e-7 with fp32's roundings near zero, and v^2 2^-24 more by the exponent's further down), and of |v| one less that: relative to the
 // result everywhere.  (1 + erf loses below -4 what a 16-bit result still shows.)  Where the distribution ends, |v| is held at 32, so that infinities are
-// multiplied with zero and one.  erfcf instead took 492 us for 16384 x 2048 -> 8192.
+// multiplied with zero and one.  16384 x 2048 -> 8192: 409 us, 492 with erfcf, 428 with 1 + erf.
 __device__ __forceinline__ uint64_t normal2(uint64_t v, uint64_t& e) {
   auto k = [](float c) { return pack2(c, c); };
   const float2 x = unpack2(v);

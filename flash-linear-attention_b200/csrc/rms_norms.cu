@@ -8,8 +8,9 @@
 // HBM streaming, in the manner of layer_norm.cu: the threads of a group share a row, E elements each, which are worked on as E / 2 fp32 pairs;
 // groups walk the rows, so that a thread's columns stay its own: parameters are read once, their gradients are sums in registers, which a
 // second kernel joins in a fixed order.  The second norm needs what the first one gives: two barriers a row, forward as well as backward.
-// Rows of more than 256 elements come by bulk copies into a ring of shared memory, two rows ahead; shorter ones, of tensors that do not begin on
-// 16 bytes, and backward those whose width is no multiple of 16 bytes, to registers, one row ahead.
+// Rows of more than 256 elements come by bulk copies into a ring of shared memory, two rows ahead (backward in fp32 above 512 columns one); shorter ones, of
+// tensors that do not begin on 16 bytes, and backward those whose width is no multiple of 16 bytes, to registers, one row ahead (backward with more than 16 bytes of
+// a row a thread, so in fp32, where they are used).
 // Measured, bf16: 65536 x 4096 with both norms and a scale forward 330 us (328 at copy rate), backward 525 (492); 16384 x 2048 with a sigmoid gate as
 // well 62 (51) and 119 (82), where instructions count: 28 and 57 an element; 8191 x 1003 fp32 37 (25) and 58 (40), 8191 x 1002 bf16 25 and 45 (13 and 20).
 // Rows of other widths than multiples of 16 bytes beyond 4096 elements spill backward (260 to 576 bytes a thread); beyond 8192 elements a
