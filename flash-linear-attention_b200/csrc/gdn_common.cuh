@@ -120,8 +120,8 @@ __device__ __forceinline__ bool successor_cta(int dist, int& c2, int& h2) {
 }
 
 // Kernels of a chain on one stream are launched while their predecessor finishes (its CTAs leave room SM by SM) and wait
-// here, as the first thing they do, until it is complete and its writes are visible: no tensor memory is allocated and nothing
-// global is touched before.  The successor's launch is released after that, so at most two kernels of a chain are resident.
+// here, before all but their own barriers, until it is complete and its writes are visible (to ordinary loads: the non-coherent path promises
+// nothing): no tensor memory is allocated and nothing global is touched before.  The successor's launch is released after that, so at most two kernels of a chain are resident.
 __device__ __forceinline__ void wait_for_predecessor() {
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
@@ -212,7 +212,7 @@ int ensure_smem(Kern kern, size_t bytes) {   // `bytes` is a constant of the ker
 }
 
 // Launch that may begin while the kernel before it on the stream is finishing (`overlap`); the kernel calls
-// wait_for_predecessor() before anything else.  Measured: 1 x 1024 tokens, 4 heads of 64, forward (two kernels) 29.5 -> 26.0 us;
+// wait_for_predecessor() before anything but setting up its barriers.  Measured: 1 x 1024 tokens, 4 heads of 64, forward (two kernels) 29.5 -> 26.0 us;
 // 16 x 86 tokens, 24 heads of 64, 39.8 -> 35.8.  With many waves of CTAs there is nothing to hide and the waiting CTAs are in the
 // way: B4 T4096 16 heads forward and backward 513 -> 519 us, 65536 tokens, 32 heads 3890 -> 3960; so up to 2048 chunk-heads.
 inline bool overlaps(const b200gdn_chunk_args& a) { return (int64_t)a.n_chunks * a.HV <= 2048; }
