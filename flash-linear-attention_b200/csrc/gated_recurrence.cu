@@ -187,11 +187,13 @@ __device__ __forceinline__ void send(uint32_t to, uint32_t from, uint32_t bytes,
                : "memory");
 }
 
-// A wait that has run out is told at the end and not repeated: what follows is invalid, but every thread still comes to the end.
+// A wait that has run out is told at the end and not repeated: what follows is invalid, but every thread still comes to the end.  Nothing more is
+// loaded then, and at the end the first warp, which loads, waits once more for what is on its way, so that no copy outlives its CTA.
 struct Patience {
-  bool ok = true;
-  __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
-    if (ok) ok = tc5::mbar_wait_warp(bar, parity);
+  int stopped = -1;   // the first step whose tokens were not waited for
+  __device__ __forceinline__ bool ok() const { return stopped < 0; }
+  __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int step) {
+    if (ok() && !tc5::mbar_wait_warp(bar, parity)) stopped = step;
   }
 };
 
@@ -220,8 +222,12 @@ struct Exchange {
   __device__ __forceinline__ void enter(uint64_t s) {   // what enters the first step
     if (W > 1 && !CLUSTER && threadIdx.x < 32) carry[0][threadIdx.x] = s;
   }
-  __device__ __forceinline__ void leave() {   // no CTA ends while another one may still send to it
-    if constexpr (CLUSTER) cluster_sync();
+  __device__ __forceinline__ void leave(int n, bool ok) {   // after n steps; no CTA ends while another one may still send to it
+    if constexpr (CLUSTER) {
+      if (!ok && threadIdx.x < 32)
+        for (int i = n > 2 ? n - 2 : 0; i < n; ++i) (void)tc5::mbar_wait_warp(&came[i & 1], (i >> 1) & 1);
+      cluster_sync();
+    }
   }
 };
 
@@ -314,7 +320,7 @@ __device__ __forceinline__ uint64_t join(Exchange<W, CLUSTER>& x, int i, int war
         if constexpr (REVERSE) ahead = ahead_at(W - 1);
         else ahead = {pack2(1.f, 1.f), 0ull};
       }
-      patience.wait(&x.came[turn], (i >> 1) & 1);
+      patience.wait(&x.came[turn], (i >> 1) & 1, i + 1);
       const uint64_t first = s;
       uint64_t entering = s;
 #pragma unroll 4
@@ -386,6 +392,10 @@ struct Tiles {
 #pragma unroll
     for (int i = 0; i < N; ++i) tma::load_2d(base + stage * offset[N] + offset[i], maps[i], channel, row, &full[stage]);
   }
+  // the warp that loads, where a wait has run out: what was loaded of the n steps from `first` on
+  __device__ __forceinline__ void land(int first, int n) const {
+    for (int i = first; i < first + STAGES && i < n; ++i) (void)tc5::mbar_wait_warp(&full[i % STAGES], (i / STAGES) & 1);
+  }
   __device__ __forceinline__ const unsigned char* row(int stage, int i, int r) const { return base + stage * offset[N] + offset[i] + r * bytes[i]; }
 };
 constexpr int stages_of(int stage_bytes, bool cluster) {   // two CTAs an SM
@@ -446,7 +456,7 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     const int rows = seq.len - t;
     Joined own = {pack2(1.f, 1.f), 0ull};
     if constexpr (TMA) {
-      patience.wait(&full[stage], phase);
+      patience.wait(&full[stage], phase, i);
       const unsigned char *px = tiles.row(stage, 0, in_step) + 2 * lane * sizeof(T), *pg = tiles.row(stage, 1, in_step) + 2 * lane * sizeof(G);
       if (rows >= R) {
 #pragma unroll
@@ -483,7 +493,7 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
   };
   // once all warps have step i in registers
   auto next = [&](int i) {
-    if (TMA && threadIdx.x == 0 && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + (i + STAGES) * step + at.rank * ROWS);
+    if (TMA && threadIdx.x == 0 && patience.ok() && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + (i + STAGES) * step + at.rank * ROWS);
     if (++stage == STAGES) {
       stage = 0;
       phase ^= 1u;
@@ -515,8 +525,11 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     finish(t0, h);
   }
   if (a.ht && live && knows_the_end<W, CLUSTER, false>(n, warp, at.rank)) store_state<APART>(a.ht, (int64_t)at.seq * a.D + at.channel, s, two);
-  if (!patience.ok && lane == 0) atomicExch(&g_recurrence_timeout, 1);
-  exchange.leave();
+  if (!patience.ok()) {
+    if (TMA && warp == 0) tiles.land(patience.stopped, n);
+    if (lane == 0) atomicExch(&g_recurrence_timeout, 1);
+  }
+  exchange.leave(n, patience.ok());
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
@@ -583,7 +596,7 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     Joined own = {pack2(1.f, 1.f), 0ull};
     const int rows = seq.len - t0;
     if constexpr (TMA) {
-      patience.wait(&full[stage], phase);
+      patience.wait(&full[stage], phase, i);
       const unsigned char *px = tiles.row(stage, 0, in_step) + 2 * lane * sizeof(T), *pg = tiles.row(stage, 1, in_step) + 2 * lane * sizeof(G),
                           *pd = tiles.row(stage, 2, in_step) + 2 * lane * sizeof(T);
       if (rows >= R) {
@@ -628,7 +641,7 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     }
     if constexpr (W > 1) left[i & 1][warp][lane] = make_ulonglong2(own.a, own_left);
     auto next = [&] {
-      if (TMA && threadIdx.x == 0 && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + last - (i + STAGES) * step);
+      if (TMA && threadIdx.x == 0 && patience.ok() && i + STAGES < n) tiles.load(stage, maps, at.tile, (int)seq.first + last - (i + STAGES) * step);
     };
     uint64_t u = join<W, CLUSTER, true>(exchange, i, warp, at.rank, at.n_ranks, own, s, patience, next);
     if (++stage == STAGES) {
@@ -676,8 +689,11 @@ __global__ void __launch_bounds__(W * 32, W == 1 ? 8 : 2)
     else finish(std::false_type());
   }
   if (a.dh0 && live && knows_the_end<W, CLUSTER, true>(n, warp, at.rank)) store_state<APART>(a.dh0, (int64_t)at.seq * a.D + at.channel, s, two);
-  if (!patience.ok && lane == 0) atomicExch(&g_recurrence_timeout, 1);
-  exchange.leave();
+  if (!patience.ok()) {
+    if (TMA && warp == 0) tiles.land(patience.stopped, n);
+    if (lane == 0) atomicExch(&g_recurrence_timeout, 1);
+  }
+  exchange.leave(n, patience.ok());
 }
 
 // ---- one token a sequence ------------------------------------------------------------------------------------------------

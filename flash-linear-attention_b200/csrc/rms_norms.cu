@@ -128,7 +128,7 @@ struct Ring {
   uint64_t* full;
   int slot = 0;
   uint32_t phase = 0;
-  bool ok = true;
+  int stopped = -1;   // slot and phase of a wait that has run out
 
   // one thread of the group
   template <typename T>
@@ -151,8 +151,18 @@ struct Ring {
   __device__ __forceinline__ const T* first(int n, int64_t row, int row_bytes) const {   // of the tensors of the row that is there now
     return reinterpret_cast<const T*>(base + slot * n * room_of(row_bytes) + (row * row_bytes & 15));
   }
-  __device__ __forceinline__ void wait() {   // (a wait that has run out is told at the end and not repeated)
-    if (ok) ok = tc5::mbar_wait_warp(&full[slot], phase);
+  // A wait that has run out is not repeated: nothing more is copied, and at the end what is on its way is waited for once more, so that no copy
+  // outlives its CTA, and the flag set.
+  __device__ __forceinline__ void wait() {
+    if (stopped < 0 && !tc5::mbar_wait_warp(&full[slot], phase)) stopped = slot << 1 | (int)phase;
+  }
+  __device__ __forceinline__ bool ok() const { return stopped < 0; }
+  __device__ __forceinline__ void finish() {   // a warp of the group
+    if (stopped < 0) return;
+    slot = stopped >> 1;
+    phase = stopped & 1;
+    for (int i = 0; i < SLOTS; ++i, next()) (void)tc5::mbar_wait_warp(&full[slot], phase);
+    if ((threadIdx.x & 31) == 0) atomicExch(&g_norms_timeout, 1);
   }
   __device__ __forceinline__ void next() {
     if (++slot == SLOTS) {
@@ -279,7 +289,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     row_sums<TPR>(s, scratch[turn][1]);
     if constexpr (RING) {   // (the whole group has passed: what it read is in registers)
       if (TPR == 32) __syncwarp();
-      if (sub == 0 && row + SLOTS * step < a.rows) ring.template fill<T>(ring.slot, tensors, n_tensors, row + SLOTS * step, a.rows, row_bytes);
+      if (sub == 0 && ring.ok() && row + SLOTS * step < a.rows) ring.template fill<T>(ring.slot, tensors, n_tensors, row + SLOTS * step, a.rows, row_bytes);
       ring.next();
     }
     const float r2 = __frsqrt_rn(s[0] * up + a.eps);
@@ -299,7 +309,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
       a.rstd_z[row] = r2;
     }
   }
-  if (RING && !ring.ok && sub == 0) atomicExch(&g_norms_timeout, 1);
+  if constexpr (RING) ring.finish();
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
@@ -468,7 +478,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     }
     if constexpr (RING) {
       if (TPR == 32) __syncwarp();
-      if (sub == 0 && row + SLOTS * step < a.rows) ring.template fill<T>(ring.slot, tensors, n_tensors, row + SLOTS * step, a.rows, row_bytes);
+      if (sub == 0 && ring.ok() && row + SLOTS * step < a.rows) ring.template fill<T>(ring.slot, tensors, n_tensors, row + SLOTS * step, a.rows, row_bytes);
       ring.next();
     }
     if (!live || !a.dy) continue;
@@ -476,7 +486,7 @@ __global__ void __launch_bounds__(threads_of(TPR), 512 / threads_of(TPR)) rms_no
     for (int i = 0; i < P; ++i) y.set(i, mul2(fma2(mul2(y.pair(i), r1), mean, z[i]), r1));   // (r1 is one without the first norm)
     y.store(static_cast<T*>(a.dy) + row * a.D, sub, a.D);
   }
-  if (RING && !ring.ok && sub == 0) atomicExch(&g_norms_timeout, 1);
+  if constexpr (RING) ring.finish();
   if (a.partials == nullptr) return;
   constexpr int COLUMNS = TPR * E;
   auto leave = [&](int which, int i, uint64_t x) {
