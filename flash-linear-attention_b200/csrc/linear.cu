@@ -14,7 +14,7 @@
 // TMA wants rows 16 bytes apart: operands of other widths are first copied to rows that are.
 // Bound by the tensor pipe (88 to 92 % of its cycles) and the clock it is left: 16384 x 2048 -> 8192 bf16 with bias and SiLU, z kept, 343 us
 // (1.60 PFLOP/s; 1.64 is the library's burst), dx 345, dW 366, dz with db 135 (123 at copy rate).  Small products: 2 us until the first operands are there,
-// 0.3 us a step of 64, 2 us for the last epilogue and the end.  4 tokens, 2048 -> 8192: 7.8 us a call (5.1 for W at copy rate).
+// 0.3 us a step of 64, 2 us for the last epilogue and the end.  4 tokens, 2048 -> 8192: 7.6 us a call (5.1 for W at copy rate).
 // Rounded to 16 bits beside the results: dz, since the products read 16 bits (bf16 dx and dW are off by 0.0024 of their size against 64 bits, 0.0017 of it by
 // their own rounding), and the z kept for the backward pass, which in 32 would take as many bytes again as y: the slope changes by at most 0.8 of what z does.
 #include "gdn_common.cuh"
